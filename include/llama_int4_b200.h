@@ -359,6 +359,90 @@ int li4_argmax_rows_allreduce(const void* logits, int dtype, int64_t rows, int64
 int li4_gather_rows(const void* table, int64_t table_rows, int64_t cols, int64_t stride_t, const int64_t* ids,
                     int64_t rows, void* out, int64_t stride_o, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * A paged KV cache: pages of page_size rows (a power of two from 8 to 1024) named by block tables.
+ * Cache slot = page * page_size + row in the page.  No counterpart in the reference, whose cache is one
+ * [max_batch, max_seq] block per layer (llama/model.py:195-215) that pads every prompt to the longest.
+ * --------------------------------------------------------------------------- */
+
+/* The bookkeeping of one serving step, in one launch.  Request b holds kv_lens[b] tokens and
+ * appends new_lens[b]; its fresh pages, ceil((kv + new) / page_size) - ceil(kv / page_size), come from
+ * the top of the stack free_pages[0 .. *n_free): the k-th fresh page of the step, in request order then
+ * block order, is free_pages[*n_free - 1 - k].  Writes
+ *   block_tables  [n_requests, table_width] (row stride table_stride), the entries of the fresh pages only
+ *   cu_seqlens    [n_requests + 1], the first token of each request in the step's packed tokens
+ *   positions     [n_tokens], each packed token's position in its request
+ *   slots         [n_tokens], its cache slot
+ *   kv_lens_out, n_free_out   the lengths and the stack's height after the step (may be kv_lens, n_free)
+ *   granted       [n_requests], 1, or 0 where the table is too narrow, the pages taken in request order
+ *                 exceed *n_free (a request that needs none is granted) or the tokens pass n_tokens.
+ * A request that is not granted keeps its length and takes no page; its tokens get slot -1, which
+ * li4_rope_paged_write skips.  n_tokens is the host's count of the new tokens; tokens past
+ * cu_seqlens[n_requests] get position 0 and slot -1.  At most 8192 requests.  free_pages is read only:
+ * the popped entries lie above the new height.  free_capacity: entries of free_pages (*n_free is
+ * clamped to it). */
+int li4_paged_append(const int32_t* kv_lens, const int32_t* new_lens, int64_t n_requests, int32_t* block_tables,
+                     int64_t table_stride, int64_t table_width, const int32_t* free_pages, int64_t free_capacity,
+                     const int32_t* n_free, int64_t page_size, int64_t n_tokens, int32_t* cu_seqlens,
+                     int32_t* positions, int64_t* slots, int32_t* kv_lens_out, int32_t* n_free_out,
+                     uint8_t* granted, void* stream);
+
+/* RoPE on packed queries and keys and the cache write of keys and values, in one launch.  q
+ * [n_tokens, n_heads, head_dim], k and v [n_tokens, n_kv_heads, head_dim], LI4_F16 or LI4_BF16; pairs
+ * (2i, 2i + 1) turn by the angle of table row positions[t], column i, in fp32, rounded once
+ * (apply_rotary_emb, llama/model.py:126-152).  q_out and k_out (k_out may be null) may be q and k.
+ * The turned key and the value of token t go to cache slot slots[t]; a negative slot is skipped.
+ * strides: 16 element strides -- q token, head; k token, head; v token, head; q_out token, head; k_out
+ * token, head; cache_k page, row, head; cache_v page, row, head -- all multiples of 8 (rows start on
+ * 16-byte boundaries).  A position outside [0, max_pos) is clamped, a slot past the cache skipped; both
+ * set bit 7 of li4_device_errors.  Tokens that share a slot are the caller's mistake: one of them stays. */
+int li4_rope_paged_write(const void* q, const void* k, const void* v, int dtype, int64_t n_tokens, int64_t n_heads,
+                         int64_t n_kv_heads, int64_t head_dim, const int64_t* strides, const float* rope_cos,
+                         const float* rope_sin, int64_t rope_stride, int64_t max_pos, const int32_t* positions,
+                         const int64_t* slots, void* q_out, void* k_out, void* cache_k, void* cache_v,
+                         int64_t num_pages, int64_t page_size, void* stream);
+
+/* Causal grouped-query attention of packed sequences.  Sequence b's queries are rows cu_seqlens[b] ..
+ * cu_seqlens[b + 1] - 1 of q [n_tokens, n_heads, head_dim]; query i of n sees keys 0 .. L - n + i of its
+ * sequence's L.  A query that sees no key gives zeros; rows past cu_seqlens[n_seqs] are left as they
+ * were.  Scores, softmax statistics and sums in fp32; probabilities rounded to the type for the second
+ * product; one rounding at the end.  A value row's NaN or infinity reaches only queries that see it. */
+typedef struct li4_attention {
+  const void* q;
+  const void* k;                /* prompt: [n_tokens, n_kv_heads, head_dim]; paged: the cache's pages */
+  const void* v;
+  void* out;                    /* [n_tokens, n_heads, head_dim] */
+  int dtype;                    /* LI4_F16 or LI4_BF16, all four */
+  float scale;                  /* of the scores, usually 1 / sqrt(head_dim) */
+  int64_t stride_qt, stride_qh; /* element strides, multiples of 8: token, head */
+  int64_t stride_ot, stride_oh;
+  int64_t stride_kp, stride_kt, stride_kh; /* page (paged only), row, KV head */
+  int64_t stride_vp, stride_vt, stride_vh;
+  const int32_t* cu_seqlens;    /* device, [n_seqs + 1], rising, within n_tokens */
+  int64_t n_seqs, n_tokens, n_heads, n_kv_heads;
+  int64_t head_dim;             /* a multiple of 8 up to 128 */
+  int64_t max_queries;          /* the longest sequence's queries, known to the host: picks the kernels */
+  /* paged only */
+  const int32_t* kv_lens;       /* device, [n_seqs]: L, with the new tokens' keys already in the cache */
+  const int32_t* block_tables;  /* device, [n_seqs, table_width]; entries outside the cache read as zero rows */
+  int64_t table_stride, table_width;
+  int64_t num_pages, page_size;
+} li4_attention;
+
+/* Bytes of workspace the two calls below need for these sizes (its contents do not matter; calls that may
+ * overlap need separate ones). */
+size_t li4_attention_workspace_bytes(const li4_attention* args);
+
+/* Whole prompts: sequence b's keys and values are its own rows of k and v (L = n).
+ * Replaces: Attention.forward's repeat_kv, mask, two matmuls and softmax on padded prompts
+ * (llama/model.py:262-275). */
+int li4_prompt_attention(const li4_attention* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* New tokens (one each, a few, or a chunk of a prompt) over a paged cache: key j of sequence b is row
+ * j % page_size of page block_tables[b][j / page_size]; L = kv_lens[b], at most table_width * page_size.
+ * Replaces: the same, over cache_k / cache_v (llama/model.py:251-275). */
+int li4_paged_attention(const li4_attention* args, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Device-side error flags of the current device (bit 0: a bounded pipeline wait
  * inside a GEMV kernel ran out; bit 1: a bounded wait for a peer's flag in
  * li4_allreduce_add ran out; bit 2: a decode program's wait for another op
@@ -366,7 +450,8 @@ int li4_gather_rows(const void* table, int64_t table_rows, int64_t cols, int64_t
  * outside its table; bit 4: a bounded wait inside li4_int4_gemm ran out; bit 5: an
  * LI4_EPI_ALLREDUCE_RESIDUAL epilogue's wait for a peer's words ran out; bit 6: a wait of
  * li4_argmax_rows_allreduce for a peer's key ran out -- the kernel
- * carried on and its outputs are not valid).  Synchronising: copies the flags to the host; reset != 0 clears them.
+ * carried on and its outputs are not valid; bit 7: li4_rope_paged_write met a position
+ * or slot out of range).  Synchronising: copies the flags to the host; reset != 0 clears them.
  * A diagnostic for tests and health checks, not for the decode loop. */
 int li4_device_errors(unsigned* flags, int reset);
 

@@ -1,0 +1,627 @@
+// li4_seq_attention.cu -- attention of packed sequences over paged or packed keys, sm_100a.
+//
+// Grouped-query attention by rows: the rep query heads of a KV head, over the queries of a sequence,
+// are the rows of one matrix (row = query * rep + head), so a KV head's keys and values are read once
+// for the whole group.  An item is (sequence, tile of 16 MT rows, KV head); its keys come in units of
+// 128.  Units of all items lie on one line; CTA g of G takes the g-th equal share of it, whatever the
+// lengths are (they are read on the device: the host knows none).  A CTA that covers only a part of an
+// item's keys leaves (running maximum, sum, unnormalised output) in `part`, and a second launch joins
+// the parts in key order, so the result does not depend on timing.
+//
+// Inside a CTA each of the 4 warps streams its own 32 keys of every unit through its own ring of
+// shared-memory stages (cp.async; no CTA barrier until the end): S = Q K^T and O += P V as m16n8k16
+// tensor-core tiles, softmax in fp32 in registers with the running maximum and sum of one pass.  The
+// work is bound by the bytes of the keys and values as long as the rows are few.
+#include <mutex>
+#include <utility>
+#include <vector>
+
+#include "li4_attention_args.cuh"
+#include "li4_gemv_device.cuh"
+
+namespace li4 {
+
+constexpr int kSeqThreads = 128;
+constexpr int kSeqWarps = 4;
+constexpr int kUnit = 128;      // keys per unit: 32 per warp
+constexpr int kSeqStages = 3;   // stages of 32 keys per warp
+
+__host__ __device__ constexpr int seq_stage_bytes(int D) { return 2 * 32 * D * 2; }
+__host__ __device__ constexpr int seq_smem_bytes(int D) { return kSeqWarps * kSeqStages * seq_stage_bytes(D); }
+// floats of one partial result: 16 MT rows of D outputs, then (maximum, sum) per row
+__host__ __device__ constexpr int seq_part_floats(int D, int MT) { return 16 * MT * (D + 2); }
+
+// The line of units.
+struct Line {
+  long long total;
+  int active;  // CTAs that get a share
+};
+__device__ __forceinline__ long long share(const Line& l, int g) { return l.total * g / l.active; }
+
+template <int MT>
+__device__ __forceinline__ long long seq_units(const SeqAttnArgs& a, const Seq& s, int* tiles, int* per) {
+  *tiles = (int)(((long long)s.n * a.rep + 16 * MT - 1) / (16 * MT));
+  *per = max(1, (s.len + kUnit - 1) / kUnit);
+  return (long long)*tiles * *per * a.Hkv;
+}
+
+// Finds the sequence that holds unit share(g): each thread sums a slice of the sequences.  Every thread
+// returns the line, the sequence and the units before it (b = -1: no share).
+template <int MT, bool PAGED>
+__device__ Line find_share(const SeqAttnArgs& a, int g, int* b_out, long long* before) {
+  __shared__ long long s_sum[kSeqWarps];
+  __shared__ int s_b;
+  __shared__ long long s_before;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (a.B + kSeqThreads - 1) / kSeqThreads;
+  const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+  long long mine = 0;
+  int tiles, units;
+  for (int b = b0; b < b1; ++b) mine += seq_units<MT>(a, load_seq<PAGED>(a, b), &tiles, &units);
+  long long incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long x = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += x;
+  }
+  if (lane == 31) s_sum[warp] = incl;
+  if (tid == 0) s_b = -1;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < kSeqWarps; ++w) {
+    if (w < warp) incl += s_sum[w];
+    total += s_sum[w];
+  }
+  Line line;
+  line.total = total;
+  line.active = (int)min((long long)a.grid, max(1LL, total));
+  if (g < line.active && total > 0) {
+    const long long at = share(line, g);
+    long long excl = incl - mine;
+    if (at >= excl && at < incl) {
+      for (int b = b0; b < b1; ++b) {
+        const long long u = seq_units<MT>(a, load_seq<PAGED>(a, b), &tiles, &units);
+        if (at < excl + u) {
+          s_b = b;
+          s_before = excl;
+          break;
+        }
+        excl += u;
+      }
+    }
+  }
+  __syncthreads();
+  *b_out = s_b;
+  *before = s_before;
+  return line;
+}
+
+__device__ __forceinline__ void cp_async16z(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t r[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t r[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  mma_16816(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 32 keys from j0 of the item into a stage: K rows then V rows, 16-byte chunk c of row r at c ^ (r & 7).
+// Rows at or past `end` and rows of no page are zeros.
+template <int D, bool PAGED>
+__device__ __forceinline__ void load_stage(const SeqAttnArgs& a, int b, const Seq& s, int kvh, int j0, int end,
+                                           uint32_t stage) {
+  constexpr int CH = D / 8;          // chunks per row
+  constexpr int RPI = 32 / CH;       // rows per instruction of the warp
+  const int lane = threadIdx.x & 31;
+  long long ko = 0, vo = 0;
+  bool have = false;
+  if (j0 + lane < end) have = key_offsets<PAGED>(a, b, s, j0 + lane, &ko, &vo);
+  const int c = lane % CH;
+  const bool in_head = c * 8 < a.hd;
+  const uint16_t* k = a.k + (long long)kvh * a.skh + c * 8;
+  const uint16_t* v = a.v + (long long)kvh * a.svh + c * 8;
+#pragma unroll
+  for (int i = 0; i < 32 / RPI; ++i) {
+    const int r = i * RPI + lane / CH;
+    const long long kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+    const bool ok = __shfl_sync(0xffffffffu, (int)have, r) && in_head;
+    const uint32_t at = stage + r * (D * 2) + ((c ^ (r & 7)) << 4);
+    cp_async16z(at, ok ? k + kr : a.q, ok);  // (not read where !ok)
+    cp_async16z(at + 32 * D * 2, ok ? v + vr : a.q, ok);
+  }
+}
+
+template <typename T, int D, int MT, bool PAGED>
+__global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid_constant__ SeqAttnArgs a) {
+  constexpr int RT = 16 * MT;
+  constexpr int KS = D / 16;  // k steps of Q K^T
+  constexpr int NT = D / 8;   // column tiles of the output
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ float s_ml[kSeqWarps][RT][2];
+  __shared__ int s_redo[RT];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t ring = smem_addr(smem) + warp * kSeqStages * seq_stage_bytes(D);
+  pdl_launch_dependents();
+  pdl_wait_primary();
+
+  int b;
+  long long before;
+  const int g = blockIdx.x;
+  const Line line = find_share<MT, PAGED>(a, g, &b, &before);
+  if (b < 0) return;
+  const long long at0 = share(line, g);
+  long long left = share(line, g + 1) - at0;
+  long long rem = at0 - before;  // units into sequence b
+  Seq s = load_seq<PAGED>(a, b);
+  int tiles, per;
+  seq_units<MT>(a, s, &tiles, &per);
+
+  while (left > 0) {
+    const int item = (int)(rem / per), u0 = (int)(rem - (long long)item * per);
+    const int u1 = (int)min((long long)per, u0 + left);
+    const int kvh = item % a.Hkv, tile = item / a.Hkv;
+    const int row0 = tile * RT;
+    const int rows = min(RT, s.n * a.rep - row0);
+    const int first_lim = s.len - s.n + row0 / a.rep;               // last key the tile's first query sees
+    const int last_lim = s.len - s.n + (row0 + rows - 1) / a.rep;   // and its last query
+    const int k0 = u0 * kUnit, k1 = min(min(u1 * kUnit, s.len), last_lim + 1);
+
+    // ---- queries as A fragments; rows past the tile are zero rows that see no key
+    uint32_t qf[MT][KS][4];
+    int lim[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int r = mt * 16 + hf * 8 + lane / 4;
+        const bool valid = r < rows;
+        const int pr = row0 + (valid ? r : 0);
+        const int tok = pr / a.rep;
+        lim[mt][hf] = valid ? s.len - s.n + tok : -1;
+        const uint16_t* q = a.q + (long long)(s.start + tok) * a.sqt + (long long)(kvh * a.rep + pr - tok * a.rep) * a.sqh;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int d = ks * 16 + c * 8 + (lane & 3) * 2;
+            qf[mt][ks][hf + 2 * c] = valid && d < a.hd ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
+          }
+      }
+    float o[MT][NT][4];
+    float m[MT][2], l[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
+      m[mt][0] = m[mt][1] = -INFINITY;
+      l[mt][0] = l[mt][1] = 0.f;
+    }
+
+    // ---- the warp's keys: k0 + 32 warp + 128 i
+    const int w0 = k0 + warp * 32;
+    const int steps = w0 < k1 ? (k1 - w0 + kUnit - 1) / kUnit : 0;
+#pragma unroll
+    for (int i = 0; i < kSeqStages - 1; ++i) {
+      if (i < steps) load_stage<D, PAGED>(a, b, s, kvh, w0 + i * kUnit, k1, ring + i * seq_stage_bytes(D));
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    int slot = 0;
+    for (int i = 0; i < steps; ++i) {
+      const int ahead = i + kSeqStages - 1;
+      int next = slot + kSeqStages - 1;
+      if (next >= kSeqStages) next -= kSeqStages;
+      __syncwarp();
+      if (ahead < steps) load_stage<D, PAGED>(a, b, s, kvh, w0 + ahead * kUnit, k1, ring + next * seq_stage_bytes(D));
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.wait_group %0;" ::"n"(kSeqStages - 1) : "memory");
+      __syncwarp();
+      const uint32_t ks_at = ring + slot * seq_stage_bytes(D), vs_at = ks_at + 32 * D * 2;
+      const int j0 = w0 + i * kUnit;
+      slot = slot + 1 == kSeqStages ? 0 : slot + 1;
+
+      float sc[MT][4][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int ks2 = 0; ks2 < KS / 2; ++ks2) {  // 8 keys x 32 dims: four 8x8 matrices
+          uint32_t kf[4];
+          const int r = nt * 8 + (lane & 7), c = ks2 * 4 + (lane >> 3);
+          ldmatrix_x4(kf, ks_at + r * (D * 2) + ((c ^ (r & 7)) << 4));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16816<T>(sc[mt][nt], qf[mt][ks2 * 2], kf[0], kf[1]);
+            mma16816<T>(sc[mt][nt], qf[mt][ks2 * 2 + 1], kf[2], kf[3]);
+          }
+        }
+      const bool mask = j0 + 31 > first_lim || rows < RT || j0 + 32 > k1;
+      uint32_t pf[MT][2][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = sc[mt][nt][e] * a.scale_log2;
+            const int j = j0 + nt * 8 + (lane & 3) * 2 + (e & 1);
+            if (mask && (j > lim[mt][e >> 1] || j >= k1)) x = -INFINITY;
+            sc[mt][nt][e] = x;
+            mx[e >> 1] = fmaxf(mx[e >> 1], x);
+          }
+        float base[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
+          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
+          const float mn = fmaxf(m[mt][hf], mx[hf]);
+          base[hf] = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every probability is exp2(-inf) = 0
+          const float keep = exp2_fast(m[mt][hf] - base[hf]);
+          m[mt][hf] = mn;
+          l[mt][hf] *= keep;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            o[mt][nt][hf * 2] *= keep;
+            o[mt][nt][hf * 2 + 1] *= keep;
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[mt][nt][e] = exp2_fast(sc[mt][nt][e] - base[e >> 1]);
+            l[mt][e >> 1] += sc[mt][nt][e];
+          }
+          pf[mt][nt >> 1][(nt & 1) * 2] = Type16<T>::pack(sc[mt][nt][0], sc[mt][nt][1]);
+          pf[mt][nt >> 1][(nt & 1) * 2 + 1] = Type16<T>::pack(sc[mt][nt][2], sc[mt][nt][3]);
+        }
+      }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)  // 16 keys x 16 dims: four transposed 8x8 matrices
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+          uint32_t vf[4];
+          const int r = kb * 16 + (lane & 15), c = dt * 2 + (lane >> 4);
+          ldmatrix_x4_trans(vf, vs_at + r * (D * 2) + ((c ^ (r & 7)) << 4));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16816<T>(o[mt][dt * 2], pf[mt][kb], vf[0], vf[1]);
+            mma16816<T>(o[mt][dt * 2 + 1], pf[mt][kb], vf[2], vf[3]);
+          }
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // every warp is done with its ring: the outputs may use it
+
+    // ---- join the four warps
+    float* so = reinterpret_cast<float*>(smem) + warp * RT * D;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int r = mt * 16 + hf * 8 + lane / 4;
+        float sum = l[mt][hf];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if ((lane & 3) == 0) {
+          s_ml[warp][r][0] = m[mt][hf];
+          s_ml[warp][r][1] = sum;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          *reinterpret_cast<float2*>(so + r * D + nt * 8 + (lane & 3) * 2) =
+              make_float2(o[mt][nt][hf * 2], o[mt][nt][hf * 2 + 1]);
+      }
+    if (tid < RT) s_redo[tid] = 0;
+    __syncthreads();
+    const bool whole = u0 == 0 && u1 == per;
+    const bool masked = k1 - 1 > first_lim;  // some row must not see some of the keys read
+    float* part = a.part + (size_t)(2 * g + (u0 == 0 ? 1 : 0)) * seq_part_floats(D, MT);
+    const float* all = reinterpret_cast<const float*>(smem);
+    for (int e = tid; e < RT * D / 2; e += kSeqThreads) {
+      const int r = e / (D / 2), d = (e - r * (D / 2)) * 2;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kSeqWarps; ++w) M = fmaxf(M, s_ml[w][r][0]);
+      const float base = M == -INFINITY ? 0.f : M;
+      float L = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+      for (int w = 0; w < kSeqWarps; ++w) {
+        const float f = exp2_fast(s_ml[w][r][0] - base);
+        const float2 ov = *reinterpret_cast<const float2*>(all + (w * RT + r) * D + d);
+        L += f * s_ml[w][r][1];
+        x += f * ov.x;
+        y += f * ov.y;
+      }
+      if (r >= rows) continue;
+      if (masked && isfinite(L) && !(isfinite(x) && isfinite(y))) s_redo[r] = 1;
+      if (whole) {
+        const int pr = row0 + r, tok = pr / a.rep;
+        const bool none = s.len - s.n + tok < 0;  // a row that sees no key is zero
+        const float inv = none ? 0.f : 1.f / L;
+        if (d < a.hd)
+          *reinterpret_cast<uint32_t*>(a.out + (long long)(s.start + tok) * a.sot +
+                                       (long long)(kvh * a.rep + pr - tok * a.rep) * a.soh + d) =
+              none ? 0u : Type16<T>::pack(x * inv, y * inv);
+      } else {
+        *reinterpret_cast<float2*>(part + r * D + d) = make_float2(x, y);
+        if (d == 0) *reinterpret_cast<float2*>(part + RT * D + r * 2) = make_float2(M, L);
+      }
+    }
+    __syncthreads();
+    if (masked) {
+      for (int r = warp; r < rows; r += kSeqWarps) {
+        if (!s_redo[r]) continue;
+        float M = -INFINITY, L = 0.f;
+        for (int w = 0; w < kSeqWarps; ++w) M = fmaxf(M, s_ml[w][r][0]);
+        const float base = M == -INFINITY ? 0.f : M;
+        for (int w = 0; w < kSeqWarps; ++w) L += exp2_fast(s_ml[w][r][0] - base) * s_ml[w][r][1];
+        float x[D / 32];
+        redo_row<T, PAGED, D>(a, b, s, kvh, row0 + r, k0, k1, base, x);
+        const int pr = row0 + r, tok = pr / a.rep;
+        uint16_t* out = a.out + (long long)(s.start + tok) * a.sot + (long long)(kvh * a.rep + pr - tok * a.rep) * a.soh;
+        const bool none = s.len - s.n + tok < 0;
+        for (int i = 0; i < D / 32; ++i) {
+          const int d = lane + 32 * i;
+          if (!whole) part[r * D + d] = x[i];
+          else if (d < a.hd) out[d] = none ? 0 : Type16<T>::one(x[i] / L);
+        }
+      }
+      __syncthreads();
+    }
+
+    left -= u1 - u0;
+    rem += u1 - u0;
+    while (left > 0 && rem >= (long long)tiles * per * a.Hkv) {
+      rem -= (long long)tiles * per * a.Hkv;
+      s = load_seq<PAGED>(a, ++b);
+      seq_units<MT>(a, s, &tiles, &per);
+    }
+  }
+}
+
+// Joins the parts of the item that the boundary between CTAs blockIdx.x and blockIdx.x + 1 cuts, if it is the
+// first boundary inside that item.
+template <typename T, int D, int MT, bool PAGED>
+__global__ void __launch_bounds__(kSeqThreads) seq_attention_join_kernel(const __grid_constant__ SeqAttnArgs a) {
+  constexpr int RT = 16 * MT;
+  pdl_launch_dependents();
+  pdl_wait_primary();
+  const int g = blockIdx.x + 1;
+  int b;
+  long long before;
+  const Line line = find_share<MT, PAGED>(a, g, &b, &before);
+  if (b < 0) return;
+  const Seq s = load_seq<PAGED>(a, b);
+  int tiles, per;
+  seq_units<MT>(a, s, &tiles, &per);
+  const long long rem = share(line, g) - before;
+  const int item = (int)(rem / per);
+  const long long start = before + (long long)item * per, end = start + per;
+  if (start == share(line, g) || share(line, g - 1) > start) return;
+  int last = g;  // the parts are CTAs g - 1 (from the item's start) and g .. last
+  while (last + 1 < line.active && share(line, last + 1) < end) ++last;
+  const int kvh = item % a.Hkv, row0 = item / a.Hkv * RT;
+  const int rows = min(RT, s.n * a.rep - row0);
+  const float* first = a.part + (size_t)(2 * (g - 1) + 1) * seq_part_floats(D, MT);
+  const float* rest = a.part + (size_t)(2 * g) * seq_part_floats(D, MT);
+  const size_t step = 2 * (size_t)seq_part_floats(D, MT);
+  const int n = last - g + 1;
+  for (int e = threadIdx.x; e < rows * (D / 2); e += kSeqThreads) {
+    const int r = e / (D / 2), d = (e - r * (D / 2)) * 2;
+    const float2 ml0 = __ldcg(reinterpret_cast<const float2*>(first + RT * D + r * 2));
+    float M = ml0.x;
+    for (int i = 0; i < n; ++i) M = fmaxf(M, __ldcg(rest + i * step + RT * D + r * 2));
+    const float base = M == -INFINITY ? 0.f : M;
+    float f = exp2_fast(ml0.x - base);
+    const float2 o0 = __ldcg(reinterpret_cast<const float2*>(first + r * D + d));
+    float L = f * ml0.y, x = f * o0.x, y = f * o0.y;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(rest + i * step + RT * D + r * 2));
+      const float2 o = __ldcg(reinterpret_cast<const float2*>(rest + i * step + r * D + d));
+      f = exp2_fast(ml.x - base);
+      L += f * ml.y;
+      x += f * o.x;
+      y += f * o.y;
+    }
+    const int pr = row0 + r, tok = pr / a.rep;
+    const bool none = s.len - s.n + tok < 0;
+    const float inv = 1.f / L;
+    if (d < a.hd)
+      *reinterpret_cast<uint32_t*>(a.out + (long long)(s.start + tok) * a.sot +
+                                   (long long)(kvh * a.rep + pr - tok * a.rep) * a.soh + d) =
+          none ? 0u : Type16<T>::pack(x * inv, y * inv);
+  }
+}
+
+template <typename KernelT>
+static int launch_attn_grid(KernelT kernel, const SeqAttnArgs& a, unsigned grid, size_t smem, cudaStream_t stream) {
+  if (smem > 0) {  // (the table is by kernel: instantiations of one signature share this function)
+    static std::mutex mu;
+    static std::vector<std::pair<int, const void*>> raised;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const std::pair<int, const void*> key(dev, reinterpret_cast<const void*>(kernel));
+    std::lock_guard<std::mutex> lock(mu);
+    bool seen = false;
+    for (auto& e : raised) seen |= (e == key);
+    if (!seen) {
+      const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                                "attention: shared memory limit");
+      if (rc != LI4_OK) return rc;
+      raised.push_back(key);
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(kSeqThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, a), "attention: kernel launch");
+}
+
+template <typename T, int D, int MT, bool PAGED>
+static int launch_seq(const SeqAttnArgs& a, cudaStream_t stream) {
+  int rc = launch_attn_grid(seq_attention_kernel<T, D, MT, PAGED>, a, (unsigned)a.grid, seq_smem_bytes(D), stream);
+  if (rc == LI4_OK && a.grid > 1)
+    rc = launch_attn_grid(seq_attention_join_kernel<T, D, MT, PAGED>, a, (unsigned)a.grid - 1, 0, stream);
+  return rc;
+}
+
+template <typename T, bool PAGED>
+static int launch_seq_d(const SeqAttnArgs& a, int mt, cudaStream_t stream) {
+  if (a.hd <= 64) return mt == 1 ? launch_seq<T, 64, 1, PAGED>(a, stream) : launch_seq<T, 64, 2, PAGED>(a, stream);
+  return mt == 1 ? launch_seq<T, 128, 1, PAGED>(a, stream) : launch_seq<T, 128, 2, PAGED>(a, stream);
+}
+
+static int seq_mt(int max_rows) { return max_rows <= 16 ? 1 : 2; }
+// CTAs that fit at once: two per SM at 64 dims (96 KB of stages each), one at 128 (192 KB).
+static int seq_grid(int hd, int sm) { return hd <= 64 ? 2 * sm : sm; }
+
+size_t seq_attention_part_bytes(int hd, int max_rows, int sm) {
+  return (size_t)2 * seq_grid(hd, sm) * seq_part_floats(hd <= 64 ? 64 : 128, seq_mt(max_rows)) * sizeof(float);
+}
+
+int launch_seq_attention(const SeqAttnArgs& args, bool paged, int dtype, int max_rows, cudaStream_t stream) {
+  SeqAttnArgs a = args;
+  a.grid = seq_grid(a.hd, current_sm_count());
+  const int mt = seq_mt(max_rows);
+  if (dtype == LI4_F16)
+    return paged ? launch_seq_d<__half, true>(a, mt, stream) : launch_seq_d<__half, false>(a, mt, stream);
+  return paged ? launch_seq_d<__nv_bfloat16, true>(a, mt, stream) : launch_seq_d<__nv_bfloat16, false>(a, mt, stream);
+}
+
+static int check_attention(const li4_attention* p, bool paged, const char* what) {
+  if (!p) return set_error(LI4_ERR_INVALID_ARG, "%s: null arguments", what);
+  if (p->dtype != LI4_F16 && p->dtype != LI4_BF16)
+    return set_error(LI4_ERR_UNSUPPORTED, "%s: dtype %d (LI4_F16 or LI4_BF16)", what, p->dtype);
+  if (p->n_seqs < 0 || p->n_tokens < 0 || p->n_kv_heads < 1 || p->n_heads < p->n_kv_heads ||
+      p->n_heads % p->n_kv_heads != 0 || p->max_queries < 0)
+    return set_error(LI4_ERR_INVALID_ARG, "%s: n_seqs=%lld n_tokens=%lld n_heads=%lld n_kv_heads=%lld max_queries=%lld",
+                     what, (long long)p->n_seqs, (long long)p->n_tokens, (long long)p->n_heads,
+                     (long long)p->n_kv_heads, (long long)p->max_queries);
+  if (p->head_dim < 8 || p->head_dim > 128 || p->head_dim % 8 != 0)
+    return set_error(LI4_ERR_UNSUPPORTED, "%s: head_dim=%lld (a multiple of 8 up to 128)", what,
+                     (long long)p->head_dim);
+  if (p->n_heads / p->n_kv_heads > 128 || p->n_heads > 65535 || p->n_seqs > (1 << 24) ||
+      p->n_tokens > (1LL << 30) / p->n_heads)
+    return set_error(LI4_ERR_UNSUPPORTED, "%s: n_seqs=%lld n_tokens=%lld n_heads=%lld too large", what,
+                     (long long)p->n_seqs, (long long)p->n_tokens, (long long)p->n_heads);
+  if (!(p->scale == p->scale) || p->scale > 3e38f || p->scale < -3e38f)
+    return set_error(LI4_ERR_INVALID_ARG, "%s: the scale is not finite", what);
+  if (paged) {
+    if (!is_pow2(p->page_size) || p->page_size < 8 || p->page_size > 1024)
+      return set_error(LI4_ERR_UNSUPPORTED, "%s: page_size=%lld (a power of two from 8 to 1024)", what,
+                       (long long)p->page_size);
+    if (p->num_pages < 0 || p->num_pages > (1LL << 31) - 1 || p->table_width < 0 || p->table_stride < p->table_width ||
+        p->table_width * p->page_size > (1LL << 30))
+      return set_error(LI4_ERR_INVALID_ARG, "%s: num_pages=%lld table_width=%lld table_stride=%lld", what,
+                       (long long)p->num_pages, (long long)p->table_width, (long long)p->table_stride);
+  }
+  if (p->n_seqs == 0 || p->n_tokens == 0) return LI4_OK;
+  if (!p->q || !p->out || !p->cu_seqlens || ((!p->k || !p->v) && !(paged && p->num_pages == 0)) ||
+      (paged && (!p->kv_lens || (!p->block_tables && p->table_width > 0))))
+    return set_error(LI4_ERR_INVALID_ARG, "%s: null pointer", what);
+  const int64_t st[] = {p->stride_qt, p->stride_qh, p->stride_ot, p->stride_oh, p->stride_kt, p->stride_kh,
+                        p->stride_vt, p->stride_vh, paged ? p->stride_kp : 0, paged ? p->stride_vp : 0};
+  bool aligned = aligned16(p->q) && aligned16(p->k) && aligned16(p->v) && aligned16(p->out);
+  for (int64_t s : st) aligned = aligned && s >= 0 && s % 8 == 0;
+  if (!aligned)
+    return set_error(LI4_ERR_ALIGNMENT, "%s: every row must start on a 16-byte boundary, at a non-negative stride", what);
+  return LI4_OK;
+}
+
+static int attention_rows(const li4_attention* p) {
+  const int64_t rows = p->max_queries * (p->n_heads / p->n_kv_heads);
+  return (int)(rows > (1 << 30) ? (1 << 30) : rows);
+}
+
+static int run_attention(const li4_attention* p, bool paged, void* workspace, size_t workspace_bytes, void* stream,
+                         const char* what) {
+  int rc = check_attention(p, paged, what);
+  if (rc != LI4_OK) return rc;
+  if (p->n_seqs == 0 || p->n_tokens == 0) {
+    clear_error();
+    return LI4_OK;
+  }
+  const size_t need = li4_attention_workspace_bytes(p);
+  if (workspace_bytes < need || (need && !workspace) || !aligned16(workspace))
+    return set_error(LI4_ERR_WORKSPACE, "%s: %zu bytes of 16-byte aligned workspace needed, %zu given", what, need,
+                     workspace_bytes);
+  SeqAttnArgs a = {};
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.k = static_cast<const uint16_t*>(p->k);
+  a.v = static_cast<const uint16_t*>(p->v);
+  a.out = static_cast<uint16_t*>(p->out);
+  a.sqt = p->stride_qt, a.sqh = p->stride_qh, a.sot = p->stride_ot, a.soh = p->stride_oh;
+  a.skp = p->stride_kp, a.skt = p->stride_kt, a.skh = p->stride_kh;
+  a.svp = p->stride_vp, a.svt = p->stride_vt, a.svh = p->stride_vh;
+  a.cu = p->cu_seqlens;
+  a.kv_lens = p->kv_lens;
+  a.tables = p->block_tables;
+  a.table_stride = p->table_stride;
+  a.table_width = paged ? (int)p->table_width : 0;
+  a.num_pages = paged ? (int)p->num_pages : 0;
+  a.log_page = paged ? ilog2(p->page_size) : 0;
+  a.B = (int)p->n_seqs;
+  a.T = (int)p->n_tokens;
+  a.Hkv = (int)p->n_kv_heads;
+  a.rep = (int)(p->n_heads / p->n_kv_heads);
+  a.hd = (int)p->head_dim;
+  a.scale_log2 = p->scale * 1.44269504088896340736f;
+  a.small_rows = 0;
+  a.big_rows = 0x7fffffff;
+  a.part = static_cast<float*>(workspace);
+  rc = launch_seq_attention(a, paged, p->dtype, attention_rows(p), static_cast<cudaStream_t>(stream));
+  if (rc == LI4_OK) clear_error();
+  return rc;
+}
+
+}  // namespace li4
+
+extern "C" size_t li4_attention_workspace_bytes(const li4_attention* p) {
+  using namespace li4;
+  if (!p || p->n_seqs <= 0 || p->n_tokens <= 0 || p->n_kv_heads < 1 || p->max_queries < 0) return 0;
+  return seq_attention_part_bytes((int)p->head_dim, attention_rows(p), current_sm_count());
+}
+
+extern "C" int li4_prompt_attention(const li4_attention* args, void* workspace, size_t workspace_bytes, void* stream) {
+  return li4::run_attention(args, false, workspace, workspace_bytes, stream, "prompt_attention");
+}
+
+extern "C" int li4_paged_attention(const li4_attention* args, void* workspace, size_t workspace_bytes, void* stream) {
+  return li4::run_attention(args, true, workspace, workspace_bytes, stream, "paged_attention");
+}

@@ -81,6 +81,20 @@ class Fusion(ctypes.Structure):
     ]
 
 
+class Attention(ctypes.Structure):
+    """struct li4_attention (include/llama_int4_b200.h): packed-sequence attention."""
+
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("dtype", ctypes.c_int), ("scale", ctypes.c_float)] + \
+        [(name, ctypes.c_int64) for name in ("stride_qt", "stride_qh", "stride_ot", "stride_oh", "stride_kp",
+                                             "stride_kt", "stride_kh", "stride_vp", "stride_vt", "stride_vh")] + \
+        [("cu_seqlens", ctypes.c_void_p)] + \
+        [(name, ctypes.c_int64) for name in ("n_seqs", "n_tokens", "n_heads", "n_kv_heads", "head_dim",
+                                             "max_queries")] + \
+        [("kv_lens", ctypes.c_void_p), ("block_tables", ctypes.c_void_p)] + \
+        [(name, ctypes.c_int64) for name in ("table_stride", "table_width", "num_pages", "page_size")]
+
+
 # name -> (restype, argtypes); mirrors include/llama_int4_b200.h
 SIGNATURES = {
     "li4_version": (_INT, []),
@@ -124,6 +138,12 @@ SIGNATURES = {
     "li4_program_launch": (_INT, [_P, _P]),
     "li4_program_set_trace": (_INT, [_P, _P, _I64]),
     "li4_program_info": (_INT, [_P, ctypes.POINTER(_INT), ctypes.POINTER(_INT), ctypes.POINTER(_SZ)]),
+    "li4_paged_append": (_INT, [_P, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P]),
+    "li4_rope_paged_write": (_INT, [_P, _P, _P, _INT, _I64, _I64, _I64, _I64, ctypes.POINTER(_I64), _P, _P, _I64,
+                                    _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _P]),
+    "li4_attention_workspace_bytes": (_SZ, [ctypes.POINTER(Attention)]),
+    "li4_prompt_attention": (_INT, [ctypes.POINTER(Attention), _P, _SZ, _P]),
+    "li4_paged_attention": (_INT, [ctypes.POINTER(Attention), _P, _SZ, _P]),
     "li4_dequantize": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
     "li4_quantize": (_INT, [_P, _INT, _P, _P, _P, _I64, _I64, _I64, _I64, _P]),
 }

@@ -338,6 +338,31 @@ class Llama(Generation):
             self._fused = None
         return self
 
+    def paged_cache(self, num_pages: int, page_size: int = 16, max_requests: Optional[int] = None,
+                    max_len: Optional[int] = None):
+        """A PagedKVCache (llama.paged) for this model's layers, type and device.  max_len (default
+        max_seq_len) is at most the RoPE table's 2 * max_seq_len positions."""
+        from .paged import PagedKVCache
+
+        p, att, w = self.params, self.layers[0].attention, self.tok_embeddings.weight
+        max_len = p.max_seq_len if max_len is None else max_len
+        if max_len > self.freqs_cis.shape[0]:
+            raise ValueError(f"max_len {max_len} exceeds the {self.freqs_cis.shape[0]} positions of the RoPE table")
+        return PagedKVCache(p.n_layers, num_pages, page_size, att.n_local_kv_heads, att.head_dim,
+                            p.max_batch_size if max_requests is None else max_requests, max_len, w.dtype, w.device)
+
+    @torch.no_grad()
+    def forward_paged(self, tokens: torch.Tensor, step, cache, max_new: int, whole_prompts: bool = False):
+        """fp32 logits [requests, vocab] of each request's last new token: tokens [T] are the step's new
+        tokens of all requests, packed in request order, step = cache.append(new_lens, T), max_new the
+        most new tokens of a request.  whole_prompts: every request with new tokens was empty before
+        the step, so attention reads the packed keys instead of the cache.  Requests of any length
+        side by side, without padding; no host synchronisation, so a step of fixed T can be captured
+        in a CUDA graph."""
+        from .paged import forward_paged
+
+        return forward_paged(self, tokens, step, cache, max_new, whole_prompts)
+
     def reset_cache(self):
         for layer in self.layers:
             layer.attention.cache_k = None
