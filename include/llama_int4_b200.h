@@ -451,7 +451,8 @@ int li4_paged_attention(const li4_attention* args, void* workspace, size_t works
  * LI4_EPI_ALLREDUCE_RESIDUAL epilogue's wait for a peer's words ran out; bit 6: a wait of
  * li4_argmax_rows_allreduce for a peer's key ran out -- the kernel
  * carried on and its outputs are not valid; bit 7: li4_rope_paged_write met a position
- * or slot out of range).  Synchronising: copies the flags to the host; reset != 0 clears them.
+ * or slot out of range; bit 8: a bounded wait inside li4_prompt_attention or li4_paged_attention ran
+ * out).  Synchronising: copies the flags to the host; reset != 0 clears them.
  * A diagnostic for tests and health checks, not for the decode loop. */
 int li4_device_errors(unsigned* flags, int reset);
 

@@ -150,6 +150,7 @@ __device__ __noinline__ void redo_row(const SeqAttnArgs& a, int b, const Seq s, 
 
 // ---- launches shared by the entry points ----
 int launch_seq_attention(const SeqAttnArgs& a, bool paged, int dtype, int max_rows, cudaStream_t stream);
+int launch_tile_attention(const SeqAttnArgs& a, bool paged, int dtype, cudaStream_t stream);
 size_t seq_attention_part_bytes(int hd, int max_rows, int sm);
 
 }  // namespace li4

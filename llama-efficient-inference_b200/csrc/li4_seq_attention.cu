@@ -524,6 +524,8 @@ int launch_seq_attention(const SeqAttnArgs& args, bool paged, int dtype, int max
   return paged ? launch_seq_d<__nv_bfloat16, true>(a, mt, stream) : launch_seq_d<__nv_bfloat16, false>(a, mt, stream);
 }
 
+constexpr int kFewRows = 32;  // rows (queries x heads of a KV head) up to which a sequence is streamed
+
 static int check_attention(const li4_attention* p, bool paged, const char* what) {
   if (!p) return set_error(LI4_ERR_INVALID_ARG, "%s: null arguments", what);
   if (p->dtype != LI4_F16 && p->dtype != LI4_BF16)
@@ -558,9 +560,13 @@ static int check_attention(const li4_attention* p, bool paged, const char* what)
   const int64_t st[] = {p->stride_qt, p->stride_qh, p->stride_ot, p->stride_oh, p->stride_kt, p->stride_kh,
                         p->stride_vt, p->stride_vh, paged ? p->stride_kp : 0, paged ? p->stride_vp : 0};
   bool aligned = aligned16(p->q) && aligned16(p->k) && aligned16(p->v) && aligned16(p->out);
-  for (int64_t s : st) aligned = aligned && s >= 0 && s % 8 == 0;
-  if (!aligned)
-    return set_error(LI4_ERR_ALIGNMENT, "%s: every row must start on a 16-byte boundary, at a non-negative stride", what);
+  const int64_t rep = p->n_heads / p->n_kv_heads;
+  const int64_t size[] = {p->n_tokens, p->n_heads, p->n_tokens, p->n_heads, paged ? p->page_size : p->n_tokens,
+                          p->n_kv_heads, paged ? p->page_size : p->n_tokens, p->n_kv_heads, p->num_pages, p->num_pages};
+  for (int i = 0; i < 10; ++i)  // (the stride of a dimension of one element is not used)
+    aligned = aligned && st[i] % 8 == 0 && (st[i] > 0 || (st[i] == 0 && (size[i] <= 1 || (!paged && i >= 8))));
+  if (!aligned || rep < 1)
+    return set_error(LI4_ERR_ALIGNMENT, "%s: every row must start on a 16-byte boundary, at a positive stride", what);
   return LI4_OK;
 }
 
@@ -602,10 +608,25 @@ static int run_attention(const li4_attention* p, bool paged, void* workspace, si
   a.rep = (int)(p->n_heads / p->n_kv_heads);
   a.hd = (int)p->head_dim;
   a.scale_log2 = p->scale * 1.44269504088896340736f;
-  a.small_rows = 0;
-  a.big_rows = 0x7fffffff;
   a.part = static_cast<float*>(workspace);
-  rc = launch_seq_attention(a, paged, p->dtype, attention_rows(p), static_cast<cudaStream_t>(stream));
+  // Which kernel: the streaming one takes sequences of few rows, whose time is the reading of the keys, the
+  // tensor-memory one (positive scales, some page) the rest.  The host knows the longest sequence as the caller
+  // claims it; the device looks at each sequence's own rows, so a wrong claim only costs time.
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int rows = attention_rows(p);
+  const bool tiles = rows > kFewRows && a.scale_log2 > 0.f && !(paged && p->num_pages == 0);
+  const bool both = tiles && paged && p->n_seqs > 1;
+  rc = LI4_OK;
+  if (!tiles || both) {
+    a.small_rows = 0;
+    a.big_rows = both ? kFewRows : 0x7fffffff;
+    rc = launch_seq_attention(a, paged, p->dtype, both ? kFewRows : rows, st);
+  }
+  if (rc == LI4_OK && tiles) {
+    a.small_rows = both ? kFewRows : 0;
+    a.big_rows = 0x7fffffff;
+    rc = launch_tile_attention(a, paged, p->dtype, st);
+  }
   if (rc == LI4_OK) clear_error();
   return rc;
 }
