@@ -5,7 +5,9 @@
 Compiles csrc/*.cu with nvcc for sm_100a (cross-compiles without a GPU) and
 links lib/libllama_int4_b200.so -- a plain C-ABI shared library (see
 include/llama_int4_b200.h) with the CUDA runtime linked statically, so it
-loads with or without torch in the process.
+loads with or without torch in the process -- and compiles csrc/li4_torch.cpp
+against this interpreter's torch into lib/li4_torch.so, the binding of the
+paged-cache entry points to torch tensors (it links the C-ABI library).
 """
 from __future__ import annotations
 
@@ -16,6 +18,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG_DIR)
@@ -23,6 +26,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libllama_int4_b200.so")
+EXT_PATH = os.path.join(LIB_DIR, "li4_torch.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
@@ -41,15 +45,49 @@ def sources() -> list[str]:
 
 
 def _deps() -> list[str]:
-    return sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) + \
+    return sources() + glob.glob(os.path.join(CSRC, "*.cpp")) + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) + \
         glob.glob(os.path.join(REPO, "include", "*.h")) + [os.path.abspath(__file__)]
 
 
 def up_to_date() -> bool:
-    if not os.path.exists(LIB_PATH):
+    if not os.path.exists(LIB_PATH) or not os.path.exists(EXT_PATH):
         return False
-    t = os.path.getmtime(LIB_PATH)
+    t = min(os.path.getmtime(LIB_PATH), os.path.getmtime(EXT_PATH))
     return all(os.path.getmtime(d) <= t for d in _deps())
+
+
+def compile_binding(verbose: bool) -> str:
+    """csrc/li4_torch.cpp as an object file (host code only)."""
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    obj = os.path.join(BUILD_DIR, "li4_torch.o")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-fvisibility=hidden", f"-I{os.path.join(REPO, 'include')}",
+           f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}",
+           f"-I{cuda}", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-c",
+           os.path.join(CSRC, "li4_torch.cpp"), "-o", obj]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on li4_torch.cpp:\n{r.stdout}\n{r.stderr}")
+    return obj
+
+
+def link_binding(obj: str, verbose: bool) -> None:
+    import torch
+
+    tmp = EXT_PATH + ".tmp"
+    cmd = ["g++", "-shared", "-o", tmp, obj, f"-L{LIB_DIR}", "-l:libllama_int4_b200.so", "-Wl,-rpath,$ORIGIN",
+           f"-L{os.path.join(os.path.dirname(torch.__file__), 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_cuda", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, EXT_PATH)
 
 
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
@@ -61,8 +99,13 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
     cc = nvcc()
     extra = ["-Xptxas", "-v"] if ptxas_info else []
 
+    shared = [d for d in _deps() if not d.endswith((".cu", ".cpp"))]
+
     def compile_one(src: str) -> str:
         obj = os.path.join(BUILD_DIR, os.path.basename(src)[:-3] + ".o")
+        if not force and not ptxas_info and os.path.exists(obj) and \
+                all(os.path.getmtime(d) <= os.path.getmtime(obj) for d in [src] + shared):
+            return obj  # newer than its source, every header and this file
         cmd = [cc] + NVCC_FLAGS + extra + ["-c", src, "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)
@@ -74,6 +117,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
         return obj
 
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        binding = ex.submit(compile_binding, verbose)
         objs = list(ex.map(compile_one, sources()))
     tmp = LIB_PATH + ".tmp"
     cmd = [cc] + ARCH_FLAGS + ["-shared", "-o", tmp] + objs
@@ -83,6 +127,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB_PATH)
+    link_binding(binding.result(), verbose)
     return LIB_PATH
 
 

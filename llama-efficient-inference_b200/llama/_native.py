@@ -7,6 +7,8 @@ entry point raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
@@ -150,6 +152,7 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_ext = None
 
 
 class Li4Error(RuntimeError):
@@ -177,6 +180,25 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = l
     return _lib
+
+
+def ext():
+    """The paged-cache entry points on torch tensors (csrc/li4_torch.cpp), loaded once after the library."""
+    global _ext
+    if _ext is None:
+        lib()
+        with _lock:
+            if _ext is None:
+                path = os.path.join(PKG_DIR, "lib", "li4_torch.so")
+                if not os.path.exists(path):
+                    raise ImportError(f"{path} is missing: build it with "
+                                      f"`python {os.path.join(PKG_DIR, 'build.py')}`")
+                loader = importlib.machinery.ExtensionFileLoader("li4_torch", path)
+                spec = importlib.util.spec_from_loader("li4_torch", loader)
+                module = importlib.util.module_from_spec(spec)
+                loader.exec_module(module)
+                _ext = module
+    return _ext
 
 
 def last_error() -> str:
