@@ -74,6 +74,15 @@ __device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, 
       : "memory");
 }
 
+// One thread of a converged warp.  Issuing through elect.sync (not a lane test) tells the compiler that one thread is
+// active: a tcgen05.mma then takes a few cycles to issue, where under `lane == 0` each took about 100 (prompts of 8192
+// tokens at 128 dims: see the launch notes below).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -301,81 +310,92 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (!ok)  // copies in flight land before the memory goes
       for (int i = max(0, n - NS); i < n; ++i) tile_wait(&kv_full[i % NS], (i / NS) & 1);
   } else if (warp == kMmaWarp) {
-    // ---- products
+    // ---- products: one thread issues them, with addresses that are constants beyond the slot's base
     constexpr uint32_t IDESC_S = tile_idesc(kTileKeys, TYPE, 0), IDESC_O = tile_idesc(D, TYPE, 1);
-    const uint32_t q_at = smem_addr(smem), ring_at = smem_addr(ring);
+    const uint64_t q_desc = desc_k_major(smem_addr(smem)), k_desc = desc_k_major(smem_addr(ring)),
+                   v_desc = desc_n_major(smem_addr(ring), TB / SUB);
     auto scores = [&](int i, int slot) {
-      const uint32_t k_at = ring_at + slot * TB;
-      if (lane == 0) {
+      const uint64_t qd = q_desc + i * (TB >> 4), kd = k_desc + slot * (TB >> 4);
 #pragma unroll
-        for (int c = 0; c < SUB; ++c)
+      for (int c = 0; c < SUB; ++c)
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_ss(tmem + S_COL + i * 128, desc_k_major(q_at + i * TB + c * (TB / SUB) + kk * 32),
-                   desc_k_major(k_at + c * (TB / SUB) + kk * 32), IDESC_S, c + kk > 0);
-        tc_commit(&s_full[i]);
-      }
-      __syncwarp();
+        for (int kk = 0; kk < 4; ++kk)
+          mma_ss(tmem + S_COL + i * 128, qd + ((c * (TB / SUB) + kk * 32) >> 4), kd + ((c * (TB / SUB) + kk * 32) >> 4),
+                 IDESC_S, c + kk > 0);
+      tc_commit(&s_full[i]);
     };
-    if (nk > 0) {
-      ok = tile_wait(q_full, 0) && tile_wait(&kv_full[0], 0);
-      if (ok) {
-        tc_fence_after();
-        if (steps[0] > 0) scores(0, 0);
-        if (steps[1] > 0) scores(1, 0);
-        if (lane == 0) tc_commit(&kv_empty[0]);
+    auto outputs = [&](int i, int slot, bool first, int groups) {
+      const uint64_t vd = v_desc + slot * (TB >> 4);
+      const uint32_t o = tmem + O_COL + i * 128, pr = tmem + S_COL + i * 128;
+      mma_ts(o, pr, vd, IDESC_O, !first);
+      if (groups == 8) {
+#pragma unroll
+        for (int kk = 1; kk < 8; ++kk) mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, true);
+      } else {
+        for (int kk = 1; kk < groups; ++kk) mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, true);
       }
-    }
-    for (int j = 0; j < nk && ok; ++j) {
+      tc_commit(&o_done[i]);
+    };
+    const int tail = s.len - (nk - 1) * kTileKeys;  // keys of the sequence from the last step on
+    const int tail_rows = min(kTileKeys, tail), tail_groups = (tail_rows + 15) / 16;
+    // step j's P V and step j + 1's scores
+    auto step = [&](int j) {
       const int nv = 2 * j + 1, vs = nv % NS, nkey = 2 * j + 2, ks = nkey % NS;
-      ok = tile_wait(&kv_full[vs], (nv / NS) & 1);
-      if (!ok) break;
-      const uint32_t v_at = ring_at + vs * TB;
-      // the sequence's last tile: only the keys it has, whole groups of 16; rows past the end are made zeros
-      // (what lies there may be anything, and 0 x NaN is NaN)
-      const int rows = min(kTileKeys, s.len - j * kTileKeys);
-      const int groups = (rows + 15) / 16;
-      if (rows < groups * 16) {
-        for (int e = lane; e < (groups * 16 - rows) * SUB * 8; e += 32) {
-          const int r = rows + e / (SUB * 8), c = e % (SUB * 8);
-          *reinterpret_cast<uint4*>(ring + vs * TB + (c >> 3) * (TB / SUB) + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-      }
+      if (!tile_wait(&kv_full[vs], (nv / NS) & 1)) return false;
       bool key_here = false;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (j < steps[i]) {
-          ok = ok && tile_wait(&p_full[i], j & 1);
-          if (!ok) break;
+          if (!tile_wait(&p_full[i], j & 1)) return false;
           tc_fence_after();
-          if (lane == 0) {
-            for (int kk = 0; kk < groups; ++kk)
-              mma_ts(tmem + O_COL + i * 128, tmem + S_COL + i * 128 + kk * 8, desc_n_major(v_at + kk * 2048, TB / SUB),
-                     IDESC_O, j + kk > 0);
-            tc_commit(&o_done[i]);
-          }
-          __syncwarp();
+          outputs(i, vs, j == 0, j == nk - 1 ? tail_groups : 8);
         }
         if (j + 1 < steps[i]) {
           if (!key_here) {
-            ok = ok && tile_wait(&kv_full[ks], (nkey / NS) & 1);
-            if (!ok) break;
+            if (!tile_wait(&kv_full[ks], (nkey / NS) & 1)) return false;
             key_here = true;
             tc_fence_after();
           }
           scores(i, ks);
         }
       }
-      if (ok && lane == 0) {
-        tc_commit(&kv_empty[vs]);
-        if (j + 1 < nk) tc_commit(&kv_empty[ks]);
+      tc_commit(&kv_empty[vs]);
+      if (j + 1 < nk) tc_commit(&kv_empty[ks]);
+      return true;
+    };
+    if (nk > 0) {
+      const bool one = elect_one();
+      if (one) {
+        ok = tile_wait(q_full, 0) && tile_wait(&kv_full[0], 0);
+        if (ok) {
+          tc_fence_after();
+          if (steps[0] > 0) scores(0, 0);
+          if (steps[1] > 0) scores(1, 0);
+          tc_commit(&kv_empty[0]);
+        }
+        for (int j = 0; j + 1 < nk && ok; ++j) ok = step(j);
       }
-    }
-    if (!ok) {  // MMAs in flight finish before the memory goes
-      if (lane == 0) tc_commit(q_full);
-      tile_wait(q_full, 1);
+      ok = __all_sync(0xffffffffu, ok);
+      // the sequence's last tile: only the keys it has, whole groups of 16; rows past the end are made zeros
+      // (what lies there may be anything, and 0 x NaN is NaN)
+      if (ok && tail_rows < tail_groups * 16) {
+        const int nv = 2 * (nk - 1) + 1, vs = nv % NS;
+        ok = __all_sync(0xffffffffu, tile_wait(&kv_full[vs], (nv / NS) & 1));
+        for (int e = lane; ok && e < (tail_groups * 16 - tail_rows) * SUB * 8; e += 32) {
+          const int r = tail_rows + e / (SUB * 8), c = e % (SUB * 8);
+          *reinterpret_cast<uint4*>(ring + vs * TB + (c >> 3) * (TB / SUB) + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+      if (one) {
+        if (ok) ok = step(nk - 1);
+        if (!ok) {  // MMAs in flight finish before the memory goes
+          tc_commit(q_full);
+          tile_wait(q_full, 1);
+        }
+      }
+      __syncwarp();
     }
   } else {
     // ---- softmax of tile i: this thread's row
