@@ -42,7 +42,7 @@ int tile_device_errors(unsigned* flags, bool reset) {
 
 constexpr int kTileRows = 128;       // rows of a tile: tensor-memory lanes
 constexpr int kTileKeys = 128;       // keys of a step
-constexpr int kTileThreads = 320;    // 8 softmax warps, the TMA warp, the MMA warp
+constexpr int kTileThreads = 384;    // 8 softmax warps, the TMA warp, the MMA warp, 2 that only fill their group
 constexpr int kTmaWarp = 8, kMmaWarp = 9;
 constexpr unsigned kTileWaitLimit = 1u << 22;
 constexpr float kLazyLog2 = 8.f;     // how far the maximum in use may lag, in powers of two
@@ -50,6 +50,11 @@ constexpr float kLazyLog2 = 8.f;     // how far the maximum in use may lag, in p
 __host__ __device__ constexpr int tile_slots(int D) { return D == 64 ? 8 : 4; }
 __host__ __device__ constexpr int tile_bytes(int D) { return 128 * D * 2; }  // a tile of queries, keys or values
 __host__ __device__ constexpr int tile_smem_bytes(int D) { return 1024 + (2 + tile_slots(D)) * tile_bytes(D) + 512; }
+
+#ifndef POLY
+#define POLY 0x8888
+#endif
+constexpr unsigned kPolyPairs = POLY;  // which of 16 pairs of probabilities the polynomial takes
 
 struct TileArgs {
   SeqAttnArgs s;
@@ -161,6 +166,56 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
       "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
       : "memory");
 }
+// Two fp32 lanes at once (the packed forms halve the issue slots of the softmax's multiply-adds and sums).
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float* x, float* y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*x), "=f"(*y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x and 2^y for x, y <= 64 on the multiply-add pipe.  The 16-per-cycle exponential unit bounds the softmax, so part of
+// its exponentials are taken here: x = n + f with n the nearest integer (added to 1.5 * 2^23, which leaves n in the low
+// bits), 2^f on [-1/2, 1/2] by a polynomial with value 1 at 0 fitted for the least largest relative error
+// (degree 5: 9.2e-8; 1.7e-7 evaluated in fp32, the size of the unit's own error), n added to the exponent bits.  x is
+// held at -127, where the sum of bits is exactly zero: a masked score gives probability 0.  NaN passes the bound; its
+// bits end up as a huge value that the 16-bit type turns into an infinity.
+__device__ __forceinline__ void exp2_pair(uint64_t v, float* x, float* y) {
+  unpack2(v, x, y);
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(*x));  // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(*y));
+  v = pack2(*x, *y);
+  const uint64_t t = add2(v, pack2(12582912.f, 12582912.f));
+  const uint64_t n = add2(t, pack2(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(n, pack2(-1.f, -1.f), v);
+  uint64_t p = pack2(0x1.5bba14p-10f, 0x1.5bba14p-10f);
+  p = fma2(p, f, pack2(0x1.3cea88p-7f, 0x1.3cea88p-7f));
+  p = fma2(p, f, pack2(0x1.c6b752p-5f, 0x1.c6b752p-5f));
+  p = fma2(p, f, pack2(0x1.ebf9bcp-3f, 0x1.ebf9bcp-3f));
+  p = fma2(p, f, pack2(0x1.62e42ap-1f, 0x1.62e42ap-1f));
+  p = fma2(p, f, pack2(1.f, 1.f));
+  float tx, ty, px, py;
+  unpack2(t, &tx, &ty);
+  unpack2(p, &px, &py);
+  *x = __uint_as_float(__float_as_uint(px) + (__float_as_uint(tx) << 23));
+  *y = __uint_as_float(__float_as_uint(py) + (__float_as_uint(ty) << 23));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Item `index` of the launch: sequences in order, inside a sequence the later (longer) pairs of tiles first, KV
@@ -214,8 +269,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* kv_empty = kv_full + NS;
   uint64_t* q_full = kv_empty + NS;
   uint64_t* s_full = q_full + 1;   // [2] S_i written
-  uint64_t* p_full = s_full + 2;   // [2] P_i written, O_i rescaled (4 warps)
-  uint64_t* o_done = p_full + 2;   // [2] the last P_i V finished
+  uint64_t* p_full = s_full + 2;   // [2][2] half of P_i written (4 warps), O_i rescaled before the first
+  uint64_t* o_done = p_full + 4;   // [2] the last P_i V finished
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_done + 2);
   TileItem* s_item = reinterpret_cast<TileItem*>(tmem_holder + 1);
 
@@ -234,7 +289,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_done[i], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -266,6 +322,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const uint32_t tmem = *tmem_holder;
   bool ok = true;
 
+  // 384 threads x 168 registers at the launch: the softmax's two groups take 208 each, the third keeps 80
+  // (2 x 128 x 208 + 128 x 80 <= 384 x 168)
+  if (warp >= kTmaWarp) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
   if (warp == kTmaWarp) {
     // ---- copies
     if (lane == 0 && nk > 0) {
@@ -324,17 +384,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                  IDESC_S, c + kk > 0);
       tc_commit(&s_full[i]);
     };
-    auto outputs = [&](int i, int slot, bool first, int groups) {
-      const uint64_t vd = v_desc + slot * (TB >> 4);
-      const uint32_t o = tmem + O_COL + i * 128, pr = tmem + S_COL + i * 128;
-      mma_ts(o, pr, vd, IDESC_O, !first);
+    // half h of P_i V: groups of 16 keys 4 h .. min(groups, 4 h + 4) - 1
+    auto outputs = [&](int i, int slot, int h, bool first, int groups) {
+      const uint64_t vd = v_desc + slot * (TB >> 4) + h * 512;
+      const uint32_t o = tmem + O_COL + i * 128, pr = tmem + S_COL + i * 128 + h * 32;
       if (groups == 8) {
 #pragma unroll
-        for (int kk = 1; kk < 8; ++kk) mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, true);
+        for (int kk = 0; kk < 4; ++kk) mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, !(first && h + kk == 0));
       } else {
-        for (int kk = 1; kk < groups; ++kk) mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, true);
+        for (int kk = 0; kk < 4 && h * 4 + kk < groups; ++kk)
+          mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, !(first && h + kk == 0));
       }
-      tc_commit(&o_done[i]);
     };
     const int tail = s.len - (nk - 1) * kTileKeys;  // keys of the sequence from the last step on
     const int tail_rows = min(kTileKeys, tail), tail_groups = (tail_rows + 15) / 16;
@@ -346,9 +406,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (j < steps[i]) {
-          if (!tile_wait(&p_full[i], j & 1)) return false;
-          tc_fence_after();
-          outputs(i, vs, j == 0, j == nk - 1 ? tail_groups : 8);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!tile_wait(&p_full[2 * i + h], j & 1)) return false;
+            tc_fence_after();
+            outputs(i, vs, h, j == 0, j == nk - 1 ? tail_groups : 8);
+          }
+          tc_commit(&o_done[i]);
         }
         if (j + 1 < steps[i]) {
           if (!key_here) {
@@ -397,7 +461,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       __syncwarp();
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax of tile i: this thread's row
     const int i = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
@@ -426,10 +492,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int e = 0; e < 128; ++e)
           if (e > rel) x[e] = -INFINITY;
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int e = 0; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], x[e]);
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      for (int e = 4; e < 124; e += 8) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mx[w] = max3(mx[w], x[e + w], x[e + 4 + w]);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mx[w] = fmaxf(mx[w], x[124 + w]);
+      const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
       // (the difference is NaN for two infinities of one sign: no move)
       if (__any_sync(0xffffffffu, (top - m) * c > kLazyLog2)) {
         const float mn = fmaxf(m, top);
@@ -454,25 +525,38 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         m = mn;
         base = nb;
       }
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t cc = pack2(c, c), nb2 = pack2(-base, -base);
+      uint64_t sum0 = 0, sum1 = 0;  // pairs of zeros
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint32_t p[16];
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p0 = exp2_fast(fmaf(x[g * 32 + 2 * e], c, -base));
-          const float p1 = exp2_fast(fmaf(x[g * 32 + 2 * e + 1], c, -base));
-          sum[(2 * e) & 3] += p0;
-          sum[(2 * e + 1) & 3] += p1;
-          p[e] = Type16<T>::pack(p0, p1);
+        for (int g = 2 * h; g < 2 * h + 2; ++g) {
+          uint32_t p[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float p0, p1;
+            const uint64_t t = fma2(pack2(x[g * 32 + 2 * e], x[g * 32 + 2 * e + 1]), cc, nb2);
+            if ((kPolyPairs >> e) & 1) {
+              exp2_pair(t, &p0, &p1);
+            } else {
+              unpack2(t, &p0, &p1);
+              p0 = exp2_fast(p0);
+              p1 = exp2_fast(p1);
+            }
+            uint64_t& sum = e & 1 ? sum1 : sum0;
+            sum = add2(sum, pack2(p0, p1));
+            p[e] = Type16<T>::pack(p0, p1);
+          }
+          tmem_st16(s_at + g * 16, p);
         }
-        tmem_st16(s_at + g * 16, p);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[i]);
+      float s0, s1;
+      unpack2(add2(sum0, sum1), &s0, &s1);
+      l += s0 + s1;
     }
     // ---- the row's output
     if (my_steps > 0 && ok) {
