@@ -44,7 +44,7 @@ constexpr int kTileRows = 128;       // rows of a tile: tensor-memory lanes
 constexpr int kTileKeys = 128;       // keys of a step
 constexpr int kTileThreads = 384;    // 8 softmax warps, the TMA warp, the MMA warp, 2 that only fill their group
 constexpr int kTmaWarp = 8, kMmaWarp = 9;
-constexpr unsigned kTileWaitLimit = 1u << 22;
+constexpr unsigned kTileWaitLimit = 1u << 24;  // polls
 constexpr float kLazyLog2 = 8.f;     // how far the maximum in use may lag, in powers of two
 
 __host__ __device__ constexpr int tile_slots(int D) { return D == 64 ? 8 : 4; }
@@ -65,8 +65,26 @@ struct TileArgs {
 // ---- mbarriers, tensor memory ----
 __device__ __forceinline__ bool tile_wait(uint64_t* bar, unsigned parity) {
   for (unsigned i = 0; i < kTileWaitLimit; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_test_wait(bar, parity)) return true;
   atomicOr(&g_tile_device_error, 256u);
+  return false;
+}
+__device__ __forceinline__ bool tile_wait2(uint64_t* bar, unsigned parity, uint64_t* bar2, unsigned parity2) {
+  for (unsigned i = 0; i < kTileWaitLimit; ++i) {
+    const bool a = mbar_test_wait(bar, parity), b = mbar_test_wait(bar2, parity2);
+    if (a && b) return true;
+  }
+  atomicOr(&g_tile_device_error, 256u);
+  return false;
+}
+// A converged warp: tests, or waits; every lane returns the same.
+__device__ __forceinline__ bool tile_test_warp(uint64_t* bar, unsigned parity) {
+  return __all_sync(0xffffffffu, mbar_test_wait(bar, parity));
+}
+__device__ __forceinline__ bool tile_wait_warp(uint64_t* bar, unsigned parity) {
+  for (unsigned i = 0; i < kTileWaitLimit; ++i)
+    if (tile_test_warp(bar, parity)) return true;
+  if ((threadIdx.x & 31) == 0) atomicOr(&g_tile_device_error, 256u);
   return false;
 }
 
@@ -80,8 +98,8 @@ __device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, 
 }
 
 // One thread of a converged warp.  Issuing through elect.sync (not a lane test) tells the compiler that one thread is
-// active: a tcgen05.mma then takes a few cycles to issue, where under `lane == 0` each took about 100 (prompts of 8192
-// tokens at 128 dims: see the launch notes below).
+// active; under `lane == 0` each tcgen05.mma took about 100 cycles to issue (8192-token prompts at 128 dims: 601 us
+// against 513).
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
@@ -261,7 +279,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                           const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   constexpr int NS = tile_slots(D), TB = tile_bytes(D), SUB = D / 64;
   constexpr int TYPE = sizeof(T) == 2 && __is_same(T, __half) ? 0 : 1;
-  constexpr uint32_t S_COL = 0, O_COL = 256;  // tensor-memory columns: S_i at 128 i (P_i in its first 64), O_i at 256 + 128 i
+  // Tensor-memory columns: S_i at 128 i, O_i at 256 + D i.  At 64 dims there is room for P_i beside them (64 columns
+  // each), so S_i of the next step is computed as soon as the softmax has read the last one; at 128 dims P_i lies in
+  // S_i's first 64 columns and the next S_i follows P_i V.
+  constexpr bool EARLY = D == 64;
+  constexpr uint32_t S_COL = 0, O_COL = 256, P_COL = EARLY ? 384 : 0, P_STEP = EARLY ? 64 : 128;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + 2 * TB;
@@ -271,7 +293,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* s_full = q_full + 1;   // [2] S_i written
   uint64_t* p_full = s_full + 2;   // [2][2] half of P_i written (4 warps), O_i rescaled before the first
   uint64_t* o_done = p_full + 4;   // [2] the last P_i V finished
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_done + 2);
+  uint64_t* s_free = o_done + 2;   // [2] S_i read (4 warps); 64 dims only
+  uint64_t* v_tail = s_free + 2;   // the last value tile's missing rows are zeros
+  uint64_t* drained = v_tail + 1;  // the product warp gave up and its MMAs have finished
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
   TileItem* s_item = reinterpret_cast<TileItem*>(tmem_holder + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -292,7 +317,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&p_full[2 * i], 4);
       mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_done[i], 1);
+      mbar_init(&s_free[i], 4);
     }
+    mbar_init(v_tail, 1);
+    mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
@@ -316,6 +344,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     steps[i] = (keys + kTileKeys - 1) / kTileKeys;
   }
   const int nk = max(steps[0], steps[1]);
+  // place of key tile j and value tile j in the ring's order: the order in which the products take them
+  auto key_at = [](int j) { return !EARLY ? 2 * j : j == 0 ? 0 : 2 * j - 1; };
+  auto value_at = [nk](int j) { return !EARLY || j == nk - 1 ? 2 * j + 1 : 2 * j + 2; };
+  // the sequence's last tile: only the keys it has, whole groups of 16; rows past the end are made zeros (what lies
+  // there may be anything, and 0 x NaN is NaN)
+  const int tail_rows = min(kTileKeys, s.len - (nk - 1) * kTileKeys), tail_groups = (tail_rows + 15) / 16;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -338,8 +372,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     s.start + tok0 + i * TPT);
     }
     int n = 0;  // tiles issued
-    const int pages = PAGED ? kTileKeys / a.box_rows : 1;
-    for (int j = 0; j < nk && ok; ++j) {
+    for (; n < 2 * nk && ok; ++n) {
+      // tile n of the ring's order
+      const bool value = !EARLY ? n & 1 : n == 2 * nk - 1 || (n > 0 && !(n & 1));
+      const int j = !EARLY ? n / 2 : n == 2 * nk - 1 ? nk - 1 : value ? n / 2 - 1 : (n + 1) / 2;
       const int key0 = j * kTileKeys;
       const int rows = min(kTileKeys, s.len - key0);
       int row = s.start + key0, page = 0;
@@ -353,29 +389,40 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // an entry outside the cache is a coordinate outside the tensor: zeros
         if (mine) page = a.s.tables[(long long)item.b * a.s.table_stride + (key >> a.s.log_page)];
       }
-      (void)pages;
-#pragma unroll 1
-      for (int kv = 0; kv < 2; ++kv, ++n) {
-        const int slot = n % NS;
-        if (n >= NS) ok = ok && tile_wait(&kv_empty[slot], ((n / NS) - 1) & 1);
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], boxes * a.box_rows * SUB * 128);
-        __syncwarp();
-        if (mine)
-          for (int c = 0; c < SUB; ++c)
-            tma_load4(smem_addr(ring + slot * TB + c * (TB / SUB)) + lane * a.box_rows * 128, kv ? &map_v : &map_k,
-                      &kv_full[slot], c * 64, row, item.kvh, page);
+      const int slot = n % NS;
+      if (n >= NS) ok = tile_wait_warp(&kv_empty[slot], ((n / NS) - 1) & 1);
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], boxes * a.box_rows * SUB * 128);
+      __syncwarp();
+      if (mine)
+        for (int c = 0; c < SUB; ++c)
+          tma_load4(smem_addr(ring + slot * TB + c * (TB / SUB)) + lane * a.box_rows * 128, value ? &map_v : &map_k,
+                    &kv_full[slot], c * 64, row, item.kvh, page);
+    }
+    if (ok && nk > 0 && tail_rows < tail_groups * 16) {
+      const int last = 2 * nk - 1, slot = last % NS;
+      ok = tile_wait_warp(&kv_full[slot], (last / NS) & 1);
+      for (int e = lane; ok && e < (tail_groups * 16 - tail_rows) * SUB * 8; e += 32) {
+        const int r = tail_rows + e / (SUB * 8), c = e % (SUB * 8);
+        *reinterpret_cast<uint4*>(ring + slot * TB + (c >> 3) * (TB / SUB) + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(v_tail);
     }
     if (!ok)  // copies in flight land before the memory goes
-      for (int i = max(0, n - NS); i < n; ++i) tile_wait(&kv_full[i % NS], (i / NS) & 1);
+      for (int i = max(0, n - NS); i < n; ++i) tile_wait_warp(&kv_full[i % NS], (i / NS) & 1);
   } else if (warp == kMmaWarp) {
-    // ---- products: one thread issues them, with addresses that are constants beyond the slot's base
+    // ---- products: one elected thread, tile 0 then tile 1 (a warp per tile was slower: their products then share the
+    // tensor cores and both finish late).  Any barrier read costs it 160-220 cycles and several at once hardly more, so
+    // what a group of products needs is tested together.
     constexpr uint32_t IDESC_S = tile_idesc(kTileKeys, TYPE, 0), IDESC_O = tile_idesc(D, TYPE, 1);
     const uint64_t q_desc = desc_k_major(smem_addr(smem)), k_desc = desc_k_major(smem_addr(ring)),
                    v_desc = desc_n_major(smem_addr(ring), TB / SUB);
-    auto scores = [&](int i, int slot) {
-      const uint64_t qd = q_desc + i * (TB >> 4), kd = k_desc + slot * (TB >> 4);
+    auto full = [&](int n) { return &kv_full[n % NS]; };
+    auto phase = [&](int n) { return (unsigned)(n / NS) & 1u; };
+    auto scores = [&](int i, int j) {  // S_i of step j
+      const uint64_t qd = q_desc + i * (TB >> 4), kd = k_desc + key_at(j) % NS * (TB >> 4);
 #pragma unroll
       for (int c = 0; c < SUB; ++c)
 #pragma unroll
@@ -384,83 +431,80 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                  IDESC_S, c + kk > 0);
       tc_commit(&s_full[i]);
     };
-    // half h of P_i V: groups of 16 keys 4 h .. min(groups, 4 h + 4) - 1
-    auto outputs = [&](int i, int slot, int h, bool first, int groups) {
-      const uint64_t vd = v_desc + slot * (TB >> 4) + h * 512;
-      const uint32_t o = tmem + O_COL + i * 128, pr = tmem + S_COL + i * 128 + h * 32;
-      if (groups == 8) {
+    auto outputs = [&](int i, int j, int h) {  // half h (64 keys) of P_i V of step j
+      const uint64_t vd = v_desc + value_at(j) % NS * (TB >> 4) + h * 512;
+      const uint32_t o = tmem + O_COL + i * D, pr = tmem + P_COL + i * P_STEP + h * 32;
+      if (j < nk - 1 || tail_groups == 8) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, !(first && h + kk == 0));
+        for (int kk = 0; kk < 4; ++kk) mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, j + h + kk > 0);
       } else {
-        for (int kk = 0; kk < 4 && h * 4 + kk < groups; ++kk)
-          mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, !(first && h + kk == 0));
+#pragma unroll 1
+        for (int kk = 0; kk < 4 && 4 * h + kk < tail_groups; ++kk)
+          mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, j + h + kk > 0);
       }
     };
-    const int tail = s.len - (nk - 1) * kTileKeys;  // keys of the sequence from the last step on
-    const int tail_rows = min(kTileKeys, tail), tail_groups = (tail_rows + 15) / 16;
-    // step j's P V and step j + 1's scores
-    auto step = [&](int j) {
-      const int nv = 2 * j + 1, vs = nv % NS, nkey = 2 * j + 2, ks = nkey % NS;
-      if (!tile_wait(&kv_full[vs], (nv / NS) & 1)) return false;
-      bool key_here = false;
+    if (elect_one() && nk > 0) {
+      ok = tile_wait2(q_full, 0, full(0), 0);
+      if (ok) {
+        tc_fence_after();
+        if (steps[0] > 0) scores(0, 0);
+        if (steps[1] > 0) scores(1, 0);
+        tc_commit(&kv_empty[0]);
+      }
+      if (nk == 1 && ok && tail_rows < tail_groups * 16) ok = tile_wait(v_tail, 0);
+#pragma unroll 1
+      for (int j = 0; j < nk && ok; ++j) {
+        const int kn = j + 1 < nk ? key_at(j + 1) : 0, vn = value_at(j);  // (kn 0: a tile that is long there)
+        if (j > 0 && j == nk - 1 && tail_rows < tail_groups * 16) ok = tile_wait(v_tail, 0);
+        if constexpr (EARLY) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (j < steps[i]) {
+          for (int i = 0; i < 2; ++i)
+            if (ok && j + 1 < steps[i]) {
+              ok = tile_wait2(&s_free[i], j & 1, full(kn), phase(kn));
+              if (!ok) break;
+              tc_fence_after();
+              scores(i, j + 1);
+            }
+          if (j + 1 < nk) tc_commit(&kv_empty[kn % NS]);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (!tile_wait(&p_full[2 * i + h], j & 1)) return false;
-            tc_fence_after();
-            outputs(i, vs, h, j == 0, j == nk - 1 ? tail_groups : 8);
-          }
-          tc_commit(&o_done[i]);
-        }
-        if (j + 1 < steps[i]) {
-          if (!key_here) {
-            if (!tile_wait(&kv_full[ks], (nkey / NS) & 1)) return false;
-            key_here = true;
-            tc_fence_after();
-          }
-          scores(i, ks);
-        }
-      }
-      tc_commit(&kv_empty[vs]);
-      if (j + 1 < nk) tc_commit(&kv_empty[ks]);
-      return true;
-    };
-    if (nk > 0) {
-      const bool one = elect_one();
-      if (one) {
-        ok = tile_wait(q_full, 0) && tile_wait(&kv_full[0], 0);
-        if (ok) {
-          tc_fence_after();
-          if (steps[0] > 0) scores(0, 0);
-          if (steps[1] > 0) scores(1, 0);
-          tc_commit(&kv_empty[0]);
-        }
-        for (int j = 0; j + 1 < nk && ok; ++j) ok = step(j);
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      // the sequence's last tile: only the keys it has, whole groups of 16; rows past the end are made zeros
-      // (what lies there may be anything, and 0 x NaN is NaN)
-      if (ok && tail_rows < tail_groups * 16) {
-        const int nv = 2 * (nk - 1) + 1, vs = nv % NS;
-        ok = __all_sync(0xffffffffu, tile_wait(&kv_full[vs], (nv / NS) & 1));
-        for (int e = lane; ok && e < (tail_groups * 16 - tail_rows) * SUB * 8; e += 32) {
-          const int r = tail_rows + e / (SUB * 8), c = e % (SUB * 8);
-          *reinterpret_cast<uint4*>(ring + vs * TB + (c >> 3) * (TB / SUB) + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-      }
-      if (one) {
-        if (ok) ok = step(nk - 1);
-        if (!ok) {  // MMAs in flight finish before the memory goes
-          tc_commit(q_full);
-          tile_wait(q_full, 1);
+          for (int i = 0; i < 2; ++i)
+            if (ok && j < steps[i]) {
+              ok = tile_wait2(&p_full[2 * i], j & 1, full(vn), phase(vn));
+              if (!ok) break;
+              tc_fence_after();
+              outputs(i, j, 0);
+              ok = tile_wait(&p_full[2 * i + 1], j & 1);
+              if (!ok) break;
+              tc_fence_after();
+              outputs(i, j, 1);
+              tc_commit(&o_done[i]);
+            }
+          tc_commit(&kv_empty[vn % NS]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (ok && j < steps[i]) {
+              ok = tile_wait2(&p_full[2 * i], j & 1, full(vn), phase(vn));
+              if (!ok) break;
+              tc_fence_after();
+              outputs(i, j, 0);
+              ok = j + 1 < nk ? tile_wait2(&p_full[2 * i + 1], j & 1, full(kn), phase(kn)) : tile_wait(&p_full[2 * i + 1], j & 1);
+              if (!ok) break;
+              tc_fence_after();
+              outputs(i, j, 1);
+              tc_commit(&o_done[i]);
+              if (j + 1 < steps[i]) scores(i, j + 1);
+            }
+          tc_commit(&kv_empty[vn % NS]);
+          if (j + 1 < nk) tc_commit(&kv_empty[kn % NS]);
         }
       }
-      __syncwarp();
+      if (!ok) {  // MMAs in flight finish before the memory goes
+        tc_commit(drained);
+        tile_wait(drained, 0);
+      }
     }
+    __syncwarp();
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -472,12 +516,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int lim = valid ? s.len - s.n + tok : -1;            // last key the row sees
     const int first_lim = s.len - s.n + tok0 + i * TPT;        // the tile's first row's
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + S_COL + i * 128, o_at = tmem + lanes + O_COL + i * 128;
+    const uint32_t s_at = tmem + lanes + S_COL + i * 128, o_at = tmem + lanes + O_COL + i * D,
+                   p_at = tmem + lanes + P_COL + i * P_STEP;
     const float c = a.s.scale_log2;
     float m = -INFINITY, base = 0.f, l = 0.f;  // maximum in use (raw score), m * c or 0, sum against it
     const int my_steps = i == 0 ? steps[0] : steps[1];
+    bool s_here = false;
     for (int j = 0; j < my_steps && ok; ++j) {
-      ok = __all_sync(0xffffffffu, tile_wait(&s_full[i], j & 1));
+      if (!s_here) ok = tile_wait_warp(&s_full[i], j & 1);
       if (!ok) break;
       tc_fence_after();
       float x[128];
@@ -485,6 +531,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int g = 0; g < 4; ++g) tmem_ld32(s_at + g * 32, x + g * 32);
 #pragma unroll
       for (int g = 0; g < 4; ++g) tmem_ld_wait(x + g * 32);
+      if constexpr (EARLY) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[i]);
+      }
+      // (asked here, used after the maximum: the answer takes a while)
+      const bool o_here = !EARLY || j == 0 || mbar_test_wait(&o_done[i], (j - 1) & 1);
       const int key0 = j * kTileKeys;
       if (key0 + kTileKeys - 1 > first_lim) {
         const int rel = lim - key0;
@@ -508,7 +561,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const float f = exp2_fast(m * c - nb);
         l = m == -INFINITY ? 0.f : l * f;
         if (j > 0) {
-          ok = __all_sync(0xffffffffu, tile_wait(&o_done[i], (j - 1) & 1));
+          ok = tile_wait_warp(&o_done[i], (j - 1) & 1);
           if (!ok) break;
           tc_fence_after();
           const float fo = m == -INFINITY ? 0.f : f;
@@ -524,6 +577,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         m = mn;
         base = nb;
+      }
+      if constexpr (EARLY) {  // the last P_i V has read P_i
+        if (!__all_sync(0xffffffffu, o_here)) ok = tile_wait_warp(&o_done[i], (j - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
       }
       const uint64_t cc = pack2(c, c), nb2 = pack2(-base, -base);
       uint64_t sum0 = 0, sum1 = 0;  // pairs of zeros
@@ -547,20 +605,22 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             sum = add2(sum, pack2(p0, p1));
             p[e] = Type16<T>::pack(p0, p1);
           }
-          tmem_st16(s_at + g * 16, p);
+          tmem_st16(p_at + g * 16, p);
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
+        if (h == 0) s_here = EARLY && j + 1 < my_steps && mbar_test_wait(&s_full[i], (j + 1) & 1);
       }
+      s_here = __all_sync(0xffffffffu, s_here);
       float s0, s1;
       unpack2(add2(sum0, sum1), &s0, &s1);
       l += s0 + s1;
     }
     // ---- the row's output
     if (my_steps > 0 && ok) {
-      ok = __all_sync(0xffffffffu, tile_wait(&o_done[i], (my_steps - 1) & 1));
+      ok = tile_wait_warp(&o_done[i], (my_steps - 1) & 1);
       tc_fence_after();
     }
     if (ok) {
