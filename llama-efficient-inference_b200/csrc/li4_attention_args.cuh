@@ -27,6 +27,7 @@ struct SeqAttnArgs {
   float scale_log2;                // softmax scale times log2(e)
   int small_rows, big_rows;        // this launch takes sequences of small_rows < n * rep <= big_rows
   int grid;                        // CTAs that share the work
+  long long max_keys;              // no sequence has more, as far as the host knows
   float* part;                     // partial results of split items (see li4_seq_attention.cu)
 };
 
@@ -151,6 +152,7 @@ __device__ __noinline__ void redo_row(const SeqAttnArgs& a, int b, const Seq s, 
 // ---- launches shared by the entry points ----
 int launch_seq_attention(const SeqAttnArgs& a, bool paged, int dtype, int max_rows, cudaStream_t stream);
 int launch_tile_attention(const SeqAttnArgs& a, bool paged, int dtype, cudaStream_t stream);
+size_t tile_attention_part_bytes(int hd, int rep, int64_t tokens, int64_t kv_heads, int64_t max_keys, int sm);
 size_t seq_attention_part_bytes(int hd, int max_rows, int sm);
 
 }  // namespace li4

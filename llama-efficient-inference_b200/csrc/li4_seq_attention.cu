@@ -575,6 +575,11 @@ static int attention_rows(const li4_attention* p) {
   return (int)(rows > (1 << 30) ? (1 << 30) : rows);
 }
 
+// The most keys a sequence can have, as far as the host knows.
+static int64_t attention_keys(const li4_attention* p) {
+  return p->kv_lens ? p->table_width * p->page_size : p->max_queries;
+}
+
 static int run_attention(const li4_attention* p, bool paged, void* workspace, size_t workspace_bytes, void* stream,
                          const char* what) {
   int rc = check_attention(p, paged, what);
@@ -609,6 +614,7 @@ static int run_attention(const li4_attention* p, bool paged, void* workspace, si
   a.hd = (int)p->head_dim;
   a.scale_log2 = p->scale * 1.44269504088896340736f;
   a.part = static_cast<float*>(workspace);
+  a.max_keys = attention_keys(p);
   // Which kernel: the streaming one takes sequences of few rows, whose time is the reading of the keys, the
   // tensor-memory one (positive scales, some page) the rest.  The host knows the longest sequence as the caller
   // claims it; the device looks at each sequence's own rows, so a wrong claim only costs time.
@@ -636,7 +642,14 @@ static int run_attention(const li4_attention* p, bool paged, void* workspace, si
 extern "C" size_t li4_attention_workspace_bytes(const li4_attention* p) {
   using namespace li4;
   if (!p || p->n_seqs <= 0 || p->n_tokens <= 0 || p->n_kv_heads < 1 || p->max_queries < 0) return 0;
-  return seq_attention_part_bytes((int)p->head_dim, attention_rows(p), current_sm_count());
+  const int64_t rep = p->n_heads / p->n_kv_heads;
+  if (rep < 1 || rep > 128) return 0;
+  const size_t seq = seq_attention_part_bytes((int)p->head_dim, attention_rows(p), current_sm_count());
+  const size_t tile = attention_rows(p) > kFewRows ? tile_attention_part_bytes((int)p->head_dim, (int)rep, p->n_tokens,
+                                                                               p->n_kv_heads, attention_keys(p),
+                                                                               current_sm_count())
+                                                   : 0;
+  return seq > tile ? seq : tile;  // (the two kernels run one after the other)
 }
 
 extern "C" int li4_prompt_attention(const li4_attention* args, void* workspace, size_t workspace_bytes, void* stream) {

@@ -17,7 +17,8 @@
 // behind (P <= 256 fits both 16-bit types, the sum is fp32), so the accumulated output is rescaled only
 // when a row's maximum grows by more than that -- rarely after the first tiles.
 // Every mbarrier wait is bounded: one that runs out sets bit 8 of li4_device_errors; every role then
-// leaves its loop, copies and MMAs in flight are waited for (bounded) and the tensor memory is freed.
+// runs to its end without waiting, copies and MMAs in flight are waited for (bounded) and the tensor
+// memory is freed.
 #include <cuda.h>
 
 #include <mutex>
@@ -45,6 +46,7 @@ constexpr int kTileKeys = 128;       // keys of a step
 constexpr int kTileThreads = 384;    // 8 softmax warps, the TMA warp, the MMA warp, 2 that only fill their group
 constexpr int kTmaWarp = 8, kMmaWarp = 9;
 constexpr unsigned kTileWaitLimit = 1u << 24;  // polls
+constexpr int kTileMinSteps = 8;     // key tiles below which a range is not cut
 constexpr float kLazyLog2 = 8.f;     // how far the maximum in use may lag, in powers of two
 
 __host__ __device__ constexpr int tile_slots(int D) { return D == 64 ? 8 : 4; }
@@ -59,33 +61,35 @@ constexpr unsigned kPolyPairs = POLY;  // which of 16 pairs of probabilities the
 struct TileArgs {
   SeqAttnArgs s;
   int tokens_per_tile;  // whole queries of a tile: 128 / rep
+  int part_slots;       // items whose partial results fit the workspace (0: keys are not split)
   int box_rows;         // key rows of one copy
 };
 
 // ---- mbarriers, tensor memory ----
-__device__ __forceinline__ bool tile_wait(uint64_t* bar, unsigned parity) {
-  for (unsigned i = 0; i < kTileWaitLimit; ++i)
-    if (mbar_test_wait(bar, parity)) return true;
-  atomicOr(&g_tile_device_error, 256u);
-  return false;
+// A converged warp waits for a phase, at most `limit` polls; a wait that runs out leaves limit = 1, which makes every later
+// wait of the warp give up at once: the roles then run to their ends on whatever is there, no role misses another's
+// arrival, and the warp reports at the end.  (Written as one PTX loop for a whole warp: a ready barrier costs 63 cycles,
+// against 120 in a branch of one thread and 150 with a check after it.)
+__device__ __forceinline__ void tile_wait(uint64_t* bar, unsigned parity, unsigned& limit) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, %0;\n"
+      "LAB_WAIT:\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra LAB_DONE;\n\t"
+      "sub.u32 n, n, 1;\n\tsetp.ne.u32 q, n, 0;\n\t@q bra LAB_WAIT;\n\tmov.u32 %0, 1;\nLAB_DONE:\n\t}"
+      : "+r"(limit)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
 }
-__device__ __forceinline__ bool tile_wait2(uint64_t* bar, unsigned parity, uint64_t* bar2, unsigned parity2) {
-  for (unsigned i = 0; i < kTileWaitLimit; ++i) {
-    const bool a = mbar_test_wait(bar, parity), b = mbar_test_wait(bar2, parity2);
-    if (a && b) return true;
-  }
-  atomicOr(&g_tile_device_error, 256u);
-  return false;
-}
-// A converged warp: tests, or waits; every lane returns the same.
-__device__ __forceinline__ bool tile_test_warp(uint64_t* bar, unsigned parity) {
-  return __all_sync(0xffffffffu, mbar_test_wait(bar, parity));
-}
-__device__ __forceinline__ bool tile_wait_warp(uint64_t* bar, unsigned parity) {
-  for (unsigned i = 0; i < kTileWaitLimit; ++i)
-    if (tile_test_warp(bar, parity)) return true;
-  if ((threadIdx.x & 31) == 0) atomicOr(&g_tile_device_error, 256u);
-  return false;
+// Both of two barriers (two tests together cost hardly more than one).
+__device__ __forceinline__ void tile_wait2(uint64_t* bar, unsigned parity, uint64_t* bar2, unsigned parity2,
+                                           unsigned& limit) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, %0;\n"
+      "LAB_WAIT:\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 q, [%3], %4;\n\tand.pred p, p, q;\n\t@p bra LAB_DONE;\n\t"
+      "sub.u32 n, n, 1;\n\tsetp.ne.u32 q, n, 0;\n\t@q bra LAB_WAIT;\n\tmov.u32 %0, 1;\nLAB_DONE:\n\t}"
+      : "+r"(limit)
+      : "r"(smem_addr(bar)), "r"(parity), "r"(smem_addr(bar2)), "r"(parity2)
+      : "memory");
 }
 
 __device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
@@ -116,33 +120,31 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
 
 // Shared-memory operand, 128-byte swizzle (see int4_gemm_kernel): K-major rows of 64 values, 8-row groups
 // 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)1u << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1u << 46 |
-         (uint64_t)2u << 61;
-}
+// (the high word of both forms below: stride offset 1024, version 1, 128-byte swizzle)
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_k_major(uint32_t addr) { return ((addr >> 4) & 0x3FFFu) | 1u << 16; }
 // The same rows read along the other axis (N-major operand: a row is one k, its 64 values are 64 n): the
 // next 64 n are `chunk` bytes on (leading offset), the next 8 k 1024 bytes (stride offset).
-__device__ __forceinline__ uint64_t desc_n_major(uint32_t addr, uint32_t chunk) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)(chunk >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
-         (uint64_t)1u << 46 | (uint64_t)2u << 61;
+__device__ __forceinline__ uint32_t desc_n_major(uint32_t addr, uint32_t chunk) {
+  return ((addr >> 4) & 0x3FFFu) | (chunk >> 4) << 16;
 }
 // Instruction descriptor, kind::f16: fp32 accumulator, A and B of one type (0 fp16, 1 bf16), B N-major or not.
 __host__ __device__ constexpr uint32_t tile_idesc(int n, int type, int b_n_major) {
   return (1u << 4) | ((uint32_t)type << 7) | ((uint32_t)type << 10) | ((uint32_t)b_n_major << 16) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "r"(kDescHigh)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tmov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "r"(kDescHigh)
       : "memory");
 }
 
@@ -236,21 +238,48 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Item `index` of the launch: sequences in order, inside a sequence the later (longer) pairs of tiles first, KV
-// heads innermost.  One warp; every lane returns the same.
-struct TileItem {
-  int b, pair, kvh;  // b = -1: no such item
+// The launch's items: sequences in order, inside a sequence the later (longer) pairs of tiles first, then the KV heads,
+// the ranges of keys innermost.  One warp; every lane returns the same.
+struct TileWork {
+  int b;              // sequence; -1: no such item
+  int kvh;
+  int start, n, len;  // the sequence (Seq)
+  int tok0;           // first query of tile 0
+  int first;          // first key tile of the item's range
+  int steps[2];       // key tiles of each tile of rows: up to the last key its last query sees
+  int part;           // the item's place among the partial results; -1: it has all its keys
 };
+
+// Ranges of keys per (pair of tiles, KV head): more than one where these alone leave SMs idle.
 template <bool PAGED>
-__device__ __forceinline__ TileItem find_item(const TileArgs& a, int index) {
+__device__ __forceinline__ int item_splits(const TileArgs& a) {
+  if (a.part_slots == 0) return 1;
+  const int lane = threadIdx.x & 31, per_pair = 2 * a.tokens_per_tile;
+  int pairs = 0, len = 0;
+  for (int b = lane; b < a.s.B; b += 32) {
+    const Seq s = load_seq<PAGED>(a.s, b);
+    pairs += (s.n + per_pair - 1) / per_pair;
+    if (s.n > 0) len = max(len, s.len);
+  }
+  pairs = __reduce_add_sync(0xffffffffu, pairs);
+  len = __reduce_max_sync(0xffffffffu, len);
+  const int most = (len + kTileMinSteps * kTileKeys - 1) / (kTileMinSteps * kTileKeys);
+  return max(1, min(most, a.part_slots / max(1, pairs * a.s.Hkv)));
+}
+
+template <bool PAGED>
+__device__ __forceinline__ TileWork find_item(const TileArgs& a, int index, int splits) {
   const int lane = threadIdx.x & 31;
-  const int per_pair = 2 * a.tokens_per_tile;
-  TileItem it = {-1, 0, 0};
+  const int per_pair = 2 * a.tokens_per_tile, number = index;
+  TileWork w;
+  w.b = -1;
   for (int b0 = 0; b0 < a.s.B; b0 += 32) {
     int items = 0, pairs = 0;
+    Seq s = {0, 0, 0};
     if (b0 + lane < a.s.B) {
-      pairs = (load_seq<PAGED>(a.s, b0 + lane).n + per_pair - 1) / per_pair;
-      items = pairs * a.s.Hkv;
+      s = load_seq<PAGED>(a.s, b0 + lane);
+      pairs = (s.n + per_pair - 1) / per_pair;
+      items = pairs * a.s.Hkv * splits;
     }
     int incl = items;
 #pragma unroll
@@ -263,22 +292,61 @@ __device__ __forceinline__ TileItem find_item(const TileArgs& a, int index) {
       const int src = __ffs(hit) - 1;
       const int rel = index - __shfl_sync(0xffffffffu, incl - items, src);
       pairs = __shfl_sync(0xffffffffu, pairs, src);
-      it.b = b0 + src;
-      it.pair = pairs - 1 - rel / a.s.Hkv;
-      it.kvh = rel % a.s.Hkv;
-      return it;
+      w.b = b0 + src;
+      w.part = splits > 1 ? number : -1;
+      w.start = __shfl_sync(0xffffffffu, s.start, src);
+      w.n = __shfl_sync(0xffffffffu, s.n, src);
+      w.len = __shfl_sync(0xffffffffu, s.len, src);
+      const int head = rel / splits, split = rel - head * splits;
+      w.kvh = head % a.s.Hkv;
+      w.tok0 = (pairs - 1 - head / a.s.Hkv) * per_pair;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int first = w.tok0 + i * a.tokens_per_tile, last = min(w.n, first + a.tokens_per_tile) - 1;
+        const int keys = first < w.n ? max(0, w.len - w.n + last + 1) : 0;
+        w.steps[i] = (keys + kTileKeys - 1) / kTileKeys;
+      }
+      const int all = max(w.steps[0], w.steps[1]), per = max(kTileMinSteps, (all + splits - 1) / splits);
+      w.first = min(all, split * per);
+      const int end = min(all, w.first + per);
+      w.steps[0] = max(0, min(w.steps[0], end) - w.first);
+      w.steps[1] = max(0, min(w.steps[1], end) - w.first);
+      return w;
     }
     index -= __shfl_sync(0xffffffffu, incl, 31);
   }
-  return it;
+  return w;
 }
+
+// Cluster launch control: asks for a CTA of this launch that has not started yet; its index arrives in `reply` on `bar`.
+__device__ __forceinline__ void ask_next(uint32_t reply, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(reply),
+      "r"(smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ int read_next(uint32_t reply) {  // -1: none is left
+  int x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 lo, hi;\n\t.reg .b128 h;\n\t"
+      "ld.shared.v2.b64 {lo, hi}, [%1];\n\tmov.b128 h, {lo, hi};\n\tmov.b32 %0, -1;\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n\t}"
+      : "=r"(x)
+      : "r"(reply)
+      : "memory");
+  return x;
+}
+
+// floats of one item's partial results: 2 x 128 rows of D outputs, then (exponent base, sum) per row
+__host__ __device__ constexpr size_t tile_part_floats(int D) { return (size_t)2 * kTileRows * (D + 2); }
 
 template <typename T, int D, bool PAGED>
 __global__ void __launch_bounds__(kTileThreads, 1)
     tile_attention_kernel(const __grid_constant__ TileArgs a, const __grid_constant__ CUtensorMap map_q,
                           const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   constexpr int NS = tile_slots(D), TB = tile_bytes(D), SUB = D / 64;
-  constexpr int TYPE = sizeof(T) == 2 && __is_same(T, __half) ? 0 : 1;
+  constexpr int TYPE = __is_same(T, __half) ? 0 : 1;
   // Tensor-memory columns: S_i at 128 i, O_i at 256 + D i.  At 64 dims there is room for P_i beside them (64 columns
   // each), so S_i of the next step is computed as soon as the softmax has read the last one; at 128 dims P_i lies in
   // S_i's first 64 columns and the next S_i follows P_i V.
@@ -287,347 +355,430 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + 2 * TB;
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(ring + NS * TB);
+  uint8_t* reply = ring + NS * TB;       // 16 bytes
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(reply + 16);
   uint64_t* kv_empty = kv_full + NS;
   uint64_t* q_full = kv_empty + NS;
-  uint64_t* s_full = q_full + 1;   // [2] S_i written
-  uint64_t* p_full = s_full + 2;   // [2][2] half of P_i written (4 warps), O_i rescaled before the first
-  uint64_t* o_done = p_full + 4;   // [2] the last P_i V finished
-  uint64_t* s_free = o_done + 2;   // [2] S_i read (4 warps); 64 dims only
-  uint64_t* v_tail = s_free + 2;   // the last value tile's missing rows are zeros
-  uint64_t* drained = v_tail + 1;  // the product warp gave up and its MMAs have finished
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
-  TileItem* s_item = reinterpret_cast<TileItem*>(tmem_holder + 1);
+  uint64_t* q_empty = q_full + 1;        // the item's last scores have read the queries
+  uint64_t* s_full = q_empty + 1;        // [2] S_i written
+  uint64_t* p_full = s_full + 2;         // [2][2] half of P_i written (4 warps), O_i rescaled before the first
+  uint64_t* o_done = p_full + 4;         // [2] the last P_i V finished
+  uint64_t* s_free = o_done + 2;         // [2] S_i read (4 warps); 64 dims only
+  uint64_t* v_tail = s_free + 2;         // the last value tile's rows are there, its missing rows not yet zeros
+  uint64_t* drained = v_tail + 1;        // the product warp gave up and its MMAs have finished
+  uint64_t* work_full = drained + 1;     // [2] work[i] names an item
+  uint64_t* work_empty = work_full + 2;  // [2] the 10 working warps have read it
+  uint64_t* replied = work_empty + 2;    // the reply is there
+  uint64_t* ending = replied + 1;        // the products are near the item's end
+  TileWork* work = reinterpret_cast<TileWork*>(ending + 1);  // [2]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(work + 2);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
-  pdl_wait_primary();
-  if (warp == 0) {
-    const TileItem it = find_item<PAGED>(a, (int)blockIdx.x);
-    if (lane == 0) *s_item = it;
-  }
-  if (tid == 32) {
+  if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
     }
     mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[2 * i], 4);
       mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_done[i], 1);
       mbar_init(&s_free[i], 4);
+      mbar_init(&work_full[i], 1);
+      mbar_init(&work_empty[i], 10);
     }
     mbar_init(v_tail, 1);
     mbar_init(drained, 1);
+    mbar_init(replied, 1);
+    mbar_init(ending, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  __syncthreads();
-  const TileItem item = *s_item;
-  if (item.b < 0) return;
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_holder)),
                  "n"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  const Seq s = load_seq<PAGED>(a.s, item.b);
-  const int TPT = a.tokens_per_tile;
-  const int tok0 = item.pair * 2 * TPT;  // first query of tile 0
-  // steps of each tile: up to the last key its last query sees
-  int steps[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int first = tok0 + i * TPT, last = min(s.n, first + TPT) - 1;
-    const int keys = first < s.n ? max(0, s.len - s.n + last + 1) : 0;
-    steps[i] = (keys + kTileKeys - 1) / kTileKeys;
-  }
-  const int nk = max(steps[0], steps[1]);
-  // place of key tile j and value tile j in the ring's order: the order in which the products take them
-  auto key_at = [](int j) { return !EARLY ? 2 * j : j == 0 ? 0 : 2 * j - 1; };
-  auto value_at = [nk](int j) { return !EARLY || j == nk - 1 ? 2 * j + 1 : 2 * j + 2; };
-  // the sequence's last tile: only the keys it has, whole groups of 16; rows past the end are made zeros (what lies
-  // there may be anything, and 0 x NaN is NaN)
-  const int tail_rows = min(kTileKeys, s.len - (nk - 1) * kTileKeys), tail_groups = (tail_rows + 15) / 16;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_wait_primary();
   const uint32_t tmem = *tmem_holder;
-  bool ok = true;
+  const int TPT = a.tokens_per_tile;
+  unsigned limit = kTileWaitLimit;
+
+  // Place of key tile j and value tile j in an item's order of the ring: the order in which the products take them.
+  auto key_at = [](int j) { return !EARLY ? 2 * j : j == 0 ? 0 : 2 * j - 1; };
+  auto value_at = [](int j, int nk) { return !EARLY || j == nk - 1 ? 2 * j + 1 : 2 * j + 2; };
+  // The working warps' next item (this CTA's k-th); b = -1 ends.
+  auto next_work = [&](int k) {
+    tile_wait(&work_full[k & 1], (k >> 1) & 1, limit);
+    TileWork w = work[k & 1];
+    if (limit == 1) w.b = -1;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&work_empty[k & 1]);
+    return w;
+  };
+  // Keys of the item's last key tile; P V takes them in groups of 16, and rows of the last group past the end are made
+  // zeros (what lies there may be anything, and 0 x NaN is NaN).
+  auto tail_rows_of = [](const TileWork& w, int nk) { return min(kTileKeys, w.len - (w.first + nk - 1) * kTileKeys); };
 
   // 384 threads x 168 registers at the launch: the softmax's two groups take 208 each, the third keeps 80
   // (2 x 128 x 208 + 128 x 80 <= 384 x 168)
   if (warp >= kTmaWarp) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-  if (warp == kTmaWarp) {
-    // ---- copies
-    if (lane == 0 && nk > 0) {
-      // a tile whose queries all lie past the tensor is not loaded (its rows are not used)
-      const int tiles = steps[1] > 0 ? 2 : 1;
-      mbar_arrive_expect_tx(q_full, tiles * SUB * TPT * a.s.rep * 128);
-      for (int i = 0; i < tiles; ++i)
-        for (int c = 0; c < SUB; ++c)
-          tma_load4(smem_addr(smem + i * TB + c * (TB / SUB)), &map_q, q_full, c * 64, 0, item.kvh,
-                    s.start + tok0 + i * TPT);
-    }
-    int n = 0;  // tiles issued
-    for (; n < 2 * nk && ok; ++n) {
-      // tile n of the ring's order
-      const bool value = !EARLY ? n & 1 : n == 2 * nk - 1 || (n > 0 && !(n & 1));
-      const int j = !EARLY ? n / 2 : n == 2 * nk - 1 ? nk - 1 : value ? n / 2 - 1 : (n + 1) / 2;
-      const int key0 = j * kTileKeys;
-      const int rows = min(kTileKeys, s.len - key0);
-      int row = s.start + key0, page = 0;
-      bool mine = lane == 0;
-      int boxes = 1;
-      if constexpr (PAGED) {
-        boxes = (rows + a.box_rows - 1) / a.box_rows;
-        mine = lane < boxes;
-        const int key = key0 + lane * a.box_rows;
-        row = key & ((1 << a.s.log_page) - 1);
-        // an entry outside the cache is a coordinate outside the tensor: zeros
-        if (mine) page = a.s.tables[(long long)item.b * a.s.table_stride + (key >> a.s.log_page)];
-      }
-      const int slot = n % NS;
-      if (n >= NS) ok = tile_wait_warp(&kv_empty[slot], ((n / NS) - 1) & 1);
-      if (!ok) break;
-      if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], boxes * a.box_rows * SUB * 128);
-      __syncwarp();
-      if (mine)
-        for (int c = 0; c < SUB; ++c)
-          tma_load4(smem_addr(ring + slot * TB + c * (TB / SUB)) + lane * a.box_rows * 128, value ? &map_v : &map_k,
-                    &kv_full[slot], c * 64, row, item.kvh, page);
-    }
-    if (ok && nk > 0 && tail_rows < tail_groups * 16) {
-      const int last = 2 * nk - 1, slot = last % NS;
-      ok = tile_wait_warp(&kv_full[slot], (last / NS) & 1);
-      for (int e = lane; ok && e < (tail_groups * 16 - tail_rows) * SUB * 8; e += 32) {
-        const int r = tail_rows + e / (SUB * 8), c = e % (SUB * 8);
-        *reinterpret_cast<uint4*>(ring + slot * TB + (c >> 3) * (TB / SUB) + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(v_tail);
-    }
-    if (!ok)  // copies in flight land before the memory goes
-      for (int i = max(0, n - NS); i < n; ++i) tile_wait_warp(&kv_full[i % NS], (i / NS) & 1);
-  } else if (warp == kMmaWarp) {
-    // ---- products: one elected thread, tile 0 then tile 1 (a warp per tile was slower: their products then share the
-    // tensor cores and both finish late).  Any barrier read costs it 160-220 cycles and several at once hardly more, so
-    // what a group of products needs is tested together.
-    constexpr uint32_t IDESC_S = tile_idesc(kTileKeys, TYPE, 0), IDESC_O = tile_idesc(D, TYPE, 1);
-    const uint64_t q_desc = desc_k_major(smem_addr(smem)), k_desc = desc_k_major(smem_addr(ring)),
-                   v_desc = desc_n_major(smem_addr(ring), TB / SUB);
-    auto full = [&](int n) { return &kv_full[n % NS]; };
-    auto phase = [&](int n) { return (unsigned)(n / NS) & 1u; };
-    auto scores = [&](int i, int j) {  // S_i of step j
-      const uint64_t qd = q_desc + i * (TB >> 4), kd = k_desc + key_at(j) % NS * (TB >> 4);
-#pragma unroll
-      for (int c = 0; c < SUB; ++c)
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          mma_ss(tmem + S_COL + i * 128, qd + ((c * (TB / SUB) + kk * 32) >> 4), kd + ((c * (TB / SUB) + kk * 32) >> 4),
-                 IDESC_S, c + kk > 0);
-      tc_commit(&s_full[i]);
-    };
-    auto outputs = [&](int i, int j, int h) {  // half h (64 keys) of P_i V of step j
-      const uint64_t vd = v_desc + value_at(j) % NS * (TB >> 4) + h * 512;
-      const uint32_t o = tmem + O_COL + i * D, pr = tmem + P_COL + i * P_STEP + h * 32;
-      if (j < nk - 1 || tail_groups == 8) {
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, j + h + kk > 0);
-      } else {
-#pragma unroll 1
-        for (int kk = 0; kk < 4 && 4 * h + kk < tail_groups; ++kk)
-          mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, j + h + kk > 0);
-      }
-    };
-    if (elect_one() && nk > 0) {
-      ok = tile_wait2(q_full, 0, full(0), 0);
-      if (ok) {
-        tc_fence_after();
-        if (steps[0] > 0) scores(0, 0);
-        if (steps[1] > 0) scores(1, 0);
-        tc_commit(&kv_empty[0]);
-      }
-      if (nk == 1 && ok && tail_rows < tail_groups * 16) ok = tile_wait(v_tail, 0);
-#pragma unroll 1
-      for (int j = 0; j < nk && ok; ++j) {
-        const int kn = j + 1 < nk ? key_at(j + 1) : 0, vn = value_at(j);  // (kn 0: a tile that is long there)
-        if (j > 0 && j == nk - 1 && tail_rows < tail_groups * 16) ok = tile_wait(v_tail, 0);
-        if constexpr (EARLY) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (ok && j + 1 < steps[i]) {
-              ok = tile_wait2(&s_free[i], j & 1, full(kn), phase(kn));
-              if (!ok) break;
-              tc_fence_after();
-              scores(i, j + 1);
-            }
-          if (j + 1 < nk) tc_commit(&kv_empty[kn % NS]);
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (ok && j < steps[i]) {
-              ok = tile_wait2(&p_full[2 * i], j & 1, full(vn), phase(vn));
-              if (!ok) break;
-              tc_fence_after();
-              outputs(i, j, 0);
-              ok = tile_wait(&p_full[2 * i + 1], j & 1);
-              if (!ok) break;
-              tc_fence_after();
-              outputs(i, j, 1);
-              tc_commit(&o_done[i]);
-            }
-          tc_commit(&kv_empty[vn % NS]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (ok && j < steps[i]) {
-              ok = tile_wait2(&p_full[2 * i], j & 1, full(vn), phase(vn));
-              if (!ok) break;
-              tc_fence_after();
-              outputs(i, j, 0);
-              ok = j + 1 < nk ? tile_wait2(&p_full[2 * i + 1], j & 1, full(kn), phase(kn)) : tile_wait(&p_full[2 * i + 1], j & 1);
-              if (!ok) break;
-              tc_fence_after();
-              outputs(i, j, 1);
-              tc_commit(&o_done[i]);
-              if (j + 1 < steps[i]) scores(i, j + 1);
-            }
-          tc_commit(&kv_empty[vn % NS]);
-          if (j + 1 < nk) tc_commit(&kv_empty[kn % NS]);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == kTmaWarp) {
+      // ---- copies
+      unsigned base = 0, qn = 0, tails = 0;  // ring tiles, query loads and mended tails of earlier items
+      for (int k = 0;; ++k) {
+        const TileWork w = next_work(k);
+        if (w.b < 0) break;
+        const int nk = max(w.steps[0], w.steps[1]);
+        if (nk == 0) continue;
+        if (qn > 0) tile_wait(q_empty, (qn - 1) & 1, limit);
+        ++qn;
+        if (lane == 0) {
+          // a tile whose queries all lie past the sequence, or that sees no key of the range, is not loaded
+          const int lo = w.steps[0] > 0 ? 0 : 1, hi = w.steps[1] > 0 ? 2 : 1;
+          mbar_arrive_expect_tx(q_full, (hi - lo) * SUB * TPT * a.s.rep * 128);
+          for (int i = lo; i < hi; ++i)
+            for (int c = 0; c < SUB; ++c)
+              tma_load4(smem_addr(smem + i * TB + c * (TB / SUB)), &map_q, q_full, c * 64, 0, w.kvh,
+                        w.start + w.tok0 + i * TPT);
         }
+        const int tail = tail_rows_of(w, nk), end = (tail + 15) / 16 * 16;
+        for (int n = 0; n < 2 * nk; ++n) {
+          const bool value = !EARLY ? n & 1 : n == 2 * nk - 1 || (n > 0 && !(n & 1));
+          const int j = !EARLY ? n / 2 : n == 2 * nk - 1 ? nk - 1 : value ? n / 2 - 1 : (n + 1) / 2;
+          const int key0 = (w.first + j) * kTileKeys;
+          int row = w.start + key0, page = 0;
+          bool mine = lane == 0;
+          int boxes = 1;
+          if constexpr (PAGED) {
+            boxes = (min(kTileKeys, w.len - key0) + a.box_rows - 1) / a.box_rows;
+            mine = lane < boxes;
+            const int key = key0 + lane * a.box_rows;
+            row = key & ((1 << a.s.log_page) - 1);
+            // an entry outside the cache is a coordinate outside the tensor: zeros
+            if (mine) page = a.s.tables[(long long)w.b * a.s.table_stride + (key >> a.s.log_page)];
+          }
+          // the last value tile with missing rows arrives on a barrier of its own and counts as full once they are zeros
+          const bool mend = n == 2 * nk - 1 && tail < end;
+          const unsigned g = base + n, slot = g % NS;
+          uint64_t* bar = mend ? v_tail : &kv_full[slot];
+          if (g >= NS) tile_wait(&kv_empty[slot], ((g / NS) - 1) & 1, limit);
+          if (lane == 0) mbar_arrive_expect_tx(bar, boxes * a.box_rows * SUB * 128);
+          __syncwarp();
+          if (mine)
+            for (int c = 0; c < SUB; ++c)
+              tma_load4(smem_addr(ring + slot * TB + c * (TB / SUB)) + lane * a.box_rows * 128, value ? &map_v : &map_k,
+                        bar, c * 64, row, w.kvh, page);
+          if (mend) {
+            tile_wait(v_tail, tails & 1, limit);
+            ++tails;
+            for (int e = lane; e < (end - tail) * SUB * 8; e += 32) {
+              const int r = tail + e / (SUB * 8), c = e % (SUB * 8);
+              *reinterpret_cast<uint4*>(ring + slot * TB + (c >> 3) * (TB / SUB) + r * 128 + (c & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&kv_full[slot]);
+          }
+        }
+        base += 2 * nk;
       }
-      if (!ok) {  // MMAs in flight finish before the memory goes
-        tc_commit(drained);
-        tile_wait(drained, 0);
+      if (limit == 1) {  // a wait ran out: copies in flight land before the memory goes
+        unsigned more = kTileWaitLimit;
+        for (unsigned i = base > NS ? base - NS : 0; i < base; ++i) tile_wait(&kv_full[i % NS], (i / NS) & 1, more);
+        if (qn > 0) tile_wait(q_full, (qn - 1) & 1, more);
+      }
+    } else if (warp == kMmaWarp) {
+      // ---- products, tile 0 then tile 1 (a warp per tile was slower: their products then share the tensor cores and
+      // both finish late).  The warp waits together; one thread issues a group of products.
+      constexpr uint32_t IDESC_S = tile_idesc(kTileKeys, TYPE, 0), IDESC_O = tile_idesc(D, TYPE, 1);
+      const uint32_t q_desc = desc_k_major(smem_addr(smem)), k_desc = desc_k_major(smem_addr(ring)),
+                     v_desc = desc_n_major(smem_addr(ring), TB / SUB);
+      unsigned base = 0, qn = 0, done0 = 0, done1 = 0;  // of earlier items: ring tiles, query loads, steps
+      for (int k = 0;; ++k) {
+        const TileWork w = next_work(k);
+        if (w.b < 0) break;
+        const int nk = max(w.steps[0], w.steps[1]);
+        if (nk == 0) {
+          if (lane == 0) mbar_arrive(ending);
+          continue;
+        }
+        const int tail_groups = (tail_rows_of(w, nk) + 15) / 16;
+        auto full = [&](unsigned n) { return &kv_full[(base + n) % NS]; };
+        auto phase = [&](unsigned n) { return (base + n) / NS & 1u; };
+        auto scores = [&](int i, unsigned slot) {  // S_i against the key tile in a slot
+          const uint32_t qd = q_desc + i * (TB >> 4), kd = k_desc + slot * (TB >> 4);
+#pragma unroll
+          for (int c = 0; c < SUB; ++c)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_ss(tmem + S_COL + i * 128, qd + ((c * (TB / SUB) + kk * 32) >> 4),
+                     kd + ((c * (TB / SUB) + kk * 32) >> 4), IDESC_S, c + kk > 0);
+          tc_commit(&s_full[i]);
+        };
+        // keys 64 h .. 64 h + 64 of P_i V with the value tile in a slot
+        auto outputs = [&](int i, unsigned slot, int h, bool first, int groups) {
+          const uint32_t vd = v_desc + slot * (TB >> 4) + h * 512;
+          const uint32_t o = tmem + O_COL + i * D, pr = tmem + P_COL + i * P_STEP + h * 32;
+          if (groups == 8) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, !first || h + kk > 0);
+          } else {
+#pragma unroll 1
+            for (int kk = 0; kk < 4 && 4 * h + kk < groups; ++kk)
+              mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, !first || h + kk > 0);
+          }
+        };
+        tile_wait2(q_full, qn & 1, full(0), phase(0), limit);
+        if (EARLY && done0 > 0 && w.steps[0] > 0) tile_wait(&s_free[0], (done0 - 1) & 1, limit);
+        if (EARLY && done1 > 0 && w.steps[1] > 0) tile_wait(&s_free[1], (done1 - 1) & 1, limit);
+        tc_fence_after();
+        if (elect_one()) {
+          if (w.steps[0] > 0) scores(0, base % NS);
+          if (w.steps[1] > 0) scores(1, base % NS);
+          tc_commit(&kv_empty[base % NS]);
+          if (nk == 1) tc_commit(q_empty);
+        }
+#pragma unroll 1
+        for (int j = 0; j < nk; ++j) {
+          if (j == max(0, nk - 3) && lane == 0) mbar_arrive(ending);
+          const unsigned kn = key_at(j + 1), vn = value_at(j, nk);
+          const unsigned kslot = (base + kn) % NS, vslot = (base + vn) % NS;
+          const int groups = j == nk - 1 ? tail_groups : 8;
+          const bool more0 = j + 1 < w.steps[0], more1 = j + 1 < w.steps[1];
+          if constexpr (EARLY) {
+            // the next scores of both tiles, then the step's P V of each
+            if (j + 1 < nk) {
+              if (more0 && more1) tile_wait2(&s_free[0], (done0 + j) & 1, &s_free[1], (done1 + j) & 1, limit);
+              else if (more0) tile_wait(&s_free[0], (done0 + j) & 1, limit);
+              else tile_wait(&s_free[1], (done1 + j) & 1, limit);
+              tile_wait(full(kn), phase(kn), limit);
+              tc_fence_after();
+              if (elect_one()) {
+                if (more0) scores(0, kslot);
+                if (more1) scores(1, kslot);
+                tc_commit(&kv_empty[kslot]);
+                if (j + 1 == nk - 1) tc_commit(q_empty);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (j < w.steps[i]) {
+                const unsigned par = ((i ? done1 : done0) + j) & 1;
+                tile_wait2(&p_full[2 * i + 1], par, full(vn), phase(vn), limit);
+                tc_fence_after();
+                if (elect_one()) {
+                  outputs(i, vslot, 0, j == 0, groups);
+                  outputs(i, vslot, 1, j == 0, groups);
+                  tc_commit(&o_done[i]);
+                }
+              }
+            if (elect_one()) tc_commit(&kv_empty[vslot]);
+          } else {
+            // each tile's P V, as its halves come, then its next scores
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (j < w.steps[i]) {
+                const unsigned par = ((i ? done1 : done0) + j) & 1;
+                tile_wait2(&p_full[2 * i], par, full(vn), phase(vn), limit);
+                tc_fence_after();
+                if (elect_one()) outputs(i, vslot, 0, j == 0, groups);
+                const bool more = i ? more1 : more0;
+                if (more) tile_wait2(&p_full[2 * i + 1], par, full(kn), phase(kn), limit);
+                else tile_wait(&p_full[2 * i + 1], par, limit);
+                tc_fence_after();
+                if (elect_one()) {
+                  outputs(i, vslot, 1, j == 0, groups);
+                  tc_commit(&o_done[i]);
+                  if (more) scores(i, kslot);
+                }
+              }
+            if (elect_one()) {
+              tc_commit(&kv_empty[vslot]);
+              if (j + 1 < nk) tc_commit(&kv_empty[kslot]);
+              if (j + 1 == nk - 1) tc_commit(q_empty);
+            }
+          }
+        }
+        ++qn;
+        base += 2 * nk;
+        done0 += w.steps[0];
+        done1 += w.steps[1];
+      }
+      if (limit == 1) {  // a wait ran out: MMAs in flight finish before the memory goes
+        unsigned more = kTileWaitLimit;
+        if (elect_one()) tc_commit(drained);
+        tile_wait(drained, 0, more);
+      }
+    } else if (warp == kTmaWarp + 2) {
+      // ---- items: the CTA's own, then those of CTAs that have not started.  Heavy items come first in a launch and the
+      // next is taken three steps before the present one ends, so the SMs finish together whatever the lengths are
+      // (taken at the present one's start, prompts of 2048 tokens at 64 dims ran 42 us instead of 31)
+      const int splits = item_splits<PAGED>(a);
+      int index = (int)blockIdx.x;
+      for (int k = 0;; ++k) {
+        TileWork w;
+        w.b = -1;
+        if (index >= 0) w = find_item<PAGED>(a, index, splits);
+        if (lane == 0) {
+          work[k & 1] = w;
+          mbar_arrive(&work_full[k & 1]);
+        }
+        if (w.b < 0 || limit == 1) break;
+        tile_wait2(&work_empty[k & 1], (k >> 1) & 1, ending, k & 1, limit);
+        if (limit == 1) break;
+        if (lane == 0) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the last reply has been read
+          mbar_arrive_expect_tx(replied, 16);
+          ask_next(smem_addr(reply), replied);
+        }
+        __syncwarp();
+        tile_wait(replied, k & 1, limit);
+        index = read_next(smem_addr(reply));
+        __syncwarp();
       }
     }
-    __syncwarp();
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax of tile i: this thread's row
     const int i = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
-    const int tok = tok0 + i * TPT + row / a.s.rep;
-    const bool valid = row < TPT * a.s.rep && tok < s.n;
-    const int lim = valid ? s.len - s.n + tok : -1;            // last key the row sees
-    const int first_lim = s.len - s.n + tok0 + i * TPT;        // the tile's first row's
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + S_COL + i * 128, o_at = tmem + lanes + O_COL + i * D,
                    p_at = tmem + lanes + P_COL + i * P_STEP;
     const float c = a.s.scale_log2;
-    float m = -INFINITY, base = 0.f, l = 0.f;  // maximum in use (raw score), m * c or 0, sum against it
-    const int my_steps = i == 0 ? steps[0] : steps[1];
-    bool s_here = false;
-    for (int j = 0; j < my_steps && ok; ++j) {
-      if (!s_here) ok = tile_wait_warp(&s_full[i], j & 1);
-      if (!ok) break;
-      tc_fence_after();
-      float x[128];
+    const int row_tok = row / a.s.rep, row_head = row - row_tok * a.s.rep;
+    int done = 0;  // steps of earlier items
+    for (int k = 0;; ++k) {
+      // (the item stays in work[k & 1] until this warp has asked for the next: read again for the output)
+      tile_wait(&work_full[k & 1], (k >> 1) & 1, limit);
+      const volatile TileWork& item = work[k & 1];
+      const int first = item.first, my_steps = item.b < 0 || limit == 1 ? -1 : item.steps[i];
+      const int first_tok = item.tok0 + i * TPT, hidden = item.len - item.n;
+      const bool valid = row < TPT * a.s.rep && first_tok + row_tok < item.n;
+      const int lim = valid ? hidden + first_tok + row_tok : -1;  // last key the row sees
+      const int first_lim = hidden + first_tok;                   // the tile's first row's
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&work_empty[k & 1]);
+      if (my_steps < 0) break;
+      float m = -INFINITY, base = 0.f, l = 0.f;  // maximum in use (raw score), m * c or 0, sum against it
+      bool s_here = false;
+      for (int j = 0; j < my_steps; ++j) {
+        if (!s_here) tile_wait(&s_full[i], (done + j) & 1, limit);
+        tc_fence_after();
+        float x[128];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) tmem_ld32(s_at + g * 32, x + g * 32);
+        for (int g = 0; g < 4; ++g) tmem_ld32(s_at + g * 32, x + g * 32);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) tmem_ld_wait(x + g * 32);
-      if constexpr (EARLY) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[i]);
-      }
-      // (asked here, used after the maximum: the answer takes a while)
-      const bool o_here = !EARLY || j == 0 || mbar_test_wait(&o_done[i], (j - 1) & 1);
-      const int key0 = j * kTileKeys;
-      if (key0 + kTileKeys - 1 > first_lim) {
-        const int rel = lim - key0;
-#pragma unroll
-        for (int e = 0; e < 128; ++e)
-          if (e > rel) x[e] = -INFINITY;
-      }
-      float mx[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-      for (int e = 4; e < 124; e += 8) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) mx[w] = max3(mx[w], x[e + w], x[e + 4 + w]);
-      }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) mx[w] = fmaxf(mx[w], x[124 + w]);
-      const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-      // (the difference is NaN for two infinities of one sign: no move)
-      if (__any_sync(0xffffffffu, (top - m) * c > kLazyLog2)) {
-        const float mn = fmaxf(m, top);
-        const float nb = mn == -INFINITY ? 0.f : mn * c;
-        const float f = exp2_fast(m * c - nb);
-        l = m == -INFINITY ? 0.f : l * f;
-        if (j > 0) {
-          ok = tile_wait_warp(&o_done[i], (j - 1) & 1);
-          if (!ok) break;
-          tc_fence_after();
-          const float fo = m == -INFINITY ? 0.f : f;
-#pragma unroll 1
-          for (int g = 0; g < D / 32; ++g) {
-            float o[32];
-            tmem_ld32(o_at + g * 32, o);
-            tmem_ld_wait(o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= fo;
-            tmem_st32(o_at + g * 32, o);
-          }
+        for (int g = 0; g < 4; ++g) tmem_ld_wait(x + g * 32);
+        if constexpr (EARLY) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[i]);
         }
-        m = mn;
-        base = nb;
+        // (asked here, used after the maximum: the answer takes a while)
+        const bool o_here = !EARLY || j == 0 || mbar_test_wait(&o_done[i], (done + j - 1) & 1);
+        const int key0 = (first + j) * kTileKeys;
+        if (key0 + kTileKeys - 1 > first_lim) {
+          const int rel = lim - key0;
+#pragma unroll
+          for (int e = 0; e < 128; ++e)
+            if (e > rel) x[e] = -INFINITY;
+        }
+        float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int e = 4; e < 124; e += 8) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) mx[v] = max3(mx[v], x[e + v], x[e + 4 + v]);
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v) mx[v] = fmaxf(mx[v], x[124 + v]);
+        const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+        // (the difference is NaN for two infinities of one sign: no move)
+        if (__any_sync(0xffffffffu, (top - m) * c > kLazyLog2)) {
+          const float mn = fmaxf(m, top);
+          const float nb = mn == -INFINITY ? 0.f : mn * c;
+          const float f = m == -INFINITY ? 0.f : exp2_fast(m * c - nb);
+          l = m == -INFINITY ? 0.f : l * f;
+          if (j > 0) {
+            tile_wait(&o_done[i], (done + j - 1) & 1, limit);
+            tc_fence_after();
+#pragma unroll 1
+            for (int g = 0; g < D / 32; ++g) {
+              float o[32];
+              tmem_ld32(o_at + g * 32, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= f;
+              tmem_st32(o_at + g * 32, o);
+            }
+          }
+          m = mn;
+          base = nb;
+        }
+        if constexpr (EARLY) {  // the last P_i V has read P_i
+          if (!__all_sync(0xffffffffu, o_here)) tile_wait(&o_done[i], (done + j - 1) & 1, limit);
+          tc_fence_after();
+        }
+        const uint64_t cc = pack2(c, c), nb2 = pack2(-base, -base);
+        uint64_t sum0 = 0, sum1 = 0;  // pairs of zeros
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int g = 2 * h; g < 2 * h + 2; ++g) {
+            uint32_t p[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float p0, p1;
+              const uint64_t t = fma2(pack2(x[g * 32 + 2 * e], x[g * 32 + 2 * e + 1]), cc, nb2);
+              if ((kPolyPairs >> e) & 1) {
+                exp2_pair(t, &p0, &p1);
+              } else {
+                unpack2(t, &p0, &p1);
+                p0 = exp2_fast(p0);
+                p1 = exp2_fast(p1);
+              }
+              uint64_t& sum = e & 1 ? sum1 : sum0;
+              sum = add2(sum, pack2(p0, p1));
+              p[e] = Type16<T>::pack(p0, p1);
+            }
+            tmem_st16(p_at + g * 16, p);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
+          if (h == 0) s_here = EARLY && j + 1 < my_steps && mbar_test_wait(&s_full[i], (done + j + 1) & 1);
+        }
+        s_here = __all_sync(0xffffffffu, s_here);
+        float s0, s1;
+        unpack2(add2(sum0, sum1), &s0, &s1);
+        l += s0 + s1;
       }
-      if constexpr (EARLY) {  // the last P_i V has read P_i
-        if (!__all_sync(0xffffffffu, o_here)) ok = tile_wait_warp(&o_done[i], (j - 1) & 1);
-        if (!ok) break;
+      // ---- the row's output, or its part of it
+      done += my_steps;
+      if (my_steps > 0) {
+        tile_wait(&o_done[i], (done - 1) & 1, limit);
         tc_fence_after();
       }
-      const uint64_t cc = pack2(c, c), nb2 = pack2(-base, -base);
-      uint64_t sum0 = 0, sum1 = 0;  // pairs of zeros
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int g = 2 * h; g < 2 * h + 2; ++g) {
-          uint32_t p[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float p0, p1;
-            const uint64_t t = fma2(pack2(x[g * 32 + 2 * e], x[g * 32 + 2 * e + 1]), cc, nb2);
-            if ((kPolyPairs >> e) & 1) {
-              exp2_pair(t, &p0, &p1);
-            } else {
-              unpack2(t, &p0, &p1);
-              p0 = exp2_fast(p0);
-              p1 = exp2_fast(p1);
-            }
-            uint64_t& sum = e & 1 ? sum1 : sum0;
-            sum = add2(sum, pack2(p0, p1));
-            p[e] = Type16<T>::pack(p0, p1);
-          }
-          tmem_st16(p_at + g * 16, p);
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
-        if (h == 0) s_here = EARLY && j + 1 < my_steps && mbar_test_wait(&s_full[i], (j + 1) & 1);
-      }
-      s_here = __all_sync(0xffffffffu, s_here);
-      float s0, s1;
-      unpack2(add2(sum0, sum1), &s0, &s1);
-      l += s0 + s1;
-    }
-    // ---- the row's output
-    if (my_steps > 0 && ok) {
-      ok = tile_wait_warp(&o_done[i], (my_steps - 1) & 1);
-      tc_fence_after();
-    }
-    if (ok) {
+      TileWork w;
+      w.b = item.b, w.kvh = item.kvh, w.start = item.start, w.n = item.n, w.len = item.len, w.tok0 = item.tok0;
+      w.first = first, w.part = item.part;
+      const int tok = first_tok + row_tok;
+      const bool whole = w.part < 0;
       const bool none = lim < 0;
       const float inv = 1.f / l;
-      uint16_t* out = a.s.out + (long long)(s.start + tok) * a.s.sot +
-                      (long long)(item.kvh * a.s.rep + row % a.s.rep) * a.s.soh;
+      uint16_t* out = a.s.out + (long long)(w.start + tok) * a.s.sot + (long long)(w.kvh * a.s.rep + row_head) * a.s.soh;
+      float* part = a.s.part + tile_part_floats(D) * (whole ? 0 : w.part) + (size_t)(i * kTileRows) * D;
       float odd = 0.f;  // becomes NaN with the first output that is not finite
       if (my_steps > 0) {
 #pragma unroll 1
@@ -637,42 +788,120 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tmem_ld_wait(o);
 #pragma unroll
           for (int e = 0; e < 32; ++e) odd = fmaf(o[e], 0.f, odd);
-          if (valid) {
+          if (!valid) continue;
+          if (whole) {
 #pragma unroll
             for (int v = 0; v < 4; ++v)
               if (g * 32 + v * 8 < a.s.hd) {
-                uint4 w;
-                w.x = Type16<T>::pack(o[v * 8] * inv, o[v * 8 + 1] * inv);
-                w.y = Type16<T>::pack(o[v * 8 + 2] * inv, o[v * 8 + 3] * inv);
-                w.z = Type16<T>::pack(o[v * 8 + 4] * inv, o[v * 8 + 5] * inv);
-                w.w = Type16<T>::pack(o[v * 8 + 6] * inv, o[v * 8 + 7] * inv);
-                *reinterpret_cast<uint4*>(out + g * 32 + v * 8) = none ? make_uint4(0, 0, 0, 0) : w;
+                uint4 u;
+                u.x = Type16<T>::pack(o[v * 8] * inv, o[v * 8 + 1] * inv);
+                u.y = Type16<T>::pack(o[v * 8 + 2] * inv, o[v * 8 + 3] * inv);
+                u.z = Type16<T>::pack(o[v * 8 + 4] * inv, o[v * 8 + 5] * inv);
+                u.w = Type16<T>::pack(o[v * 8 + 6] * inv, o[v * 8 + 7] * inv);
+                *reinterpret_cast<uint4*>(out + g * 32 + v * 8) = none ? make_uint4(0, 0, 0, 0) : u;
               }
+          } else {
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              *reinterpret_cast<float4*>(part + (size_t)row * D + g * 32 + v * 4) =
+                  make_float4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
           }
         }
-      } else if (valid) {
+      } else if (valid && whole) {
         for (int d = 0; d < a.s.hd; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
       }
-      unsigned again = __ballot_sync(0xffffffffu, valid && !none && isfinite(l) && !(odd == 0.f));
+      float2* ml = reinterpret_cast<float2*>(part + (size_t)(2 - i) * kTileRows * D) + i * kTileRows;
+      if (!whole && valid) ml[row] = m == -INFINITY ? make_float2(-INFINITY, l) : make_float2(base, l);
+      unsigned again = __ballot_sync(0xffffffffu, valid && !none && my_steps > 0 && isfinite(l) && !(odd == 0.f));
       while (again) {
         const int src = __ffs(again) - 1;
         again &= again - 1;
         const float mb = __shfl_sync(0xffffffffu, base, src), ll = __shfl_sync(0xffffffffu, l, src);
-        const int pr = (tok0 + i * TPT) * a.s.rep + (warp & 3) * 32 + src;
+        const int r = (warp & 3) * 32 + src;
+        const int pr = (w.tok0 + i * TPT) * a.s.rep + r;
+        const Seq s = {w.start, w.n, w.len};
         float o[D / 32];
-        redo_row<T, PAGED, D>(a.s, item.b, s, item.kvh, pr, 0, s.len, mb, o);
+        redo_row<T, PAGED, D>(a.s, w.b, s, w.kvh, pr, w.first * kTileKeys, min(w.len, (w.first + my_steps) * kTileKeys), mb, o);
         const int rt = pr / a.s.rep;
-        uint16_t* ro = a.s.out + (long long)(s.start + rt) * a.s.sot + (long long)(item.kvh * a.s.rep + pr % a.s.rep) * a.s.soh;
-        for (int e = 0; e < D / 32; ++e)
-          if (lane + 32 * e < a.s.hd) ro[lane + 32 * e] = Type16<T>::one(o[e] / ll);
+        uint16_t* ro = a.s.out + (long long)(w.start + rt) * a.s.sot + (long long)(w.kvh * a.s.rep + pr % a.s.rep) * a.s.soh;
+        for (int e = 0; e < D / 32; ++e) {
+          if (!whole) part[(size_t)r * D + lane + 32 * e] = o[e];
+          else if (lane + 32 * e < a.s.hd) ro[lane + 32 * e] = Type16<T>::one(o[e] / ll);
+        }
       }
+      __syncwarp();
     }
   }
+  if (limit == 1 && lane == 0) atomicOr(&g_tile_device_error, 256u);
   tc_fence_before();
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+  }
+}
+
+// Joins the ranges of keys of an item, 32 of its rows per CTA; returns at once where the launch did not split.
+template <typename T, int D, bool PAGED>
+__global__ void __launch_bounds__(256) tile_join_kernel(const __grid_constant__ TileArgs a) {
+  __shared__ TileWork s_work;
+  __shared__ int s_splits;
+  pdl_launch_dependents();
+  pdl_wait_primary();
+  if (threadIdx.x < 32) {
+    const int splits = item_splits<PAGED>(a);
+    TileWork w;
+    w.b = -1;
+    if (splits > 1) w = find_item<PAGED>(a, (int)blockIdx.x * splits, splits);
+    if (threadIdx.x == 0) {
+      s_work = w;
+      s_splits = splits;
+    }
+  }
+  __syncthreads();
+  const TileWork w = s_work;
+  if (w.b < 0) return;
+  const int splits = s_splits;
+  const int r = blockIdx.y * 32 + threadIdx.x / 8, i = r >> 7, row = r & 127;
+  constexpr int W = D / 8;
+  const int d0 = (threadIdx.x & 7) * W;
+  const int row_tok = row / a.s.rep, tok = w.tok0 + i * a.tokens_per_tile + row_tok;
+  if (row >= a.tokens_per_tile * a.s.rep || tok >= w.n || d0 >= a.s.hd) return;
+  const float* part = a.s.part + tile_part_floats(D) * ((size_t)blockIdx.x * splits);
+  float M = -INFINITY;
+  for (int p = 0; p < splits; ++p)
+    M = fmaxf(M, __ldcg(part + p * tile_part_floats(D) + (size_t)2 * kTileRows * D + r * 2));
+  float L = 0.f, o[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) o[e] = 0.f;
+  for (int p = 0; p < splits; ++p) {
+    const float* q = part + p * tile_part_floats(D);
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + (size_t)2 * kTileRows * D) + r);
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw no key: its outputs were not written
+    const float f = exp2_fast(ml.x - M);
+    L += f * ml.y;
+#pragma unroll
+    for (int e = 0; e < W; e += 4) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(q + (size_t)r * D + d0 + e));
+      o[e] += f * v.x;
+      o[e + 1] += f * v.y;
+      o[e + 2] += f * v.z;
+      o[e + 3] += f * v.w;
+    }
+  }
+  const bool none = w.len - w.n + tok < 0;
+  const float inv = 1.f / L;
+  uint16_t* out = a.s.out + (long long)(w.start + tok) * a.s.sot +
+                  (long long)(w.kvh * a.s.rep + row - row_tok * a.s.rep) * a.s.soh + d0;
+#pragma unroll
+  for (int e = 0; e < W; e += 8) {
+    if (d0 + e >= a.s.hd) break;
+    uint4 u;
+    u.x = Type16<T>::pack(o[e] * inv, o[e + 1] * inv);
+    u.y = Type16<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
+    u.z = Type16<T>::pack(o[e + 4] * inv, o[e + 5] * inv);
+    u.w = Type16<T>::pack(o[e + 6] * inv, o[e + 7] * inv);
+    *reinterpret_cast<uint4*>(out + e) = none ? make_uint4(0, 0, 0, 0) : u;
   }
 }
 
@@ -740,8 +969,24 @@ static int launch_tile(const TileArgs& a, const CUtensorMap& q, const CUtensorMa
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, tile_attention_kernel<T, D, PAGED>, a, q, k, v),
-                    "attention: kernel launch");
+  int rc = check_cuda(cudaLaunchKernelEx(&cfg, tile_attention_kernel<T, D, PAGED>, a, q, k, v),
+                      "attention: kernel launch");
+  if (rc != LI4_OK || a.part_slots == 0) return rc;
+  cfg.gridDim = dim3((unsigned)a.part_slots / 2, 2 * kTileRows / 32, 1);  // (a split item has two parts at least)
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.dynamicSmemBytes = 0;
+  return check_cuda(cudaLaunchKernelEx(&cfg, tile_join_kernel<T, D, PAGED>, a), "attention: kernel launch");
+}
+
+// Items whose partial results the workspace has room for: two per SM, where the pairs of tiles that the tokens alone
+// make do not fill the SMs and some sequence may have enough keys to cut.
+static int tile_part_slots(int rep, int64_t tokens, int64_t kv_heads, int64_t max_keys, int sm) {
+  const int64_t pairs = tokens / (2 * (kTileRows / rep));
+  return pairs * kv_heads >= sm || max_keys <= kTileMinSteps * kTileKeys ? 0 : 2 * sm;
+}
+size_t tile_attention_part_bytes(int hd, int rep, int64_t tokens, int64_t kv_heads, int64_t max_keys, int sm) {
+  return (size_t)tile_part_slots(rep, tokens, kv_heads, max_keys, sm) * tile_part_floats(hd <= 64 ? 64 : 128) *
+         sizeof(float);
 }
 
 int launch_tile_attention(const SeqAttnArgs& args, bool paged, int dtype, cudaStream_t stream) {
@@ -760,8 +1005,11 @@ int launch_tile_attention(const SeqAttnArgs& args, bool paged, int dtype, cudaSt
   if (rc == LI4_OK)
     rc = make_map(&v, dtype, args.v, args.hd, y, args.svt, args.Hkv, args.svh, w, args.svp, a.box_rows, 1);
   if (rc != LI4_OK) return rc;
+  const int sm = current_sm_count();
+  a.part_slots = tile_part_slots(rep, args.T, args.Hkv, args.max_keys, sm);
   const int64_t pairs = args.T / (2 * a.tokens_per_tile) + args.B;  // at least the sequences' pairs of tiles
-  const int64_t grid = pairs * args.Hkv;
+  int64_t grid = pairs * args.Hkv;
+  if (grid < a.part_slots) grid = a.part_slots;
   if (grid > 0x7fffffff) return set_error(LI4_ERR_UNSUPPORTED, "attention: too many items");
   const unsigned g = (unsigned)grid;
   const bool half = dtype == LI4_F16;
