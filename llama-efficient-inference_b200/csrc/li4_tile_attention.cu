@@ -53,10 +53,9 @@ __host__ __device__ constexpr int tile_slots(int D) { return D == 64 ? 8 : 4; }
 __host__ __device__ constexpr int tile_bytes(int D) { return 128 * D * 2; }  // a tile of queries, keys or values
 __host__ __device__ constexpr int tile_smem_bytes(int D) { return 1024 + (2 + tile_slots(D)) * tile_bytes(D) + 512; }
 
-#ifndef POLY
-#define POLY 0x8888
-#endif
-constexpr unsigned kPolyPairs = POLY;  // which of 16 pairs of probabilities the polynomial takes
+// Which of 16 pairs of probabilities the polynomial takes (8192 tokens at 64 dims: none 387 us, 2 378 us, 4 360 us,
+// 5 370 us; at 128 dims, where the products and the power limit bound, 459, 456, 460, 466 us).
+constexpr unsigned kPolyPairs = 0x8888;
 
 struct TileArgs {
   SeqAttnArgs s;
@@ -558,10 +557,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if constexpr (EARLY) {
             // the next scores of both tiles, then the step's P V of each
             if (j + 1 < nk) {
+              tile_wait(full(kn), phase(kn), limit);
               if (more0 && more1) tile_wait2(&s_free[0], (done0 + j) & 1, &s_free[1], (done1 + j) & 1, limit);
               else if (more0) tile_wait(&s_free[0], (done0 + j) & 1, limit);
               else tile_wait(&s_free[1], (done1 + j) & 1, limit);
-              tile_wait(full(kn), phase(kn), limit);
               tc_fence_after();
               if (elect_one()) {
                 if (more0) scores(0, kslot);
@@ -580,9 +579,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                   outputs(i, vslot, 0, j == 0, groups);
                   outputs(i, vslot, 1, j == 0, groups);
                   tc_commit(&o_done[i]);
+                  if (i == 1 || j >= w.steps[1]) tc_commit(&kv_empty[vslot]);
                 }
               }
-            if (elect_one()) tc_commit(&kv_empty[vslot]);
           } else {
             // each tile's P V, as its halves come, then its next scores
 #pragma unroll
@@ -599,14 +598,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if (elect_one()) {
                   outputs(i, vslot, 1, j == 0, groups);
                   tc_commit(&o_done[i]);
+                  if (i == 1 || j >= w.steps[1]) tc_commit(&kv_empty[vslot]);
                   if (more) scores(i, kslot);
+                  if (more && (i == 1 || !more1)) {
+                    tc_commit(&kv_empty[kslot]);
+                    if (j + 1 == nk - 1) tc_commit(q_empty);
+                  }
                 }
               }
-            if (elect_one()) {
-              tc_commit(&kv_empty[vslot]);
-              if (j + 1 < nk) tc_commit(&kv_empty[kslot]);
-              if (j + 1 == nk - 1) tc_commit(q_empty);
-            }
           }
         }
         ++qn;
@@ -622,7 +621,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     } else if (warp == kTmaWarp + 2) {
       // ---- items: the CTA's own, then those of CTAs that have not started.  Heavy items come first in a launch and the
       // next is taken three steps before the present one ends, so the SMs finish together whatever the lengths are
-      // (taken at the present one's start, prompts of 2048 tokens at 64 dims ran 42 us instead of 31)
+      // (taken at the present one's start, a prompt of 2048 tokens at 64 dims ran 42 us instead of 33)
       const int splits = item_splits<PAGED>(a);
       int index = (int)blockIdx.x;
       for (int k = 0;; ++k) {
@@ -685,8 +684,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_free[i]);
         }
-        // (asked here, used after the maximum: the answer takes a while)
-        const bool o_here = !EARLY || j == 0 || mbar_test_wait(&o_done[i], (done + j - 1) & 1);
         const int key0 = (first + j) * kTileKeys;
         if (key0 + kTileKeys - 1 > first_lim) {
           const int rel = lim - key0;
@@ -702,6 +699,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
 #pragma unroll
         for (int v = 0; v < 4; ++v) mx[v] = fmaxf(mx[v], x[124 + v]);
+        // (asked here, used a little later: the answer takes a while)
+        const bool o_here = !EARLY || j == 0 || mbar_test_wait(&o_done[i], (done + j - 1) & 1);
         const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
         // (the difference is NaN for two infinities of one sign: no move)
         if (__any_sync(0xffffffffu, (top - m) * c > kLazyLog2)) {
@@ -752,12 +751,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               p[e] = Type16<T>::pack(p0, p1);
             }
             tmem_st16(p_at + g * 16, p);
+            if (g == 2) s_here = EARLY && j + 1 < my_steps && mbar_test_wait(&s_full[i], (done + j + 1) & 1);
           }
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
-          if (h == 0) s_here = EARLY && j + 1 < my_steps && mbar_test_wait(&s_full[i], (done + j + 1) & 1);
         }
         s_here = __all_sync(0xffffffffu, s_here);
         float s0, s1;
