@@ -2,16 +2,19 @@
 //
 // Grouped-query attention by rows: the rep query heads of a KV head, over the queries of a sequence,
 // are the rows of one matrix (row = query * rep + head), so a KV head's keys and values are read once
-// for the whole group.  An item is (sequence, tile of 16 MT rows, KV head); its keys come in units of
+// for the whole group.  An item is (sequence, tile of 8 NT rows, KV head); its keys come in units of
 // 128.  Units of all items lie on one line; CTA g of G takes the g-th equal share of it, whatever the
 // lengths are (they are read on the device: the host knows none).  A CTA that covers only a part of an
 // item's keys leaves (running maximum, sum, unnormalised output) in `part`, and a second launch joins
 // the parts in key order, so the result does not depend on timing.
 //
 // Inside a CTA each of the 4 warps streams its own 32 keys of every unit through its own ring of
-// shared-memory stages (cp.async; no CTA barrier until the end): S = Q K^T and O += P V as m16n8k16
-// tensor-core tiles, softmax in fp32 in registers with the running maximum and sum of one pass.  The
-// work is bound by the bytes of the keys and values as long as the rows are few.
+// shared-memory stages (cp.async; no CTA barrier until the end): S^T = K Q^T and O^T += V^T P^T as
+// m16n8k16 tensor-core tiles, softmax in fp32 in registers with the running maximum and sum of one
+// pass.  The keys are the 16-wide side and the rows the 8-wide one, so a group of 4 or 8 heads wastes
+// half of a tile or nothing (rows as the 16-wide side: 985 instead of NEWCOUNT instructions per 32 keys of a
+// warp, 64 requests of 300-16000 tokens 85 us instead of NEWTIME).  The work is bound by the bytes of the keys
+// and values as long as the rows are few.
 #include <mutex>
 #include <utility>
 #include <vector>
@@ -28,8 +31,8 @@ constexpr int kSeqStages = 3;   // stages of 32 keys per warp
 
 __host__ __device__ constexpr int seq_stage_bytes(int D) { return 2 * 32 * D * 2; }
 __host__ __device__ constexpr int seq_smem_bytes(int D) { return kSeqWarps * kSeqStages * seq_stage_bytes(D); }
-// floats of one partial result: 16 MT rows of D outputs, then (maximum, sum) per row
-__host__ __device__ constexpr int seq_part_floats(int D, int MT) { return 16 * MT * (D + 2); }
+// floats of one partial result: 8 NT rows of D outputs, then (maximum, sum) per row
+__host__ __device__ constexpr int seq_part_floats(int D, int NT) { return 8 * NT * (D + 2); }
 
 // The line of units.
 struct Line {
@@ -38,16 +41,16 @@ struct Line {
 };
 __device__ __forceinline__ long long share(const Line& l, int g) { return l.total * g / l.active; }
 
-template <int MT>
+template <int NT>
 __device__ __forceinline__ long long seq_units(const SeqAttnArgs& a, const Seq& s, int* tiles, int* per) {
-  *tiles = (int)(((long long)s.n * a.rep + 16 * MT - 1) / (16 * MT));
+  *tiles = (int)(((long long)s.n * a.rep + 8 * NT - 1) / (8 * NT));
   *per = max(1, (s.len + kUnit - 1) / kUnit);
   return (long long)*tiles * *per * a.Hkv;
 }
 
 // Finds the sequence that holds unit share(g): each thread sums a slice of the sequences.  Every thread
 // returns the line, the sequence and the units before it (b = -1: no share).
-template <int MT, bool PAGED>
+template <int NT, bool PAGED>
 __device__ Line find_share(const SeqAttnArgs& a, int g, int* b_out, long long* before) {
   __shared__ long long s_sum[kSeqWarps];
   __shared__ int s_b;
@@ -57,7 +60,7 @@ __device__ Line find_share(const SeqAttnArgs& a, int g, int* b_out, long long* b
   const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
   long long mine = 0;
   int tiles, units;
-  for (int b = b0; b < b1; ++b) mine += seq_units<MT>(a, load_seq<PAGED>(a, b), &tiles, &units);
+  for (int b = b0; b < b1; ++b) mine += seq_units<NT>(a, load_seq<PAGED>(a, b), &tiles, &units);
   long long incl = mine;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -81,7 +84,7 @@ __device__ Line find_share(const SeqAttnArgs& a, int g, int* b_out, long long* b
     long long excl = incl - mine;
     if (at >= excl && at < incl) {
       for (int b = b0; b < b1; ++b) {
-        const long long u = seq_units<MT>(a, load_seq<PAGED>(a, b), &tiles, &units);
+        const long long u = seq_units<NT>(a, load_seq<PAGED>(a, b), &tiles, &units);
         if (at < excl + u) {
           s_b = b;
           s_before = excl;
@@ -129,37 +132,66 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float c[4], const uint32
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 32 keys from j0 of the item into a stage: K rows then V rows, 16-byte chunk c of row r at c ^ (r & 7).
-// Rows at or past `end` and rows of no page are zeros.
-template <int D, bool PAGED>
-__device__ __forceinline__ void load_stage(const SeqAttnArgs& a, int b, const Seq& s, int kvh, int j0, int end,
-                                           uint32_t stage) {
-  constexpr int CH = D / 8;          // chunks per row
-  constexpr int RPI = 32 / CH;       // rows per instruction of the warp
-  const int lane = threadIdx.x & 31;
-  long long ko = 0, vo = 0;
-  bool have = false;
-  if (j0 + lane < end) have = key_offsets<PAGED>(a, b, s, j0 + lane, &ko, &vo);
-  const int c = lane % CH;
-  const bool in_head = c * 8 < a.hd;
-  const uint16_t* k = a.k + (long long)kvh * a.skh + c * 8;
-  const uint16_t* v = a.v + (long long)kvh * a.svh + c * 8;
+// 8x8 values of 16 bits across the warp, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+// The pages of 32 keys from j0, 8 keys each (a page has 8 rows at least and j0 is a multiple of 32, so 8 keys share one);
+// asked for a stage ahead of their copy, as the block table's answer takes a trip to L2.  -1: past the end.
+struct KeyPages {
+  int page[4];
+};
+template <bool PAGED>
+__device__ __forceinline__ KeyPages key_pages(const SeqAttnArgs& a, int b, int j0, int end) {
+  KeyPages k;
 #pragma unroll
-  for (int i = 0; i < 32 / RPI; ++i) {
-    const int r = i * RPI + lane / CH;
-    const long long kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
-    const bool ok = __shfl_sync(0xffffffffu, (int)have, r) && in_head;
-    const uint32_t at = stage + r * (D * 2) + ((c ^ (r & 7)) << 4);
-    cp_async16z(at, ok ? k + kr : a.q, ok);  // (not read where !ok)
-    cp_async16z(at + 32 * D * 2, ok ? v + vr : a.q, ok);
+  for (int q = 0; q < 4; ++q) {
+    k.page[q] = -1;
+    if (j0 + 8 * q < end)
+      k.page[q] = PAGED ? a.tables[(long long)b * a.table_stride + ((j0 + 8 * q) >> a.log_page)] : 0;
+  }
+  return k;
+}
+
+// 32 keys of the item into a stage: K rows then V rows, 16-byte chunk c of row r at c ^ (r & 7).  Rows past the end and
+// rows of no page are zeros.
+template <int D, bool PAGED>
+__device__ __forceinline__ void load_stage(const SeqAttnArgs& a, const KeyPages& kp, const Seq& s, int kvh, int j0, int end,
+                                           uint32_t stage) {
+  constexpr int CH = D / 8;           // chunks per row
+  constexpr int RPI = 32 / CH;        // rows per instruction of the warp
+  const int lane = threadIdx.x & 31;
+  const int c = lane % CH, r0 = lane / CH;
+  const bool in_head = c * 8 < a.hd;
+  const uint16_t* k = a.k + (long long)kvh * a.skh + (long long)r0 * a.skt + c * 8;
+  const uint16_t* v = a.v + (long long)kvh * a.svh + (long long)r0 * a.svt + c * 8;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int row = PAGED ? (j0 + 8 * q) & ((1 << a.log_page) - 1) : s.start + j0 + 8 * q;
+    const long long page = PAGED ? kp.page[q] : 0;
+    const bool have = (PAGED ? (unsigned)kp.page[q] < (unsigned)a.num_pages : kp.page[q] == 0) && in_head;
+    const uint16_t* kq = k + page * a.skp + (long long)row * a.skt;
+    const uint16_t* vq = v + page * a.svp + (long long)row * a.svt;
+#pragma unroll
+    for (int i = 0; i < 8 / RPI; ++i) {
+      const int r = q * 8 + i * RPI + r0;
+      const bool ok = have && j0 + r < end;
+      const uint32_t at = stage + r * (D * 2) + ((c ^ (r & 7)) << 4);
+      cp_async16z(at, ok ? kq + (long long)(i * RPI) * a.skt : a.q, ok);  // (not read where !ok)
+      cp_async16z(at + 32 * D * 2, ok ? vq + (long long)(i * RPI) * a.svt : a.q, ok);
+    }
   }
 }
 
-template <typename T, int D, int MT, bool PAGED>
+template <typename T, int D, int NT, bool PAGED>
 __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid_constant__ SeqAttnArgs a) {
-  constexpr int RT = 16 * MT;
-  constexpr int KS = D / 16;  // k steps of Q K^T
-  constexpr int NT = D / 8;   // column tiles of the output
+  constexpr int RT = 8 * NT;
+  constexpr int KS = D / 16;  // k steps of K Q^T
+  constexpr int DT = D / 16;  // 16-dim tiles of the output
+  constexpr int LD = D + 8;   // floats per row of the warps' outputs in shared memory
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ float s_ml[kSeqWarps][RT][2];
   __shared__ int s_redo[RT];
@@ -171,14 +203,14 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
   int b;
   long long before;
   const int g = blockIdx.x;
-  const Line line = find_share<MT, PAGED>(a, g, &b, &before);
+  const Line line = find_share<NT, PAGED>(a, g, &b, &before);
   if (b < 0) return;
   const long long at0 = share(line, g);
   long long left = share(line, g + 1) - at0;
   long long rem = at0 - before;  // units into sequence b
   Seq s = load_seq<PAGED>(a, b);
   int tiles, per;
-  seq_units<MT>(a, s, &tiles, &per);
+  seq_units<NT>(a, s, &tiles, &per);
 
   while (left > 0) {
     const int item = (int)(rem / per), u0 = (int)(rem - (long long)item * per);
@@ -190,160 +222,175 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
     const int last_lim = s.len - s.n + (row0 + rows - 1) / a.rep;   // and its last query
     const int k0 = u0 * kUnit, k1 = min(min(u1 * kUnit, s.len), last_lim + 1);
 
-    // ---- queries as A fragments; rows past the tile are zero rows that see no key
-    uint32_t qf[MT][KS][4];
-    int lim[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int r = mt * 16 + hf * 8 + lane / 4;
-        const bool valid = r < rows;
-        const int pr = row0 + (valid ? r : 0);
-        const int tok = pr / a.rep;
-        lim[mt][hf] = valid ? s.len - s.n + tok : -1;
-        const uint16_t* q = a.q + (long long)(s.start + tok) * a.sqt + (long long)(kvh * a.rep + pr - tok * a.rep) * a.sqh;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int d = ks * 16 + c * 8 + (lane & 3) * 2;
-            qf[mt][ks][hf + 2 * c] = valid && d < a.hd ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
-          }
-      }
-    float o[MT][NT][4];
-    float m[MT][2], l[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
-      m[mt][0] = m[mt][1] = -INFINITY;
-      l[mt][0] = l[mt][1] = 0.f;
-    }
-
-    // ---- the warp's keys: k0 + 32 warp + 128 i
+    // ---- the warp's keys: k0 + 32 warp + 128 i, their first stages under way
     const int w0 = k0 + warp * 32;
     const int steps = w0 < k1 ? (k1 - w0 + kUnit - 1) / kUnit : 0;
+    KeyPages pages[kSeqStages];
+#pragma unroll
+    for (int i = 0; i < kSeqStages; ++i) pages[i] = key_pages<PAGED>(a, b, w0 + i * kUnit, k1);
 #pragma unroll
     for (int i = 0; i < kSeqStages - 1; ++i) {
-      if (i < steps) load_stage<D, PAGED>(a, b, s, kvh, w0 + i * kUnit, k1, ring + i * seq_stage_bytes(D));
+      if (i < steps) load_stage<D, PAGED>(a, pages[i], s, kvh, w0 + i * kUnit, k1, ring + i * seq_stage_bytes(D));
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    KeyPages next_pages = pages[kSeqStages - 1];
+
+    // ---- queries as B fragments (n = row, k = dim); rows past the tile are zero rows
+    uint32_t qf[NT][KS][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + lane / 4;
+      const bool valid = r < rows;
+      const int pr = row0 + (valid ? r : 0), tok = pr / a.rep;
+      const uint16_t* q = a.q + (long long)(s.start + tok) * a.sqt + (long long)(kvh * a.rep + pr - tok * a.rep) * a.sqh;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int d = ks * 16 + c * 8 + (lane & 3) * 2;
+          qf[nt][ks][c] = valid && d < a.hd ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
+        }
+    }
+    // ---- this thread's rows of the scores and outputs: nt * 8 + (lane & 3) * 2 + {0, 1}
+    int lim[NT][2];
+    float o[DT][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = nt * 8 + (lane & 3) * 2 + e;
+        lim[nt][e] = r < rows ? s.len - s.n + (row0 + r) / a.rep : -1;
+        m[nt][e] = -INFINITY;
+        l[nt][e] = 0.f;
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt][nt][0] = o[dt][nt][1] = o[dt][nt][2] = o[dt][nt][3] = 0.f;
+    }
+
     int slot = 0;
     for (int i = 0; i < steps; ++i) {
       const int ahead = i + kSeqStages - 1;
       int next = slot + kSeqStages - 1;
       if (next >= kSeqStages) next -= kSeqStages;
       __syncwarp();
-      if (ahead < steps) load_stage<D, PAGED>(a, b, s, kvh, w0 + ahead * kUnit, k1, ring + next * seq_stage_bytes(D));
+      if (ahead < steps)
+        load_stage<D, PAGED>(a, next_pages, s, kvh, w0 + ahead * kUnit, k1, ring + next * seq_stage_bytes(D));
       asm volatile("cp.async.commit_group;" ::: "memory");
+      next_pages = key_pages<PAGED>(a, b, w0 + (ahead + 1) * kUnit, k1);
       asm volatile("cp.async.wait_group %0;" ::"n"(kSeqStages - 1) : "memory");
       __syncwarp();
       const uint32_t ks_at = ring + slot * seq_stage_bytes(D), vs_at = ks_at + 32 * D * 2;
       const int j0 = w0 + i * kUnit;
       slot = slot + 1 == kSeqStages ? 0 : slot + 1;
 
-      float sc[MT][4][4];
+      // S^T: 32 keys x 8 NT rows
+      float sc[2][NT][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-        for (int ks2 = 0; ks2 < KS / 2; ++ks2) {  // 8 keys x 32 dims: four 8x8 matrices
+        for (int ks = 0; ks < KS; ++ks) {  // 16 keys x 16 dims: four 8x8 matrices
           uint32_t kf[4];
-          const int r = nt * 8 + (lane & 7), c = ks2 * 4 + (lane >> 3);
+          const int r = mt * 16 + (lane & 15), c = ks * 2 + (lane >> 4);
           ldmatrix_x4(kf, ks_at + r * (D * 2) + ((c ^ (r & 7)) << 4));
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma16816<T>(sc[mt][nt], qf[mt][ks2 * 2], kf[0], kf[1]);
-            mma16816<T>(sc[mt][nt], qf[mt][ks2 * 2 + 1], kf[2], kf[3]);
-          }
-        }
-      const bool mask = j0 + 31 > first_lim || rows < RT || j0 + 32 > k1;
-      uint32_t pf[MT][2][4];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = sc[mt][nt][e] * a.scale_log2;
-            const int j = j0 + nt * 8 + (lane & 3) * 2 + (e & 1);
-            if (mask && (j > lim[mt][e >> 1] || j >= k1)) x = -INFINITY;
-            sc[mt][nt][e] = x;
-            mx[e >> 1] = fmaxf(mx[e >> 1], x);
-          }
-        float base[2];
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
-          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
-          const float mn = fmaxf(m[mt][hf], mx[hf]);
-          base[hf] = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every probability is exp2(-inf) = 0
-          const float keep = exp2_fast(m[mt][hf] - base[hf]);
-          m[mt][hf] = mn;
-          l[mt][hf] *= keep;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            o[mt][nt][hf * 2] *= keep;
-            o[mt][nt][hf * 2 + 1] *= keep;
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            sc[mt][nt][e] = exp2_fast(sc[mt][nt][e] - base[e >> 1]);
-            l[mt][e >> 1] += sc[mt][nt][e];
-          }
-          pf[mt][nt >> 1][(nt & 1) * 2] = Type16<T>::pack(sc[mt][nt][0], sc[mt][nt][1]);
-          pf[mt][nt >> 1][(nt & 1) * 2 + 1] = Type16<T>::pack(sc[mt][nt][2], sc[mt][nt][3]);
+          for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[mt][nt], kf, qf[nt][ks][0], qf[nt][ks][1]);
         }
       }
+      if (j0 + 31 > first_lim || j0 + 32 > k1) {  // some key of the 32 is hidden from some row
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)  // 16 keys x 16 dims: four transposed 8x8 matrices
+        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) {
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = j0 + mt * 16 + (e >> 1) * 8 + lane / 4;
+              sc[mt][nt][e] = j > lim[nt][e & 1] || j >= k1 ? -INFINITY : sc[mt][nt][e] * a.scale_log2;
+            }
+      } else {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[mt][nt][e] *= a.scale_log2;
+      }
+      uint32_t pf[2][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float base[2], keep[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float mn = fmaxf(m[nt][e], mx);
+          base[e] = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every probability is exp2(-inf) = 0
+          keep[e] = exp2_fast(m[nt][e] - base[e]);
+          m[nt][e] = mn;
+          l[nt][e] *= keep[e];
+        }
+        if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[dt][nt][e] *= keep[e & 1];
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[mt][nt][e] = exp2_fast(sc[mt][nt][e] - base[e & 1]);
+            l[nt][e & 1] += sc[mt][nt][e];
+          }
+          // [key][row] as the scores lie -> [row][key] as a B fragment wants it
+          pf[mt][nt][0] = transpose8(Type16<T>::pack(sc[mt][nt][0], sc[mt][nt][1]));
+          pf[mt][nt][1] = transpose8(Type16<T>::pack(sc[mt][nt][2], sc[mt][nt][3]));
+        }
+      }
+      // O^T += V^T P^T: 16 dims x 16 keys by four transposed 8x8 matrices
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
           uint32_t vf[4];
-          const int r = kb * 16 + (lane & 15), c = dt * 2 + (lane >> 4);
+          const int r = mt * 16 + (lane >> 4) * 8 + (lane & 7), c = dt * 2 + ((lane >> 3) & 1);
           ldmatrix_x4_trans(vf, vs_at + r * (D * 2) + ((c ^ (r & 7)) << 4));
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma16816<T>(o[mt][dt * 2], pf[mt][kb], vf[0], vf[1]);
-            mma16816<T>(o[mt][dt * 2 + 1], pf[mt][kb], vf[2], vf[3]);
-          }
+          for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[dt][nt], vf, pf[mt][nt][0], pf[mt][nt][1]);
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();  // every warp is done with its ring: the outputs may use it
 
     // ---- join the four warps
-    float* so = reinterpret_cast<float*>(smem) + warp * RT * D;
+    float* so = reinterpret_cast<float*>(smem) + warp * RT * LD;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int r = mt * 16 + hf * 8 + lane / 4;
-        float sum = l[mt][hf];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if ((lane & 3) == 0) {
-          s_ml[warp][r][0] = m[mt][hf];
+      for (int e = 0; e < 2; ++e) {
+        const int r = nt * 8 + (lane & 3) * 2 + e;
+        float sum = l[nt][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (lane < 4) {
+          s_ml[warp][r][0] = m[nt][e];
           s_ml[warp][r][1] = sum;
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          *reinterpret_cast<float2*>(so + r * D + nt * 8 + (lane & 3) * 2) =
-              make_float2(o[mt][nt][hf * 2], o[mt][nt][hf * 2 + 1]);
+        for (int dt = 0; dt < DT; ++dt) {
+          so[r * LD + dt * 16 + lane / 4] = o[dt][nt][e];
+          so[r * LD + dt * 16 + 8 + lane / 4] = o[dt][nt][e + 2];
+        }
       }
     if (tid < RT) s_redo[tid] = 0;
     __syncthreads();
     const bool whole = u0 == 0 && u1 == per;
     const bool masked = k1 - 1 > first_lim;  // some row must not see some of the keys read
-    float* part = a.part + (size_t)(2 * g + (u0 == 0 ? 1 : 0)) * seq_part_floats(D, MT);
+    float* part = a.part + (size_t)(2 * g + (u0 == 0 ? 1 : 0)) * seq_part_floats(D, NT);
     const float* all = reinterpret_cast<const float*>(smem);
     for (int e = tid; e < RT * D / 2; e += kSeqThreads) {
       const int r = e / (D / 2), d = (e - r * (D / 2)) * 2;
@@ -355,7 +402,7 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
 #pragma unroll
       for (int w = 0; w < kSeqWarps; ++w) {
         const float f = exp2_fast(s_ml[w][r][0] - base);
-        const float2 ov = *reinterpret_cast<const float2*>(all + (w * RT + r) * D + d);
+        const float2 ov = *reinterpret_cast<const float2*>(all + (w * RT + r) * LD + d);
         L += f * s_ml[w][r][1];
         x += f * ov.x;
         y += f * ov.y;
@@ -402,69 +449,83 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
     while (left > 0 && rem >= (long long)tiles * per * a.Hkv) {
       rem -= (long long)tiles * per * a.Hkv;
       s = load_seq<PAGED>(a, ++b);
-      seq_units<MT>(a, s, &tiles, &per);
+      seq_units<NT>(a, s, &tiles, &per);
     }
   }
 }
 
 // Joins the parts of the item that the boundary between CTAs blockIdx.x and blockIdx.x + 1 cuts, if it is the
-// first boundary inside that item.
-template <typename T, int D, int MT, bool PAGED>
+// first boundary inside that item; blockIdx.y takes a share of its outputs.  The parts' weights come first, all loads in
+// flight together, then the outputs.
+constexpr int kJoinShares = 4;
+template <typename T, int D, int NT, bool PAGED>
 __global__ void __launch_bounds__(kSeqThreads) seq_attention_join_kernel(const __grid_constant__ SeqAttnArgs a) {
-  constexpr int RT = 16 * MT;
+  constexpr int RT = 8 * NT;
+  extern __shared__ float s_w[];  // [parts][RT] weight of a part in a row's output
   pdl_launch_dependents();
   pdl_wait_primary();
   const int g = blockIdx.x + 1;
   int b;
   long long before;
-  const Line line = find_share<MT, PAGED>(a, g, &b, &before);
+  const Line line = find_share<NT, PAGED>(a, g, &b, &before);
   if (b < 0) return;
   const Seq s = load_seq<PAGED>(a, b);
   int tiles, per;
-  seq_units<MT>(a, s, &tiles, &per);
+  seq_units<NT>(a, s, &tiles, &per);
   const long long rem = share(line, g) - before;
   const int item = (int)(rem / per);
   const long long start = before + (long long)item * per, end = start + per;
   if (start == share(line, g) || share(line, g - 1) > start) return;
-  int last = g;  // the parts are CTAs g - 1 (from the item's start) and g .. last
-  while (last + 1 < line.active && share(line, last + 1) < end) ++last;
+  // the parts are CTAs g - 1 (from the item's start) and g .. last, the last CTA with share(last) < end
+  const int last = (int)min((long long)line.active - 1, (end * line.active - 1) / line.total);
   const int kvh = item % a.Hkv, row0 = item / a.Hkv * RT;
   const int rows = min(RT, s.n * a.rep - row0);
-  const float* first = a.part + (size_t)(2 * (g - 1) + 1) * seq_part_floats(D, MT);
-  const float* rest = a.part + (size_t)(2 * g) * seq_part_floats(D, MT);
-  const size_t step = 2 * (size_t)seq_part_floats(D, MT);
-  const int n = last - g + 1;
-  for (int e = threadIdx.x; e < rows * (D / 2); e += kSeqThreads) {
-    const int r = e / (D / 2), d = (e - r * (D / 2)) * 2;
-    const float2 ml0 = __ldcg(reinterpret_cast<const float2*>(first + RT * D + r * 2));
-    float M = ml0.x;
-    for (int i = 0; i < n; ++i) M = fmaxf(M, __ldcg(rest + i * step + RT * D + r * 2));
+  const float* first = a.part + (size_t)(2 * (g - 1) + 1) * seq_part_floats(D, NT);
+  const float* rest = a.part + (size_t)(2 * g) * seq_part_floats(D, NT);
+  const size_t step = 2 * (size_t)seq_part_floats(D, NT);
+  const int n = last - g + 2;
+  auto part = [&](int i) { return i == 0 ? first : rest + (i - 1) * step; };
+  // row r by lanes: the largest maximum, then every part's exp2(maximum - largest) / sum
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = warp; r < rows; r += kSeqWarps) {
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(part(i) + RT * D + r * 2));
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
     const float base = M == -INFINITY ? 0.f : M;
-    float f = exp2_fast(ml0.x - base);
-    const float2 o0 = __ldcg(reinterpret_cast<const float2*>(first + r * D + d));
-    float L = f * ml0.y, x = f * o0.x, y = f * o0.y;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(rest + i * step + RT * D + r * 2));
-      const float2 o = __ldcg(reinterpret_cast<const float2*>(rest + i * step + r * D + d));
-      f = exp2_fast(ml.x - base);
+    float L = 0.f;
+    for (int i = lane; i < n; i += 32) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(part(i) + RT * D + r * 2));
+      const float f = exp2_fast(ml.x - base);
+      s_w[i * RT + r] = f;
       L += f * ml.y;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) L += __shfl_xor_sync(0xffffffffu, L, d);
+    for (int i = lane; i < n; i += 32) s_w[i * RT + r] *= 1.f / L;
+  }
+  __syncthreads();
+  for (int e = blockIdx.y * kSeqThreads + threadIdx.x; e < rows * (D / 2); e += kSeqThreads * kJoinShares) {
+    const int r = e / (D / 2), d = (e - r * (D / 2)) * 2;
+    float x = 0.f, y = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float2 o = __ldcg(reinterpret_cast<const float2*>(part(i) + r * D + d));
+      const float f = s_w[i * RT + r];
       x += f * o.x;
       y += f * o.y;
     }
     const int pr = row0 + r, tok = pr / a.rep;
-    const bool none = s.len - s.n + tok < 0;
-    const float inv = 1.f / L;
     if (d < a.hd)
       *reinterpret_cast<uint32_t*>(a.out + (long long)(s.start + tok) * a.sot +
                                    (long long)(kvh * a.rep + pr - tok * a.rep) * a.soh + d) =
-          none ? 0u : Type16<T>::pack(x * inv, y * inv);
+          s.len - s.n + tok < 0 ? 0u : Type16<T>::pack(x, y);
   }
 }
 
 template <typename KernelT>
-static int launch_attn_grid(KernelT kernel, const SeqAttnArgs& a, unsigned grid, size_t smem, cudaStream_t stream) {
-  if (smem > 0) {  // (the table is by kernel: instantiations of one signature share this function)
+static int launch_attn_grid(KernelT kernel, const SeqAttnArgs& a, dim3 grid, size_t smem, cudaStream_t stream) {
+  if (smem > 40 * 1024) {  // (the table is by kernel: instantiations of one signature share this function)
     static std::mutex mu;
     static std::vector<std::pair<int, const void*>> raised;
     int dev = 0;
@@ -481,7 +542,7 @@ static int launch_attn_grid(KernelT kernel, const SeqAttnArgs& a, unsigned grid,
     }
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(kSeqThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -493,38 +554,47 @@ static int launch_attn_grid(KernelT kernel, const SeqAttnArgs& a, unsigned grid,
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, a), "attention: kernel launch");
 }
 
-template <typename T, int D, int MT, bool PAGED>
+template <typename T, int D, int NT, bool PAGED>
 static int launch_seq(const SeqAttnArgs& a, cudaStream_t stream) {
-  int rc = launch_attn_grid(seq_attention_kernel<T, D, MT, PAGED>, a, (unsigned)a.grid, seq_smem_bytes(D), stream);
+  int rc = launch_attn_grid(seq_attention_kernel<T, D, NT, PAGED>, a, dim3((unsigned)a.grid), seq_smem_bytes(D), stream);
   if (rc == LI4_OK && a.grid > 1)
-    rc = launch_attn_grid(seq_attention_join_kernel<T, D, MT, PAGED>, a, (unsigned)a.grid - 1, 0, stream);
+    rc = launch_attn_grid(seq_attention_join_kernel<T, D, NT, PAGED>, a, dim3((unsigned)a.grid - 1, kJoinShares),
+                          (size_t)a.grid * 8 * NT * sizeof(float), stream);
   return rc;
 }
 
 template <typename T, bool PAGED>
-static int launch_seq_d(const SeqAttnArgs& a, int mt, cudaStream_t stream) {
-  if (a.hd <= 64) return mt == 1 ? launch_seq<T, 64, 1, PAGED>(a, stream) : launch_seq<T, 64, 2, PAGED>(a, stream);
-  return mt == 1 ? launch_seq<T, 128, 1, PAGED>(a, stream) : launch_seq<T, 128, 2, PAGED>(a, stream);
+static int launch_seq_d(const SeqAttnArgs& a, int nt, cudaStream_t stream) {
+  if (a.hd <= 64)
+    return nt == 1   ? launch_seq<T, 64, 1, PAGED>(a, stream)
+           : nt == 2 ? launch_seq<T, 64, 2, PAGED>(a, stream)
+                     : launch_seq<T, 64, 4, PAGED>(a, stream);
+  return nt == 1   ? launch_seq<T, 128, 1, PAGED>(a, stream)
+         : nt == 2 ? launch_seq<T, 128, 2, PAGED>(a, stream)
+                   : launch_seq<T, 128, 4, PAGED>(a, stream);
 }
 
-static int seq_mt(int max_rows) { return max_rows <= 16 ? 1 : 2; }
+static int seq_nt(int max_rows) { return max_rows <= 8 ? 1 : max_rows <= 16 ? 2 : 4; }
 // CTAs that fit at once: two per SM at 64 dims (96 KB of stages each), one at 128 (192 KB).
 static int seq_grid(int hd, int sm) { return hd <= 64 ? 2 * sm : sm; }
 
 size_t seq_attention_part_bytes(int hd, int max_rows, int sm) {
-  return (size_t)2 * seq_grid(hd, sm) * seq_part_floats(hd <= 64 ? 64 : 128, seq_mt(max_rows)) * sizeof(float);
+  return (size_t)2 * seq_grid(hd, sm) * seq_part_floats(hd <= 64 ? 64 : 128, seq_nt(max_rows)) * sizeof(float);
 }
 
 int launch_seq_attention(const SeqAttnArgs& args, bool paged, int dtype, int max_rows, cudaStream_t stream) {
   SeqAttnArgs a = args;
   a.grid = seq_grid(a.hd, current_sm_count());
-  const int mt = seq_mt(max_rows);
+  const int nt = seq_nt(max_rows);
   if (dtype == LI4_F16)
-    return paged ? launch_seq_d<__half, true>(a, mt, stream) : launch_seq_d<__half, false>(a, mt, stream);
-  return paged ? launch_seq_d<__nv_bfloat16, true>(a, mt, stream) : launch_seq_d<__nv_bfloat16, false>(a, mt, stream);
+    return paged ? launch_seq_d<__half, true>(a, nt, stream) : launch_seq_d<__half, false>(a, nt, stream);
+  return paged ? launch_seq_d<__nv_bfloat16, true>(a, nt, stream) : launch_seq_d<__nv_bfloat16, false>(a, nt, stream);
 }
 
-constexpr int kFewRows = 32;  // rows (queries x heads of a KV head) up to which a sequence is streamed
+// Rows (queries x heads of a KV head) up to which a sequence is streamed: where no sequence has more the streaming
+// kernel runs alone, with tiles of 32 rows; beside longer ones it takes those of one 16-row tile (a decode step's, whose
+// keys then pass through half the registers: 31 requests beside a chunk, 112 us of streaming with 32-row tiles).
+constexpr int kFewRows = 32, kFewRowsBeside = 16;
 
 static int check_attention(const li4_attention* p, bool paged, const char* what) {
   if (!p) return set_error(LI4_ERR_INVALID_ARG, "%s: null arguments", what);
@@ -625,11 +695,11 @@ static int run_attention(const li4_attention* p, bool paged, void* workspace, si
   rc = LI4_OK;
   if (!tiles || both) {
     a.small_rows = 0;
-    a.big_rows = both ? kFewRows : 0x7fffffff;
-    rc = launch_seq_attention(a, paged, p->dtype, both ? kFewRows : rows, st);
+    a.big_rows = both ? kFewRowsBeside : 0x7fffffff;
+    rc = launch_seq_attention(a, paged, p->dtype, both ? kFewRowsBeside : rows, st);
   }
   if (rc == LI4_OK && tiles) {
-    a.small_rows = both ? kFewRows : 0;
+    a.small_rows = both ? kFewRowsBeside : 0;
     a.big_rows = 0x7fffffff;
     rc = launch_tile_attention(a, paged, p->dtype, st);
   }
