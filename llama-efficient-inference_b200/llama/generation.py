@@ -74,6 +74,45 @@ class DecodeGraph:
         return torch.cat(out, 1)
 
 
+class PagedDecodeGraph:
+    """Greedy decode steps of every request of a PagedKVCache, replayed from one CUDA graph.
+
+    tok int64 [requests] is a static buffer; replay() appends one token to every request (li4_paged_append), runs the
+    blocks over the cache and leaves each request's next token in tok.  The lengths, tables and free pages live on the
+    GPU, so the one graph serves every length.  Made after the prompts are in the cache: the warm-up steps run on the
+    requests as they are and the cache's bookkeeping is put back."""
+
+    @torch.no_grad()
+    def __init__(self, model: nn.Module, cache, tok: torch.Tensor, warmup: int = 2):
+        self.model, self.cache, self.tok = model, cache, tok.clone()
+        self.one = torch.ones_like(cache.kv_lens)
+        state = (cache.kv_lens, cache.n_free, cache.block_tables, self.tok)
+        saved = [t.clone() for t in state]
+        dev = tok.device
+        side = torch.cuda.Stream(dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side):
+            for _ in range(warmup):  # sizes every workspace before capture
+                self._step()
+                for t, s in zip(state, saved):
+                    t.copy_(s)
+        torch.cuda.current_stream(dev).wait_stream(side)
+        torch.cuda.synchronize(dev)
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self.logits = self._step()
+        torch.cuda.synchronize(dev)
+
+    def _step(self):
+        step = self.cache.append(self.one, self.tok.shape[0])
+        logits = self.model.forward_paged(self.tok, step, self.cache, 1)
+        self.tok.copy_(logits.argmax(-1))
+        return logits
+
+    def replay(self):
+        self.graph.replay()
+
+
 @torch.no_grad()
 def eager_tokens(model: nn.Module, tokens: torch.Tensor, n_steps: int) -> torch.Tensor:
     """Greedy tokens from the eager reference-style loop (the reference's bench.py:154-161)."""
@@ -135,6 +174,63 @@ class Generation(nn.Module):
         results = []
         for row, n in enumerate(lengths):
             gen = buf[row, n:n + max_gen_len].tolist()
+            if tokenizer.eos_id in gen:
+                gen = gen[:gen.index(tokenizer.eos_id)]
+            results.append({"generation": tokenizer.decode(gen)})
+        return results
+
+    @torch.no_grad()
+    def generate_paged(self, tokenizer, prompts, max_gen_len, temperature, top_p, device, page_size=16,
+                       cuda_graph=False):
+        """generate() over a paged KV cache (llama.paged), without padding: the prompts run packed as one step, then
+        every unfinished request gets a token per step, and a finished one returns its pages at once.
+        cuda_graph=True (greedy only) replays one captured step for all requests until max_gen_len and cuts the
+        answers at eos afterwards."""
+        if cuda_graph and temperature > 0:
+            raise ValueError("cuda_graph decode needs greedy sampling (temperature 0)")
+        encoded = [tokenizer.encode(text, bos=True, eos=False) for text in prompts]
+        n, lengths = len(encoded), [len(t) for t in encoded]
+        if n == 0 or min(lengths) < 1:
+            raise ValueError("generate_paged: every prompt needs a token")
+        total = max(lengths) + max_gen_len
+        pages = sum(-(-(l + max_gen_len) // page_size) for l in lengths)
+        cache = self.paged_cache(pages, page_size, max_requests=n, max_len=total)
+
+        def pick(logits):
+            if temperature > 0:
+                return sample_top_p(torch.softmax(logits / temperature, dim=-1), top_p).view(-1)
+            return logits.argmax(dim=-1)
+
+        answers = [[] for _ in range(n)]
+        if max_gen_len > 0:
+            packed = torch.tensor([t for toks in encoded for t in toks], dtype=torch.long, device=device)
+            step = cache.append(torch.tensor(lengths, dtype=torch.int32, device=device), sum(lengths))
+            choice = pick(self.forward_paged(packed, step, cache, max(lengths), whole_prompts=True))
+            if cuda_graph:
+                graph = PagedDecodeGraph(self, cache, choice)
+                chosen = [choice]
+                for _ in range(max_gen_len - 1):
+                    graph.replay()
+                    chosen.append(graph.tok.clone())
+                answers = torch.stack(chosen, 1).tolist()
+            else:
+                going = [True] * n
+                while True:
+                    for row, token in enumerate(choice.tolist()):
+                        if going[row]:
+                            answers[row].append(token)
+                    ended = [g and (answers[r][-1] == tokenizer.eos_id or len(answers[r]) == max_gen_len)
+                             for r, g in enumerate(going)]
+                    if any(ended):
+                        cache.release(torch.tensor(ended, device=device))
+                        going = [g and not e for g, e in zip(going, ended)]
+                    if not any(going):
+                        break
+                    new = torch.tensor([int(g) for g in going], dtype=torch.int32, device=device)
+                    fed = torch.tensor([answers[r][-1] for r in range(n) if going[r]], dtype=torch.long, device=device)
+                    choice = pick(self.forward_paged(fed, cache.append(new, fed.shape[0]), cache, 1))
+        results = []
+        for gen in answers:
             if tokenizer.eos_id in gen:
                 gen = gen[:gen.index(tokenizer.eos_id)]
             results.append({"generation": tokenizer.decode(gen)})

@@ -574,3 +574,50 @@ def test_model_steps_over_the_paged_cache(paged, heads, kv_heads, page):
         cache.release(torch.tensor([True, True, True], device="cuda"))
         assert int(cache.n_free) == cache.free_pages.numel()
         assert sorted(cache.free_pages.tolist()) == list(range(cache.free_pages.numel()))
+
+
+class Letters:
+    """A tokenizer of one token per character."""
+
+    pad_id, eos_id = 0, 1
+
+    def encode(self, text, bos, eos):
+        return [2] + [3 + ord(c) % 490 for c in text]
+
+    def decode(self, ids):
+        return " ".join(map(str, ids))
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_generate_paged(paged, quantized):
+    """Every greedy token of every answer is the best of Llama.forward's logits for the text before it, up to 2% of
+    their range (the two paths round at different places); the captured step gives the eager loop's answers."""
+    from llama import quantize
+
+    model = tiny_model(seed=3)
+    if quantized:
+        quantize.quantize_model(model, 128)
+        quantize.set_dequant_impl("v4")
+    try:
+        prompts, tok = ["a", "some longer prompt " * 5, "of three", "the fourth"], Letters()
+        got = model.generate_paged(tok, prompts, 12, 0.0, 1.0, "cuda", page_size=8)
+        again = model.generate_paged(tok, prompts, 12, 0.0, 1.0, "cuda", page_size=32, cuda_graph=True)
+        assert [len(g["generation"].split()) for g in got] == [12] * 4 or all(g["generation"] for g in got)
+        for text, a, b in zip(prompts, got, again):
+            for answer in (a, b):
+                ids = tok.encode(text, True, False)
+                gen = [int(x) for x in answer["generation"].split()]
+                with torch.no_grad():
+                    model.reset_cache()
+                    logits = model(torch.tensor([ids + gen], device="cuda"), 0)[0].float()
+                for i, t in enumerate(gen):
+                    row = logits[len(ids) - 1 + i]
+                    assert float(row.max() - row[t]) <= 2e-2 * float(row.max() - row.min())
+        sampled = model.generate_paged(tok, prompts, 5, 0.8, 0.9, "cuda")
+        assert len(sampled) == 4
+        with pytest.raises(ValueError):
+            model.generate_paged(tok, prompts, 5, 0.8, 0.9, "cuda", cuda_graph=True)
+        with pytest.raises(ValueError):
+            model.generate_paged(tok, ["x" * 600], 5, 0.0, 0.9, "cuda")
+    finally:
+        quantize.set_dequant_impl("v1")
