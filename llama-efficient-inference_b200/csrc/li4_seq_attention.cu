@@ -3,12 +3,12 @@
 // Grouped-query attention by rows: the rep query heads of a KV head, over the queries of a sequence,
 // are the rows of one matrix (row = query * rep + head), so a KV head's keys and values are read once
 // for the whole group.  An item is (sequence, tile of 8 NT rows, KV head); its keys come in units of
-// 128.  Units of all items lie on one line; CTA g of G takes the g-th equal share of it, whatever the
+// 128 (64 dims) or 64 (128 dims).  Units of all items lie on one line; CTA g of G takes the g-th equal share of it, whatever the
 // lengths are (they are read on the device: the host knows none).  A CTA that covers only a part of an
 // item's keys leaves (running maximum, sum, unnormalised output) in `part`, and a second launch joins
 // the parts in key order, so the result does not depend on timing.
 //
-// Inside a CTA each of the 4 warps streams its own 32 keys of every unit through its own ring of
+// Inside a CTA each of the 4 warps streams its own quarter of every unit through its own ring of
 // shared-memory stages (cp.async; no CTA barrier until the end): S^T = K Q^T and O^T += V^T P^T as
 // m16n8k16 tensor-core tiles, softmax in fp32 in registers with the running maximum and sum of one
 // pass.  The keys are the 16-wide side and the rows the 8-wide one, so a group of 4 or 8 heads wastes
@@ -26,10 +26,13 @@ namespace li4 {
 
 constexpr int kSeqThreads = 128;
 constexpr int kSeqWarps = 4;
-constexpr int kUnit = 128;      // keys per unit: 32 per warp
-constexpr int kSeqStages = 3;   // stages of 32 keys per warp
-
-__host__ __device__ constexpr int seq_stage_bytes(int D) { return 2 * 32 * D * 2; }
+constexpr int kSeqStages = 3;   // stages per warp
+// Keys of a warp's stage: 8 KB of keys and values, 96 KB of stages per CTA, two CTAs per SM (while one joins its warps or
+// starts an item the other's copies go on: one CTA of 32-key stages at 128 dims, 32 requests of 1000-8000 tokens 81 us
+// instead of NEW128).
+__host__ __device__ constexpr int seq_keys(int D) { return 32 * 64 / D; }
+__host__ __device__ constexpr int seq_unit(int D) { return kSeqWarps * seq_keys(D); }  // keys per unit
+__host__ __device__ constexpr int seq_stage_bytes(int D) { return 2 * seq_keys(D) * D * 2; }
 __host__ __device__ constexpr int seq_smem_bytes(int D) { return kSeqWarps * kSeqStages * seq_stage_bytes(D); }
 // floats of one partial result: 8 NT rows of D outputs, then (maximum, sum) per row
 __host__ __device__ constexpr int seq_part_floats(int D, int NT) { return 8 * NT * (D + 2); }
@@ -41,16 +44,16 @@ struct Line {
 };
 __device__ __forceinline__ long long share(const Line& l, int g) { return l.total * g / l.active; }
 
-template <int NT>
+template <int D, int NT>
 __device__ __forceinline__ long long seq_units(const SeqAttnArgs& a, const Seq& s, int* tiles, int* per) {
   *tiles = (int)(((long long)s.n * a.rep + 8 * NT - 1) / (8 * NT));
-  *per = max(1, (s.len + kUnit - 1) / kUnit);
+  *per = max(1, (s.len + seq_unit(D) - 1) / seq_unit(D));
   return (long long)*tiles * *per * a.Hkv;
 }
 
 // Finds the sequence that holds unit share(g): each thread sums a slice of the sequences.  Every thread
 // returns the line, the sequence and the units before it (b = -1: no share).
-template <int NT, bool PAGED>
+template <int D, int NT, bool PAGED>
 __device__ Line find_share(const SeqAttnArgs& a, int g, int* b_out, long long* before) {
   __shared__ long long s_sum[kSeqWarps];
   __shared__ int s_b;
@@ -60,7 +63,7 @@ __device__ Line find_share(const SeqAttnArgs& a, int g, int* b_out, long long* b
   const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
   long long mine = 0;
   int tiles, units;
-  for (int b = b0; b < b1; ++b) mine += seq_units<NT>(a, load_seq<PAGED>(a, b), &tiles, &units);
+  for (int b = b0; b < b1; ++b) mine += seq_units<D, NT>(a, load_seq<PAGED>(a, b), &tiles, &units);
   long long incl = mine;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -84,7 +87,7 @@ __device__ Line find_share(const SeqAttnArgs& a, int g, int* b_out, long long* b
     long long excl = incl - mine;
     if (at >= excl && at < incl) {
       for (int b = b0; b < b1; ++b) {
-        const long long u = seq_units<NT>(a, load_seq<PAGED>(a, b), &tiles, &units);
+        const long long u = seq_units<D, NT>(a, load_seq<PAGED>(a, b), &tiles, &units);
         if (at < excl + u) {
           s_b = b;
           s_before = excl;
@@ -139,16 +142,17 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return r;
 }
 
-// The pages of 32 keys from j0, 8 keys each (a page has 8 rows at least and j0 is a multiple of 32, so 8 keys share one);
+// The pages of a stage's keys from j0, 8 keys each (a page has 8 rows at least and j0 is a multiple of 16, so 8 keys share one);
 // asked for a stage ahead of their copy, as the block table's answer takes a trip to L2.  -1: past the end.
+template <int D>
 struct KeyPages {
-  int page[4];
+  int page[seq_keys(D) / 8];
 };
-template <bool PAGED>
-__device__ __forceinline__ KeyPages key_pages(const SeqAttnArgs& a, int b, int j0, int end) {
-  KeyPages k;
+template <int D, bool PAGED>
+__device__ __forceinline__ KeyPages<D> key_pages(const SeqAttnArgs& a, int b, int j0, int end) {
+  KeyPages<D> k;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < seq_keys(D) / 8; ++q) {
     k.page[q] = -1;
     if (j0 + 8 * q < end)
       k.page[q] = PAGED ? a.tables[(long long)b * a.table_stride + ((j0 + 8 * q) >> a.log_page)] : 0;
@@ -156,10 +160,10 @@ __device__ __forceinline__ KeyPages key_pages(const SeqAttnArgs& a, int b, int j
   return k;
 }
 
-// 32 keys of the item into a stage: K rows then V rows, 16-byte chunk c of row r at c ^ (r & 7).  Rows past the end and
+// A stage's keys: K rows then V rows, 16-byte chunk c of row r at c ^ (r & 7).  Rows past the end and
 // rows of no page are zeros.
 template <int D, bool PAGED>
-__device__ __forceinline__ void load_stage(const SeqAttnArgs& a, const KeyPages& kp, const Seq& s, int kvh, int j0, int end,
+__device__ __forceinline__ void load_stage(const SeqAttnArgs& a, const KeyPages<D>& kp, const Seq& s, int kvh, int j0, int end,
                                            uint32_t stage) {
   constexpr int CH = D / 8;           // chunks per row
   constexpr int RPI = 32 / CH;        // rows per instruction of the warp
@@ -169,7 +173,7 @@ __device__ __forceinline__ void load_stage(const SeqAttnArgs& a, const KeyPages&
   const uint16_t* k = a.k + (long long)kvh * a.skh + (long long)r0 * a.skt + c * 8;
   const uint16_t* v = a.v + (long long)kvh * a.svh + (long long)r0 * a.svt + c * 8;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < seq_keys(D) / 8; ++q) {
     const int row = PAGED ? (j0 + 8 * q) & ((1 << a.log_page) - 1) : s.start + j0 + 8 * q;
     const long long page = PAGED ? kp.page[q] : 0;
     const bool have = (PAGED ? (unsigned)kp.page[q] < (unsigned)a.num_pages : kp.page[q] == 0) && in_head;
@@ -181,7 +185,7 @@ __device__ __forceinline__ void load_stage(const SeqAttnArgs& a, const KeyPages&
       const bool ok = have && j0 + r < end;
       const uint32_t at = stage + r * (D * 2) + ((c ^ (r & 7)) << 4);
       cp_async16z(at, ok ? kq + (long long)(i * RPI) * a.skt : a.q, ok);  // (not read where !ok)
-      cp_async16z(at + 32 * D * 2, ok ? vq + (long long)(i * RPI) * a.svt : a.q, ok);
+      cp_async16z(at + seq_keys(D) * D * 2, ok ? vq + (long long)(i * RPI) * a.svt : a.q, ok);
     }
   }
 }
@@ -191,6 +195,7 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
   constexpr int RT = 8 * NT;
   constexpr int KS = D / 16;  // k steps of K Q^T
   constexpr int DT = D / 16;  // 16-dim tiles of the output
+  constexpr int KW = seq_keys(D), KT = KW / 16, UNIT = seq_unit(D);  // a warp's keys per stage, their 16-key tiles
   constexpr int LD = D + 8;   // floats per row of the warps' outputs in shared memory
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ float s_ml[kSeqWarps][RT][2];
@@ -203,14 +208,14 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
   int b;
   long long before;
   const int g = blockIdx.x;
-  const Line line = find_share<NT, PAGED>(a, g, &b, &before);
+  const Line line = find_share<D, NT, PAGED>(a, g, &b, &before);
   if (b < 0) return;
   const long long at0 = share(line, g);
   long long left = share(line, g + 1) - at0;
   long long rem = at0 - before;  // units into sequence b
   Seq s = load_seq<PAGED>(a, b);
   int tiles, per;
-  seq_units<NT>(a, s, &tiles, &per);
+  seq_units<D, NT>(a, s, &tiles, &per);
 
   while (left > 0) {
     const int item = (int)(rem / per), u0 = (int)(rem - (long long)item * per);
@@ -220,20 +225,20 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
     const int rows = min(RT, s.n * a.rep - row0);
     const int first_lim = s.len - s.n + row0 / a.rep;               // last key the tile's first query sees
     const int last_lim = s.len - s.n + (row0 + rows - 1) / a.rep;   // and its last query
-    const int k0 = u0 * kUnit, k1 = min(min(u1 * kUnit, s.len), last_lim + 1);
+    const int k0 = u0 * UNIT, k1 = min(min(u1 * UNIT, s.len), last_lim + 1);
 
-    // ---- the warp's keys: k0 + 32 warp + 128 i, their first stages under way
-    const int w0 = k0 + warp * 32;
-    const int steps = w0 < k1 ? (k1 - w0 + kUnit - 1) / kUnit : 0;
-    KeyPages pages[kSeqStages];
+    // ---- the warp's keys: k0 + KW warp + UNIT i, their first stages under way
+    const int w0 = k0 + warp * KW;
+    const int steps = w0 < k1 ? (k1 - w0 + UNIT - 1) / UNIT : 0;
+    KeyPages<D> pages[kSeqStages];
 #pragma unroll
-    for (int i = 0; i < kSeqStages; ++i) pages[i] = key_pages<PAGED>(a, b, w0 + i * kUnit, k1);
+    for (int i = 0; i < kSeqStages; ++i) pages[i] = key_pages<D, PAGED>(a, b, w0 + i * UNIT, k1);
 #pragma unroll
     for (int i = 0; i < kSeqStages - 1; ++i) {
-      if (i < steps) load_stage<D, PAGED>(a, pages[i], s, kvh, w0 + i * kUnit, k1, ring + i * seq_stage_bytes(D));
+      if (i < steps) load_stage<D, PAGED>(a, pages[i], s, kvh, w0 + i * UNIT, k1, ring + i * seq_stage_bytes(D));
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    KeyPages next_pages = pages[kSeqStages - 1];
+    KeyPages<D> next_pages = pages[kSeqStages - 1];
 
     // ---- queries as B fragments (n = row, k = dim); rows past the tile are zero rows
     uint32_t qf[NT][KS][2];
@@ -274,19 +279,19 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
       if (next >= kSeqStages) next -= kSeqStages;
       __syncwarp();
       if (ahead < steps)
-        load_stage<D, PAGED>(a, next_pages, s, kvh, w0 + ahead * kUnit, k1, ring + next * seq_stage_bytes(D));
+        load_stage<D, PAGED>(a, next_pages, s, kvh, w0 + ahead * UNIT, k1, ring + next * seq_stage_bytes(D));
       asm volatile("cp.async.commit_group;" ::: "memory");
-      next_pages = key_pages<PAGED>(a, b, w0 + (ahead + 1) * kUnit, k1);
+      next_pages = key_pages<D, PAGED>(a, b, w0 + (ahead + 1) * UNIT, k1);
       asm volatile("cp.async.wait_group %0;" ::"n"(kSeqStages - 1) : "memory");
       __syncwarp();
-      const uint32_t ks_at = ring + slot * seq_stage_bytes(D), vs_at = ks_at + 32 * D * 2;
-      const int j0 = w0 + i * kUnit;
+      const uint32_t ks_at = ring + slot * seq_stage_bytes(D), vs_at = ks_at + KW * D * 2;
+      const int j0 = w0 + i * UNIT;
       slot = slot + 1 == kSeqStages ? 0 : slot + 1;
 
-      // S^T: 32 keys x 8 NT rows
-      float sc[2][NT][4];
+      // S^T: KW keys x 8 NT rows
+      float sc[KT][NT][4];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
+      for (int mt = 0; mt < KT; ++mt) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
 #pragma unroll
@@ -298,9 +303,9 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
           for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[mt][nt], kf, qf[nt][ks][0], qf[nt][ks][1]);
         }
       }
-      if (j0 + 31 > first_lim || j0 + 32 > k1) {  // some key of the 32 is hidden from some row
+      if (j0 + KW - 1 > first_lim || j0 + KW > k1) {  // some key of them is hidden from some row
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -310,19 +315,20 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
             }
       } else {
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[mt][nt][e] *= a.scale_log2;
       }
-      uint32_t pf[2][NT][2];
+      uint32_t pf[KT][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float base[2], keep[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2]));
+          float mx = fmaxf(sc[0][nt][e], sc[0][nt][e + 2]);
+          if constexpr (KT == 2) mx = fmaxf(mx, fmaxf(sc[KT - 1][nt][e], sc[KT - 1][nt][e + 2]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -339,7 +345,7 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
             for (int e = 0; e < 4; ++e) o[dt][nt][e] *= keep[e & 1];
         }
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+        for (int mt = 0; mt < KT; ++mt) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             sc[mt][nt][e] = exp2_fast(sc[mt][nt][e] - base[e & 1]);
@@ -352,7 +358,7 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
       }
       // O^T += V^T P^T: 16 dims x 16 keys by four transposed 8x8 matrices
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           uint32_t vf[4];
@@ -449,7 +455,7 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
     while (left > 0 && rem >= (long long)tiles * per * a.Hkv) {
       rem -= (long long)tiles * per * a.Hkv;
       s = load_seq<PAGED>(a, ++b);
-      seq_units<NT>(a, s, &tiles, &per);
+      seq_units<D, NT>(a, s, &tiles, &per);
     }
   }
 }
@@ -467,11 +473,11 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_join_kernel(const _
   const int g = blockIdx.x + 1;
   int b;
   long long before;
-  const Line line = find_share<NT, PAGED>(a, g, &b, &before);
+  const Line line = find_share<D, NT, PAGED>(a, g, &b, &before);
   if (b < 0) return;
   const Seq s = load_seq<PAGED>(a, b);
   int tiles, per;
-  seq_units<NT>(a, s, &tiles, &per);
+  seq_units<D, NT>(a, s, &tiles, &per);
   const long long rem = share(line, g) - before;
   const int item = (int)(rem / per);
   const long long start = before + (long long)item * per, end = start + per;
@@ -575,16 +581,15 @@ static int launch_seq_d(const SeqAttnArgs& a, int nt, cudaStream_t stream) {
 }
 
 static int seq_nt(int max_rows) { return max_rows <= 8 ? 1 : max_rows <= 16 ? 2 : 4; }
-// CTAs that fit at once: two per SM at 64 dims (96 KB of stages each), one at 128 (192 KB).
-static int seq_grid(int hd, int sm) { return hd <= 64 ? 2 * sm : sm; }
+static int seq_grid(int sm) { return 2 * sm; }  // CTAs that fit at once
 
 size_t seq_attention_part_bytes(int hd, int max_rows, int sm) {
-  return (size_t)2 * seq_grid(hd, sm) * seq_part_floats(hd <= 64 ? 64 : 128, seq_nt(max_rows)) * sizeof(float);
+  return (size_t)2 * seq_grid(sm) * seq_part_floats(hd <= 64 ? 64 : 128, seq_nt(max_rows)) * sizeof(float);
 }
 
 int launch_seq_attention(const SeqAttnArgs& args, bool paged, int dtype, int max_rows, cudaStream_t stream) {
   SeqAttnArgs a = args;
-  a.grid = seq_grid(a.hd, current_sm_count());
+  a.grid = seq_grid(current_sm_count());
   const int nt = seq_nt(max_rows);
   if (dtype == LI4_F16)
     return paged ? launch_seq_d<__half, true>(a, nt, stream) : launch_seq_d<__half, false>(a, nt, stream);
