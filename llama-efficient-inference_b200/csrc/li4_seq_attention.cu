@@ -12,9 +12,11 @@
 // shared-memory stages (cp.async; no CTA barrier until the end): S^T = K Q^T and O^T += V^T P^T as
 // m16n8k16 tensor-core tiles, softmax in fp32 in registers with the running maximum and sum of one
 // pass.  The keys are the 16-wide side and the rows the 8-wide one, so a group of 4 or 8 heads wastes
-// half of a tile or nothing (rows as the 16-wide side: 985 instead of NEWCOUNT instructions per 32 keys of a
-// warp, 64 requests of 300-16000 tokens 85 us instead of NEWTIME).  The work is bound by the bytes of the keys
-// and values as long as the rows are few.
+// half of a tile or nothing (with the rows as the 16-wide side 64 requests of 300-16000 tokens took
+// 85 us instead of 81).  The work is bound by the bytes of the keys and values as long as the rows
+// are few: those 419 MB are read at 5.2 TB/s, and no faster with the products left out.
+#include <cooperative_groups.h>
+
 #include <mutex>
 #include <utility>
 #include <vector>
@@ -24,12 +26,14 @@
 
 namespace li4 {
 
+namespace cg = cooperative_groups;
+
 constexpr int kSeqThreads = 128;
 constexpr int kSeqWarps = 4;
 constexpr int kSeqStages = 3;   // stages per warp
 // Keys of a warp's stage: 8 KB of keys and values, 96 KB of stages per CTA, two CTAs per SM (while one joins its warps or
 // starts an item the other's copies go on: one CTA of 32-key stages at 128 dims, 32 requests of 1000-8000 tokens 81 us
-// instead of NEW128).
+// instead of 75).
 __host__ __device__ constexpr int seq_keys(int D) { return 32 * 64 / D; }
 __host__ __device__ constexpr int seq_unit(int D) { return kSeqWarps * seq_keys(D); }  // keys per unit
 __host__ __device__ constexpr int seq_stage_bytes(int D) { return 2 * seq_keys(D) * D * 2; }
@@ -190,13 +194,16 @@ __device__ __forceinline__ void load_stage(const SeqAttnArgs& a, const KeyPages<
   }
 }
 
-template <typename T, int D, int NT, bool PAGED>
+// CL: few requests of short contexts.  A cluster of CTAs takes all keys of a (request, KV head) and joins its parts through
+// distributed shared memory, so there is no second launch (see seq_cluster).
+template <typename T, int D, int NT, bool PAGED, bool CL>
 __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid_constant__ SeqAttnArgs a) {
   constexpr int RT = 8 * NT;
   constexpr int KS = D / 16;  // k steps of K Q^T
   constexpr int DT = D / 16;  // 16-dim tiles of the output
   constexpr int KW = seq_keys(D), KT = KW / 16, UNIT = seq_unit(D);  // a warp's keys per stage, their 16-key tiles
   constexpr int LD = D + 8;   // floats per row of the warps' outputs in shared memory
+  static_assert((kSeqWarps * RT * LD + RT * (D + 2)) * 4 <= seq_smem_bytes(D), "outputs and a part fit the ring");
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ float s_ml[kSeqWarps][RT][2];
   __shared__ int s_redo[RT];
@@ -205,22 +212,44 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
   pdl_launch_dependents();
   pdl_wait_primary();
 
-  int b;
-  long long before;
   const int g = blockIdx.x;
-  const Line line = find_share<D, NT, PAGED>(a, g, &b, &before);
-  if (b < 0) return;
-  const long long at0 = share(line, g);
-  long long left = share(line, g + 1) - at0;
-  long long rem = at0 - before;  // units into sequence b
-  Seq s = load_seq<PAGED>(a, b);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = CL ? (int)cluster.block_rank() : 0, ranks = CL ? (int)cluster.num_blocks() : 1;
+  int b;
+  long long left, rem;  // units of the share left; units into sequence b (CL: tiles left; tiles done)
+  Seq s;
   int tiles, per;
-  seq_units<D, NT>(a, s, &tiles, &per);
+  if constexpr (CL) {
+    b = g / ranks / a.Hkv;
+    s = load_seq<PAGED>(a, b);
+    seq_units<D, NT>(a, s, &tiles, &per);
+    left = tiles;
+    rem = 0;
+  } else {
+    long long before;
+    const Line line = find_share<D, NT, PAGED>(a, g, &b, &before);
+    if (b < 0) return;
+    const long long at0 = share(line, g);
+    left = share(line, g + 1) - at0;
+    rem = at0 - before;
+    s = load_seq<PAGED>(a, b);
+    seq_units<D, NT>(a, s, &tiles, &per);
+  }
 
   while (left > 0) {
-    const int item = (int)(rem / per), u0 = (int)(rem - (long long)item * per);
-    const int u1 = (int)min((long long)per, u0 + left);
-    const int kvh = item % a.Hkv, tile = item / a.Hkv;
+    int kvh, tile, u0, u1;
+    if constexpr (CL) {
+      kvh = g / ranks % a.Hkv;
+      tile = (int)rem;
+      u0 = per * rank / ranks;
+      u1 = per * (rank + 1) / ranks;
+    } else {
+      const int item = (int)(rem / per);
+      u0 = (int)(rem - (long long)item * per);
+      u1 = (int)min((long long)per, u0 + left);
+      kvh = item % a.Hkv;
+      tile = item / a.Hkv;
+    }
     const int row0 = tile * RT;
     const int rows = min(RT, s.n * a.rep - row0);
     const int first_lim = s.len - s.n + row0 / a.rep;               // last key the tile's first query sees
@@ -394,9 +423,11 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
       }
     if (tid < RT) s_redo[tid] = 0;
     __syncthreads();
-    const bool whole = u0 == 0 && u1 == per;
+    const bool whole = !CL && u0 == 0 && u1 == per;
     const bool masked = k1 - 1 > first_lim;  // some row must not see some of the keys read
-    float* part = a.part + (size_t)(2 * g + (u0 == 0 ? 1 : 0)) * seq_part_floats(D, NT);
+    // where a part of the item's result goes: the workspace, or this CTA's shared memory past the warps' outputs
+    float* part = CL ? reinterpret_cast<float*>(smem) + kSeqWarps * RT * LD
+                     : a.part + (size_t)(2 * g + (u0 == 0 ? 1 : 0)) * seq_part_floats(D, NT);
     const float* all = reinterpret_cast<const float*>(smem);
     for (int e = tid; e < RT * D / 2; e += kSeqThreads) {
       const int r = e / (D / 2), d = (e - r * (D / 2)) * 2;
@@ -450,6 +481,36 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
       __syncthreads();
     }
 
+    if constexpr (CL) {
+      cluster.sync();  // every CTA's part is there
+      for (int e = rank * kSeqThreads + tid; e < rows * (D / 2); e += ranks * kSeqThreads) {
+        const int r = e / (D / 2), d = (e - r * (D / 2)) * 2;
+        float M = -INFINITY;
+        for (int c = 0; c < ranks; ++c) M = fmaxf(M, cluster.map_shared_rank(part, c)[RT * D + r * 2]);
+        const float base = M == -INFINITY ? 0.f : M;
+        float L = 0.f, x = 0.f, y = 0.f;
+#pragma unroll 4
+        for (int c = 0; c < ranks; ++c) {
+          const float* pc = cluster.map_shared_rank(part, c);
+          const float2 ml = *reinterpret_cast<const float2*>(pc + RT * D + r * 2);
+          const float2 ov = *reinterpret_cast<const float2*>(pc + r * D + d);
+          const float f = exp2_fast(ml.x - base);
+          L += f * ml.y;
+          x += f * ov.x;
+          y += f * ov.y;
+        }
+        const int pr = row0 + r, tok = pr / a.rep;
+        const float inv = 1.f / L;
+        if (d < a.hd)
+          *reinterpret_cast<uint32_t*>(a.out + (long long)(s.start + tok) * a.sot +
+                                       (long long)(kvh * a.rep + pr - tok * a.rep) * a.soh + d) =
+              s.len - s.n + tok < 0 ? 0u : Type16<T>::pack(x * inv, y * inv);
+      }
+      cluster.sync();  // read by every CTA: the memory may go
+      --left;
+      ++rem;
+      continue;
+    }
     left -= u1 - u0;
     rem += u1 - u0;
     while (left > 0 && rem >= (long long)tiles * per * a.Hkv) {
@@ -530,7 +591,8 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_join_kernel(const _
 }
 
 template <typename KernelT>
-static int launch_attn_grid(KernelT kernel, const SeqAttnArgs& a, dim3 grid, size_t smem, cudaStream_t stream) {
+static int launch_attn_grid(KernelT kernel, const SeqAttnArgs& a, dim3 grid, size_t smem, int cluster,
+                            cudaStream_t stream) {
   if (smem > 40 * 1024) {  // (the table is by kernel: instantiations of one signature share this function)
     static std::mutex mu;
     static std::vector<std::pair<int, const void*>> raised;
@@ -552,20 +614,39 @@ static int launch_attn_grid(KernelT kernel, const SeqAttnArgs& a, dim3 grid, siz
   cfg.blockDim = dim3(kSeqThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, a), "attention: kernel launch");
+}
+
+// CTAs of a cluster per (request, KV head), 1: the shares of a line.  Where the pairs alone leave half of the CTAs that fit
+// at once idle and no request can have more than 1024 keys per CTA, a cluster saves the second launch (a request of 576
+// tokens: 4.9 us, 9.9 us by shares; 16 of them 6.9 and 13.8 us); with longer contexts equal shares are worth it (one request of 32000: 18.6 us by
+// shares).
+static int seq_cluster(const SeqAttnArgs& a) {
+  int c = 1;
+  while (c < 8 && 2LL * c * a.B * a.Hkv <= a.grid) c *= 2;
+  return c > 1 && a.max_keys <= 1024LL * c ? c : 1;
 }
 
 template <typename T, int D, int NT, bool PAGED>
 static int launch_seq(const SeqAttnArgs& a, cudaStream_t stream) {
-  int rc = launch_attn_grid(seq_attention_kernel<T, D, NT, PAGED>, a, dim3((unsigned)a.grid), seq_smem_bytes(D), stream);
-  if (rc == LI4_OK && a.grid > 1)
+  const int c = seq_cluster(a);
+  if (c > 1)
+    return launch_attn_grid(seq_attention_kernel<T, D, NT, PAGED, true>, a, dim3((unsigned)(a.B * a.Hkv * c)),
+                            seq_smem_bytes(D), c, stream);
+  int rc = launch_attn_grid(seq_attention_kernel<T, D, NT, PAGED, false>, a, dim3((unsigned)a.grid), seq_smem_bytes(D), 1,
+                            stream);
+  if (rc == LI4_OK)
     rc = launch_attn_grid(seq_attention_join_kernel<T, D, NT, PAGED>, a, dim3((unsigned)a.grid - 1, kJoinShares),
-                          (size_t)a.grid * 8 * NT * sizeof(float), stream);
+                          (size_t)a.grid * 8 * NT * sizeof(float), 1, stream);
   return rc;
 }
 
