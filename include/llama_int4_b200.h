@@ -68,7 +68,7 @@ typedef enum li4_kernel {
 
 /* Library version, (major << 16) | (minor << 8) | patch.  0.2: li4_fusion has the argmax_*
  * fields (callers built against 0.1 pass a shorter struct); the li4_program_* and
- * li4_gather_rows entry points. */
+ * li4_gather_rows entry points.  0.3: the paged KV cache. */
 int li4_version(void);
 
 /* Message describing the last failed call on this host thread ("" if none). */

@@ -55,33 +55,37 @@ struct AppendArgs {
   int vector_out;  // positions and slots start on 16-byte boundaries
 };
 
+// Sums of 64 bits: the lengths are the caller's, and a wrong one must not wrap into a grant.
+struct Sums {
+  long long tokens, pages;
+};
 template <int THREADS>
-__device__ __forceinline__ int2 block_scan2(int2 v, int2* warp_sums, int2* total) {  // exclusive, over the CTA
+__device__ __forceinline__ Sums block_scan2(Sums v, Sums* warp_sums, Sums* total) {  // exclusive, over the CTA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int2 s = v;
+  Sums s = v;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
-    const int x = __shfl_up_sync(0xffffffffu, s.x, d), y = __shfl_up_sync(0xffffffffu, s.y, d);
+    const long long x = __shfl_up_sync(0xffffffffu, s.tokens, d), y = __shfl_up_sync(0xffffffffu, s.pages, d);
     if (lane >= d) {
-      s.x += x;
-      s.y += y;
+      s.tokens += x;
+      s.pages += y;
     }
   }
   if (lane == 31) warp_sums[warp] = s;
   __syncthreads();
-  int2 base = make_int2(0, 0), all = make_int2(0, 0);
+  Sums base = {0, 0}, all = {0, 0};
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) {
-    const int2 p = warp_sums[w];
+    const Sums p = warp_sums[w];
     if (w < warp) {
-      base.x += p.x;
-      base.y += p.y;
+      base.tokens += p.tokens;
+      base.pages += p.pages;
     }
-    all.x += p.x;
-    all.y += p.y;
+    all.tokens += p.tokens;
+    all.pages += p.pages;
   }
   *total = all;
-  return make_int2(base.x + s.x - v.x, base.y + s.y - v.y);
+  return {base.tokens + s.tokens - v.tokens, base.pages + s.pages - v.pages};
 }
 
 // The step of one request: its lengths, checked, and the fresh pages it asks for.
@@ -107,7 +111,7 @@ __global__ void __launch_bounds__(THREADS) paged_append_kernel(const __grid_cons
   int* s_cu = sm;                // [B + 1] first token of each request
   int* s_ctx = s_cu + a.B + 1;   // [B] tokens held before the step
   int* s_rank = s_ctx + a.B;     // [B] number of the request's first fresh page; -1: refused
-  __shared__ int2 warp_sums[THREADS / 32];
+  __shared__ Sums warp_sums[THREADS / 32];
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, rank = (int)cluster.block_rank(), C = (int)cluster.num_blocks();
   const int page = 1 << a.log_page;
@@ -117,29 +121,29 @@ __global__ void __launch_bounds__(THREADS) paged_append_kernel(const __grid_cons
   const int n_free = max(0, min(*a.n_free, a.capacity));
   const int per = (a.B + THREADS - 1) / THREADS;
   const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
-  int2 sum = make_int2(0, 0);  // tokens, pages
+  Sums sum = {0, 0};
   for (int b = b0; b < b1; ++b) {
     int c, n, need;
     append_request(a, b, &c, &n, &need);
-    sum.x += n;
-    sum.y += need;
+    sum.tokens += n;
+    sum.pages += need;
   }
-  int2 total;
-  int2 at = block_scan2<THREADS>(sum, warp_sums, &total);
+  Sums total;
+  Sums at = block_scan2<THREADS>(sum, warp_sums, &total);
   int taken = 0;
   for (int b = b0; b < b1; ++b) {
     int c, n, need;
     const bool fits = append_request(a, b, &c, &n, &need);
     // granted: the table is wide enough, the pages are there, the tokens are among the step's T
-    const bool ok = fits && (need == 0 || at.y + need <= n_free) && at.x + n <= a.T;
-    s_cu[b] = at.x;
+    const bool ok = fits && (need == 0 || at.pages + need <= n_free) && at.tokens + n <= a.T;
+    s_cu[b] = (int)min(at.tokens, 0x7fffffffLL);
     s_ctx[b] = c;
-    s_rank[b] = ok ? at.y : -1;
+    s_rank[b] = !ok ? -1 : need == 0 ? 0 : (int)at.pages;
     if (ok) taken += need;
-    at.x += n;
-    at.y += need;
+    at.tokens += n;
+    at.pages += need;
   }
-  if (tid == 0) s_cu[a.B] = total.x;
+  if (tid == 0) s_cu[a.B] = (int)min(total.tokens, 0x7fffffffLL);
   if (C > 1) cluster.sync();  // everyone has read the lengths and the stack's height
   else __syncthreads();
   if (rank == 0) {
@@ -150,9 +154,8 @@ __global__ void __launch_bounds__(THREADS) paged_append_kernel(const __grid_cons
       a.kv_out[b] = s_rank[b] >= 0 ? s_ctx[b] + n : s_ctx[b];
     }
     __syncthreads();
-    const int2 t = block_scan2<THREADS>(make_int2(0, taken), warp_sums, &total);
-    (void)t;
-    if (tid == 0) *a.n_free_out = n_free - total.y;
+    block_scan2<THREADS>({0, taken}, warp_sums, &total);
+    if (tid == 0) *a.n_free_out = n_free - (int)total.pages;
   }
   const int used = min(s_cu[a.B], a.T);
   const bool wide = a.vector_out != 0;

@@ -698,7 +698,7 @@ static int check_attention(const li4_attention* p, bool paged, const char* what)
       p->n_tokens > (1LL << 30) / p->n_heads)
     return set_error(LI4_ERR_UNSUPPORTED, "%s: n_seqs=%lld n_tokens=%lld n_heads=%lld too large", what,
                      (long long)p->n_seqs, (long long)p->n_tokens, (long long)p->n_heads);
-  if (!(p->scale == p->scale) || p->scale > 3e38f || p->scale < -3e38f)
+  if (!(p->scale == p->scale) || p->scale > 1e38f || p->scale < -1e38f)
     return set_error(LI4_ERR_INVALID_ARG, "%s: the scale is not finite", what);
   if (paged) {
     if (!is_pow2(p->page_size) || p->page_size < 8 || p->page_size > 1024)

@@ -160,6 +160,8 @@ def forward_paged(model, tokens: torch.Tensor, step: PagedStep, cache: PagedKVCa
                   whole_prompts: bool = False) -> torch.Tensor:
     """fp32 logits [requests, vocab] of each request's last token of the step (rows of requests without new tokens
     hold another token's): see Llama.forward_paged."""
+    if tokens.dim() != 1 or tokens.shape[0] == 0:
+        raise ValueError(f"forward_paged: a step has at least one token, tokens [T]; got {list(tokens.shape)}")
     cos, sin = rope_tables(model)
     h = model.tok_embeddings(tokens)
     T = tokens.shape[0]

@@ -426,6 +426,25 @@ def test_paged_append(paged, case, in_place):
         assert kv.tolist() == ctx and nf.tolist() == [free]
 
 
+def test_paged_append_refuses_lengths_out_of_range(paged):
+    """Lengths that are negative or whose sums pass 32 bits take nothing and hurt no one before them."""
+    big = 1 << 29
+    tables = torch.full((9, 6), -1, dtype=torch.int32, device="cuda")
+    ctx = [3, 0, -4, 0, 0, 0, 0, 7, big]
+    new = [2, big, 1, big, big, big, -9, big, 2 * big]
+    nf = i32([5])
+    step = paged.paged_append(i32(ctx), i32(new), tables, i32([4, 5, 6, 7, 8]), nf, 16, 2)
+    assert step.granted.tolist() == [True] + [False] * 8
+    assert step.kv_lens.tolist() == [5] + ctx[1:] and step.n_free.tolist() == [5]
+    assert step.positions.tolist() == [3, 4] and bool((tables == -1).all())
+    assert step.cu_seqlens[:2].tolist() == [0, 2] and step.slots.tolist() == [-16 + 3, -16 + 4]
+    # more tokens than the host counted: the first requests that fit are served
+    tables = torch.full((3, 4), -1, dtype=torch.int32, device="cuda")
+    step = paged.paged_append(i32([0, 0, 0]), i32([3, 4, 5]), tables, i32([1, 2, 3]), i32([3]), 16, 8)
+    assert step.granted.tolist() == [True, True, False] and step.n_free.tolist() == [1]
+    assert step.slots.tolist() == [48, 49, 50, 32, 33, 34, 35, -1]
+
+
 def test_paged_append_table_rows_with_a_stride(paged):
     wide = torch.full((3, 20), -1, dtype=torch.int32, device="cuda")
     step = paged.paged_append(i32([0, 0, 0]), i32([17, 0, 5]), wide[:, :6], i32(list(range(8))), i32([8]), 16, 22)
@@ -548,6 +567,8 @@ def test_model_steps_over_the_paged_cache(paged, heads, kv_heads, page):
     rng = random.Random(1)
     texts = [[rng.randrange(500) for _ in range(200)] for _ in range(4)]
     cache = model.paged_cache(num_pages=-(-200 // page) * 3 + 3, page_size=page, max_requests=3)
+    with pytest.raises(ValueError):
+        model.forward_paged(torch.zeros(0, dtype=torch.long, device="cuda"), None, cache, 0)
     fed, owner = [0, 0, 0], [0, 1, 2]
 
     def step(new, whole=False):
