@@ -678,9 +678,9 @@ int launch_seq_attention(const SeqAttnArgs& args, bool paged, int dtype, int max
 }
 
 // Rows (queries x heads of a KV head) up to which a sequence is streamed: where no sequence has more the streaming
-// kernel runs alone, with tiles of 32 rows; beside longer ones it takes those of one 16-row tile (a decode step's, whose
-// keys then pass through half the registers: 31 requests beside a chunk, 112 us of streaming with 32-row tiles).
-constexpr int kFewRows = 32, kFewRowsBeside = 16;
+// kernel runs alone, with tiles of 8, 16 or 32 rows; beside longer ones it takes those of one 8-row tile (31 requests of
+// 8-row tiles beside a chunk 8 us less than with 16-row tiles).
+constexpr int kFewRows = 32, kFewRowsBeside = 8;
 
 static int check_attention(const li4_attention* p, bool paged, const char* what) {
   if (!p) return set_error(LI4_ERR_INVALID_ARG, "%s: null arguments", what);

@@ -337,8 +337,10 @@ __device__ __forceinline__ int read_next(uint32_t reply) {  // -1: none is left
   return x;
 }
 
-// floats of one item's partial results: 2 x 128 rows of D outputs, then (exponent base, sum) per row
+// One item's partial results: 2 x 128 rows of D outputs, four dims of all rows after four dims of all rows (a warp's lanes
+// are rows), then (exponent base, sum) per row.
 __host__ __device__ constexpr size_t tile_part_floats(int D) { return (size_t)2 * kTileRows * (D + 2); }
+__device__ __forceinline__ size_t tile_part_at(int row, int d) { return ((size_t)(d >> 2) * 2 * kTileRows + row) * 4 + (d & 3); }
 
 template <typename T, int D, bool PAGED>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -777,7 +779,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const bool none = lim < 0;
       const float inv = 1.f / l;
       uint16_t* out = a.s.out + (long long)(w.start + tok) * a.s.sot + (long long)(w.kvh * a.s.rep + row_head) * a.s.soh;
-      float* part = a.s.part + tile_part_floats(D) * (whole ? 0 : w.part) + (size_t)(i * kTileRows) * D;
+      float* part = a.s.part + tile_part_floats(D) * (whole ? 0 : w.part);
       float odd = 0.f;  // becomes NaN with the first output that is not finite
       if (my_steps > 0) {
 #pragma unroll 1
@@ -802,14 +804,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           } else {
 #pragma unroll
             for (int v = 0; v < 8; ++v)
-              *reinterpret_cast<float4*>(part + (size_t)row * D + g * 32 + v * 4) =
+              *reinterpret_cast<float4*>(part + tile_part_at(i * kTileRows + row, g * 32 + v * 4)) =
                   make_float4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
           }
         }
       } else if (valid && whole) {
         for (int d = 0; d < a.s.hd; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
       }
-      float2* ml = reinterpret_cast<float2*>(part + (size_t)(2 - i) * kTileRows * D) + i * kTileRows;
+      float2* ml = reinterpret_cast<float2*>(part + (size_t)2 * kTileRows * D) + i * kTileRows;
       if (!whole && valid) ml[row] = m == -INFINITY ? make_float2(-INFINITY, l) : make_float2(base, l);
       unsigned again = __ballot_sync(0xffffffffu, valid && !none && my_steps > 0 && isfinite(l) && !(odd == 0.f));
       while (again) {
@@ -824,7 +826,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int rt = pr / a.s.rep;
         uint16_t* ro = a.s.out + (long long)(w.start + rt) * a.s.sot + (long long)(w.kvh * a.s.rep + pr % a.s.rep) * a.s.soh;
         for (int e = 0; e < D / 32; ++e) {
-          if (!whole) part[(size_t)r * D + lane + 32 * e] = o[e];
+          if (!whole) part[tile_part_at(i * kTileRows + r, lane + 32 * e)] = o[e];
           else if (lane + 32 * e < a.s.hd) ro[lane + 32 * e] = Type16<T>::one(o[e] / ll);
         }
       }
@@ -861,9 +863,9 @@ __global__ void __launch_bounds__(256) tile_join_kernel(const __grid_constant__ 
   const TileWork w = s_work;
   if (w.b < 0) return;
   const int splits = s_splits;
-  const int r = blockIdx.y * 32 + threadIdx.x / 8, i = r >> 7, row = r & 127;
+  const int r = blockIdx.y * 32 + (threadIdx.x & 31), i = r >> 7, row = r & 127;  // a lane is a row, a warp some dims
   constexpr int W = D / 8;
-  const int d0 = (threadIdx.x & 7) * W;
+  const int d0 = (threadIdx.x >> 5) * W;
   const int row_tok = row / a.s.rep, tok = w.tok0 + i * a.tokens_per_tile + row_tok;
   if (row >= a.tokens_per_tile * a.s.rep || tok >= w.n || d0 >= a.s.hd) return;
   const float* part = a.s.part + tile_part_floats(D) * ((size_t)blockIdx.x * splits);
@@ -881,7 +883,7 @@ __global__ void __launch_bounds__(256) tile_join_kernel(const __grid_constant__ 
     L += f * ml.y;
 #pragma unroll
     for (int e = 0; e < W; e += 4) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(q + (size_t)r * D + d0 + e));
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(q + tile_part_at(r, d0 + e)));
       o[e] += f * v.x;
       o[e + 1] += f * v.y;
       o[e + 2] += f * v.z;
@@ -977,11 +979,12 @@ static int launch_tile(const TileArgs& a, const CUtensorMap& q, const CUtensorMa
   return check_cuda(cudaLaunchKernelEx(&cfg, tile_join_kernel<T, D, PAGED>, a), "attention: kernel launch");
 }
 
-// Items whose partial results the workspace has room for: two per SM, where the pairs of tiles that the tokens alone
-// make do not fill the SMs and some sequence may have enough keys to cut.
+// Items whose partial results the workspace has room for: one per SM, where the pairs of tiles that the tokens alone
+// make do not fill the SMs and some sequence may have enough keys to cut.  (Up to two per SM, a chunk of 512 tokens beside
+// 31 decoding requests took 113 us instead of 100, one of 128 tokens over 32000 keys 74 instead of 67.)
 static int tile_part_slots(int rep, int64_t tokens, int64_t kv_heads, int64_t max_keys, int sm) {
   const int64_t pairs = tokens / (2 * (kTileRows / rep));
-  return pairs * kv_heads >= sm || max_keys <= kTileMinSteps * kTileKeys ? 0 : 2 * sm;
+  return pairs * kv_heads >= sm || max_keys <= kTileMinSteps * kTileKeys ? 0 : sm;
 }
 size_t tile_attention_part_bytes(int hd, int rep, int64_t tokens, int64_t kv_heads, int64_t max_keys, int sm) {
   return (size_t)tile_part_slots(rep, tokens, kv_heads, max_keys, sm) * tile_part_floats(hd <= 64 ? 64 : 128) *
