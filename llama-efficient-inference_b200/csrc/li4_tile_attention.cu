@@ -780,6 +780,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const float inv = 1.f / l;
       uint16_t* out = a.s.out + (long long)(w.start + tok) * a.s.sot + (long long)(w.kvh * a.s.rep + row_head) * a.s.soh;
       float* part = a.s.part + tile_part_floats(D) * (whole ? 0 : w.part);
+      // a row's outputs go out a 32-byte sector at a time where they start on one (16 prompts of 15001 tokens together:
+      // 180 us, 184 with 16-byte stores)
+      const bool sectors = __all_sync(0xffffffffu, (reinterpret_cast<uintptr_t>(out) & 31u) == 0);
       float odd = 0.f;  // becomes NaN with the first output that is not finite
       if (my_steps > 0) {
 #pragma unroll 1
@@ -792,15 +795,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (!valid) continue;
           if (whole) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (g * 32 + v * 8 < a.s.hd) {
-                uint4 u;
-                u.x = Type16<T>::pack(o[v * 8] * inv, o[v * 8 + 1] * inv);
-                u.y = Type16<T>::pack(o[v * 8 + 2] * inv, o[v * 8 + 3] * inv);
-                u.z = Type16<T>::pack(o[v * 8 + 4] * inv, o[v * 8 + 5] * inv);
-                u.w = Type16<T>::pack(o[v * 8 + 6] * inv, o[v * 8 + 7] * inv);
-                *reinterpret_cast<uint4*>(out + g * 32 + v * 8) = none ? make_uint4(0, 0, 0, 0) : u;
+            for (int v = 0; v < 2; ++v) {  // 16 dims: a sector
+              uint32_t u[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                u[e] = none ? 0u : Type16<T>::pack(o[v * 16 + 2 * e] * inv, o[v * 16 + 2 * e + 1] * inv);
+              uint16_t* to = out + g * 32 + v * 16;
+              if (sectors && g * 32 + v * 16 + 16 <= a.s.hd) {
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(u[0]), "r"(u[1]),
+                             "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                             : "memory");
+              } else {
+                if (g * 32 + v * 16 < a.s.hd) *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
+                if (g * 32 + v * 16 + 8 < a.s.hd) *reinterpret_cast<uint4*>(to + 8) = make_uint4(u[4], u[5], u[6], u[7]);
               }
+            }
           } else {
 #pragma unroll
             for (int v = 0; v < 8; ++v)
