@@ -116,6 +116,62 @@ def test_prompt_attention_long_against_tiles(paged, d):
         check(got[i:i + 1], q[i:i + 1], [k[:i + 1]], [v[:i + 1]], [1])
 
 
+def test_prompt_attention_very_long(paged):
+    n, dtype = 70001, torch.float16
+    q, k, v = rand((n, 2, 64), dtype, 4), rand((n, 1, 64), dtype, 5), rand((n, 1, 64), dtype, 6)
+    got = paged.prompt_attention(q, k, v, i32([0, n]), n)
+    for i in [0, 1, 127, 128, 4095, 32768, 65535, 65536, 69999, 70000]:
+        check(got[i:i + 1], q[i:i + 1], [k[:i + 1]], [v[:i + 1]], [1])
+
+
+@pytest.mark.parametrize("claim", [1, 50])
+def test_prompt_attention_many_prompts(paged, claim):
+    """More sequences than one round of the item search looks at, some of them empty."""
+    lens = [(7 * b) % 50 for b in range(150)]
+    T = sum(lens)
+    q, k, v = rand((T, 4, 32), torch.bfloat16, 7), rand((T, 2, 32), torch.bfloat16, 8), rand((T, 2, 32), torch.bfloat16, 9)
+    got = paged.prompt_attention(q, k, v, i32(cumulative(lens)), claim)
+    check(got, q, list(k.split(lens)), list(v.split(lens)), lens)
+
+
+def test_two_prompt_batches_at_once(paged):
+    """Calls on two streams at the same time give what they give alone."""
+    batches = []
+    for i in range(2):
+        lens = [900 + 100 * i, 333, 1500]
+        T = sum(lens)
+        q, k, v = (rand((T, h, 128), torch.float16, 60 + 3 * i + h) for h in (8, 2, 2))
+        batches.append((q, k, v, i32(cumulative(lens)), 1500))
+    want = [paged.prompt_attention(*b) for b in batches]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(paged.prompt_attention(*batches[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_long_chunk_is_cut_and_joined_alike_every_time(paged, d):
+    """Few items over many keys: ranges of keys on different SMs, joined in order."""
+    ck, cv, tables, keys, values = make_cache([9001, 40], 2, d, 32, torch.bfloat16, 70)
+    q = rand((170, 8, d), torch.bfloat16, 71)
+    args = (q, ck, cv, tables, i32([9001, 40]), i32([0, 130, 170]), 130)
+    got = paged.paged_attention(*args)
+    check(got, q, keys, values, [130, 40])
+    for _ in range(3):
+        assert torch.equal(got, paged.paged_attention(*args))
+
+
+def test_no_bounded_wait_ran_out(paged):
+    from llama import _native
+
+    assert _native.device_errors() == 0
+
+
 def test_prompt_attention_wrong_max_len_is_only_slower(paged):
     lens = [200, 31]
     q, k, v = (rand((231, h, 64), torch.float16, 7 + h) for h in (8, 2, 2))
@@ -142,6 +198,10 @@ def test_prompt_attention_strided_rows_and_rows_past_the_end(paged, dtype):
     n = sum(lens)
     check(out[:n], q[:n], list(k[:n].split(lens)), list(v[:n].split(lens)), lens)
     assert bool((wide[n:] == 7).all()) and bool((wide[..., d:] == 7).all())
+    # rows of the output that start 16 bytes past a 32-byte sector
+    odd_out = torch.full((T, H, d + 16), 7.0, dtype=dtype, device="cuda")
+    assert torch.equal(paged.prompt_attention(q, k, v, i32(cumulative(lens)), 100, out=odd_out[..., 8:8 + d])[:n], out[:n])
+    assert bool((odd_out[n:] == 7).all()) and bool((odd_out[..., :8] == 7).all()) and bool((odd_out[..., 8 + d:] == 7).all())
     # other layouts: heads outermost, a misaligned first element, a broadcast key head
     q2 = q[:n].transpose(0, 1).contiguous().transpose(0, 1)
     odd = torch.empty(n * Hkv * d + 1, dtype=dtype, device="cuda")[1:].view(n, Hkv, d)
