@@ -3,10 +3,10 @@
 // Grouped-query attention by rows: the rep query heads of a KV head, over the queries of a sequence,
 // are the rows of one matrix (row = query * rep + head), so a KV head's keys and values are read once
 // for the whole group.  An item is (sequence, tile of 8 NT rows, KV head); its keys come in units of
-// 128 (64 dims) or 64 (128 dims).  Units of all items lie on one line; CTA g of G takes the g-th equal share of it, whatever the
-// lengths are (they are read on the device: the host knows none).  A CTA that covers only a part of an
-// item's keys leaves (running maximum, sum, unnormalised output) in `part`, and a second launch joins
-// the parts in key order, so the result does not depend on timing.
+// 128 (64 dims) or 64 (128 dims).  Units of all items lie on one line; CTA g of G takes the g-th equal
+// share of it, whatever the lengths are (they are read on the device: the host knows none).  A CTA that
+// covers only a part of an item's keys leaves (running maximum, sum, unnormalised output) in `part`, and
+// a second launch joins the parts in key order, so the result does not depend on timing.
 //
 // Inside a CTA each of the 4 warps streams its own quarter of every unit through its own ring of
 // shared-memory stages (cp.async; no CTA barrier until the end): S^T = K Q^T and O^T += V^T P^T as

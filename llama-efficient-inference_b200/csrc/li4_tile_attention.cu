@@ -11,7 +11,11 @@
 //   warp 9  (MMA)   S_i = Q_i K^T (M 128, N 128 keys) into tensor memory, O_i += P_i V (A = P_i from tensor
 //                   memory, N = dims, V as it lies: N-major) accumulated there over the whole item
 //   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a row (tensor-memory lane) and needs no exchange;
-//                   P in the 16-bit type replaces S in its columns
+//                   writes P in the 16-bit type
+//   warp 10         the CTA's next item, when the present one nears its end
+//
+// Prompts of 8192 tokens (32 / 8 heads, fp16): 457 us at 128 dims, 1.2 PFLOP/s, where the power limit holds the clock
+// near 1.6 GHz; 360 us at 64 dims, bound by the softmax's issue and latency.
 //
 // The running maximum moves lazily: probabilities are taken against a maximum that may lag up to 2^8
 // behind (P <= 256 fits both 16-bit types, the sum is fp32), so the accumulated output is rescaled only
@@ -43,7 +47,7 @@ int tile_device_errors(unsigned* flags, bool reset) {
 
 constexpr int kTileRows = 128;       // rows of a tile: tensor-memory lanes
 constexpr int kTileKeys = 128;       // keys of a step
-constexpr int kTileThreads = 384;    // 8 softmax warps, the TMA warp, the MMA warp, 2 that only fill their group
+constexpr int kTileThreads = 384;    // 8 softmax warps, the TMA, MMA and item warps, one that only fills its group
 constexpr int kTmaWarp = 8, kMmaWarp = 9;
 constexpr unsigned kTileWaitLimit = 1u << 24;  // polls
 constexpr int kTileMinSteps = 8;     // key tiles below which a range is not cut
@@ -497,6 +501,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         unsigned more = kTileWaitLimit;
         for (unsigned i = base > NS ? base - NS : 0; i < base; ++i) tile_wait(&kv_full[i % NS], (i / NS) & 1, more);
         if (qn > 0) tile_wait(q_full, (qn - 1) & 1, more);
+        if (tails > 0) tile_wait(v_tail, (tails - 1) & 1, more);
       }
     } else if (warp == kMmaWarp) {
       // ---- products, tile 0 then tile 1 (a warp per tile was slower: their products then share the tensor cores and
@@ -644,6 +649,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         __syncwarp();
         tile_wait(replied, k & 1, limit);
+        if (limit == 1) {  // (the reply is still to land: once more before the memory goes)
+          unsigned more = kTileWaitLimit;
+          tile_wait(replied, k & 1, more);
+          break;
+        }
         index = read_next(smem_addr(reply));
         __syncwarp();
       }
