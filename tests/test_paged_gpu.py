@@ -82,7 +82,7 @@ def check(got, q, keys, values, lens, scale=None):
 
 
 HEADS = [(32, 8, 64), (8, 2, 128), (4, 4, 64), (7, 1, 128), (6, 2, 32), (12, 4, 80), (2, 1, 8), (40, 8, 64),
-         (16, 1, 64), (5, 1, 112)]
+         (16, 1, 64), (5, 1, 112), (128, 1, 64), (100, 1, 24)]
 PROMPTS = [[1], [2, 1], [33], [128], [0, 5, 0, 17, 0], [129, 127, 1, 64], [300, 3, 257]]
 
 
@@ -266,7 +266,7 @@ STEPS = [  # (new tokens, tokens of the cache with them) per request
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("step", STEPS, ids=str)
 @pytest.mark.parametrize("H,Hkv,d,page", [(32, 8, 64, 16), (8, 2, 128, 64), (7, 1, 128, 8), (6, 2, 32, 256),
-                                          (4, 4, 64, 128), (12, 4, 80, 32)])
+                                          (4, 4, 64, 128), (12, 4, 80, 32), (24, 1, 128, 1024)])
 def test_paged_attention(paged, H, Hkv, d, page, step, dtype):
     new, kv = [s[0] for s in step], [s[1] for s in step]
     ck, cv, tables, keys, values = make_cache(kv, Hkv, d, page, dtype, 20)
