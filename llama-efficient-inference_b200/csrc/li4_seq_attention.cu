@@ -14,7 +14,7 @@
 // pass.  The keys are the 16-wide side and the rows the 8-wide one, so a group of 4 or 8 heads wastes
 // half of a tile or nothing (with the rows as the 16-wide side 64 requests of 300-16000 tokens took
 // 85 us instead of 81).  The work is bound by the bytes of the keys and values as long as the rows
-// are few: those 419 MB are read at 5.2 TB/s, and no faster with the products left out.
+// are few: those 419 MB now take 77 us, 5.5 TB/s with the join, and with the products left out no less.
 #include <cooperative_groups.h>
 
 #include <mutex>
@@ -41,18 +41,22 @@ __host__ __device__ constexpr int seq_smem_bytes(int D) { return kSeqWarps * kSe
 // floats of one partial result: 8 NT rows of D outputs, then (maximum, sum) per row
 __host__ __device__ constexpr int seq_part_floats(int D, int NT) { return 8 * NT * (D + 2); }
 
-// The line of units.
+// The line of units.  An item takes kItemUnits more than its keys do: starting it and joining its warps cost about that
+// much time (256 requests of 100-4000 tokens: 143 us without, 108 with 4, 107 with 2, 109 with 6; 64 of
+// 300-16000 tokens 81, 77, 79, 78 us).
+constexpr int kItemUnits = 4;
 struct Line {
   long long total;
   int active;  // CTAs that get a share
 };
 __device__ __forceinline__ long long share(const Line& l, int g) { return l.total * g / l.active; }
 
+// Key units of an item and the units that a sequence takes.
 template <int D, int NT>
 __device__ __forceinline__ long long seq_units(const SeqAttnArgs& a, const Seq& s, int* tiles, int* per) {
   *tiles = (int)(((long long)s.n * a.rep + 8 * NT - 1) / (8 * NT));
   *per = max(1, (s.len + seq_unit(D) - 1) / seq_unit(D));
-  return (long long)*tiles * *per * a.Hkv;
+  return (long long)*tiles * (*per + kItemUnits) * a.Hkv;
 }
 
 // Finds the sequence that holds unit share(g): each thread sums a slice of the sequences.  Every thread
@@ -237,16 +241,18 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
   }
 
   while (left > 0) {
-    int kvh, tile, u0, u1;
+    int kvh, tile, u0, u1, r0 = 0, r1 = 0;  // key units; units of the item
     if constexpr (CL) {
       kvh = g / ranks % a.Hkv;
       tile = (int)rem;
       u0 = per * rank / ranks;
       u1 = per * (rank + 1) / ranks;
     } else {
-      const int item = (int)(rem / per);
-      u0 = (int)(rem - (long long)item * per);
-      u1 = (int)min((long long)per, u0 + left);
+      const int span = per + kItemUnits, item = (int)(rem / span);
+      r0 = (int)(rem - (long long)item * span);
+      r1 = (int)min((long long)span, r0 + left);
+      u0 = max(0, r0 - kItemUnits);
+      u1 = max(0, r1 - kItemUnits);
       kvh = item % a.Hkv;
       tile = item / a.Hkv;
     }
@@ -423,11 +429,11 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
       }
     if (tid < RT) s_redo[tid] = 0;
     __syncthreads();
-    const bool whole = !CL && u0 == 0 && u1 == per;
+    const bool whole = !CL && r0 == 0 && r1 == per + kItemUnits;
     const bool masked = k1 - 1 > first_lim;  // some row must not see some of the keys read
     // where a part of the item's result goes: the workspace, or this CTA's shared memory past the warps' outputs
     float* part = CL ? reinterpret_cast<float*>(smem) + kSeqWarps * RT * LD
-                     : a.part + (size_t)(2 * g + (u0 == 0 ? 1 : 0)) * seq_part_floats(D, NT);
+                     : a.part + (size_t)(2 * g + (r0 == 0 ? 1 : 0)) * seq_part_floats(D, NT);
     const float* all = reinterpret_cast<const float*>(smem);
     for (int e = tid; e < RT * D / 2; e += kSeqThreads) {
       const int r = e / (D / 2), d = (e - r * (D / 2)) * 2;
@@ -511,10 +517,10 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
       ++rem;
       continue;
     }
-    left -= u1 - u0;
-    rem += u1 - u0;
-    while (left > 0 && rem >= (long long)tiles * per * a.Hkv) {
-      rem -= (long long)tiles * per * a.Hkv;
+    left -= r1 - r0;
+    rem += r1 - r0;
+    while (left > 0 && rem >= (long long)tiles * (per + kItemUnits) * a.Hkv) {
+      rem -= (long long)tiles * (per + kItemUnits) * a.Hkv;
       s = load_seq<PAGED>(a, ++b);
       seq_units<D, NT>(a, s, &tiles, &per);
     }
@@ -540,8 +546,8 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_join_kernel(const _
   int tiles, per;
   seq_units<D, NT>(a, s, &tiles, &per);
   const long long rem = share(line, g) - before;
-  const int item = (int)(rem / per);
-  const long long start = before + (long long)item * per, end = start + per;
+  const int span = per + kItemUnits, item = (int)(rem / span);
+  const long long start = before + (long long)item * span, end = start + span;
   if (start == share(line, g) || share(line, g - 1) > start) return;
   // the parts are CTAs g - 1 (from the item's start) and g .. last, the last CTA with share(last) < end
   const int last = (int)min((long long)line.active - 1, (end * line.active - 1) / line.total);
