@@ -802,8 +802,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tmem_ld_wait(o);
 #pragma unroll
           for (int e = 0; e < 32; ++e) odd = fmaf(o[e], 0.f, odd);
-          if (!valid) continue;
-          if (whole) {
+          if (valid && whole) {
 #pragma unroll
             for (int v = 0; v < 2; ++v) {  // 16 dims: a sector
               uint32_t u[8];
@@ -820,18 +819,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if (g * 32 + v * 16 + 8 < a.s.hd) *reinterpret_cast<uint4*>(to + 8) = make_uint4(u[4], u[5], u[6], u[7]);
               }
             }
-          } else {
+          } else if (valid) {
 #pragma unroll
             for (int v = 0; v < 8; ++v)
               *reinterpret_cast<float4*>(part + tile_part_at(i * kTileRows + row, g * 32 + v * 4)) =
                   make_float4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
           }
+          __syncwarp();  // (the next load takes the whole warp)
         }
       } else if (valid && whole) {
         for (int d = 0; d < a.s.hd; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
       }
       float2* ml = reinterpret_cast<float2*>(part + (size_t)2 * kTileRows * D) + i * kTileRows;
       if (!whole && valid) ml[row] = m == -INFINITY ? make_float2(-INFINITY, l) : make_float2(base, l);
+      __syncwarp();  // (other lanes write a row again below)
       unsigned again = __ballot_sync(0xffffffffu, valid && !none && my_steps > 0 && isfinite(l) && !(odd == 0.f));
       while (again) {
         const int src = __ffs(again) - 1;
