@@ -20,12 +20,20 @@
 // The running maximum moves lazily: probabilities are taken against a maximum that may lag up to 2^8
 // behind (P <= 256 fits both 16-bit types, the sum is fp32), so the accumulated output is rescaled only
 // when a row's maximum grows by more than that -- rarely after the first tiles.
+//
+// A masked key's probability is zero, but zero times a NaN or an infinity is NaN: a value that a row must not see can
+// reach it through the last few key tiles of an item, where some keys are hidden from some rows.  A CTA that meets an
+// output that is not finite therefore runs that item again, and its later ones from the start, with care (every role's
+// code exists twice, so the usual pass is spared the tests): the copying warp takes the values that are not finite out of those tiles before the products may have them and notes where in each
+// dim the first +inf, -inf or NaN stood, and a row that sees that key gets it added at the end (added to a
+// sum, what is not finite does not depend on its weight).  At most two items of a CTA run twice, whatever the context.
 // Every mbarrier wait is bounded: one that runs out sets bit 8 of li4_device_errors; every role then
 // runs to its end without waiting, copies and MMAs in flight are waited for (bounded) and the tensor
 // memory is freed.
 #include <cuda.h>
 
 #include <mutex>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -51,11 +59,12 @@ constexpr int kTileThreads = 384;    // 8 softmax warps, the TMA, MMA and item w
 constexpr int kTmaWarp = 8, kMmaWarp = 9;
 constexpr unsigned kTileWaitLimit = 1u << 24;  // polls
 constexpr int kTileMinSteps = 8;     // key tiles below which a range is not cut
+constexpr int kUnseen = 0x7fffffff;   // no key
 constexpr float kLazyLog2 = 8.f;     // how far the maximum in use may lag, in powers of two
 
 __host__ __device__ constexpr int tile_slots(int D) { return D == 64 ? 8 : 4; }
 __host__ __device__ constexpr int tile_bytes(int D) { return 128 * D * 2; }  // a tile of queries, keys or values
-__host__ __device__ constexpr int tile_smem_bytes(int D) { return 1024 + (2 + tile_slots(D)) * tile_bytes(D) + 512; }
+__host__ __device__ constexpr int tile_smem_bytes(int D) { return 1024 + (2 + tile_slots(D)) * tile_bytes(D) + 512 + 16 * D; }
 
 // Which of 16 pairs of probabilities the polynomial takes (8192 tokens at 64 dims: none 387 us, 2 378 us, 4 360 us,
 // 5 370 us; at 128 dims, where the products and the power limit bound, 459, 456, 460, 466 us).
@@ -212,8 +221,8 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // its exponentials are taken here: x = n + f with n the nearest integer (added to 1.5 * 2^23, which leaves n in the low
 // bits), 2^f on [-1/2, 1/2] by a polynomial with value 1 at 0 fitted for the least largest relative error
 // (degree 5: 9.2e-8; 1.7e-7 evaluated in fp32, the size of the unit's own error), n added to the exponent bits.  x is
-// held at -127, where the sum of bits is exactly zero: a masked score gives probability 0.  NaN passes the bound; its
-// bits end up as a huge value that the 16-bit type turns into an infinity.
+// held at -127, where the sum of bits is exactly zero: a masked score gives probability 0.  NaN passes the bound and its
+// bits end up as the largest finite value; the row's maximum is NaN then, which makes its sum NaN.
 __device__ __forceinline__ void exp2_pair(uint64_t v, float* x, float* y) {
   unpack2(v, x, y);
   asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(*x));  // -127
@@ -234,9 +243,15 @@ __device__ __forceinline__ void exp2_pair(uint64_t v, float* x, float* y) {
   *x = __uint_as_float(__float_as_uint(px) + (__float_as_uint(tx) << 23));
   *y = __uint_as_float(__float_as_uint(py) + (__float_as_uint(ty) << 23));
 }
+// (NaN where one of them is)
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -274,7 +289,7 @@ template <bool PAGED>
 __device__ __forceinline__ TileWork find_item(const TileArgs& a, int index, int splits) {
   const int lane = threadIdx.x & 31;
   const int per_pair = 2 * a.tokens_per_tile, number = index;
-  TileWork w;
+  TileWork w = {};
   w.b = -1;
   for (int b0 = 0; b0 < a.s.B; b0 += 32) {
     int items = 0, pairs = 0;
@@ -346,6 +361,48 @@ __device__ __forceinline__ int read_next(uint32_t reply) {  // -1: none is left
 __host__ __device__ constexpr size_t tile_part_floats(int D) { return (size_t)2 * kTileRows * (D + 2); }
 __device__ __forceinline__ size_t tile_part_at(int row, int d) { return ((size_t)(d >> 2) * 2 * kTileRows + row) * 4 + (d & 3); }
 
+// Takes what is not finite out of rows [from, to) of a value tile (the warp's lanes are rows) and notes, per dim, the first
+// key with +inf or NaN and the first with -inf or NaN: `first` is [2][D].
+template <typename T, int D>
+__device__ __noinline__ void take_out(uint8_t* tile, int from, int to, int key0, int* first) {
+  constexpr uint16_t INF = __is_same(T, __half) ? 0x7c00 : 0x7f80;
+  for (int r = from + (threadIdx.x & 31); r < to; r += 32) {
+#pragma unroll 1
+    for (int c = 0; c < D / 8; ++c) {  // the chunk of dims 8 c .. 8 c + 7: at c ^ r of its row (128-byte swizzle)
+      uint4* at = reinterpret_cast<uint4*>(tile + (c >> 3) * (tile_bytes(D) * 64 / D) + r * 128 + ((c ^ r) & 7) * 16);
+      const uint4 v = *at;
+      uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint16_t x = (uint16_t)(u[e >> 1] >> (e & 1) * 16);
+        if ((x & 0x7fff) < INF) continue;
+        if (x != (INF | 0x8000)) atomicMin(first + 8 * c + e, key0 + r);
+        if (x != INF) atomicMin(first + D + 8 * c + e, key0 + r);
+        u[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+        *at = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+    }
+  }
+}
+
+// Adds what was taken out to the outputs of the warp's rows (lane's row sees keys up to last).
+template <int D>
+__device__ __noinline__ void put_back(uint32_t o_at, const int* first, int last) {
+#pragma unroll 1
+  for (int g = 0; g < D / 32; ++g) {
+    float o[32];
+    tmem_ld32(o_at + g * 32, o);
+    tmem_ld_wait(o);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      if (last >= first[g * 32 + e]) o[e] += INFINITY;
+      if (last >= first[g * 32 + e + D]) o[e] -= INFINITY;
+    }
+    tmem_st32(o_at + g * 32, o);
+  }
+  tmem_st_wait();
+}
+
 template <typename T, int D, bool PAGED>
 __global__ void __launch_bounds__(kTileThreads, 1)
     tile_attention_kernel(const __grid_constant__ TileArgs a, const __grid_constant__ CUtensorMap map_q,
@@ -375,8 +432,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* work_empty = work_full + 2;  // [2] the 10 working warps have read it
   uint64_t* replied = work_empty + 2;    // the reply is there
   uint64_t* ending = replied + 1;        // the products are near the item's end
-  TileWork* work = reinterpret_cast<TileWork*>(ending + 1);  // [2]
+  uint64_t* taken_out = ending + 1;      // [2] an item's infinities and NaNs are noted (items taken with care alone)
+  TileWork* work = reinterpret_cast<TileWork*>(taken_out + 2);  // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(work + 2);
+  volatile int* again = reinterpret_cast<int*>(tmem_holder + 1);  // [2] by item parity: one to run again
+  volatile int* gave_up = again + 2;             // a wait of the usual pass ran out
+  int* first_bad = const_cast<int*>(again) + 3;  // [2][2][D] of items taken with care: see take_out
+  static_assert(16 + (2 * NS + 22) * 8 + 2 * sizeof(TileWork) + 16 <= 512, "what lies behind the tiles fits");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
@@ -400,6 +462,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     mbar_init(drained, 1);
     mbar_init(replied, 1);
     mbar_init(ending, 1);
+    mbar_init(&taken_out[0], 1);
+    mbar_init(&taken_out[1], 1);
+    again[0] = again[1] = *gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -428,6 +493,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (lane == 0) mbar_arrive(&work_empty[k & 1]);
     return w;
   };
+  // The end of the usual pass, where every warp meets.  True: a pass with care follows.
+  auto go_again = [&]() {
+    if (limit == 1 && lane == 0) *gave_up = 1;
+    tc_fence_before();
+    __syncthreads();
+    return *gave_up == 0 && again[0] + again[1] > 0;
+  };
+  auto end_care = [&]() {
+    tc_fence_before();
+    __syncthreads();
+  };
+  // The item's first key tile with a key that some row of it must not see.
+  auto masked_from = [](const TileWork& w) {
+    return max(0, (max(0, w.len - w.n + w.tok0 + 1) >> 7) - w.first);
+  };
   // Keys of the item's last key tile; P V takes them in groups of 16, and rows of the last group past the end are made
   // zeros (what lies there may be anything, and 0 x NaN is NaN).
   auto tail_rows_of = [](const TileWork& w, int nk) { return min(kTileKeys, w.len - (w.first + nk - 1) * kTileKeys); };
@@ -438,70 +518,93 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == kTmaWarp) {
       // ---- copies
+      int k = 0;
       unsigned base = 0, qn = 0, tails = 0;  // ring tiles, query loads and mended tails of earlier items
-      for (int k = 0;; ++k) {
-        const TileWork w = next_work(k);
-        if (w.b < 0) break;
-        const int nk = max(w.steps[0], w.steps[1]);
-        if (nk == 0) continue;
-        if (qn > 0) tile_wait(q_empty, (qn - 1) & 1, limit);
-        ++qn;
-        if (lane == 0) {
-          // a tile whose queries all lie past the sequence, or that sees no key of the range, is not loaded
-          const int lo = w.steps[0] > 0 ? 0 : 1, hi = w.steps[1] > 0 ? 2 : 1;
-          mbar_arrive_expect_tx(q_full, (hi - lo) * SUB * TPT * a.s.rep * 128);
-          for (int i = lo; i < hi; ++i)
-            for (int c = 0; c < SUB; ++c)
-              tma_load4(smem_addr(smem + i * TB + c * (TB / SUB)), &map_q, q_full, c * 64, 0, w.kvh,
-                        w.start + w.tok0 + i * TPT);
-        }
-        const int tail = tail_rows_of(w, nk), end = (tail + 15) / 16 * 16;
-        for (int n = 0; n < 2 * nk; ++n) {
-          const bool value = !EARLY ? n & 1 : n == 2 * nk - 1 || (n > 0 && !(n & 1));
-          const int j = !EARLY ? n / 2 : n == 2 * nk - 1 ? nk - 1 : value ? n / 2 - 1 : (n + 1) / 2;
-          const int key0 = (w.first + j) * kTileKeys;
-          int row = w.start + key0, page = 0;
-          bool mine = lane == 0;
-          int boxes = 1;
-          if constexpr (PAGED) {
-            boxes = (min(kTileKeys, w.len - key0) + a.box_rows - 1) / a.box_rows;
-            mine = lane < boxes;
-            const int key = key0 + lane * a.box_rows;
-            row = key & ((1 << a.s.log_page) - 1);
-            // an entry outside the cache is a coordinate outside the tensor: zeros
-            if (mine) page = a.s.tables[(long long)w.b * a.s.table_stride + (key >> a.s.log_page)];
+      auto pass = [&](auto care) {
+        constexpr bool CARE = decltype(care)::value;
+        unsigned cares = 0;
+        for (;;) {
+          const TileWork w = next_work(k++);
+          if (w.b < 0) break;
+          const int nk = max(w.steps[0], w.steps[1]);
+          if (nk == 0) continue;
+          if (qn > 0) tile_wait(q_empty, (qn - 1) & 1, limit);
+          ++qn;
+          if (lane == 0) {
+            // a tile whose queries all lie past the sequence, or that sees no key of the range, is not loaded
+            const int lo = w.steps[0] > 0 ? 0 : 1, hi = w.steps[1] > 0 ? 2 : 1;
+            mbar_arrive_expect_tx(q_full, (hi - lo) * SUB * TPT * a.s.rep * 128);
+            for (int i = lo; i < hi; ++i)
+              for (int c = 0; c < SUB; ++c)
+                tma_load4(smem_addr(smem + i * TB + c * (TB / SUB)), &map_q, q_full, c * 64, 0, w.kvh,
+                          w.start + w.tok0 + i * TPT);
           }
-          // the last value tile with missing rows arrives on a barrier of its own and counts as full once they are zeros
-          const bool mend = n == 2 * nk - 1 && tail < end;
-          const unsigned g = base + n, slot = g % NS;
-          uint64_t* bar = mend ? v_tail : &kv_full[slot];
-          if (g >= NS) tile_wait(&kv_empty[slot], ((g / NS) - 1) & 1, limit);
-          if (lane == 0) mbar_arrive_expect_tx(bar, boxes * a.box_rows * SUB * 128);
-          __syncwarp();
-          if (mine)
-            for (int c = 0; c < SUB; ++c)
-              tma_load4(smem_addr(ring + slot * TB + c * (TB / SUB)) + lane * a.box_rows * 128, value ? &map_v : &map_k,
-                        bar, c * 64, row, w.kvh, page);
-          if (mend) {
-            tile_wait(v_tail, tails & 1, limit);
-            ++tails;
-            for (int e = lane; e < (end - tail) * SUB * 8; e += 32) {
-              const int r = tail + e / (SUB * 8), c = e % (SUB * 8);
-              *reinterpret_cast<uint4*>(ring + slot * TB + (c >> 3) * (TB / SUB) + r * 128 + (c & 7) * 16) =
-                  make_uint4(0, 0, 0, 0);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          const int tail = tail_rows_of(w, nk), end = (tail + 15) / 16 * 16;
+          const int care_from = CARE ? masked_from(w) : nk;
+          int* bad = first_bad + (cares & 1) * 2 * D;
+          if constexpr (CARE) {
+            for (int e = lane; e < 2 * D; e += 32) bad[e] = kUnseen;
             __syncwarp();
-            if (lane == 0) mbar_arrive(&kv_full[slot]);
           }
+          for (int n = 0; n < 2 * nk; ++n) {
+            const bool value = !EARLY ? n & 1 : n == 2 * nk - 1 || (n > 0 && !(n & 1));
+            const int j = !EARLY ? n / 2 : n == 2 * nk - 1 ? nk - 1 : value ? n / 2 - 1 : (n + 1) / 2;
+            const int key0 = (w.first + j) * kTileKeys;
+            int row = w.start + key0, page = 0;
+            bool mine = lane == 0;
+            int boxes = 1;
+            if constexpr (PAGED) {
+              boxes = (min(kTileKeys, w.len - key0) + a.box_rows - 1) / a.box_rows;
+              mine = lane < boxes;
+              const int key = key0 + lane * a.box_rows;
+              row = key & ((1 << a.s.log_page) - 1);
+              // an entry outside the cache is a coordinate outside the tensor: zeros
+              if (mine) page = a.s.tables[(long long)w.b * a.s.table_stride + (key >> a.s.log_page)];
+            }
+            // the last value tile with missing rows, and with care each that has hidden keys, arrives on a barrier of its
+            // own and counts as full once its rows are mended
+            const bool mend = (n == 2 * nk - 1 && tail < end) || (value && j >= care_from);
+            const unsigned g = base + n, slot = g % NS;
+            uint64_t* bar = mend ? v_tail : &kv_full[slot];
+            if (g >= NS) tile_wait(&kv_empty[slot], ((g / NS) - 1) & 1, limit);
+            if (lane == 0) mbar_arrive_expect_tx(bar, boxes * a.box_rows * SUB * 128);
+            __syncwarp();
+            if (mine)
+              for (int c = 0; c < SUB; ++c)
+                tma_load4(smem_addr(ring + slot * TB + c * (TB / SUB)) + lane * a.box_rows * 128, value ? &map_v : &map_k,
+                          bar, c * 64, row, w.kvh, page);
+            if (mend) {
+              tile_wait(v_tail, tails & 1, limit);
+              ++tails;
+              for (int e = n < 2 * nk - 1 ? kTileKeys * SUB * 8 : lane; e < (end - tail) * SUB * 8; e += 32) {
+                const int r = tail + e / (SUB * 8), c = e % (SUB * 8);
+                *reinterpret_cast<uint4*>(ring + slot * TB + (c >> 3) * (TB / SUB) + r * 128 + (c & 7) * 16) =
+                    make_uint4(0, 0, 0, 0);
+              }
+              if constexpr (CARE) take_out<T, D>(ring + slot * TB, 0, n < 2 * nk - 1 ? kTileKeys : tail, key0, bad);
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&kv_full[slot]);
+            }
+          }
+          if constexpr (CARE) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&taken_out[cares & 1]);
+            ++cares;
+          }
+          base += 2 * nk;
         }
-        base += 2 * nk;
-      }
-      if (limit == 1) {  // a wait ran out: copies in flight land before the memory goes
-        unsigned more = kTileWaitLimit;
-        for (unsigned i = base > NS ? base - NS : 0; i < base; ++i) tile_wait(&kv_full[i % NS], (i / NS) & 1, more);
-        if (qn > 0) tile_wait(q_full, (qn - 1) & 1, more);
-        if (tails > 0) tile_wait(v_tail, (tails - 1) & 1, more);
+        if (limit == 1) {  // a wait ran out: copies in flight land before the memory goes
+          unsigned more = kTileWaitLimit;
+          for (unsigned i = base > NS ? base - NS : 0; i < base; ++i) tile_wait(&kv_full[i % NS], (i / NS) & 1, more);
+          if (qn > 0) tile_wait(q_full, (qn - 1) & 1, more);
+          if (tails > 0) tile_wait(v_tail, (tails - 1) & 1, more);
+        }
+      };
+      pass(std::false_type{});
+      if (go_again()) {
+        pass(std::true_type{});
+        end_care();
       }
     } else if (warp == kMmaWarp) {
       // ---- products, tile 0 then tile 1 (a warp per tile was slower: their products then share the tensor cores and
@@ -510,153 +613,186 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const uint32_t q_desc = desc_k_major(smem_addr(smem)), k_desc = desc_k_major(smem_addr(ring)),
                      v_desc = desc_n_major(smem_addr(ring), TB / SUB);
       unsigned base = 0, qn = 0, done0 = 0, done1 = 0;  // of earlier items: ring tiles, query loads, steps
-      for (int k = 0;; ++k) {
-        const TileWork w = next_work(k);
-        if (w.b < 0) break;
-        const int nk = max(w.steps[0], w.steps[1]);
-        if (nk == 0) {
-          if (lane == 0) mbar_arrive(ending);
-          continue;
-        }
-        const int tail_groups = (tail_rows_of(w, nk) + 15) / 16;
-        auto full = [&](unsigned n) { return &kv_full[(base + n) % NS]; };
-        auto phase = [&](unsigned n) { return (base + n) / NS & 1u; };
-        auto scores = [&](int i, unsigned slot) {  // S_i against the key tile in a slot
-          const uint32_t qd = q_desc + i * (TB >> 4), kd = k_desc + slot * (TB >> 4);
-#pragma unroll
-          for (int c = 0; c < SUB; ++c)
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_ss(tmem + S_COL + i * 128, qd + ((c * (TB / SUB) + kk * 32) >> 4),
-                     kd + ((c * (TB / SUB) + kk * 32) >> 4), IDESC_S, c + kk > 0);
-          tc_commit(&s_full[i]);
-        };
-        // keys 64 h .. 64 h + 64 of P_i V with the value tile in a slot
-        auto outputs = [&](int i, unsigned slot, int h, bool first, int groups) {
-          const uint32_t vd = v_desc + slot * (TB >> 4) + h * 512;
-          const uint32_t o = tmem + O_COL + i * D, pr = tmem + P_COL + i * P_STEP + h * 32;
-          if (groups == 8) {
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, !first || h + kk > 0);
-          } else {
-#pragma unroll 1
-            for (int kk = 0; kk < 4 && 4 * h + kk < groups; ++kk)
-              mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, !first || h + kk > 0);
+      int k = 0;
+      auto pass = [&](auto) {
+        for (;;) {
+          const TileWork w = next_work(k++);
+          if (w.b < 0) {
+            if (lane == 0) mbar_arrive(ending);
+            break;
           }
-        };
-        tile_wait2(q_full, qn & 1, full(0), phase(0), limit);
-        if (EARLY && done0 > 0 && w.steps[0] > 0) tile_wait(&s_free[0], (done0 - 1) & 1, limit);
-        if (EARLY && done1 > 0 && w.steps[1] > 0) tile_wait(&s_free[1], (done1 - 1) & 1, limit);
-        tc_fence_after();
-        if (elect_one()) {
-          if (w.steps[0] > 0) scores(0, base % NS);
-          if (w.steps[1] > 0) scores(1, base % NS);
-          tc_commit(&kv_empty[base % NS]);
-          if (nk == 1) tc_commit(q_empty);
-        }
-#pragma unroll 1
-        for (int j = 0; j < nk; ++j) {
-          if (j == max(0, nk - 3) && lane == 0) mbar_arrive(ending);
-          const unsigned kn = key_at(j + 1), vn = value_at(j, nk);
-          const unsigned kslot = (base + kn) % NS, vslot = (base + vn) % NS;
-          const int groups = j == nk - 1 ? tail_groups : 8;
-          const bool more0 = j + 1 < w.steps[0], more1 = j + 1 < w.steps[1];
-          if constexpr (EARLY) {
-            // the next scores of both tiles, then the step's P V of each
-            if (j + 1 < nk) {
-              tile_wait(full(kn), phase(kn), limit);
-              if (more0 && more1) tile_wait2(&s_free[0], (done0 + j) & 1, &s_free[1], (done1 + j) & 1, limit);
-              else if (more0) tile_wait(&s_free[0], (done0 + j) & 1, limit);
-              else tile_wait(&s_free[1], (done1 + j) & 1, limit);
-              tc_fence_after();
-              if (elect_one()) {
-                if (more0) scores(0, kslot);
-                if (more1) scores(1, kslot);
-                tc_commit(&kv_empty[kslot]);
-                if (j + 1 == nk - 1) tc_commit(q_empty);
-              }
+          const int nk = max(w.steps[0], w.steps[1]);
+          if (nk == 0) {
+            if (lane == 0) mbar_arrive(ending);
+            continue;
+          }
+          const int tail_groups = (tail_rows_of(w, nk) + 15) / 16;
+          auto full = [&](unsigned n) { return &kv_full[(base + n) % NS]; };
+          auto phase = [&](unsigned n) { return (base + n) / NS & 1u; };
+          auto scores = [&](int i, unsigned slot) {  // S_i against the key tile in a slot
+            const uint32_t qd = q_desc + i * (TB >> 4), kd = k_desc + slot * (TB >> 4);
+  #pragma unroll
+            for (int c = 0; c < SUB; ++c)
+  #pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_ss(tmem + S_COL + i * 128, qd + ((c * (TB / SUB) + kk * 32) >> 4),
+                       kd + ((c * (TB / SUB) + kk * 32) >> 4), IDESC_S, c + kk > 0);
+            tc_commit(&s_full[i]);
+          };
+          // keys 64 h .. 64 h + 64 of P_i V with the value tile in a slot
+          auto outputs = [&](int i, unsigned slot, int h, bool first, int groups) {
+            const uint32_t vd = v_desc + slot * (TB >> 4) + h * 512;
+            const uint32_t o = tmem + O_COL + i * D, pr = tmem + P_COL + i * P_STEP + h * 32;
+            if (groups == 8) {
+  #pragma unroll
+              for (int kk = 0; kk < 4; ++kk) mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, !first || h + kk > 0);
+            } else {
+  #pragma unroll 1
+              for (int kk = 0; kk < 4 && 4 * h + kk < groups; ++kk)
+                mma_ts(o, pr + kk * 8, vd + kk * 128, IDESC_O, !first || h + kk > 0);
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (j < w.steps[i]) {
-                const unsigned par = ((i ? done1 : done0) + j) & 1;
-                tile_wait2(&p_full[2 * i + 1], par, full(vn), phase(vn), limit);
+          };
+          tile_wait2(q_full, qn & 1, full(0), phase(0), limit);
+          if (EARLY && done0 > 0 && w.steps[0] > 0) tile_wait(&s_free[0], (done0 - 1) & 1, limit);
+          if (EARLY && done1 > 0 && w.steps[1] > 0) tile_wait(&s_free[1], (done1 - 1) & 1, limit);
+          tc_fence_after();
+          if (elect_one()) {
+            if (w.steps[0] > 0) scores(0, base % NS);
+            if (w.steps[1] > 0) scores(1, base % NS);
+            tc_commit(&kv_empty[base % NS]);
+            if (nk == 1) tc_commit(q_empty);
+          }
+  #pragma unroll 1
+          for (int j = 0; j < nk; ++j) {
+            if (j == max(0, nk - 3) && lane == 0) mbar_arrive(ending);
+            const unsigned kn = key_at(j + 1), vn = value_at(j, nk);
+            const unsigned kslot = (base + kn) % NS, vslot = (base + vn) % NS;
+            const int groups = j == nk - 1 ? tail_groups : 8;
+            const bool more0 = j + 1 < w.steps[0], more1 = j + 1 < w.steps[1];
+            if constexpr (EARLY) {
+              // the next scores of both tiles, then the step's P V of each
+              if (j + 1 < nk) {
+                tile_wait(full(kn), phase(kn), limit);
+                if (more0 && more1) tile_wait2(&s_free[0], (done0 + j) & 1, &s_free[1], (done1 + j) & 1, limit);
+                else if (more0) tile_wait(&s_free[0], (done0 + j) & 1, limit);
+                else tile_wait(&s_free[1], (done1 + j) & 1, limit);
                 tc_fence_after();
                 if (elect_one()) {
-                  outputs(i, vslot, 0, j == 0, groups);
-                  outputs(i, vslot, 1, j == 0, groups);
-                  tc_commit(&o_done[i]);
-                  if (i == 1 || j >= w.steps[1]) tc_commit(&kv_empty[vslot]);
+                  if (more0) scores(0, kslot);
+                  if (more1) scores(1, kslot);
+                  tc_commit(&kv_empty[kslot]);
+                  if (j + 1 == nk - 1) tc_commit(q_empty);
                 }
               }
-          } else {
-            // each tile's P V, as its halves come, then its next scores
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (j < w.steps[i]) {
-                const unsigned par = ((i ? done1 : done0) + j) & 1;
-                tile_wait2(&p_full[2 * i], par, full(vn), phase(vn), limit);
-                tc_fence_after();
-                if (elect_one()) outputs(i, vslot, 0, j == 0, groups);
-                const bool more = i ? more1 : more0;
-                if (more) tile_wait2(&p_full[2 * i + 1], par, full(kn), phase(kn), limit);
-                else tile_wait(&p_full[2 * i + 1], par, limit);
-                tc_fence_after();
-                if (elect_one()) {
-                  outputs(i, vslot, 1, j == 0, groups);
-                  tc_commit(&o_done[i]);
-                  if (i == 1 || j >= w.steps[1]) tc_commit(&kv_empty[vslot]);
-                  if (more) scores(i, kslot);
-                  if (more && (i == 1 || !more1)) {
-                    tc_commit(&kv_empty[kslot]);
-                    if (j + 1 == nk - 1) tc_commit(q_empty);
+  #pragma unroll
+              for (int i = 0; i < 2; ++i)
+                if (j < w.steps[i]) {
+                  const unsigned par = ((i ? done1 : done0) + j) & 1;
+                  tile_wait2(&p_full[2 * i + 1], par, full(vn), phase(vn), limit);
+                  tc_fence_after();
+                  if (elect_one()) {
+                    outputs(i, vslot, 0, j == 0, groups);
+                    outputs(i, vslot, 1, j == 0, groups);
+                    tc_commit(&o_done[i]);
+                    if (i == 1 || j >= w.steps[1]) tc_commit(&kv_empty[vslot]);
                   }
                 }
-              }
+            } else {
+              // each tile's P V, as its halves come, then its next scores
+  #pragma unroll
+              for (int i = 0; i < 2; ++i)
+                if (j < w.steps[i]) {
+                  const unsigned par = ((i ? done1 : done0) + j) & 1;
+                  tile_wait2(&p_full[2 * i], par, full(vn), phase(vn), limit);
+                  tc_fence_after();
+                  if (elect_one()) outputs(i, vslot, 0, j == 0, groups);
+                  const bool more = i ? more1 : more0;
+                  if (more) tile_wait2(&p_full[2 * i + 1], par, full(kn), phase(kn), limit);
+                  else tile_wait(&p_full[2 * i + 1], par, limit);
+                  tc_fence_after();
+                  if (elect_one()) {
+                    outputs(i, vslot, 1, j == 0, groups);
+                    tc_commit(&o_done[i]);
+                    if (i == 1 || j >= w.steps[1]) tc_commit(&kv_empty[vslot]);
+                    if (more) scores(i, kslot);
+                    if (more && (i == 1 || !more1)) {
+                      tc_commit(&kv_empty[kslot]);
+                      if (j + 1 == nk - 1) tc_commit(q_empty);
+                    }
+                  }
+                }
+            }
           }
+          ++qn;
+          base += 2 * nk;
+          done0 += w.steps[0];
+          done1 += w.steps[1];
         }
-        ++qn;
-        base += 2 * nk;
-        done0 += w.steps[0];
-        done1 += w.steps[1];
-      }
-      if (limit == 1) {  // a wait ran out: MMAs in flight finish before the memory goes
-        unsigned more = kTileWaitLimit;
-        if (elect_one()) tc_commit(drained);
-        tile_wait(drained, 0, more);
+        if (limit == 1) {  // a wait ran out: MMAs in flight finish before the memory goes
+          unsigned more = kTileWaitLimit;
+          if (elect_one()) tc_commit(drained);
+          tile_wait(drained, 0, more);
+        }
+      };
+      pass(std::false_type{});
+      if (go_again()) {
+        pass(std::true_type{});
+        end_care();
       }
     } else if (warp == kTmaWarp + 2) {
       // ---- items: the CTA's own, then those of CTAs that have not started.  Heavy items come first in a launch and the
       // next is taken three steps before the present one ends, so the SMs finish together whatever the lengths are
       // (taken at the present one's start, a prompt of 2048 tokens at 64 dims ran 42 us instead of 33)
       const int splits = item_splits<PAGED>(a);
-      int index = (int)blockIdx.x;
-      for (int k = 0;; ++k) {
-        TileWork w;
-        w.b = -1;
-        if (index >= 0) w = find_item<PAGED>(a, index, splits);
-        if (lane == 0) {
-          work[k & 1] = w;
-          mbar_arrive(&work_full[k & 1]);
+      int index = (int)blockIdx.x, k = 0, asked = 0, held[2] = {-1, -1};
+      auto pass = [&](auto care) {
+        constexpr bool CARE = decltype(care)::value;
+        for (;; ++k) {
+          TileWork w;
+          w.b = -1;
+          int at = -1;
+          if constexpr (CARE) {
+            for (int i = 0; i < 2 && at < 0; ++i)
+              if (again[i] != 0) at = held[i], held[i] = -1;
+          }
+          const bool repeat = at >= 0;
+          if (!repeat) at = index;
+          // (an output that is not finite ends the usual pass: it has come from one of the last two items)
+          if (at >= 0 && (CARE || !__any_sync(0xffffffffu, again[0] + again[1] > 0))) w = find_item<PAGED>(a, at, splits);
+          if (!CARE && w.b >= 0) held[k & 1] = at;
+          if (lane == 0) {
+            work[k & 1] = w;
+            mbar_arrive(&work_full[k & 1]);
+          }
+          if (w.b < 0 || limit == 1) break;
+          tile_wait2(&work_empty[k & 1], (k >> 1) & 1, ending, k & 1, limit);
+          if (limit == 1) break;
+          if (repeat) continue;
+          if (lane == 0) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the last reply has been read
+            mbar_arrive_expect_tx(replied, 16);
+            ask_next(smem_addr(reply), replied);
+          }
+          __syncwarp();
+          tile_wait(replied, asked & 1, limit);
+          if (limit == 1) {  // (the reply is still to land: once more before the memory goes)
+            unsigned more = kTileWaitLimit;
+            tile_wait(replied, asked & 1, more);
+            break;
+          }
+          ++asked;
+          index = read_next(smem_addr(reply));
+          __syncwarp();
         }
-        if (w.b < 0 || limit == 1) break;
-        tile_wait2(&work_empty[k & 1], (k >> 1) & 1, ending, k & 1, limit);
-        if (limit == 1) break;
-        if (lane == 0) {
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the last reply has been read
-          mbar_arrive_expect_tx(replied, 16);
-          ask_next(smem_addr(reply), replied);
-        }
-        __syncwarp();
-        tile_wait(replied, k & 1, limit);
-        if (limit == 1) {  // (the reply is still to land: once more before the memory goes)
-          unsigned more = kTileWaitLimit;
-          tile_wait(replied, k & 1, more);
-          break;
-        }
-        index = read_next(smem_addr(reply));
-        __syncwarp();
+      };
+      pass(std::false_type{});
+      if (go_again()) {
+        ++k;
+        pass(std::true_type{});
+        end_care();
       }
+    } else if (go_again()) {
+      end_care();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -668,194 +804,189 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                    p_at = tmem + lanes + P_COL + i * P_STEP;
     const float c = a.s.scale_log2;
     const int row_tok = row / a.s.rep, row_head = row - row_tok * a.s.rep;
-    int done = 0;  // steps of earlier items
-    for (int k = 0;; ++k) {
-      // (the item stays in work[k & 1] until this warp has asked for the next: read again for the output)
-      tile_wait(&work_full[k & 1], (k >> 1) & 1, limit);
-      const volatile TileWork& item = work[k & 1];
-      const int first = item.first, my_steps = item.b < 0 || limit == 1 ? -1 : item.steps[i];
-      const int first_tok = item.tok0 + i * TPT, hidden = item.len - item.n;
-      const bool valid = row < TPT * a.s.rep && first_tok + row_tok < item.n;
-      const int lim = valid ? hidden + first_tok + row_tok : -1;  // last key the row sees
-      const int first_lim = hidden + first_tok;                   // the tile's first row's
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&work_empty[k & 1]);
-      if (my_steps < 0) break;
-      float m = -INFINITY, base = 0.f, l = 0.f;  // maximum in use (raw score), m * c or 0, sum against it
-      bool s_here = false;
-      for (int j = 0; j < my_steps; ++j) {
-        if (!s_here) tile_wait(&s_full[i], (done + j) & 1, limit);
-        tc_fence_after();
-        float x[128];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) tmem_ld32(s_at + g * 32, x + g * 32);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) tmem_ld_wait(x + g * 32);
-        if constexpr (EARLY) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[i]);
-        }
-        const int key0 = (first + j) * kTileKeys;
-        if (key0 + kTileKeys - 1 > first_lim) {
-          const int rel = lim - key0;
-#pragma unroll
-          for (int e = 0; e < 128; ++e)
-            if (e > rel) x[e] = -INFINITY;
-        }
-        float mx[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-        for (int e = 4; e < 124; e += 8) {
-#pragma unroll
-          for (int v = 0; v < 4; ++v) mx[v] = max3(mx[v], x[e + v], x[e + 4 + v]);
-        }
-#pragma unroll
-        for (int v = 0; v < 4; ++v) mx[v] = fmaxf(mx[v], x[124 + v]);
-        // (asked here, used a little later: the answer takes a while)
-        const bool o_here = !EARLY || j == 0 || mbar_test_wait(&o_done[i], (done + j - 1) & 1);
-        const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-        // (the difference is NaN for two infinities of one sign: no move)
-        if (__any_sync(0xffffffffu, (top - m) * c > kLazyLog2)) {
-          const float mn = fmaxf(m, top);
-          const float nb = mn == -INFINITY ? 0.f : mn * c;
-          const float f = m == -INFINITY ? 0.f : exp2_fast(m * c - nb);
-          l = m == -INFINITY ? 0.f : l * f;
-          if (j > 0) {
-            tile_wait(&o_done[i], (done + j - 1) & 1, limit);
-            tc_fence_after();
-#pragma unroll 1
-            for (int g = 0; g < D / 32; ++g) {
-              float o[32];
-              tmem_ld32(o_at + g * 32, o);
-              tmem_ld_wait(o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] *= f;
-              tmem_st32(o_at + g * 32, o);
-            }
+    int k = 0, done = 0;  // steps of earlier items
+    auto pass = [&](auto care) {
+      constexpr bool CARE = decltype(care)::value;
+      unsigned cares = 0;
+      for (;; ++k) {
+        // (the item stays in work[k & 1] until this warp has asked for the next: read again where it is needed)
+        tile_wait(&work_full[k & 1], (k >> 1) & 1, limit);
+        const volatile TileWork& item = work[k & 1];
+        const int first = item.first, my_steps = item.b < 0 || limit == 1 ? -1 : item.steps[i];
+        const int first_tok = item.tok0 + i * TPT, hidden = item.len - item.n;
+        const bool valid = row < TPT * a.s.rep && first_tok + row_tok < item.n;
+        const int lim = valid ? hidden + first_tok + row_tok : -1;  // last key the row sees
+        const int first_lim = hidden + first_tok;                   // the tile's first row's
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&work_empty[k & 1]);
+        if (my_steps < 0) break;
+        float m = -INFINITY, base = 0.f, l = 0.f;  // maximum in use (raw score), m * c or 0, sum against it
+        bool s_here = false;
+        for (int j = 0; j < my_steps; ++j) {
+          if (!s_here) tile_wait(&s_full[i], (done + j) & 1, limit);
+          tc_fence_after();
+          float x[128];
+  #pragma unroll
+          for (int g = 0; g < 4; ++g) tmem_ld32(s_at + g * 32, x + g * 32);
+  #pragma unroll
+          for (int g = 0; g < 4; ++g) tmem_ld_wait(x + g * 32);
+          if constexpr (EARLY) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[i]);
           }
-          m = mn;
-          base = nb;
+          const int key0 = (first + j) * kTileKeys;
+          if (key0 + kTileKeys - 1 > first_lim) {
+            const int rel = lim - key0;
+  #pragma unroll
+            for (int e = 0; e < 128; ++e)
+              if (e > rel) x[e] = -INFINITY;
+          }
+          float mx[4] = {x[0], x[1], x[2], x[3]};
+  #pragma unroll
+          for (int e = 4; e < 124; e += 8) {
+  #pragma unroll
+            for (int v = 0; v < 4; ++v) mx[v] = max3(mx[v], x[e + v], x[e + 4 + v]);
+          }
+  #pragma unroll
+          for (int v = 0; v < 4; ++v) mx[v] = max2(mx[v], x[124 + v]);
+          // (asked here, used a little later: the answer takes a while)
+          [[maybe_unused]] const bool o_here = !EARLY || j == 0 || mbar_test_wait(&o_done[i], (done + j - 1) & 1);
+          const float top = max2(max3(mx[0], mx[1], mx[2]), mx[3]);
+          // (the difference is NaN for two infinities of one sign and beside a NaN score: no move)
+          if (__any_sync(0xffffffffu, (top - m) * c > kLazyLog2)) {
+            const float mn = fmaxf(m, top);
+            const float nb = mn == -INFINITY ? 0.f : mn * c;
+            const float f = m == -INFINITY ? 0.f : exp2_fast(m * c - nb);
+            l *= f;  // (0 so far, or NaN, where nothing finite has been seen)
+            if (j > 0) {
+              tile_wait(&o_done[i], (done + j - 1) & 1, limit);
+              tc_fence_after();
+  #pragma unroll 1
+              for (int g = 0; g < D / 32; ++g) {
+                float o[32];
+                tmem_ld32(o_at + g * 32, o);
+                tmem_ld_wait(o);
+  #pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] *= f;
+                tmem_st32(o_at + g * 32, o);
+              }
+            }
+            m = mn;
+            base = nb;
+          }
+          if constexpr (EARLY) {  // the last P_i V has read P_i
+            if (!__all_sync(0xffffffffu, o_here)) tile_wait(&o_done[i], (done + j - 1) & 1, limit);
+            tc_fence_after();
+          }
+          const uint64_t cc = pack2(c, c), nb2 = pack2(-base, -base);
+          uint64_t sum0 = 0, sum1 = 0;  // pairs of zeros
+  #pragma unroll
+          for (int h = 0; h < 2; ++h) {
+  #pragma unroll
+            for (int g = 2 * h; g < 2 * h + 2; ++g) {
+              uint32_t p[16];
+  #pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                float p0, p1;
+                const uint64_t t = fma2(pack2(x[g * 32 + 2 * e], x[g * 32 + 2 * e + 1]), cc, nb2);
+                if ((kPolyPairs >> e) & 1) {
+                  exp2_pair(t, &p0, &p1);
+                } else {
+                  unpack2(t, &p0, &p1);
+                  p0 = exp2_fast(p0);
+                  p1 = exp2_fast(p1);
+                }
+                uint64_t& sum = e & 1 ? sum1 : sum0;
+                sum = add2(sum, pack2(p0, p1));
+                p[e] = Type16<T>::pack(p0, p1);
+              }
+              tmem_st16(p_at + g * 16, p);
+              if (g == 2) s_here = EARLY && j + 1 < my_steps && mbar_test_wait(&s_full[i], (done + j + 1) & 1);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
+          }
+          s_here = __all_sync(0xffffffffu, s_here);
+          float s0, s1;
+          unpack2(add2(sum0, sum1), &s0, &s1);
+          // a NaN score, or an infinite one (its exponent is infinity - infinity), makes the row NaN
+          l = top < INFINITY ? l + (s0 + s1) : NAN;
         }
-        if constexpr (EARLY) {  // the last P_i V has read P_i
-          if (!__all_sync(0xffffffffu, o_here)) tile_wait(&o_done[i], (done + j - 1) & 1, limit);
+        // ---- the row's output, or its part of it
+        done += my_steps;
+        if (my_steps > 0) {
+          tile_wait(&o_done[i], (done - 1) & 1, limit);
           tc_fence_after();
         }
-        const uint64_t cc = pack2(c, c), nb2 = pack2(-base, -base);
-        uint64_t sum0 = 0, sum1 = 0;  // pairs of zeros
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int g = 2 * h; g < 2 * h + 2; ++g) {
-            uint32_t p[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float p0, p1;
-              const uint64_t t = fma2(pack2(x[g * 32 + 2 * e], x[g * 32 + 2 * e + 1]), cc, nb2);
-              if ((kPolyPairs >> e) & 1) {
-                exp2_pair(t, &p0, &p1);
-              } else {
-                unpack2(t, &p0, &p1);
-                p0 = exp2_fast(p0);
-                p1 = exp2_fast(p1);
+        const int tok = first_tok + row_tok, part_at = item.part;
+        const bool whole = part_at < 0;
+        const bool none = lim < 0;
+        const float inv = 1.f / l;
+        uint16_t* out = a.s.out + (long long)(item.start + tok) * a.s.sot + (long long)(item.kvh * a.s.rep + row_head) * a.s.soh;
+        float* part = a.s.part + tile_part_floats(D) * (whole ? 0 : part_at);
+        if (CARE && max(item.steps[0], item.steps[1]) > 0) {
+          tile_wait(&taken_out[cares & 1], cares >> 1 & 1, limit);
+          if (my_steps > 0) put_back<D>(o_at, first_bad + (cares & 1) * 2 * D, lim);
+          ++cares;
+        }
+        // a row's outputs go out a 32-byte sector at a time where they start on one (16 prompts of 15001 tokens together:
+        // 180 us, 184 with 16-byte stores)
+        const bool sectors = __all_sync(0xffffffffu, (reinterpret_cast<uintptr_t>(out) & 31u) == 0);
+        float odd = 0.f;  // becomes NaN with the first output that is not finite
+        if (my_steps > 0) {
+  #pragma unroll 1
+          for (int g = 0; g < D / 32; ++g) {
+            float o[32];
+            tmem_ld32(o_at + g * 32, o);
+            tmem_ld_wait(o);
+  #pragma unroll
+            for (int e = 0; e < 32; ++e) odd = fmaf(o[e], 0.f, odd);
+            if (valid && whole) {
+  #pragma unroll
+              for (int v = 0; v < 2; ++v) {  // 16 dims: a sector
+                uint32_t u[8];
+  #pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  u[e] = none ? 0u : Type16<T>::pack(o[v * 16 + 2 * e] * inv, o[v * 16 + 2 * e + 1] * inv);
+                uint16_t* to = out + g * 32 + v * 16;
+                if (sectors && g * 32 + v * 16 + 16 <= a.s.hd) {
+                  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(u[0]), "r"(u[1]),
+                               "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                               : "memory");
+                } else {
+                  if (g * 32 + v * 16 < a.s.hd) *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
+                  if (g * 32 + v * 16 + 8 < a.s.hd) *reinterpret_cast<uint4*>(to + 8) = make_uint4(u[4], u[5], u[6], u[7]);
+                }
               }
-              uint64_t& sum = e & 1 ? sum1 : sum0;
-              sum = add2(sum, pack2(p0, p1));
-              p[e] = Type16<T>::pack(p0, p1);
+            } else if (valid) {
+  #pragma unroll
+              for (int v = 0; v < 8; ++v)
+                *reinterpret_cast<float4*>(part + tile_part_at(i * kTileRows + row, g * 32 + v * 4)) =
+                    make_float4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
             }
-            tmem_st16(p_at + g * 16, p);
-            if (g == 2) s_here = EARLY && j + 1 < my_steps && mbar_test_wait(&s_full[i], (done + j + 1) & 1);
+            __syncwarp();  // (the next load takes the whole warp)
           }
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
+        } else if (valid && whole) {
+          for (int d = 0; d < a.s.hd; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
         }
-        s_here = __all_sync(0xffffffffu, s_here);
-        float s0, s1;
-        unpack2(add2(sum0, sum1), &s0, &s1);
-        l += s0 + s1;
+        float2* ml = reinterpret_cast<float2*>(part + (size_t)2 * kTileRows * D) + i * kTileRows;
+        if (!whole && valid) ml[row] = m == -INFINITY ? make_float2(-INFINITY, l) : make_float2(base, l);
+        // an output that is not finite though the row's sum is: it may come from values that the row must not see
+        if (!CARE && valid && !none && my_steps > 0 && isfinite(l) && !(odd == 0.f)) again[k & 1] = 1;
+        __syncwarp();
       }
-      // ---- the row's output, or its part of it
-      done += my_steps;
-      if (my_steps > 0) {
-        tile_wait(&o_done[i], (done - 1) & 1, limit);
-        tc_fence_after();
-      }
-      TileWork w;
-      w.b = item.b, w.kvh = item.kvh, w.start = item.start, w.n = item.n, w.len = item.len, w.tok0 = item.tok0;
-      w.first = first, w.part = item.part;
-      const int tok = first_tok + row_tok;
-      const bool whole = w.part < 0;
-      const bool none = lim < 0;
-      const float inv = 1.f / l;
-      uint16_t* out = a.s.out + (long long)(w.start + tok) * a.s.sot + (long long)(w.kvh * a.s.rep + row_head) * a.s.soh;
-      float* part = a.s.part + tile_part_floats(D) * (whole ? 0 : w.part);
-      // a row's outputs go out a 32-byte sector at a time where they start on one (16 prompts of 15001 tokens together:
-      // 180 us, 184 with 16-byte stores)
-      const bool sectors = __all_sync(0xffffffffu, (reinterpret_cast<uintptr_t>(out) & 31u) == 0);
-      float odd = 0.f;  // becomes NaN with the first output that is not finite
-      if (my_steps > 0) {
-#pragma unroll 1
-        for (int g = 0; g < D / 32; ++g) {
-          float o[32];
-          tmem_ld32(o_at + g * 32, o);
-          tmem_ld_wait(o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) odd = fmaf(o[e], 0.f, odd);
-          if (valid && whole) {
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {  // 16 dims: a sector
-              uint32_t u[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                u[e] = none ? 0u : Type16<T>::pack(o[v * 16 + 2 * e] * inv, o[v * 16 + 2 * e + 1] * inv);
-              uint16_t* to = out + g * 32 + v * 16;
-              if (sectors && g * 32 + v * 16 + 16 <= a.s.hd) {
-                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(u[0]), "r"(u[1]),
-                             "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
-                             : "memory");
-              } else {
-                if (g * 32 + v * 16 < a.s.hd) *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
-                if (g * 32 + v * 16 + 8 < a.s.hd) *reinterpret_cast<uint4*>(to + 8) = make_uint4(u[4], u[5], u[6], u[7]);
-              }
-            }
-          } else if (valid) {
-#pragma unroll
-            for (int v = 0; v < 8; ++v)
-              *reinterpret_cast<float4*>(part + tile_part_at(i * kTileRows + row, g * 32 + v * 4)) =
-                  make_float4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
-          }
-          __syncwarp();  // (the next load takes the whole warp)
-        }
-      } else if (valid && whole) {
-        for (int d = 0; d < a.s.hd; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
-      }
-      float2* ml = reinterpret_cast<float2*>(part + (size_t)2 * kTileRows * D) + i * kTileRows;
-      if (!whole && valid) ml[row] = m == -INFINITY ? make_float2(-INFINITY, l) : make_float2(base, l);
-      __syncwarp();  // (other lanes write a row again below)
-      unsigned again = __ballot_sync(0xffffffffu, valid && !none && my_steps > 0 && isfinite(l) && !(odd == 0.f));
-      while (again) {
-        const int src = __ffs(again) - 1;
-        again &= again - 1;
-        const float mb = __shfl_sync(0xffffffffu, base, src), ll = __shfl_sync(0xffffffffu, l, src);
-        const int r = (warp & 3) * 32 + src;
-        const int pr = (w.tok0 + i * TPT) * a.s.rep + r;
-        const Seq s = {w.start, w.n, w.len};
-        float o[D / 32];
-        redo_row<T, PAGED, D>(a.s, w.b, s, w.kvh, pr, w.first * kTileKeys, min(w.len, (w.first + my_steps) * kTileKeys), mb, o);
-        const int rt = pr / a.s.rep;
-        uint16_t* ro = a.s.out + (long long)(w.start + rt) * a.s.sot + (long long)(w.kvh * a.s.rep + pr % a.s.rep) * a.s.soh;
-        for (int e = 0; e < D / 32; ++e) {
-          if (!whole) part[tile_part_at(i * kTileRows + r, lane + 32 * e)] = o[e];
-          else if (lane + 32 * e < a.s.hd) ro[lane + 32 * e] = Type16<T>::one(o[e] / ll);
-        }
-      }
-      __syncwarp();
+    };
+    pass(std::false_type{});
+    if (go_again()) {
+      ++k;
+      pass(std::true_type{});
+      end_care();
     }
   }
   if (limit == 1 && lane == 0) atomicOr(&g_tile_device_error, 256u);
-  tc_fence_before();
-  __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
