@@ -15,6 +15,10 @@
 // half of a tile or nothing (with the rows as the 16-wide side 64 requests of 300-16000 tokens took
 // 85 us instead of 81).  The work is bound by the bytes of the keys and values as long as the rows
 // are few: those 419 MB now take 77 us, 5.5 TB/s with the join, and with the products left out no less.
+//
+// A masked key's probability is zero, but zero times a NaN or an infinity is NaN.  In the steps with keys that some
+// row must not see (the last tokens' own), a value that is not finite is therefore taken out of the warp's stage before
+// the product and added to the rows that see it (a sum with what is not finite does not depend on its weight).
 #include <cooperative_groups.h>
 
 #include <mutex>
@@ -210,7 +214,6 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
   static_assert((kSeqWarps * RT * LD + RT * (D + 2)) * 4 <= seq_smem_bytes(D), "outputs and a part fit the ring");
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ float s_ml[kSeqWarps][RT][2];
-  __shared__ int s_redo[RT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t ring = smem_addr(smem) + warp * kSeqStages * seq_stage_bytes(D);
   pdl_launch_dependents();
@@ -391,6 +394,44 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
           pf[mt][nt][1] = transpose8(Type16<T>::pack(sc[mt][nt][2], sc[mt][nt][3]));
         }
       }
+      if (j0 + KW - 1 > first_lim) {
+        uint8_t* vs = smem + (vs_at - smem_addr(smem));
+        unsigned bad = 0;  // hidden keys of the stage with a value that is not finite
+        constexpr int CH = D / 8;
+#pragma unroll
+        for (int i = 0; i < KW * CH / 32; ++i) {
+          const int r = (i * 32 + lane) / CH, c = lane % CH;
+          const uint4 v = *reinterpret_cast<const uint4*>(vs + r * (D * 2) + ((c ^ (r & 7)) << 4));
+          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+          bool odd = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            odd |= Type16<T>::not_finite((uint16_t)u[e]) || Type16<T>::not_finite((uint16_t)(u[e] >> 16));
+          if (odd && j0 + r > first_lim) bad |= 1u << r;
+        }
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        for (unsigned rest = bad; rest != 0; rest &= rest - 1) {
+          const int r = __ffs(rest) - 1;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = dt * 2 + h;  // dim dt * 16 + 8 h + lane / 4
+              uint16_t* at = reinterpret_cast<uint16_t*>(vs + r * (D * 2) + ((c ^ (r & 7)) << 4)) + lane / 4;
+              const uint16_t x = *at;
+              __syncwarp();
+              if (Type16<T>::not_finite(x)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if (j0 + r <= lim[nt][e]) o[dt][nt][2 * h + e] += Type16<T>::unpack(x).x;
+                *at = 0;
+              }
+            }
+        }
+        if (bad != 0) __syncwarp();
+      }
       // O^T += V^T P^T: 16 dims x 16 keys by four transposed 8x8 matrices
 #pragma unroll
       for (int mt = 0; mt < KT; ++mt)
@@ -427,10 +468,8 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
           so[r * LD + dt * 16 + 8 + lane / 4] = o[dt][nt][e + 2];
         }
       }
-    if (tid < RT) s_redo[tid] = 0;
     __syncthreads();
     const bool whole = !CL && r0 == 0 && r1 == per + kItemUnits;
-    const bool masked = k1 - 1 > first_lim;  // some row must not see some of the keys read
     // where a part of the item's result goes: the workspace, or this CTA's shared memory past the warps' outputs
     float* part = CL ? reinterpret_cast<float*>(smem) + kSeqWarps * RT * LD
                      : a.part + (size_t)(2 * g + (r0 == 0 ? 1 : 0)) * seq_part_floats(D, NT);
@@ -451,7 +490,6 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
         y += f * ov.y;
       }
       if (r >= rows) continue;
-      if (masked && isfinite(L) && !(isfinite(x) && isfinite(y))) s_redo[r] = 1;
       if (whole) {
         const int pr = row0 + r, tok = pr / a.rep;
         const bool none = s.len - s.n + tok < 0;  // a row that sees no key is zero
@@ -466,27 +504,6 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
       }
     }
     __syncthreads();
-    if (masked) {
-      for (int r = warp; r < rows; r += kSeqWarps) {
-        if (!s_redo[r]) continue;
-        float M = -INFINITY, L = 0.f;
-        for (int w = 0; w < kSeqWarps; ++w) M = fmaxf(M, s_ml[w][r][0]);
-        const float base = M == -INFINITY ? 0.f : M;
-        for (int w = 0; w < kSeqWarps; ++w) L += exp2_fast(s_ml[w][r][0] - base) * s_ml[w][r][1];
-        float x[D / 32];
-        redo_row<T, PAGED, D>(a, b, s, kvh, row0 + r, k0, k1, base, x);
-        const int pr = row0 + r, tok = pr / a.rep;
-        uint16_t* out = a.out + (long long)(s.start + tok) * a.sot + (long long)(kvh * a.rep + pr - tok * a.rep) * a.soh;
-        const bool none = s.len - s.n + tok < 0;
-        for (int i = 0; i < D / 32; ++i) {
-          const int d = lane + 32 * i;
-          if (!whole) part[r * D + d] = x[i];
-          else if (d < a.hd) out[d] = none ? 0 : Type16<T>::one(x[i] / L);
-        }
-      }
-      __syncthreads();
-    }
-
     if constexpr (CL) {
       cluster.sync();  // every CTA's part is there
       for (int e = rank * kSeqThreads + tid; e < rows * (D / 2); e += ranks * kSeqThreads) {

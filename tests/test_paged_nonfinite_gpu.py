@@ -166,3 +166,28 @@ def test_a_bad_value_costs_little_and_hurts_no_other_prompt(paged, d):  # noqa: 
         assert torch.equal(got[:row - row % 512], want[:row - row % 512])
         assert bool(torch.isfinite(got[:lens[0]][..., others]).all()) and bool(torch.isfinite(got[:row]).all())
         assert elapsed(lambda: paged.prompt_attention(q, k, w, cu, max(lens))) < 3 * clean
+
+
+def test_a_bad_value_costs_little_over_long_contexts(paged):  # noqa: F811
+    """Requests of a few tokens over long contexts, the first value and one that the last query alone sees NaN."""
+    dtype, H, Hkv, d, page, n = torch.float16, 8, 1, 64, 64, 4
+    lens = [30000] * 40
+    ck, cv, tables, keys, values = make_cache(lens[:1], Hkv, d, page, dtype, 16)
+    tables = tables[:, :-1].expand(40, -1).contiguous()
+    q = rand((40 * n, H, d), dtype, 17)
+    args = (tables, i32(lens), i32(cumulative([n] * 40)), n)
+    want = paged.paged_attention(q, ck, cv, *args)
+    clean = elapsed(lambda: paged.paged_attention(q, ck, cv, *args))
+    bad = cv.clone(memory_format=torch.preserve_format)
+    bad[int(tables[0, 0]), 0, :, 2] = NAN
+    bad[int(tables[0, 29999 // page]), 29999 % page, :, 4] = INF
+    got = paged.paged_attention(q, ck, bad, *args).view(40, n, H, d)
+    assert bool(torch.isnan(got[..., 2]).all()) and not bool(torch.isfinite(got[:, -1, :, 4]).any())
+    same = [x for x in range(d) if x not in (2, 4)]
+    u = torch.finfo(dtype).eps
+    ref = want.view(40, n, H, d)
+    # (the last key's step sums in another order: a rounding of the type at most)
+    assert bool(((got - ref)[..., same].abs() <= u * ref[..., same].abs() + 2.0 ** -14).all())
+    assert bool(((got - ref)[:, :-1, :, 4].abs() <= u * ref[:, :-1, :, 4].abs() + 2.0 ** -14).all())
+    assert elapsed(lambda: paged.paged_attention(q, ck, bad, *args)) < 3 * clean
+    assert math.isfinite(clean)
