@@ -468,6 +468,10 @@ int li4_device_errors(unsigned* flags, int reset);
  * device waits). */
 int li4_debug_set_wait_limits(unsigned allreduce_polls, unsigned program_polls, unsigned program_wait_extra);
 
+/* The same for the waits inside li4_prompt_attention and li4_paged_attention: the poll limit of every launch made
+ * after the call, on any device (0 restores the default: half a second, and more for long contexts). */
+int li4_debug_set_attention_wait_limit(unsigned polls);
+
 /* ---------------------------------------------------------------------------
  * Tensor-parallel all-reduce over NVLink peer memory (one GPU per process).
  * Every rank allocates one communication buffer (li4_comm_alloc), exports it

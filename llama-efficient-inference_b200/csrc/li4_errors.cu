@@ -58,3 +58,9 @@ extern "C" int li4_debug_set_wait_limits(unsigned allreduce_polls, unsigned prog
   if (rc == LI4_OK) li4::clear_error();
   return rc;
 }
+
+extern "C" int li4_debug_set_attention_wait_limit(unsigned polls) {
+  const int rc = li4::tile_set_wait_limit(polls);
+  if (rc == LI4_OK) li4::clear_error();
+  return rc;
+}

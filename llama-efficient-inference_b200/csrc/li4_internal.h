@@ -35,6 +35,8 @@ int sample_set_wait_limit(unsigned polls);
 int paged_device_errors(unsigned* flags, bool reset);
 // Device error word of the tensor-memory attention kernel (bit 8).
 int tile_device_errors(unsigned* flags, bool reset);
+// Poll limit of that kernel's waits in later launches (0 = default).
+int tile_set_wait_limit(unsigned polls);
 // Poll limit of the LI4_EPI_ALLREDUCE_RESIDUAL epilogue's waits (0 = default).
 int gemv_set_ar_wait_limit(unsigned polls);
 // Poll limit of the all-reduce flag waits (li4_comm.cu); 0 restores the default.

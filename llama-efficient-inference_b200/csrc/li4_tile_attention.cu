@@ -27,11 +27,12 @@
 // code exists twice, so the usual pass is spared the tests): the copying warp takes the values that are not finite out of those tiles before the products may have them and notes where in each
 // dim the first +inf, -inf or NaN stood, and a row that sees that key gets it added at the end (added to a
 // sum, what is not finite does not depend on its weight).  At most two items of a CTA run twice, whatever the context.
-// Every mbarrier wait is bounded: one that runs out sets bit 8 of li4_device_errors; every role then
-// runs to its end without waiting, copies and MMAs in flight are waited for (bounded) and the tensor
-// memory is freed.
+// Every mbarrier wait is bounded: one that runs out sets bit 8 of li4_device_errors.  The copying warp then issues
+// nothing more (a barrier whose bytes are still to come must not be armed twice), the other roles run to the end of
+// their item without waiting, copies and MMAs in flight are waited for (bounded) and the tensor memory is freed.
 #include <cuda.h>
 
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 #include <utility>
@@ -57,7 +58,8 @@ constexpr int kTileRows = 128;       // rows of a tile: tensor-memory lanes
 constexpr int kTileKeys = 128;       // keys of a step
 constexpr int kTileThreads = 384;    // 8 softmax warps, the TMA, MMA and item warps, one that only fills its group
 constexpr int kTmaWarp = 8, kMmaWarp = 9;
-constexpr unsigned kTileWaitLimit = 1u << 24;  // polls
+constexpr unsigned kTileWaitLimit = 1u << 24;  // polls, about half a second; and for each key tile that an item may have,
+constexpr unsigned kTileWaitStep = 1u << 8;    // as some waits last an item (a step of 2900 cycles is some 60 polls)
 constexpr int kTileMinSteps = 8;     // key tiles below which a range is not cut
 constexpr int kUnseen = 0x7fffffff;   // no key
 constexpr float kLazyLog2 = 8.f;     // how far the maximum in use may lag, in powers of two
@@ -75,6 +77,7 @@ struct TileArgs {
   int tokens_per_tile;  // whole queries of a tile: 128 / rep
   int part_slots;       // items whose partial results fit the workspace (0: keys are not split)
   int box_rows;         // key rows of one copy
+  unsigned wait_limit;  // polls of a wait
 };
 
 // ---- mbarriers, tensor memory ----
@@ -427,7 +430,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* o_done = p_full + 4;         // [2] the last P_i V finished
   uint64_t* s_free = o_done + 2;         // [2] S_i read (4 warps); 64 dims only
   uint64_t* v_tail = s_free + 2;         // the last value tile's rows are there, its missing rows not yet zeros
-  uint64_t* drained = v_tail + 1;        // the product warp gave up and its MMAs have finished
+  uint64_t* drained = v_tail + 1;        // a wait ran out: the MMAs issued so far have finished
   uint64_t* work_full = drained + 1;     // [2] work[i] names an item
   uint64_t* work_empty = work_full + 2;  // [2] the 10 working warps have read it
   uint64_t* replied = work_empty + 2;    // the reply is there
@@ -436,9 +439,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   TileWork* work = reinterpret_cast<TileWork*>(taken_out + 2);  // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(work + 2);
   volatile int* again = reinterpret_cast<int*>(tmem_holder + 1);  // [2] by item parity: one to run again
-  volatile int* gave_up = again + 2;             // a wait of the usual pass ran out
-  int* first_bad = const_cast<int*>(again) + 3;  // [2][2][D] of items taken with care: see take_out
-  static_assert(16 + (2 * NS + 22) * 8 + 2 * sizeof(TileWork) + 16 <= 512, "what lies behind the tiles fits");
+  volatile int* gave_up = again + 2;             // [2] a wait of the usual pass, of the one with care ran out
+  int* first_bad = const_cast<int*>(again) + 4;  // [2][2][D] of items taken with care: see take_out
+  static_assert(16 + (2 * NS + 22) * 8 + 2 * sizeof(TileWork) + 20 <= 512, "what lies behind the tiles fits");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
@@ -464,7 +467,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     mbar_init(ending, 1);
     mbar_init(&taken_out[0], 1);
     mbar_init(&taken_out[1], 1);
-    again[0] = again[1] = *gave_up = 0;
+    again[0] = again[1] = gave_up[0] = gave_up[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -479,28 +482,30 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   pdl_wait_primary();
   const uint32_t tmem = *tmem_holder;
   const int TPT = a.tokens_per_tile;
-  unsigned limit = kTileWaitLimit;
+  unsigned limit = a.wait_limit;
 
   // Place of key tile j and value tile j in an item's order of the ring: the order in which the products take them.
   auto key_at = [](int j) { return !EARLY ? 2 * j : j == 0 ? 0 : 2 * j - 1; };
   auto value_at = [](int j, int nk) { return !EARLY || j == nk - 1 ? 2 * j + 1 : 2 * j + 2; };
+  // A wait of this warp has run out.  (All lanes of a wait test one word in one instruction, so they agree.)
+  auto ran_out = [&]() { return __any_sync(0xffffffffu, limit == 1) != 0; };
   // The working warps' next item (this CTA's k-th); b = -1 ends.
   auto next_work = [&](int k) {
     tile_wait(&work_full[k & 1], (k >> 1) & 1, limit);
     TileWork w = work[k & 1];
-    if (limit == 1) w.b = -1;
-    __syncwarp();
+    if (ran_out()) w.b = -1;
     if (lane == 0) mbar_arrive(&work_empty[k & 1]);
     return w;
   };
   // The end of the usual pass, where every warp meets.  True: a pass with care follows.
   auto go_again = [&]() {
-    if (limit == 1 && lane == 0) *gave_up = 1;
+    if (ran_out() && lane == 0) gave_up[0] = 1;
     tc_fence_before();
     __syncthreads();
-    return *gave_up == 0 && again[0] + again[1] > 0;
+    return gave_up[0] == 0 && again[0] + again[1] > 0;
   };
   auto end_care = [&]() {
+    if (ran_out() && lane == 0) gave_up[1] = 1;
     tc_fence_before();
     __syncthreads();
   };
@@ -519,7 +524,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (warp == kTmaWarp) {
       // ---- copies
       int k = 0;
-      unsigned base = 0, qn = 0, tails = 0;  // ring tiles, query loads and mended tails of earlier items
+      unsigned base = 0, issued = 0, qn = 0, tails = 0;  // ring tiles of earlier items, all issued; queries; mended tiles
       auto pass = [&](auto care) {
         constexpr bool CARE = decltype(care)::value;
         unsigned cares = 0;
@@ -530,7 +535,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (nk == 0) continue;
           if (qn > 0) tile_wait(q_empty, (qn - 1) & 1, limit);
           ++qn;
-          if (lane == 0) {
+          // (once a wait has run out nothing is armed or loaded any more)
+          if (lane == 0 && limit != 1) {
             // a tile whose queries all lie past the sequence, or that sees no key of the range, is not loaded
             const int lo = w.steps[0] > 0 ? 0 : 1, hi = w.steps[1] > 0 ? 2 : 1;
             mbar_arrive_expect_tx(q_full, (hi - lo) * SUB * TPT * a.s.rep * 128);
@@ -567,15 +573,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const unsigned g = base + n, slot = g % NS;
             uint64_t* bar = mend ? v_tail : &kv_full[slot];
             if (g >= NS) tile_wait(&kv_empty[slot], ((g / NS) - 1) & 1, limit);
-            if (lane == 0) mbar_arrive_expect_tx(bar, boxes * a.box_rows * SUB * 128);
+            if (lane == 0 && limit != 1) mbar_arrive_expect_tx(bar, boxes * a.box_rows * SUB * 128);
             __syncwarp();
-            if (mine)
+            if (mine && limit != 1)
               for (int c = 0; c < SUB; ++c)
                 tma_load4(smem_addr(ring + slot * TB + c * (TB / SUB)) + lane * a.box_rows * 128, value ? &map_v : &map_k,
                           bar, c * 64, row, w.kvh, page);
             if (mend) {
-              tile_wait(v_tail, tails & 1, limit);
-              ++tails;
+              tile_wait(v_tail, tails++ & 1, limit);
               for (int e = n < 2 * nk - 1 ? kTileKeys * SUB * 8 : lane; e < (end - tail) * SUB * 8; e += 32) {
                 const int r = tail + e / (SUB * 8), c = e % (SUB * 8);
                 *reinterpret_cast<uint4*>(ring + slot * TB + (c >> 3) * (TB / SUB) + r * 128 + (c & 7) * 16) =
@@ -584,8 +589,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               if constexpr (CARE) take_out<T, D>(ring + slot * TB, 0, n < 2 * nk - 1 ? kTileKeys : tail, key0, bad);
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
               __syncwarp();
-              if (lane == 0) mbar_arrive(&kv_full[slot]);
+              if (lane == 0 && limit != 1) mbar_arrive(&kv_full[slot]);
             }
+            if (limit != 1) issued = g + 1;  // (a tile that goes to v_tail counts once it has been mended)
           }
           if constexpr (CARE) {
             __syncwarp();
@@ -594,11 +600,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
           base += 2 * nk;
         }
-        if (limit == 1) {  // a wait ran out: copies in flight land before the memory goes
-          unsigned more = kTileWaitLimit;
-          for (unsigned i = base > NS ? base - NS : 0; i < base; ++i) tile_wait(&kv_full[i % NS], (i / NS) & 1, more);
-          if (qn > 0) tile_wait(q_full, (qn - 1) & 1, more);
-          if (tails > 0) tile_wait(v_tail, (tails - 1) & 1, more);
+        if (ran_out()) {  // copies in flight land before the memory goes
+          unsigned more;
+          for (unsigned i = issued > NS ? issued - NS : 0; i < issued; ++i)
+            tile_wait(&kv_full[i % NS], (i / NS) & 1, more = kTileWaitLimit);
+          if (qn > 0) tile_wait(q_full, (qn - 1) & 1, more = kTileWaitLimit);
+          if (tails > 0) tile_wait(v_tail, (tails - 1) & 1, more = kTileWaitLimit);
         }
       };
       pass(std::false_type{});
@@ -612,6 +619,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       constexpr uint32_t IDESC_S = tile_idesc(kTileKeys, TYPE, 0), IDESC_O = tile_idesc(D, TYPE, 1);
       const uint32_t q_desc = desc_k_major(smem_addr(smem)), k_desc = desc_k_major(smem_addr(ring)),
                      v_desc = desc_n_major(smem_addr(ring), TB / SUB);
+      // (Nothing is issued once a wait has run out: a freed slot is loaded again, so what frees it must have seen its last
+      // load land.)
       unsigned base = 0, qn = 0, done0 = 0, done1 = 0;  // of earlier items: ring tiles, query loads, steps
       int k = 0;
       auto pass = [&](auto) {
@@ -656,7 +665,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (EARLY && done0 > 0 && w.steps[0] > 0) tile_wait(&s_free[0], (done0 - 1) & 1, limit);
           if (EARLY && done1 > 0 && w.steps[1] > 0) tile_wait(&s_free[1], (done1 - 1) & 1, limit);
           tc_fence_after();
-          if (elect_one()) {
+          if (elect_one() && limit != 1) {
             if (w.steps[0] > 0) scores(0, base % NS);
             if (w.steps[1] > 0) scores(1, base % NS);
             tc_commit(&kv_empty[base % NS]);
@@ -677,7 +686,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 else if (more0) tile_wait(&s_free[0], (done0 + j) & 1, limit);
                 else tile_wait(&s_free[1], (done1 + j) & 1, limit);
                 tc_fence_after();
-                if (elect_one()) {
+                if (elect_one() && limit != 1) {
                   if (more0) scores(0, kslot);
                   if (more1) scores(1, kslot);
                   tc_commit(&kv_empty[kslot]);
@@ -690,7 +699,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                   const unsigned par = ((i ? done1 : done0) + j) & 1;
                   tile_wait2(&p_full[2 * i + 1], par, full(vn), phase(vn), limit);
                   tc_fence_after();
-                  if (elect_one()) {
+                  if (elect_one() && limit != 1) {
                     outputs(i, vslot, 0, j == 0, groups);
                     outputs(i, vslot, 1, j == 0, groups);
                     tc_commit(&o_done[i]);
@@ -705,12 +714,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                   const unsigned par = ((i ? done1 : done0) + j) & 1;
                   tile_wait2(&p_full[2 * i], par, full(vn), phase(vn), limit);
                   tc_fence_after();
-                  if (elect_one()) outputs(i, vslot, 0, j == 0, groups);
+                  if (elect_one() && limit != 1) outputs(i, vslot, 0, j == 0, groups);
                   const bool more = i ? more1 : more0;
                   if (more) tile_wait2(&p_full[2 * i + 1], par, full(kn), phase(kn), limit);
                   else tile_wait(&p_full[2 * i + 1], par, limit);
                   tc_fence_after();
-                  if (elect_one()) {
+                  if (elect_one() && limit != 1) {
                     outputs(i, vslot, 1, j == 0, groups);
                     tc_commit(&o_done[i]);
                     if (i == 1 || j >= w.steps[1]) tc_commit(&kv_empty[vslot]);
@@ -727,11 +736,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           base += 2 * nk;
           done0 += w.steps[0];
           done1 += w.steps[1];
-        }
-        if (limit == 1) {  // a wait ran out: MMAs in flight finish before the memory goes
-          unsigned more = kTileWaitLimit;
-          if (elect_one()) tc_commit(drained);
-          tile_wait(drained, 0, more);
         }
       };
       pass(std::false_type{});
@@ -764,9 +768,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             work[k & 1] = w;
             mbar_arrive(&work_full[k & 1]);
           }
-          if (w.b < 0 || limit == 1) break;
+          if (w.b < 0 || ran_out()) break;
           tile_wait2(&work_empty[k & 1], (k >> 1) & 1, ending, k & 1, limit);
-          if (limit == 1) break;
+          if (ran_out()) break;
           if (repeat) continue;
           if (lane == 0) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the last reply has been read
@@ -775,7 +779,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
           __syncwarp();
           tile_wait(replied, asked & 1, limit);
-          if (limit == 1) {  // (the reply is still to land: once more before the memory goes)
+          if (ran_out()) {  // (the reply is still to land: once more before the memory goes)
             unsigned more = kTileWaitLimit;
             tile_wait(replied, asked & 1, more);
             break;
@@ -812,7 +816,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // (the item stays in work[k & 1] until this warp has asked for the next: read again where it is needed)
         tile_wait(&work_full[k & 1], (k >> 1) & 1, limit);
         const volatile TileWork& item = work[k & 1];
-        const int first = item.first, my_steps = item.b < 0 || limit == 1 ? -1 : item.steps[i];
+        const int first = item.first, my_steps = item.b < 0 || ran_out() ? -1 : item.steps[i];
         const int first_tok = item.tok0 + i * TPT, hidden = item.len - item.n;
         const bool valid = row < TPT * a.s.rep && first_tok + row_tok < item.n;
         const int lim = valid ? hidden + first_tok + row_tok : -1;  // last key the row sees
@@ -986,8 +990,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       end_care();
     }
   }
-  if (limit == 1 && lane == 0) atomicOr(&g_tile_device_error, 256u);
+  if (ran_out() && lane == 0) atomicOr(&g_tile_device_error, 256u);
   if (warp == kMmaWarp) {
+    if (gave_up[0] + gave_up[1] > 0) {  // MMAs in flight finish before the memory goes
+      unsigned more = kTileWaitLimit;
+      if (elect_one()) tc_commit(drained);
+      tile_wait(drained, 0, more);
+    }
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
   }
@@ -1142,6 +1151,13 @@ size_t tile_attention_part_bytes(int hd, int rep, int64_t tokens, int64_t kv_hea
          sizeof(float);
 }
 
+// Poll limit of the kernel's waits in later launches, for tests (0: the default).
+static std::atomic<unsigned> g_tile_wait_polls{0};
+int tile_set_wait_limit(unsigned polls) {
+  g_tile_wait_polls = polls == 1 ? 2 : polls;  // (a limit of 1 says that a wait has run out)
+  return LI4_OK;
+}
+
 int launch_tile_attention(const SeqAttnArgs& args, bool paged, int dtype, cudaStream_t stream) {
   TileArgs a;
   a.s = args;
@@ -1160,6 +1176,8 @@ int launch_tile_attention(const SeqAttnArgs& args, bool paged, int dtype, cudaSt
   if (rc != LI4_OK) return rc;
   const int sm = current_sm_count();
   a.part_slots = tile_part_slots(rep, args.T, args.Hkv, args.max_keys, sm);
+  const unsigned polls = g_tile_wait_polls.load();
+  a.wait_limit = polls != 0 ? polls : kTileWaitLimit + kTileWaitStep * (unsigned)((paged ? args.max_keys : args.T) / kTileKeys);
   const int64_t pairs = args.T / (2 * a.tokens_per_tile) + args.B;  // at least the sequences' pairs of tiles
   int64_t grid = pairs * args.Hkv;
   if (grid < a.part_slots) grid = a.part_slots;

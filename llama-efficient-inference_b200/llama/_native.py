@@ -120,6 +120,7 @@ SIGNATURES = {
     "li4_argmax_rows_keys": (_INT, [_P, _INT, _I64, _I64, _I64, _I64, _P, _I64, _P]),
     "li4_device_errors": (_INT, [ctypes.POINTER(ctypes.c_uint), _INT]),
     "li4_debug_set_wait_limits": (_INT, [ctypes.c_uint, ctypes.c_uint, ctypes.c_uint]),
+    "li4_debug_set_attention_wait_limit": (_INT, [ctypes.c_uint]),
     "li4_comm_alloc": (_INT, [_SZ, ctypes.POINTER(_P)]),
     "li4_comm_free": (_INT, [_P]),
     "li4_ipc_get_handle": (_INT, [_P, _P]),
