@@ -13,15 +13,6 @@ pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
 
 
-@pytest.fixture(autouse=True)
-def no_device_error(paged):  # noqa: F811
-    from llama import _native
-
-    _native.device_errors()
-    yield
-    assert _native.device_errors() == 0
-
-
 def close(got, q, k, v, skip=None):
     """test_paged_gpu.check for one sequence, a head's rows at a time: got, q [n, H, d], k / v [L, Hkv, d]; outputs where
     skip [n, H, d] is true are not looked at."""
