@@ -387,6 +387,14 @@ int li4_paged_append(const int32_t* kv_lens, const int32_t* new_lens, int64_t n_
                      int32_t* positions, int64_t* slots, int32_t* kv_lens_out, int32_t* n_free_out,
                      uint8_t* granted, void* stream);
 
+/* The same with a limit on a request's length: one that would hold more than max_len tokens after the step is
+ * refused whole, as where the table is too narrow (whose pages may hold up to page_size - 1 tokens more). */
+int li4_paged_append_within(const int32_t* kv_lens, const int32_t* new_lens, int64_t n_requests, int32_t* block_tables,
+                            int64_t table_stride, int64_t table_width, const int32_t* free_pages,
+                            int64_t free_capacity, const int32_t* n_free, int64_t page_size, int64_t n_tokens,
+                            int64_t max_len, int32_t* cu_seqlens, int32_t* positions, int64_t* slots,
+                            int32_t* kv_lens_out, int32_t* n_free_out, uint8_t* granted, void* stream);
+
 /* RoPE on packed queries and keys and the cache write of keys and values, in one launch.  q
  * [n_tokens, n_heads, head_dim], k and v [n_tokens, n_kv_heads, head_dim], LI4_F16 or LI4_BF16; pairs
  * (2i, 2i + 1) turn by the angle of table row positions[t], column i, in fp32, rounded once

@@ -46,6 +46,7 @@ struct AppendArgs {
   const int* n_free;
   long long table_stride;
   int B, width, log_page, capacity, T;
+  int max_len;     // no request grows past it
   int* cu;
   int* positions;
   long long* slots;
@@ -100,8 +101,9 @@ __device__ __forceinline__ bool append_request(const AppendArgs& a, int b, int* 
     return false;
   }
   const int want = (*c + *n + page - 1) >> a.log_page, held = (*c + page - 1) >> a.log_page;
-  *need = want <= a.width ? want - held : 0;
-  return want <= a.width;
+  const bool fits = want <= a.width && *c + *n <= a.max_len;
+  *need = fits ? want - held : 0;
+  return fits;
 }
 
 // TOK tokens in a row per thread: one search for the first, then on from request to request.
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(THREADS) paged_append_kernel(const __grid_cons
   for (int b = b0; b < b1; ++b) {
     int c, n, need;
     const bool fits = append_request(a, b, &c, &n, &need);
-    // granted: the table is wide enough, the pages are there, the tokens are among the step's T
+    // granted: the table is wide enough, the length allowed, the pages are there, the tokens are among the step's T
     const bool ok = fits && (need == 0 || at.pages + need <= n_free) && at.tokens + n <= a.T;
     s_cu[b] = (int)min(at.tokens, 0x7fffffffLL);
     s_ctx[b] = c;
@@ -355,6 +357,17 @@ extern "C" int li4_paged_append(const int32_t* kv_lens, const int32_t* new_lens,
                                 int64_t page_size, int64_t n_tokens, int32_t* cu_seqlens, int32_t* positions,
                                 int64_t* slots, int32_t* kv_lens_out, int32_t* n_free_out, uint8_t* granted,
                                 void* stream) {
+  return li4_paged_append_within(kv_lens, new_lens, n_requests, block_tables, table_stride, table_width, free_pages,
+                                 free_capacity, n_free, page_size, n_tokens, li4::kAppendMaxLen, cu_seqlens, positions,
+                                 slots, kv_lens_out, n_free_out, granted, stream);
+}
+
+extern "C" int li4_paged_append_within(const int32_t* kv_lens, const int32_t* new_lens, int64_t n_requests,
+                                       int32_t* block_tables, int64_t table_stride, int64_t table_width,
+                                       const int32_t* free_pages, int64_t free_capacity, const int32_t* n_free,
+                                       int64_t page_size, int64_t n_tokens, int64_t max_len, int32_t* cu_seqlens,
+                                       int32_t* positions, int64_t* slots, int32_t* kv_lens_out, int32_t* n_free_out,
+                                       uint8_t* granted, void* stream) {
   using namespace li4;
   if (n_requests < 0 || table_width < 0 || free_capacity < 0 || n_tokens < 0 || table_stride < table_width)
     return set_error(LI4_ERR_INVALID_ARG,
@@ -367,6 +380,7 @@ extern "C" int li4_paged_append(const int32_t* kv_lens, const int32_t* new_lens,
   if (n_requests > kAppendMaxRequests)
     return set_error(LI4_ERR_UNSUPPORTED, "paged_append: n_requests=%lld (at most %d)", (long long)n_requests,
                      kAppendMaxRequests);
+  if (max_len < 0) return set_error(LI4_ERR_INVALID_ARG, "paged_append: max_len=%lld", (long long)max_len);
   if (n_tokens > kAppendMaxLen || free_capacity > kAppendMaxLen || table_width > kAppendMaxLen)
     return set_error(LI4_ERR_INVALID_ARG, "paged_append: sizes above 2^30");
   if (!n_free || !cu_seqlens || !n_free_out ||
@@ -386,6 +400,7 @@ extern "C" int li4_paged_append(const int32_t* kv_lens, const int32_t* new_lens,
   a.log_page = ilog2(page_size);
   a.capacity = (int)free_capacity;
   a.T = (int)n_tokens;
+  a.max_len = (int)(max_len < kAppendMaxLen ? max_len : kAppendMaxLen);
   a.cu = cu_seqlens;
   a.positions = positions;
   a.slots = reinterpret_cast<long long*>(slots);

@@ -315,7 +315,7 @@ PyObject* rope_paged_write(PyObject* const* v) {
   return r;
 }
 
-// (kv_lens, new_lens, block_tables, free_pages, n_free, page_size, num_tokens, kv_lens_out, n_free_out)
+// (kv_lens, new_lens, block_tables, free_pages, n_free, page_size, num_tokens, kv_lens_out, n_free_out, max_len)
 PyObject* paged_append(PyObject* const* v) {
   const char* what = "paged_append";
   const Tensor kv = tensor(what, "kv_lens", v[0]), nl = tensor(what, "new_lens", v[1]),
@@ -338,6 +338,7 @@ PyObject* paged_append(PyObject* const* v) {
   if ((width > 1 && bt.stride(1) != 1) || (B > 1 && bt.stride(0) < width)) fail(what, "block_tables rows must be contiguous");
   const int64_t page = integer(what, "page_size", v[5]), T = integer(what, "num_tokens", v[6]);
   if (T < 0 || T > (1 << 30)) fail(what, "num_tokens ", T);
+  const int64_t max_len = v[9] == Py_None ? INT64_MAX : integer(what, "max_len", v[9]);
   const c10::cuda::CUDAGuard guard(d.dev);
   const Tensor kc = kv.contiguous(), nc = nl.contiguous(), fc = fp.contiguous();
   auto result = [&](const char* name, PyObject* o, const Tensor& like) {
@@ -355,9 +356,9 @@ PyObject* paged_append(PyObject* const* v) {
   int rc;
   {
     NoGil nogil;
-    rc = li4_paged_append(kc.const_data_ptr<int32_t>(), nc.const_data_ptr<int32_t>(), B, bt.data_ptr<int32_t>(),
+    rc = li4_paged_append_within(kc.const_data_ptr<int32_t>(), nc.const_data_ptr<int32_t>(), B, bt.data_ptr<int32_t>(),
                           B > 1 ? bt.stride(0) : width, width, fc.const_data_ptr<int32_t>(), fc.size(0),
-                          nf.const_data_ptr<int32_t>(), page, T, cu.data_ptr<int32_t>(), pos.data_ptr<int32_t>(),
+                          nf.const_data_ptr<int32_t>(), page, T, max_len, cu.data_ptr<int32_t>(), pos.data_ptr<int32_t>(),
                           slots.data_ptr<int64_t>(), kv_out.data_ptr<int32_t>(), nf_out.data_ptr<int32_t>(),
                           reinterpret_cast<uint8_t*>(granted.data_ptr()), stream);
   }
@@ -398,7 +399,7 @@ PyMethodDef method(const char* name) {
 }
 
 PyMethodDef methods[] = {method<prompt_attention, 7>("prompt_attention"), method<paged_attention, 9>("paged_attention"),
-                         method<rope_paged_write, 12>("rope_paged_write"), method<paged_append, 9>("paged_append"),
+                         method<rope_paged_write, 12>("rope_paged_write"), method<paged_append, 10>("paged_append"),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "li4_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -142,6 +142,8 @@ SIGNATURES = {
     "li4_program_set_trace": (_INT, [_P, _P, _I64]),
     "li4_program_info": (_INT, [_P, ctypes.POINTER(_INT), ctypes.POINTER(_INT), ctypes.POINTER(_SZ)]),
     "li4_paged_append": (_INT, [_P, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P]),
+    "li4_paged_append_within": (_INT, [_P, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P,
+                                       _P, _P]),
     "li4_rope_paged_write": (_INT, [_P, _P, _P, _INT, _I64, _I64, _I64, _I64, ctypes.POINTER(_I64), _P, _P, _I64,
                                     _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _P]),
     "li4_attention_workspace_bytes": (_SZ, [ctypes.POINTER(Attention)]),

@@ -47,16 +47,18 @@ def _done(what: str, result):
 
 def paged_append(kv_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor, free_pages: torch.Tensor,
                  n_free: torch.Tensor, page_size: int, num_tokens: int, kv_lens_out: Optional[torch.Tensor] = None,
-                 n_free_out: Optional[torch.Tensor] = None) -> PagedStep:
-    """One step's bookkeeping (li4_paged_append): request b holds kv_lens[b] tokens and appends new_lens[b].
+                 n_free_out: Optional[torch.Tensor] = None, max_len: Optional[int] = None) -> PagedStep:
+    """One step's bookkeeping (li4_paged_append_within): request b holds kv_lens[b] tokens and appends new_lens[b].
 
     kv_lens, new_lens int32 [requests]; block_tables int32 [requests, blocks], the entries of the step's fresh
     pages are written; free_pages int32 [capacity] with the free ones in free_pages[:n_free], taken from the top;
     n_free int32 [1]; num_tokens = sum(new_lens), which the host knows.  kv_lens_out / n_free_out may be kv_lens /
-    n_free (in place); by default they are new tensors.  A request that does not fit (table too narrow, too few
-    pages for it and those before it) is refused whole: granted False, length kept, slots -1."""
+    n_free (in place); by default they are new tensors.  A request that does not fit (more than max_len tokens with
+    the new ones, table too narrow, too few pages for it and those before it) is refused whole: granted False, length
+    kept, slots -1."""
     return PagedStep._make(_done("paged_append", native.ext().paged_append(
-        kv_lens, new_lens, block_tables, free_pages, n_free, page_size, num_tokens, kv_lens_out, n_free_out)))
+        kv_lens, new_lens, block_tables, free_pages, n_free, page_size, num_tokens, kv_lens_out, n_free_out,
+        max_len)))
 
 
 def rope_paged_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -130,9 +132,10 @@ class PagedKVCache:
 
     def append(self, new_lens: torch.Tensor, num_tokens: int) -> PagedStep:
         """Takes pages for new_lens[r] more tokens of every request r (int32 [max_requests], zeros for idle rows);
-        num_tokens is their sum.  Updates the cache's lengths, tables and free pages in place."""
+        num_tokens is their sum.  Updates the cache's lengths, tables and free pages in place.  A request that does not
+        fit, or that would hold more than max_len tokens, is refused whole (step.granted)."""
         return paged_append(self.kv_lens, new_lens, self.block_tables, self.free_pages, self.n_free, self.page_size,
-                            num_tokens, kv_lens_out=self.kv_lens, n_free_out=self.n_free)
+                            num_tokens, kv_lens_out=self.kv_lens, n_free_out=self.n_free, max_len=self.max_len)
 
     def release(self, finished: torch.Tensor) -> None:
         """Returns the pages of the requests flagged in finished (bool [max_requests]) and sets their lengths to 0.

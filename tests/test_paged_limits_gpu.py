@@ -1,0 +1,54 @@
+"""Limits of the paged serving path on the GPU: what is refused, and that a refusal is the only thing that happens."""
+import pytest
+import torch
+
+from test_paged_gpu import i32, paged, rand, tiny_model  # noqa: F401 (paged: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("page,max_len", [(16, 20), (16, 16), (8, 1), (1024, 37), (32, 95)])
+def test_no_request_grows_past_max_len(paged, page, max_len):  # noqa: F811
+    """max_len that is no multiple of the page size: the last page's other rows are never given out."""
+    cache = paged.PagedKVCache(1, 40, page, 1, 8, max_requests=3, max_len=max_len)
+    step = cache.append(i32([max_len, max_len + 1, max_len - 1]), 3 * max_len)
+    assert step.granted.tolist() == [True, False, True]
+    assert cache.kv_lens.tolist() == [max_len, 0, max_len - 1]
+    assert bool((step.slots[max_len:2 * max_len + 1] == -1).all()) and bool((step.slots[2 * max_len + 1:] >= 0).all())
+    free = int(cache.n_free)
+    step = cache.append(i32([1, 1, 1]), 3)
+    assert step.granted.tolist() == [False, True, True]
+    assert cache.kv_lens.tolist() == [max_len, 1, max_len]
+    step = cache.append(i32([1, 0, 1]), 2)
+    assert step.granted.tolist() == [False, True, False]
+    assert cache.kv_lens.tolist() == [max_len, 1, max_len] and int(cache.n_free) >= free - 2
+
+
+def test_append_takes_a_limit(paged):  # noqa: F811
+    tables = torch.full((3, 4), -1, dtype=torch.int32, device="cuda")
+    args = (i32([0, 5, 9]), i32([10, 5, 2]), tables, i32([0, 1, 2, 3, 4, 5]), i32([6]), 8, 17)
+    step = paged.paged_append(*args, max_len=10)
+    assert step.granted.tolist() == [True, True, False] and step.n_free.tolist() == [3]
+    assert step.kv_lens.tolist() == [10, 10, 9]
+    assert paged.paged_append(*args, max_len=11).granted.tolist() == [True, True, True]
+    assert paged.paged_append(*args).granted.tolist() == [True, True, True]
+    assert paged.paged_append(*args, max_len=1 << 62).granted.tolist() == [True, True, True]
+    assert paged.paged_append(*args, max_len=0).granted.tolist() == [False, False, False]
+    for bad in (-1, 1.5):
+        with pytest.raises(RuntimeError):
+            paged.paged_append(*args, max_len=bad)
+
+
+def test_the_model_s_positions_stay_inside_its_rope_table(paged):  # noqa: F811
+    """A cache as long as the RoPE table, which ends inside a page: tokens past it are refused, not clamped (the error
+    words are looked at after every test)."""
+    model = tiny_model()
+    rows = model.freqs_cis.shape[0]
+    cache = model.paged_cache(num_pages=2, page_size=1024, max_requests=1, max_len=rows)
+    tokens = torch.randint(0, 500, (rows,), device="cuda")
+    step = cache.append(i32([rows]), rows)
+    assert step.granted.tolist() == [True]
+    assert bool(torch.isfinite(model.forward_paged(tokens, step, cache, rows)).all())
+    step = cache.append(i32([1]), 1)
+    assert step.granted.tolist() == [False] and step.slots.tolist() == [-1]
+    assert cache.kv_lens.tolist() == [rows]
