@@ -403,7 +403,7 @@ int li4_paged_append_within(const int32_t* kv_lens, const int32_t* new_lens, int
  * strides: 16 element strides -- q token, head; k token, head; v token, head; q_out token, head; k_out
  * token, head; cache_k page, row, head; cache_v page, row, head -- all multiples of 8 (rows start on
  * 16-byte boundaries).  A position outside [0, max_pos) is clamped, a slot past the cache skipped; both
- * set bit 7 of li4_device_errors.  Tokens that share a slot are the caller's mistake: one of them stays. */
+ * set bit 7 of li4_device_errors (a token of negative slot, refused or padding, sets none).  Tokens that share a slot are the caller's mistake: one of them stays. */
 int li4_rope_paged_write(const void* q, const void* k, const void* v, int dtype, int64_t n_tokens, int64_t n_heads,
                          int64_t n_kv_heads, int64_t head_dim, const int64_t* strides, const float* rope_cos,
                          const float* rope_sin, int64_t rope_stride, int64_t max_pos, const int32_t* positions,

@@ -290,10 +290,9 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_write_kernel(const __
   const int d = (int)(i - t * a.chunks) * 8;
   int pos = a.positions[t];
   const long long slot = a.slots[t];
-  if (pos < 0 || pos >= a.max_pos || slot >= a.num_slots) {
-    atomicOr(&g_paged_device_error, 128u);
-    pos = max(0, min(pos, a.max_pos - 1));
-  }
+  // (a token that is skipped may stand anywhere: li4_paged_append refuses a request at the table's end like any other)
+  if (slot >= a.num_slots || (slot >= 0 && (pos < 0 || pos >= a.max_pos))) atomicOr(&g_paged_device_error, 128u);
+  pos = max(0, min(pos, a.max_pos - 1));
   const bool keep = slot >= 0 && slot < a.num_slots;
   const long long page = keep ? slot >> a.log_page : 0, row = keep ? slot & ((1 << a.log_page) - 1) : 0;
   const float4 c = *reinterpret_cast<const float4*>(a.cos + (long long)pos * a.srope + d / 2);

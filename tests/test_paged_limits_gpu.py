@@ -52,3 +52,27 @@ def test_the_model_s_positions_stay_inside_its_rope_table(paged):  # noqa: F811
     step = cache.append(i32([1]), 1)
     assert step.granted.tolist() == [False] and step.slots.tolist() == [-1]
     assert cache.kv_lens.tolist() == [rows]
+
+
+def test_refused_tokens_set_no_error(paged):  # noqa: F811
+    """Refused requests through the append and the RoPE write: one at the end of its table and of the RoPE table, one of
+    a negative length.  Their tokens have positions outside the table and are skipped; nothing is reported."""
+    from llama import _native
+
+    page, H, Hkv, d, rows = 16, 4, 2, 64, 32
+    kv, new, T = i32([rows, -5, 3]), i32([2, 2, 1]), 5
+    tables = i32([[0, 1], [2, 3], [4, 5]])
+    step = paged.paged_append(kv, new, tables, i32([6, 7]), i32([2]), page, T)
+    assert step.granted.tolist() == [False, False, True] and step.slots.tolist() == [-1, -1, -1, -1, 4 * page + 3]
+    q, k, v = rand((T, H, d), torch.float16, 1), rand((T, Hkv, d), torch.float16, 2), rand((T, Hkv, d), torch.float16, 3)
+    angle = torch.rand(rows, d // 2, device="cuda")
+    ck = torch.zeros(8, page, Hkv, d, dtype=torch.float16, device="cuda")
+    cv = torch.zeros_like(ck)
+    paged.rope_paged_write(q, k, v, angle.cos(), angle.sin(), step.positions, step.slots, ck, cv)
+    assert _native.device_errors() == 0
+    assert torch.equal(cv[4, 3], v[4]) and int((cv != 0).any(-1).sum()) == Hkv
+    # a bad position that would be written is reported
+    bad = step.positions.clone()
+    bad[4] = rows
+    paged.rope_paged_write(q, k, v, angle.cos(), angle.sin(), bad, step.slots, ck, cv)
+    assert _native.device_errors() == 128
