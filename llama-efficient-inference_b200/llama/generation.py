@@ -75,18 +75,22 @@ class DecodeGraph:
 
 
 class PagedDecodeGraph:
-    """Greedy decode steps of every request of a PagedKVCache, replayed from one CUDA graph.
+    """Greedy decode steps of the requests of a PagedKVCache, replayed from one CUDA graph.
 
-    tok int64 [requests] is a static buffer; replay() appends one token to every request (li4_paged_append), runs the
-    blocks over the cache and leaves each request's next token in tok.  The lengths, tables and free pages live on the
-    GPU, so the one graph serves every length.  Made after the prompts are in the cache: the warm-up steps run on the
-    requests as they are and the cache's bookkeeping is put back."""
+    tok int64 [requests] is a static buffer; replay() appends one token to every request of the cache
+    (li4_paged_append), runs the blocks over the cache and leaves each request's next token
+    in tok.  The lengths, tables and free pages live on the GPU, so the one graph serves every length.  Made after the
+    prompts are in the cache: the warm-up steps run on the requests as they are and the cache's bookkeeping is put back.
+
+    granted bool [requests] is a static buffer too: False from the first replay on that refused the request its token
+    (no page left, or max_len reached); such a replay leaves the request's token and length as they were."""
 
     @torch.no_grad()
     def __init__(self, model: nn.Module, cache, tok: torch.Tensor, warmup: int = 2):
         self.model, self.cache, self.tok = model, cache, tok.clone()
         self.one = torch.ones_like(cache.kv_lens)
-        state = (cache.kv_lens, cache.n_free, cache.block_tables, self.tok)
+        self.granted = torch.ones_like(self.one, dtype=torch.bool)
+        state = (cache.kv_lens, cache.n_free, cache.block_tables, self.tok, self.granted)
         saved = [t.clone() for t in state]
         dev = tok.device
         side = torch.cuda.Stream(dev)
@@ -106,7 +110,8 @@ class PagedDecodeGraph:
     def _step(self):
         step = self.cache.append(self.one, self.tok.shape[0])
         logits = self.model.forward_paged(self.tok, step, self.cache, 1)
-        self.tok.copy_(logits.argmax(-1))
+        torch.where(step.granted, logits.argmax(-1), self.tok, out=self.tok)
+        self.granted.logical_and_(step.granted)
         return logits
 
     def replay(self):
@@ -212,6 +217,8 @@ class Generation(nn.Module):
                 for _ in range(max_gen_len - 1):
                     graph.replay()
                     chosen.append(graph.tok.clone())
+                if not bool(graph.granted.all()):
+                    raise RuntimeError("generate_paged: a request was refused a token")
                 answers = torch.stack(chosen, 1).tolist()
             else:
                 going = [True] * n

@@ -76,3 +76,54 @@ def test_refused_tokens_set_no_error(paged):  # noqa: F811
     bad[4] = rows
     paged.rope_paged_write(q, k, v, angle.cos(), angle.sin(), bad, step.slots, ck, cv)
     assert _native.device_errors() == 128
+
+
+def prompts_in(model, cache, lens, seed):
+    """Random prompts of the given lengths (0: the request stays idle) through the cache; the requests' next tokens."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    tokens = torch.randint(0, 500, (sum(lens),), device="cuda", generator=gen)
+    step = cache.append(i32(lens), sum(lens))
+    assert bool(step.granted.all())
+    return model.forward_paged(tokens, step, cache, max(lens), whole_prompts=True).argmax(-1)
+
+
+def eager_steps(model, cache, tok, active, steps):
+    """Tokens of a loop over the active requests that stops feeding a request once it is refused."""
+    tok, history = tok.clone(), []
+    for _ in range(steps):
+        step = cache.append(i32([int(a) for a in active]), sum(active))
+        rows = [r for r, a in enumerate(active) if a]
+        best = model.forward_paged(tok[rows], step, cache, 1).argmax(-1)
+        for r in rows:
+            if bool(step.granted[r]):
+                tok[r] = best[r]
+        history.append(tok.clone())
+    return torch.stack(history)
+
+
+def test_captured_steps_say_which_requests_were_refused(paged):  # noqa: F811
+    """Pages run out, and a request reaches max_len, in the middle of the replays: the refused request keeps its token and
+    length and granted says so; the others go on as in an eager loop."""
+    from llama.generation import PagedDecodeGraph
+
+    model = tiny_model(seed=1)
+    lens, steps = [5, 17, 8], 12
+    with torch.no_grad():
+        caches = [model.paged_cache(num_pages=6, page_size=8, max_requests=3, max_len=24) for _ in range(2)]
+        first = [prompts_in(model, c, lens, 2) for c in caches]
+        assert torch.equal(*first)
+        want = eager_steps(model, caches[0], first[0], [True] * 3, steps)
+        graph = PagedDecodeGraph(model, caches[1], first[1])
+        assert graph.granted.tolist() == [True] * 3
+        got, granted = [], []
+        for _ in range(steps):
+            graph.replay()
+            got.append(graph.tok.clone())
+            granted.append(graph.granted.tolist())
+    assert torch.equal(torch.stack(got), want)
+    assert caches[1].kv_lens.tolist() == caches[0].kv_lens.tolist()
+    for r, n in enumerate(lens):
+        served = int(caches[1].kv_lens[r]) - n
+        assert [g[r] for g in granted] == [i < served for i in range(steps)]
+        assert all(int(t[r]) == int(got[served - 1][r]) for t in got[served:])
+    assert not all(granted[-1]) and caches[1].kv_lens.max() <= 24
