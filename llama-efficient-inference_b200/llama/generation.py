@@ -77,8 +77,8 @@ class DecodeGraph:
 class PagedDecodeGraph:
     """Greedy decode steps of the requests of a PagedKVCache, replayed from one CUDA graph.
 
-    tok int64 [requests] is a static buffer; replay() appends one token to every request of the cache
-    (li4_paged_append), runs the blocks over the cache and leaves each request's next token
+    tok int64 [requests] is a static buffer; replay() appends one token to every request that held tokens when the graph
+    was made (li4_paged_append; idle rows stay idle), runs the blocks over the cache and leaves each request's next token
     in tok.  The lengths, tables and free pages live on the GPU, so the one graph serves every length.  Made after the
     prompts are in the cache: the warm-up steps run on the requests as they are and the cache's bookkeeping is put back.
 
@@ -88,7 +88,11 @@ class PagedDecodeGraph:
     @torch.no_grad()
     def __init__(self, model: nn.Module, cache, tok: torch.Tensor, warmup: int = 2):
         self.model, self.cache, self.tok = model, cache, tok.clone()
-        self.one = torch.ones_like(cache.kv_lens)
+        self.one = (cache.kv_lens > 0).to(torch.int32)
+        rows = self.one.nonzero().view(-1)
+        if rows.numel() == 0:
+            raise ValueError("PagedDecodeGraph: no request of the cache holds a token")
+        self.rows = rows if rows.numel() < self.one.numel() else None  # the active requests, where some are idle
         self.granted = torch.ones_like(self.one, dtype=torch.bool)
         state = (cache.kv_lens, cache.n_free, cache.block_tables, self.tok, self.granted)
         saved = [t.clone() for t in state]
@@ -108,9 +112,11 @@ class PagedDecodeGraph:
         torch.cuda.synchronize(dev)
 
     def _step(self):
-        step = self.cache.append(self.one, self.tok.shape[0])
-        logits = self.model.forward_paged(self.tok, step, self.cache, 1)
-        torch.where(step.granted, logits.argmax(-1), self.tok, out=self.tok)
+        fed = self.tok if self.rows is None else self.tok.index_select(0, self.rows)
+        step = self.cache.append(self.one, fed.shape[0])
+        logits = self.model.forward_paged(fed, step, self.cache, 1)
+        moved = step.granted if self.rows is None else step.granted & (self.one > 0)
+        torch.where(moved, logits.argmax(-1), self.tok, out=self.tok)
         self.granted.logical_and_(step.granted)
         return logits
 

@@ -127,3 +127,21 @@ def test_captured_steps_say_which_requests_were_refused(paged):  # noqa: F811
         assert [g[r] for g in granted] == [i < served for i in range(steps)]
         assert all(int(t[r]) == int(got[served - 1][r]) for t in got[served:])
     assert not all(granted[-1]) and caches[1].kv_lens.max() <= 24
+
+
+def test_captured_steps_leave_idle_requests_idle(paged):  # noqa: F811
+    from llama.generation import PagedDecodeGraph
+
+    model = tiny_model(seed=2)
+    lens = [0, 9, 0, 30, 1]
+    with torch.no_grad():
+        caches = [model.paged_cache(num_pages=20, page_size=8, max_requests=5) for _ in range(2)]
+        first = [prompts_in(model, c, lens, 3) for c in caches]
+        want = eager_steps(model, caches[0], first[0], [n > 0 for n in lens], 6)
+        graph = PagedDecodeGraph(model, caches[1], first[1])
+        for i in range(6):
+            graph.replay()
+            assert torch.equal(graph.tok, want[i])
+        assert caches[1].kv_lens.tolist() == [0, 15, 0, 36, 7] and bool(graph.granted.all())
+        with pytest.raises(ValueError):
+            PagedDecodeGraph(model, model.paged_cache(num_pages=4, page_size=8, max_requests=2), first[0][:2])
