@@ -7,6 +7,7 @@
 // returned as an int for the caller to turn into its error.  Every C++ exception ends at the entry.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -31,7 +32,10 @@ template <typename... Args>
 
 Tensor tensor(const char* what, const char* name, PyObject* o) {
   if (!THPVariable_Check(o)) fail(what, name, " must be a tensor");
-  return THPVariable_Unpack(o);
+  const Tensor& t = THPVariable_Unpack(o);
+  if (c10::GradMode::is_enabled() && t.requires_grad())
+    fail(what, name, " requires grad and there is no backward pass: call under torch.no_grad()");
+  return t;
 }
 
 // The call's device: the first tensor's; every other tensor must be on it.

@@ -16,7 +16,8 @@ and replayed while the requests grow.  PagedKVCache holds the pool, Llama.forwar
 blocks over it, Generation.generate_paged is the loop around them.
 
 Every function runs on the current stream of its tensors' device, allocates its outputs (unless they are
-given) and its workspace there, and raises RuntimeError subclasses for arguments it does not take.
+given) and its workspace there, and raises RuntimeError subclasses for arguments it does not take.  None has a backward
+pass: tensors that require grad are refused outside torch.no_grad().
 """
 from __future__ import annotations
 

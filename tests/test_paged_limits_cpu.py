@@ -1,5 +1,6 @@
 """Arguments that the paged-cache entry points refuse on the host (no kernel is launched, no GPU needed)."""
 import pytest
+import torch
 
 
 @pytest.fixture(scope="module")
@@ -19,3 +20,43 @@ def test_append_refuses_a_negative_limit(native):
 
     assert append(-1) == native.LI4_ERR_INVALID_ARG and "max_len" in native.last_error()
     assert append(10, page=12) == native.LI4_ERR_UNSUPPORTED
+
+
+def calls(paged, q, k, cache):
+    """Every entry point on float tensors, as (name of a tensor, call with that tensor replaced)."""
+    i32 = dict(dtype=torch.int32, device=q.device)
+    cu, lens, tables = torch.tensor([0, 4], **i32), torch.tensor([4], **i32), torch.zeros(1, 2, **i32)
+    cos, pos = torch.zeros(8, 32, device=q.device), torch.zeros(4, **i32)
+    slots = torch.zeros(4, dtype=torch.long, device=q.device)
+    a = dict(q=q, k=k, v=k.detach().clone(), cache_k=cache, cache_v=cache.detach().clone(), cos=cos, sin=cos.clone())
+
+    def prompt(**x):
+        x = {**a, **x}
+        return paged.prompt_attention(x["q"], x["k"], x["v"], cu, 4, out=x.get("out"))
+
+    def over_cache(**x):
+        x = {**a, **x}
+        return paged.paged_attention(x["q"], x["cache_k"], x["cache_v"], tables, lens, cu, 4, out=x.get("out"))
+
+    def rope(**x):
+        x = {**a, **x}
+        return paged.rope_paged_write(x["q"], x["k"], x["v"], x["cos"], x["sin"], pos, slots, x["cache_k"], x["cache_v"],
+                                      q_out=x.get("q_out"), k_out=x.get("k_out"))
+
+    return a, {prompt: ("q", "k", "v"), over_cache: ("q", "cache_k", "cache_v"),
+               rope: ("q", "k", "v", "cos", "sin", "cache_k", "cache_v")}
+
+
+def test_tensors_that_require_grad_are_refused(native):
+    """There is no backward pass: a result without a graph would lose the gradient silently."""
+    from llama import paged
+
+    q, k = torch.zeros(4, 4, 64, dtype=torch.float16), torch.zeros(4, 2, 64, dtype=torch.float16)
+    a, table = calls(paged, q, k, torch.zeros(2, 16, 2, 64, dtype=torch.float16))
+    for call, names in table.items():
+        for name in names:
+            leaf = a[name].clone().requires_grad_()
+            with pytest.raises(RuntimeError, match=f"{name} requires grad"):
+                call(**{name: leaf})
+            with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+                call(**{name: leaf})
