@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -33,6 +34,10 @@ template <typename... Args>
 Tensor tensor(const char* what, const char* name, PyObject* o) {
   if (!THPVariable_Check(o)) fail(what, name, " must be a tensor");
   const Tensor& t = THPVariable_Unpack(o);
+  // These are no registered operators: a tracer would record nothing of the call, or meet a tensor without data.
+  if (t.key_set().has(c10::DispatchKey::Python) || !t.has_storage() ||
+      c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer))
+    fail(what, name, " must be a plain tensor, outside of any tracing");
   if (c10::GradMode::is_enabled() && t.requires_grad())
     fail(what, name, " requires grad and there is no backward pass: call under torch.no_grad()");
   return t;

@@ -17,7 +17,8 @@ blocks over it, Generation.generate_paged is the loop around them.
 
 Every function runs on the current stream of its tensors' device, allocates its outputs (unless they are
 given) and its workspace there, and raises RuntimeError subclasses for arguments it does not take.  None has a backward
-pass: tensors that require grad are refused outside torch.no_grad().
+pass: tensors that require grad are refused outside torch.no_grad(); and none is a registered operator: fake tensors
+and calls under a tracer are refused.
 """
 from __future__ import annotations
 

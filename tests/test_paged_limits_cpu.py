@@ -60,3 +60,25 @@ def test_tensors_that_require_grad_are_refused(native):
                 call(**{name: leaf})
             with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
                 call(**{name: leaf})
+
+
+def test_fake_tensors_and_tracing_are_refused(native):
+    """The functions are no registered operators: a tracer would record their outputs as constants."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from llama import paged
+
+    with FakeTensorMode():
+        q, k = torch.zeros(4, 4, 64, dtype=torch.float16), torch.zeros(4, 2, 64, dtype=torch.float16)
+        _, table = calls(paged, q, k, torch.zeros(2, 16, 2, 64, dtype=torch.float16))
+        for call in table:
+            with pytest.raises(RuntimeError, match="plain tensor"):
+                call()
+        i32 = dict(dtype=torch.int32)
+        with pytest.raises(RuntimeError, match="plain tensor"):
+            paged.paged_append(torch.zeros(2, **i32), torch.zeros(2, **i32), torch.zeros(2, 4, **i32),
+                               torch.zeros(8, **i32), torch.zeros(1, **i32), 16, 0)
+    q, k = torch.zeros(4, 4, 64, dtype=torch.float16), torch.zeros(4, 2, 64, dtype=torch.float16)
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="plain tensor"):
+        torch.jit.trace(lambda x: paged.prompt_attention(x, k, k, cu, 4), (q,))
