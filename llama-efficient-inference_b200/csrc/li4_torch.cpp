@@ -102,6 +102,41 @@ Tensor output(const char* what, const char* name, PyObject* o, const Tensor& lik
   return t;
 }
 
+// Whether two tensors of 16-bit values share no memory, as far as their strides show it: their ranges lie apart, or they
+// are parts of one wider row (queries, keys and values of one projection): modulo some stride of theirs, what the
+// dimensions of other strides span lies apart.
+bool apart(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return true;
+  auto span = [](const Tensor& t, int64_t modulo) {  // elements, the dimensions of strides that are multiples left out
+    int64_t n = 1;
+    for (int64_t i = 0; i < t.dim(); ++i)
+      if (modulo == 0 || t.stride(i) % modulo != 0) n += (t.size(i) - 1) * t.stride(i);
+    return n;
+  };
+  const int64_t pa = (int64_t)(reinterpret_cast<uintptr_t>(a.data_ptr()) / 2),
+                pb = (int64_t)(reinterpret_cast<uintptr_t>(b.data_ptr()) / 2);
+  if (pa + span(a, 0) <= pb || pb + span(b, 0) <= pa) return true;
+  for (const Tensor* t : {&a, &b})
+    for (int64_t i = 0; i < t->dim(); ++i) {
+      const int64_t m = t->stride(i);
+      if (t->size(i) < 2 || m < 1) continue;
+      const int64_t ahead = ((pb - pa) % m + m) % m;
+      if (ahead >= span(a, m) && m - ahead >= span(b, m)) return true;
+    }
+  return false;
+}
+
+bool same_rows(const Tensor& a, const Tensor& b) {
+  if (a.data_ptr() != b.data_ptr()) return false;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) != b.size(i) || (a.size(i) > 1 && a.stride(i) != b.stride(i))) return false;
+  return true;
+}
+
+void not_over(const char* what, const char* out_name, const Tensor& out, const char* name, const Tensor& in) {
+  if (!apart(out, in)) fail(what, out_name, " must not overlap ", name);
+}
+
 void cache_ok(const char* what, const char* name, const Tensor& t, const Tensor& q, int64_t kv_heads) {
   if (t.dim() != 4 || t.size(2) != kv_heads || t.size(3) != q.size(2) || t.scalar_type() != q.scalar_type())
     fail(what, name, " must be ", q.scalar_type(), " [pages, page_size, ", kv_heads, ", ", q.size(2), "], got ",
@@ -173,11 +208,6 @@ void queries_ok(const char* what, const Tensor& q, const Tensor& cu, int64_t kv_
   if (max_queries < 0) fail(what, "a longest sequence of ", max_queries, " queries");
 }
 
-void out_ok(const char* what, const Tensor& out, const Tensor& q) {
-  if (out.numel() && out.data_ptr() == q.data_ptr())
-    fail(what, "out must not be q: rows are read again after others are written");
-}
-
 // (q, k, v, cu_seqlens, max_len, scale, out)
 PyObject* prompt_attention(PyObject* const* v) {
   const char* what = "prompt_attention";
@@ -197,7 +227,11 @@ PyObject* prompt_attention(PyObject* const* v) {
     fail(what, "q ", q.sizes(), ", k ", k.sizes(), " and v ", val.sizes(), " do not match");
   const c10::cuda::CUDAGuard guard(d.dev);
   const Tensor out = output(what, "out", v[6], q, d);
-  out_ok(what, out, q);
+  if (v[6] != Py_None) {  // (rows are read again after others are written)
+    not_over(what, "out", out, "q", q);
+    not_over(what, "out", out, "k", k);
+    not_over(what, "out", out, "v", val);
+  }
   const Tensor kr = readable(k), vr = readable(val);
   li4_attention a = {};
   a.k = kr.data_ptr();
@@ -236,7 +270,11 @@ PyObject* paged_attention(PyObject* const* v) {
   ints(what, "kv_lens", lens, at::kInt, {B});
   const c10::cuda::CUDAGuard guard(d.dev);
   const Tensor out = output(what, "out", v[8], q, d);
-  out_ok(what, out, q);
+  if (v[8] != Py_None) {
+    not_over(what, "out", out, "q", q);
+    not_over(what, "out", out, "cache_k", ck);
+    not_over(what, "out", out, "cache_v", cv);
+  }
   const bool table_ok = (width <= 1 || bt.stride(1) == 1) && (B <= 1 || bt.stride(0) >= width);
   const Tensor tables = table_ok ? bt : bt.contiguous(), l = lens.contiguous();
   li4_attention a = {};
@@ -296,6 +334,18 @@ PyObject* rope_paged_write(PyObject* const* v) {
   const Tensor q_out = output(what, "q_out", v[9], q, d);
   Tensor k_out;
   if (want_k) k_out = output(what, "k_out", v[10], k, d);
+  // an output may be its own input; nothing else may be written before it is read
+  auto check = [&](const char* name, const Tensor& out, const char* own_name, const Tensor& own, const char* other_name,
+                   const Tensor& other) {
+    if (!same_rows(out, own)) not_over(what, name, out, own_name, own);
+    not_over(what, name, out, other_name, other);
+    not_over(what, name, out, "v", val);
+    not_over(what, name, out, "cache_k", ck);
+    not_over(what, name, out, "cache_v", cv);
+  };
+  if (v[9] != Py_None) check("q_out", q_out, "q", q, "k", k);
+  if (v[10] != Py_None) check("k_out", k_out, "k", k, "q", q);
+  if (v[9] != Py_None && v[10] != Py_None) not_over(what, "q_out", q_out, "k_out", k_out);
   auto table = [](const Tensor& t) {
     return t.is_contiguous() && !(reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) ? t : t.clone(at::MemoryFormat::Contiguous);
   };

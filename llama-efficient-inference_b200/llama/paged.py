@@ -72,7 +72,7 @@ def rope_paged_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: tor
     Pairs (2i, 2i + 1) turn by the angle in row positions[t] of cos / sin (fp32 [positions, d / 2]), in fp32.  The
     turned key and the value of token t go to row slots[t] % page_size of page slots[t] // page_size of cache_k /
     cache_v [pages, page_size, kv_heads, d] (any strides with contiguous rows); negative slots are skipped.
-    Returns (turned q, turned k); q_out / k_out may be q / k themselves.  need_k = False leaves the packed turned
+    Returns (turned q, turned k); q_out / k_out may be q / k themselves and overlap nothing else.  need_k = False leaves the packed turned
     keys out (returns None for them): attention over the cache does not read them."""
     return _done("rope_paged_write", native.ext().rope_paged_write(q, k, v, cos, sin, positions, slots, cache_k, cache_v,
                                                                    q_out, k_out, need_k))

@@ -145,3 +145,53 @@ def test_captured_steps_leave_idle_requests_idle(paged):  # noqa: F811
         assert caches[1].kv_lens.tolist() == [0, 15, 0, 36, 7] and bool(graph.granted.all())
         with pytest.raises(ValueError):
             PagedDecodeGraph(model, model.paged_cache(num_pages=4, page_size=8, max_requests=2), first[0][:2])
+
+
+def test_outputs_that_overlap_their_inputs_are_refused(paged):  # noqa: F811
+    from test_paged_limits_cpu import calls
+
+    T, H, Hkv, d, page = 4, 4, 2, 64, 16
+    dtype = torch.float16
+    pool = torch.zeros(1 << 16, dtype=dtype, device="cuda")
+
+    def at(start, shape):
+        n = 1
+        for x in shape:
+            n *= x
+        return pool[start:start + n].view(shape)
+
+    Q, K, C = (T, H, d), (T, Hkv, d), (2, page, Hkv, d)
+    q, k, cache = at(8192, Q), at(16384, K), at(24576, C)
+    a, table = calls(paged, q, k, cache)
+    prompt, over_cache, rope = table
+    v, cache_v = at(32768, K), at(40960, C)
+    bad = [(prompt, dict(out=at(8192 + 8, Q))), (prompt, dict(out=at(8192 - 8, Q))), (prompt, dict(out=q)),
+           (prompt, dict(out=at(16384 + K[0] * Hkv * d - 8, Q))), (prompt, dict(out=at(16384 - 8, Q))),
+           (prompt, dict(v=v, out=at(32768 + 64, Q))), (over_cache, dict(out=at(24576 + 1024, Q))),
+           (over_cache, dict(cache_v=cache_v, out=at(40960 + 2048, Q))), (over_cache, dict(out=at(8192 + 64, Q))),
+           (rope, dict(q_out=at(8192 + 8, Q))), (rope, dict(q_out=at(16384, Q))), (rope, dict(k_out=at(8192, K))),
+           (rope, dict(v=v, k_out=v)), (rope, dict(q_out=at(24576, Q))), (rope, dict(cache_v=cache_v, k_out=at(40960, K))),
+           (rope, dict(q_out=at(49152, Q), k_out=at(49152 + 64, K))),
+           # the same memory in another order
+           (rope, dict(q_out=at(8192, (H, T, d)).transpose(0, 1)))]
+    for i, (call, over) in enumerate(bad):
+        with pytest.raises(RuntimeError, match="overlap"):
+            call(**over)
+            pytest.fail(f"call {i} was not refused")
+    # what touches without overlapping, in place, and parts of one wide row
+    prompt(out=at(8192 + T * H * d, Q))
+    prompt(out=at(16384 - T * H * d, Q))
+    rope(q_out=q, k_out=k)
+    rope(q_out=q)
+    wide = rand((T, (2 * H + 3 * Hkv) * d), dtype, 1)
+    parts, start = [], 0
+    for heads in (H, Hkv, Hkv, H, Hkv):
+        parts.append(wide[:, start:start + heads * d].view(T, heads, d))
+        start += heads * d
+    prompt(q=parts[0], k=parts[1], v=parts[2], out=parts[3])
+    rope(q=parts[0], k=parts[1], v=parts[2], q_out=parts[3], k_out=parts[4])
+    rope(q=parts[0], k=parts[1], v=parts[2], q_out=parts[0], k_out=parts[1])
+    # heads interleaved in pairs of rows: q and the output take turns
+    turns = rand((T, H, 2, d), dtype, 2)
+    prompt(q=turns[:, :, 0], out=turns[:, :, 1])
+    torch.cuda.synchronize()
