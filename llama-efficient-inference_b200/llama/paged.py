@@ -152,13 +152,16 @@ class PagedKVCache:
 
 
 def rope_tables(model) -> Tuple[torch.Tensor, torch.Tensor]:
-    """The model's RoPE angles as fp32 cos / sin tables on its device (made once)."""
-    dev = model.tok_embeddings.weight.device
-    tables = getattr(model, "_rope_tables", None)
-    if tables is None or tables[0].device != dev:
-        freqs = model.freqs_cis.to(dev)
-        tables = model._rope_tables = (freqs.real.float().contiguous(), freqs.imag.float().contiguous())
-    return tables
+    """The model's RoPE angles as fp32 cos / sin tables on its device, made again when freqs_cis is another tensor, has been
+    written to, or the model has moved."""
+    dev, freqs = model.tok_embeddings.weight.device, model.freqs_cis
+    version = 0 if freqs.is_inference() else freqs._version  # (inference tensors count no writes)
+    made = getattr(model, "_rope_tables", None)
+    if made is None or made[0] is not freqs or made[1] != version or made[2].device != dev:
+        here = freqs.to(dev)
+        made = model._rope_tables = (freqs, version, here.real.float().contiguous(),
+                                     here.imag.float().contiguous())
+    return made[2], made[3]
 
 
 def forward_paged(model, tokens: torch.Tensor, step: PagedStep, cache: PagedKVCache, max_new: int,

@@ -82,3 +82,22 @@ def test_fake_tensors_and_tracing_are_refused(native):
     cu = torch.tensor([0, 4], dtype=torch.int32)
     with pytest.raises(RuntimeError, match="plain tensor"):
         torch.jit.trace(lambda x: paged.prompt_attention(x, k, k, cu, 4), (q,))
+
+
+def test_rope_tables_follow_the_model(native):
+    """A freqs_cis that is replaced or written to is seen; one that is not is not turned into tables again."""
+    from llama.model import Llama, ModelArgs
+    from llama.paged import rope_tables
+
+    model = Llama(ModelArgs(dim=64, n_layers=1, n_heads=2, n_kv_heads=1, vocab_size=16, multiple_of=32, max_batch_size=1,
+                            max_seq_len=8))
+    cos, sin = rope_tables(model)
+    assert torch.equal(cos, model.freqs_cis.real.float()) and torch.equal(sin, model.freqs_cis.imag.float())
+    assert rope_tables(model)[0] is cos
+    model.freqs_cis = model.freqs_cis.conj().resolve_conj().clone()
+    assert torch.equal(rope_tables(model)[1], -sin)
+    model.freqs_cis.mul_(2)
+    assert torch.equal(rope_tables(model)[0], 2 * cos)
+    with torch.inference_mode():
+        model.freqs_cis = model.freqs_cis.clone()
+    assert torch.equal(rope_tables(model)[0], 2 * cos)
