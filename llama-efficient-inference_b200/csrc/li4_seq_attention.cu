@@ -705,6 +705,8 @@ int launch_seq_attention(const SeqAttnArgs& args, bool paged, int dtype, int max
 // 8-row tiles beside a chunk 8 us less than with 16-row tiles).
 constexpr int kFewRows = 32, kFewRowsBeside = 8;
 
+constexpr int64_t kAttentionMost = 1 << 30;  // rows of a sequence, keys: what is claimed above it counts as it
+
 static int check_attention(const li4_attention* p, bool paged, const char* what) {
   if (!p) return set_error(LI4_ERR_INVALID_ARG, "%s: null arguments", what);
   if (p->dtype != LI4_F16 && p->dtype != LI4_BF16)
@@ -728,7 +730,7 @@ static int check_attention(const li4_attention* p, bool paged, const char* what)
       return set_error(LI4_ERR_UNSUPPORTED, "%s: page_size=%lld (a power of two from 8 to 1024)", what,
                        (long long)p->page_size);
     if (p->num_pages < 0 || p->num_pages > (1LL << 31) - 1 || p->table_width < 0 || p->table_stride < p->table_width ||
-        p->table_width * p->page_size > (1LL << 30))
+        p->table_width > kAttentionMost / p->page_size)
       return set_error(LI4_ERR_INVALID_ARG, "%s: num_pages=%lld table_width=%lld table_stride=%lld", what,
                        (long long)p->num_pages, (long long)p->table_width, (long long)p->table_stride);
   }
@@ -750,13 +752,15 @@ static int check_attention(const li4_attention* p, bool paged, const char* what)
 }
 
 static int attention_rows(const li4_attention* p) {
-  const int64_t rows = p->max_queries * (p->n_heads / p->n_kv_heads);
-  return (int)(rows > (1 << 30) ? (1 << 30) : rows);
+  const int64_t rep = p->n_heads / p->n_kv_heads;
+  return (int)(p->max_queries > kAttentionMost / rep ? kAttentionMost : p->max_queries * rep);
 }
 
 // The most keys a sequence can have, as far as the host knows.
 static int64_t attention_keys(const li4_attention* p) {
-  return p->kv_lens ? p->table_width * p->page_size : p->max_queries;
+  if (!p->kv_lens) return p->max_queries < kAttentionMost ? p->max_queries : kAttentionMost;
+  if (p->page_size < 1 || p->table_width < 1) return 0;
+  return p->table_width > kAttentionMost / p->page_size ? kAttentionMost : p->table_width * p->page_size;
 }
 
 static int run_attention(const li4_attention* p, bool paged, void* workspace, size_t workspace_bytes, void* stream,

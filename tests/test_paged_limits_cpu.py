@@ -1,4 +1,6 @@
 """Arguments that the paged-cache entry points refuse on the host (no kernel is launched, no GPU needed)."""
+import ctypes
+
 import pytest
 import torch
 
@@ -101,3 +103,21 @@ def test_rope_tables_follow_the_model(native):
     with torch.inference_mode():
         model.freqs_cis = model.freqs_cis.clone()
     assert torch.equal(rope_tables(model)[0], 2 * cos)
+
+
+def attention_args(native, **over):
+    D, H, Hkv, page = 64, 8, 2, 16
+    a = native.Attention(q=16, k=16, v=16, out=16, dtype=0, scale=0.125, stride_qt=H * D, stride_qh=D,
+                         stride_ot=H * D, stride_oh=D, stride_kp=page * Hkv * D, stride_kt=Hkv * D, stride_kh=D,
+                         stride_vp=page * Hkv * D, stride_vt=Hkv * D, stride_vh=D, cu_seqlens=16, n_seqs=2, n_tokens=8,
+                         n_heads=H, n_kv_heads=Hkv, head_dim=D, max_queries=4, kv_lens=16, block_tables=16,
+                         table_stride=8, table_width=8, num_pages=20, page_size=page)
+    for name, value in over.items():
+        setattr(a, name, value)
+    return a
+
+
+def test_tables_whose_width_passes_64_bits_are_refused(native):
+    for width in (1 << 59, 1 << 60, (1 << 63) - 1):
+        a = attention_args(native, table_width=width, table_stride=width)
+        assert native.lib().li4_paged_attention(ctypes.byref(a), 16, 1 << 40, None) == native.LI4_ERR_INVALID_ARG

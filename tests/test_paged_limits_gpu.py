@@ -195,3 +195,28 @@ def test_outputs_that_overlap_their_inputs_are_refused(paged):  # noqa: F811
     turns = rand((T, H, 2, d), dtype, 2)
     prompt(q=turns[:, :, 0], out=turns[:, :, 1])
     torch.cuda.synchronize()
+
+
+def test_claims_whose_products_pass_64_bits(paged):  # noqa: F811
+    """A longest sequence or a table width near 2^62 counts as a long one; it does not wrap to a short one."""
+    import ctypes
+
+    from llama import _native as native
+    from test_paged_limits_cpu import attention_args
+
+    def need(**over):
+        return native.lib().li4_attention_workspace_bytes(ctypes.byref(attention_args(native, **over)))
+
+    for kv_lens in (None, 16):
+        long = need(kv_lens=kv_lens, table_width=128, max_queries=1 << 28)
+        assert long > need(kv_lens=kv_lens, table_width=128, max_queries=4)
+        for claim in (1 << 30, 1 << 61, 1 << 62, (1 << 63) - 1):
+            assert need(kv_lens=kv_lens, table_width=128, max_queries=claim) == long
+    wide = need(max_queries=100, table_width=1 << 26)
+    for width in (1 << 59, 1 << 60, (1 << 63) - 1):
+        assert need(max_queries=100, table_width=width) == wide
+    q, k = rand((70, 4, 64), torch.float16, 1), rand((70, 2, 64), torch.float16, 2)
+    cu = i32([0, 70])
+    want = paged.prompt_attention(q, k, k, cu, 70)
+    for claim in (1 << 61, 1 << 62, (1 << 63) - 1):
+        assert torch.equal(paged.prompt_attention(q, k, k, cu, claim), want)
