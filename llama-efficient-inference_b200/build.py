@@ -7,7 +7,9 @@ links lib/libllama_int4_b200.so -- a plain C-ABI shared library (see
 include/llama_int4_b200.h) with the CUDA runtime linked statically, so it
 loads with or without torch in the process -- and compiles csrc/li4_torch.cpp
 against this interpreter's torch into lib/li4_torch.so, the binding of the
-paged-cache entry points to torch tensors (it links the C-ABI library).
+paged-cache entry points to torch tensors (it links the C-ABI library).  Without
+g++, torch or their headers the library is built alone, and llama.paged raises
+when it is used.
 """
 from __future__ import annotations
 
@@ -50,10 +52,28 @@ def _deps() -> list[str]:
 
 
 def up_to_date() -> bool:
-    if not os.path.exists(LIB_PATH) or not os.path.exists(EXT_PATH):
+    if not os.path.exists(LIB_PATH):
         return False
-    t = min(os.path.getmtime(LIB_PATH), os.path.getmtime(EXT_PATH))
+    t = os.path.getmtime(LIB_PATH)
+    if os.path.exists(EXT_PATH):
+        t = min(t, os.path.getmtime(EXT_PATH))
+    elif not why_no_binding():
+        return False
     return all(os.path.getmtime(d) <= t for d in _deps())
+
+
+def why_no_binding() -> str:
+    """What the binding cannot be built without, "" if it can."""
+    if shutil.which("g++") is None:
+        return "no g++"
+    try:
+        import torch
+    except ImportError as e:
+        return f"no torch ({e})"
+    headers = [os.path.join(os.path.dirname(torch.__file__), "include", "ATen", "ATen.h"),
+               os.path.join(sysconfig.get_paths()["include"], "Python.h")]
+    missing = [h for h in headers if not os.path.exists(h)]
+    return f"no {missing[0]}" if missing else ""
 
 
 def compile_binding(verbose: bool) -> str:
@@ -116,8 +136,9 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
             sys.stdout.write(r.stderr)
         return obj
 
+    missing = why_no_binding()
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
-        binding = ex.submit(compile_binding, verbose)
+        binding = None if missing else ex.submit(compile_binding, verbose)
         objs = list(ex.map(compile_one, sources()))
     tmp = LIB_PATH + ".tmp"
     cmd = [cc] + ARCH_FLAGS + ["-shared", "-o", tmp] + objs
@@ -127,7 +148,12 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB_PATH)
-    link_binding(binding.result(), verbose)
+    if binding is None:
+        print(f"build.py: li4_torch.so is not built ({missing}); llama.paged needs it", file=sys.stderr)
+        if os.path.exists(EXT_PATH):
+            os.remove(EXT_PATH)  # (made for another build of the library)
+    else:
+        link_binding(binding.result(), verbose)
     return LIB_PATH
 
 
