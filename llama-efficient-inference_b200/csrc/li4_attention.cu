@@ -606,18 +606,24 @@ template <typename KernelT>
 static int launch_attn(KernelT kernel, const AttnArgs& a, int batch, int cluster, size_t smem, cudaStream_t stream) {
   if (smem + 4096 > 48 * 1024) {  // dynamic + the static softmax partials past the 48 KiB default
     static std::mutex mu;
-    static std::vector<std::pair<int, size_t>> raised;  // (device, bytes) of this instantiation
+    // (by kernel: all instantiations have one signature and so share this function)
+    struct Raised {
+      int dev;
+      KernelT kernel;
+      size_t bytes;
+    };
+    static std::vector<Raised> raised;
     int dev = 0;
     cudaGetDevice(&dev);
     std::lock_guard<std::mutex> lock(mu);
     bool ok = false;
     for (auto& e : raised)
-      if (e.first == dev && e.second >= smem) ok = true;
+      if (e.dev == dev && e.kernel == kernel && e.bytes >= smem) ok = true;
     if (!ok) {
       const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                                 "decode_attention: cudaFuncSetAttribute");
       if (rc != LI4_OK) return rc;
-      raised.emplace_back(dev, smem);
+      raised.push_back({dev, kernel, smem});
     }
   }
   cudaLaunchConfig_t cfg = {};
