@@ -23,8 +23,8 @@
 //
 // A masked key's probability is zero, but zero times a NaN or an infinity is NaN: a value that a row must not see can
 // reach it through the last few key tiles of an item, where some keys are hidden from some rows.  A CTA that meets an
-// output that is not finite therefore runs that item again, and its later ones from the start, with care (every role's
-// code exists twice, so the usual pass is spared the tests): the copying warp takes the values that are not finite out of those tiles before the products may have them and notes where in each
+// output that is not finite therefore runs that item again, and its later ones from the start, with care (a role's
+// code exists twice where that spares the usual pass time): the copying warp takes the values that are not finite out of those tiles before the products may have them and notes where in each
 // dim the first +inf, -inf or NaN stood, and a row that sees that key gets it added at the end (added to a
 // sum, what is not finite does not depend on its weight).  At most two items of a CTA run twice, whatever the context.
 // Every mbarrier wait is bounded: one that runs out sets bit 8 of li4_device_errors.  The copying warp then issues
@@ -526,8 +526,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // ---- copies
       int k = 0;
       unsigned base = 0, issued = 0, qn = 0, tails = 0;  // ring tiles of earlier items, all issued; queries; mended tiles
-      auto pass = [&](auto care) {
-        constexpr bool CARE = decltype(care)::value;
+      auto pass = [&](const bool with_care) {
         unsigned cares = 0;
         for (;;) {
           const TileWork w = next_work(k++);
@@ -547,9 +546,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                           w.start + w.tok0 + i * TPT);
           }
           const int tail = tail_rows_of(w, nk), end = (tail + 15) / 16 * 16;
-          const int care_from = CARE ? masked_from(w) : nk;
+          const int care_from = with_care ? masked_from(w) : nk;
           int* bad = first_bad + (cares & 1) * 2 * D;
-          if constexpr (CARE) {
+          if (with_care) {
             for (int e = lane; e < 2 * D; e += 32) bad[e] = kUnseen;
             __syncwarp();
           }
@@ -587,14 +586,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 *reinterpret_cast<uint4*>(ring + slot * TB + (c >> 3) * (TB / SUB) + r * 128 + (c & 7) * 16) =
                     make_uint4(0, 0, 0, 0);
               }
-              if constexpr (CARE) take_out<T, D>(ring + slot * TB, 0, n < 2 * nk - 1 ? kTileKeys : tail, key0, bad);
+              if (with_care) take_out<T, D>(ring + slot * TB, 0, n < 2 * nk - 1 ? kTileKeys : tail, key0, bad);
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
               __syncwarp();
               if (lane == 0 && limit != 1) mbar_arrive(&kv_full[slot]);
             }
             if (limit != 1) issued = g + 1;  // (a tile that goes to v_tail counts once it has been mended)
           }
-          if constexpr (CARE) {
+          if (with_care) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&taken_out[cares & 1]);
             ++cares;
@@ -609,10 +608,23 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (tails > 0) tile_wait(v_tail, (tails - 1) & 1, more = kTileWaitLimit);
         }
       };
-      pass(std::false_type{});
-      if (go_again()) {
-        pass(std::true_type{});
-        end_care();
+      // Its code twice at 64 dims (16 prompts of 15001 tokens 180 us, 184 with one), once at 128 dims (a chunk of 512 beside
+      // 31 requests 83.6 us, 87 with two: more code to fetch between the other kernels' launches).
+      if constexpr (D == 64) {
+        pass(false);
+        if (go_again()) {
+          pass(true);
+          end_care();
+        }
+      } else {
+        for (bool care = false;; care = true) {
+          pass(care);
+          if (care) {
+            end_care();
+            break;
+          }
+          if (!go_again()) break;
+        }
       }
     } else if (warp == kMmaWarp) {
       // ---- products, tile 0 then tile 1 (a warp per tile was slower: their products then share the tensor cores and
@@ -624,7 +636,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // load land.)
       unsigned base = 0, qn = 0, done0 = 0, done1 = 0;  // of earlier items: ring tiles, query loads, steps
       int k = 0;
-      auto pass = [&](auto) {
+      for (int passes = 1;; ++passes) {
         for (;;) {
           const TileWork w = next_work(k++);
           if (w.b < 0) {
@@ -738,11 +750,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           done0 += w.steps[0];
           done1 += w.steps[1];
         }
-      };
-      pass(std::false_type{});
-      if (go_again()) {
-        pass(std::true_type{});
-        end_care();
+        if (passes == 2) {
+          end_care();
+          break;
+        }
+        if (!go_again()) break;
       }
     } else if (warp == kTmaWarp + 2) {
       // ---- items: the CTA's own, then those of CTAs that have not started.  Heavy items come first in a launch and the
