@@ -68,7 +68,8 @@ typedef enum li4_kernel {
 
 /* Library version, (major << 16) | (minor << 8) | patch.  0.2: li4_fusion has the argmax_*
  * fields (callers built against 0.1 pass a shorter struct); the li4_program_* and
- * li4_gather_rows entry points.  0.3: the paged KV cache. */
+ * li4_gather_rows entry points.  0.3: the paged KV cache.  0.4:
+ * li4_paged_append_within, li4_debug_set_attention_wait_limit. */
 int li4_version(void);
 
 /* Message describing the last failed call on this host thread ("" if none). */
@@ -414,7 +415,8 @@ int li4_rope_paged_write(const void* q, const void* k, const void* v, int dtype,
  * cu_seqlens[b + 1] - 1 of q [n_tokens, n_heads, head_dim]; query i of n sees keys 0 .. L - n + i of its
  * sequence's L.  A query that sees no key gives zeros; rows past cu_seqlens[n_seqs] are left as they
  * were.  Scores, softmax statistics and sums in fp32; probabilities rounded to the type for the second
- * product; one rounding at the end.  A value row's NaN or infinity reaches only queries that see it. */
+ * product; one rounding at the end.  A value row's NaN or infinity reaches only queries that see it (a call that
+ * meets one takes up to three times as long); a NaN or infinite score makes its query's outputs NaN. */
 typedef struct li4_attention {
   const void* q;
   const void* k;                /* prompt: [n_tokens, n_kv_heads, head_dim]; paged: the cache's pages */

@@ -701,8 +701,13 @@ int launch_seq_attention(const SeqAttnArgs& args, bool paged, int dtype, int max
 }
 
 // Rows (queries x heads of a KV head) up to which a sequence is streamed: where no sequence has more the streaming
-// kernel runs alone, with tiles of 8, 16 or 32 rows; beside longer ones it takes those of one 8-row tile (31 requests of
-// 8-row tiles beside a chunk 8 us less than with 16-row tiles).
+// kernel runs alone, with tiles of 8, 16 or 32 rows; beside longer ones it takes those of one 8-row tile.  Beside a chunk
+// of 512 tokens, 31 requests of 200-6000 tokens each, with the limit at 8 / 16 / 32 rows and tiles as high (us):
+//   64 dims, 8 KV heads: 4 rows a request 63 / 64 / 71, 8 rows 64 / 65 / 72, 16 rows 96 / 67 / 77
+//   128 dims, 8 KV heads: 4 rows 83 / 88 / 99, 8 rows 84 / 90 / 102, 16 rows 120 / 94 / 108
+//   128 dims, 4 KV heads: 8 rows 68 / 71 / 78, 16 rows 94 / 77 / 82, 32 rows 94 / 95 / 93
+//   128 dims, 1 KV head: 16 rows 50 / 47 / 59, 32 rows 50 / 50 / 61; 7 requests beside it: 16 rows 28 / 34 / 41
+// So 8 is right for single tokens at groups of up to 8, and up to 1.4 times too slow for 16 rows of many requests.
 constexpr int kFewRows = 32, kFewRowsBeside = 8;
 
 constexpr int64_t kAttentionMost = 1 << 30;  // rows of a sequence, keys: what is claimed above it counts as it

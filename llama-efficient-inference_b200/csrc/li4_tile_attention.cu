@@ -14,8 +14,10 @@
 //                   writes P in the 16-bit type
 //   warp 10         the CTA's next item, when the present one nears its end
 //
-// Prompts of 8192 tokens (32 / 8 heads, fp16): 457 us at 128 dims, 1.2 PFLOP/s, where the power limit holds the clock
-// near 1.6 GHz; 360 us at 64 dims, bound by the softmax's issue and latency.
+// Prompts of 8192 tokens (32 / 8 heads, fp16), 128 dims: 463 us in a burst (1.19 PFLOP/s, 0.72 of cuBLAS's burst rate);
+// call after call for seconds 530 us (1.04 PFLOP/s, 0.75 of its sustained rate), as the power limit brings the clock to
+// 1.5 GHz: 0.82 million cycles either way.  64 dims: 370 us, bound by the softmax's issue and latency.  A NaN in the
+// first value, which runs every CTA's first two items twice: 775 and 574 us.
 //
 // The running maximum moves lazily: probabilities are taken against a maximum that may lag up to 2^8
 // behind (P <= 256 fits both 16-bit types, the sum is fp32), so the accumulated output is rescaled only
