@@ -26,9 +26,10 @@
 // A masked key's probability is zero, but zero times a NaN or an infinity is NaN: a value that a row must not see can
 // reach it through the last few key tiles of an item, where some keys are hidden from some rows.  A CTA that meets an
 // output that is not finite therefore runs that item again, and its later ones from the start, with care (a role's
-// code exists twice where that spares the usual pass time): the copying warp takes the values that are not finite out of those tiles before the products may have them and notes where in each
-// dim the first +inf, -inf or NaN stood, and a row that sees that key gets it added at the end (added to a
-// sum, what is not finite does not depend on its weight).  At most two items of a CTA run twice, whatever the context.
+// code exists twice where that spares the usual pass time): the copying warp takes the values that are not finite out
+// of those tiles before the products may have them and notes where in each dim the first +inf, -inf or NaN stood, and a
+// row that sees that key gets it added at the end (what is not finite does not depend on its weight in a sum).  At most
+// two items of a CTA run twice, whatever the context.
 // Every mbarrier wait is bounded: one that runs out sets bit 8 of li4_device_errors.  The copying warp then issues
 // nothing more (a barrier whose bytes are still to come must not be armed twice), the other roles run to the end of
 // their item without waiting, copies and MMAs in flight are waited for (bounded) and the tensor memory is freed.
