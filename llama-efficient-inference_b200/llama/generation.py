@@ -81,6 +81,7 @@ class PagedDecodeGraph:
     was made (li4_paged_append; idle rows stay idle), runs the blocks over the cache and leaves each request's next token
     in tok.  The lengths, tables and free pages live on the GPU, so the one graph serves every length.  Made after the
     prompts are in the cache: the warm-up steps run on the requests as they are and the cache's bookkeeping is put back.
+    The set of requests is the graph's: after a release or a new prompt another graph is made.
 
     granted bool [requests] is a static buffer too: False from the first replay on that refused the request its token
     (no page left, or max_len reached); such a replay leaves the request's token and length as they were."""

@@ -82,6 +82,30 @@ def test_a_bad_value_in_a_cache(paged, page, n, L, d, bad):  # noqa: F811
         split_check(got, q, k, v, row, 5)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,d", [(8, 2, 64), (3, 3, 128), (16, 1, 128), (12, 4, 72)])
+def test_bad_values_in_some_of_many_prompts(paged, H, Hkv, d, dtype):  # noqa: F811
+    """Several items per CTA, with and without bad values in turn, some with many of both signs; one KV head's bad values
+    are no other's."""
+    lens = [(37 * b) % 290 for b in range(70)]
+    T = sum(lens)
+    q, k, v0 = rand((T, H, d), dtype, 20), rand((T, Hkv, d), dtype, 21), rand((T, Hkv, d), dtype, 22)
+    v, clean, at, rep = v0.clone(), v0.clone(), cumulative(lens), H // Hkv
+    skip = torch.zeros(T, H, d, dtype=torch.bool, device="cuda")
+    for b, n in enumerate(lens):
+        for i in range((0, 0, 1, 0, 7)[b % 5] if n else 0):
+            j, h, dim = (n - 1 - 11 * i - b) % n, (b + i) % Hkv, (5 * b + 3 * i) % d
+            v[at[b] + j, h, dim] = (NAN, INF, -INF)[(b + i) % 3]
+            clean[at[b] + j, h, dim] = 0
+            skip[at[b] + j:at[b + 1], h * rep:(h + 1) * rep, dim] = True
+    got = paged.prompt_attention(q, k, v, i32(at), max(lens))
+    assert not bool((torch.isfinite(got) & skip).any())
+    for b, n in enumerate(lens):
+        if n:
+            part = slice(at[b], at[b + 1])
+            close(got[part], q[part], k[part], clean[part], skip[part])
+
+
 @pytest.mark.parametrize("d", [64, 128])
 def test_a_whole_hidden_stretch_of_bad_values(paged, d):  # noqa: F811
     """Every later value is NaN: rows that see none of them are right."""
