@@ -69,7 +69,8 @@ typedef enum li4_kernel {
 /* Library version, (major << 16) | (minor << 8) | patch.  0.2: li4_fusion has the argmax_*
  * fields (callers built against 0.1 pass a shorter struct); the li4_program_* and
  * li4_gather_rows entry points.  0.3: the paged KV cache.  0.4:
- * li4_paged_append_within, li4_debug_set_attention_wait_limit. */
+ * li4_paged_append_within, li4_debug_set_attention_wait_limit.  0.5: the paged cache in 4 bits, li4_paged_fork,
+ * li4_token_logprobs. */
 int li4_version(void);
 
 /* Message describing the last failed call on this host thread ("" if none). */
@@ -453,6 +454,89 @@ int li4_prompt_attention(const li4_attention* args, void* workspace, size_t work
  * Replaces: the same, over cache_k / cache_v (llama/model.py:251-275). */
 int li4_paged_attention(const li4_attention* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * A paged cache in 4 bits.  A row of head_dim values (a multiple of 32 up to 128) is cut into groups of 32.  A group
+ * has a scale s and an offset m of the row's 16-bit type and 32 codes c in 0 .. 15; it stands for the values
+ * c s + m, rounded once to the type.  (5 bits a value.)
+ *   codes   [pages, page_size, n_kv_heads, head_dim / 2] bytes: dims 8 w .. 8 w + 7 are the 32-bit word w of a row, dim
+ *           8 w + 2 i in bits 4 i .. 4 i + 3, dim 8 w + 2 i + 1 in bits 16 + 4 i .. 16 + 4 i + 3
+ *   params  [pages, page_size, n_kv_heads, head_dim / 32] pairs (s, m) of 16-bit values: s in the low half
+ * Rows of codes start on 16-byte boundaries (strides in bytes), rows of params on 4-byte ones (strides in pairs).
+ * --------------------------------------------------------------------------- */
+#define LI4_KV_GROUP 32
+
+typedef struct li4_int4_pages {
+  void* codes;
+  void* params;
+  int64_t stride_cp, stride_ct, stride_ch; /* bytes: page, row, KV head */
+  int64_t stride_pp, stride_pt, stride_ph; /* pairs: page, row, KV head */
+} li4_int4_pages;
+
+/* li4_rope_paged_write into such a cache.  Queries are turned as there.  Keys are turned in 64 bits and rounded to the
+ * type by way of 32 bits; then a group of 32 values x of a key or value gets
+ *   m = the smallest x, s = (the largest x - m) / 15 rounded towards zero to the type (so that c s + m never passes the
+ *   largest), c = min(15, (x - m) / s rounded to the nearest, ties to even), 0 where s is 0,
+ * the quotients as if in 64 bits: the codes are a function of the inputs alone.  A group with a value that is not finite
+ * gets s = m = NaN and reads as NaN.  k_out and v_out (each may be null, and may be k, v): the turned keys and the values
+ * as the cache holds them, c s + m, packed like k and v.
+ * strides: 12 element strides -- q, k, v, q_out, k_out, v_out: token, head -- multiples of 8.  head_dim: a multiple of 32
+ * up to 128.  Bit 7 of li4_device_errors as there. */
+int li4_rope_paged_write_int4(const void* q, const void* k, const void* v, int dtype, int64_t n_tokens, int64_t n_heads,
+                              int64_t n_kv_heads, int64_t head_dim, const int64_t* strides, const float* rope_cos,
+                              const float* rope_sin, int64_t rope_stride, int64_t max_pos, const int32_t* positions,
+                              const int64_t* slots, void* q_out, void* k_out, void* v_out,
+                              const li4_int4_pages* cache_k, const li4_int4_pages* cache_v, int64_t num_pages,
+                              int64_t page_size, void* stream);
+
+/* li4_paged_attention over such a cache: the same function of the values that the cache stands for.  args: as there,
+ * its k, v and their strides unused; head_dim a multiple of 32.  A group of not finite parameters reads as NaN, and as in
+ * li4_paged_attention reaches only queries that see it. */
+size_t li4_attention_int4_workspace_bytes(const li4_attention* args);
+int li4_paged_attention_int4(const li4_attention* args, const li4_int4_pages* cache_k, const li4_int4_pages* cache_v,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Requests that go on from others, and requests that end.  Request r holds kv_lens[r] tokens in the pages that row r of
+ * block_tables names.  parents[r] = r: it stays; = p, another request: from now on it holds p's tokens instead of its own;
+ * = -1: it ends and holds none.  Every request is read as it was before the call, so requests may change places.
+ * A request that takes p's tokens shares p's full pages; where p's last page is not full it gets a page of its own for that
+ * part, with a copy of p's, so no page that a request appends to is shared.  Those pages come from the top of the free stack in
+ * request order; where the stack runs out (or parents[r] is no request, or p's length does not fit the table) the request
+ * is refused whole: it stays as it was, granted 0.  Then pages that no request holds any more go on the stack, in the order of
+ * the requests and blocks that held them first.  Pages are recognised as shared by the tables alone: nothing else is kept.
+ * Writes
+ *   block_tables  the rows of requests that took tokens, as far as their pages go
+ *   free_pages    the entries of pages that came back
+ *   kv_lens_out, n_free_out   (may be kv_lens, n_free)
+ *   granted       [n_requests]
+ *   pools         in each of n_pools memory blocks of pages (pools[i] + page * pool_strides[i] bytes: pool_bytes[i] bytes, all
+ *                 multiples of 16), the pages of the parts that were copied
+ * pools, pool_strides and pool_bytes are host arrays.  Pages are 0 .. free_capacity - 1; other entries of the tables count as no page.
+ * At most 8192 requests, and n_requests * table_width below 2^31.  Two or more launches: the tables, then the copies, up to
+ * LI4_FORK_POOLS pools each.  No counterpart in the reference, which decodes each prompt once. */
+#define LI4_FORK_POOLS 128
+size_t li4_paged_fork_workspace_bytes(int64_t n_requests, int64_t table_width, int64_t free_capacity);
+int li4_paged_fork(const int32_t* kv_lens, const int32_t* parents, int64_t n_requests, int32_t* block_tables,
+                   int64_t table_stride, int64_t table_width, int32_t* free_pages, int64_t free_capacity,
+                   const int32_t* n_free, int64_t page_size, int32_t* kv_lens_out, int32_t* n_free_out,
+                   uint8_t* granted, void* const* pools, const int64_t* pool_strides, const int64_t* pool_bytes,
+                   int64_t n_pools, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Log probabilities.  For each row x of logits [rows, cols] (LI4_F16, LI4_BF16 or LI4_F32, row stride `stride` elements):
+ *   logprobs[r] = x[tokens[r]] - L with L = log sum_j exp(x_j); NaN where tokens[r] is outside [0, cols)
+ *   entropy[r]  = - sum_j p_j log p_j with p_j = exp(x_j - L) (a token of probability 0 adds 0)
+ *   top_ids[r, i], top_logprobs[r, i], i < top: the likeliest tokens in order, the lower index first among equals, and
+ *                 their x - L.  NaN counts as the largest value.
+ * Statistics in fp32.  A row with a NaN or a +infinity, or of nothing but -infinity, has NaN for its log probabilities and
+ * entropy.  tokens and logprobs may be null together, entropy may be null; top from 0 to LI4_MAX_TOP, at most cols.
+ * One launch, no workspace.
+ * Replaces: the log_softmax, gather and topk over logits (of llama/model.py:455-456) that a user of the reference writes. */
+#define LI4_MAX_TOP 32
+int li4_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t cols, int64_t stride, const int64_t* tokens,
+                       int64_t top, float* logprobs, float* entropy, int64_t* top_ids, float* top_logprobs,
+                       void* stream);
+
 /* Device-side error flags of the current device (bit 0: a bounded pipeline wait
  * inside a GEMV kernel ran out; bit 1: a bounded wait for a peer's flag in
  * li4_allreduce_add ran out; bit 2: a decode program's wait for another op
@@ -460,7 +544,7 @@ int li4_paged_attention(const li4_attention* args, void* workspace, size_t works
  * outside its table; bit 4: a bounded wait inside li4_int4_gemm ran out; bit 5: an
  * LI4_EPI_ALLREDUCE_RESIDUAL epilogue's wait for a peer's words ran out; bit 6: a wait of
  * li4_argmax_rows_allreduce for a peer's key ran out -- the kernel
- * carried on and its outputs are not valid; bit 7: li4_rope_paged_write met a position
+ * carried on and its outputs are not valid; bit 7: li4_rope_paged_write (or its _int4 form) met a position
  * or slot out of range; bit 8: a bounded wait inside li4_prompt_attention or li4_paged_attention ran
  * out).  Synchronising: copies the flags to the host; reset != 0 clears them.
  * A diagnostic for tests and health checks, not for the decode loop. */

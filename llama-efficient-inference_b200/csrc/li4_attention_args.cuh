@@ -31,6 +31,12 @@ struct SeqAttnArgs {
   float* part;                     // partial results of split items (see li4_seq_attention.cu)
 };
 
+// The same over a cache in 4 bits: k, v and their strides are not used.
+struct Seq4Args : SeqAttnArgs {
+  li4_int4_pages k4, v4;
+  int wide_params;  // a row's params are one aligned run of as many pairs as the kernel's row has groups
+};
+
 // One sequence as this launch sees it (n = 0: not this launch's).
 struct Seq {
   int start, n, len;
@@ -87,6 +93,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 // ---- launches shared by the entry points ----
 int launch_seq_attention(const SeqAttnArgs& a, bool paged, int dtype, int max_rows, cudaStream_t stream);
+int launch_seq_attention_int4(const Seq4Args& a, int dtype, int max_rows, cudaStream_t stream);
 int launch_tile_attention(const SeqAttnArgs& a, bool paged, int dtype, cudaStream_t stream);
 size_t tile_attention_part_bytes(int hd, int rep, int64_t tokens, int64_t kv_heads, int64_t max_keys, int sm);
 size_t seq_attention_part_bytes(int hd, int max_rows, int sm);

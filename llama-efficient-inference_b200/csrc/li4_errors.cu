@@ -46,7 +46,7 @@ int current_sm_count() {
 // 0.4.0: li4_paged_append_within, li4_debug_set_attention_wait_limit.
 // 0.3.0: the paged KV cache (li4_paged_append, li4_rope_paged_write, li4_prompt_attention, li4_paged_attention).
 // 0.2.0: li4_fusion gained the argmax_* fields (a larger struct); the decode program, li4_gather_rows.
-extern "C" int li4_version(void) { return (0 << 16) | (4 << 8) | 0; }
+extern "C" int li4_version(void) { return (0 << 16) | (5 << 8) | 0; }
 
 extern "C" const char* li4_last_error(void) { return li4::g_last_error; }
 

@@ -45,6 +45,11 @@ int comm_set_wait_limit(unsigned polls);
 int program_set_wait_limits(unsigned polls, unsigned extra);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Codes on 16-byte boundaries, params on 4-byte ones.
+inline bool int4_pages_aligned(const li4_int4_pages& p) {
+  return aligned16(p.codes) && (reinterpret_cast<uintptr_t>(p.params) & 3u) == 0 &&
+         ((p.stride_cp | p.stride_ct | p.stride_ch) & 15) == 0;
+}
 inline bool is_pow2(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
 inline int ilog2(int64_t v) { int r = 0; while ((int64_t(1) << r) < v) ++r; return r; }
 

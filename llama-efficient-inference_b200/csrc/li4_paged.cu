@@ -2,9 +2,11 @@
 //
 // li4_paged_append: the requests' lengths -> pages for the new tokens, block tables, positions, slots.
 // li4_rope_paged_write: RoPE on the packed queries and keys, keys and values into their slots.
+// li4_rope_paged_write_int4: the same into a cache in 4 bits.
 #include <cooperative_groups.h>
 
 #include "li4_common.cuh"
+#include "li4_int4_pages.cuh"
 #include "li4_internal.h"
 
 namespace li4 {
@@ -314,6 +316,139 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_write_kernel(const __
               [&](int h, uint4 x) { *reinterpret_cast<uint4*>(cv + (long long)h * a.scvh) = x; });
 }
 
+// ---------------------------------------------------------------------------
+// RoPE and the write into a cache in 4 bits.  A thread owns 8 dims of one token as above, so four neighbouring threads
+// hold a group of 32: its smallest and largest value cross them by two shuffles each, and every thread packs its eight codes
+// into one word.  Whatever decides a code is exact or in 64 bits: a key is turned in 64 bits, the scale
+// is a 64-bit quotient cut to the type, and a code whose 32-bit quotient lies near a border is found again in 64 bits.
+// ---------------------------------------------------------------------------
+struct Rope4Args {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* q_out;
+  uint16_t* k_out;  // may be null
+  uint16_t* v_out;  // may be null
+  long long sqt, sqh, skt, skh, svt, svh, sqot, sqoh, skot, skoh, svot, svoh;
+  const float* cos;
+  const float* sin;
+  long long srope;
+  const int* positions;
+  const long long* slots;
+  li4_int4_pages ck, cv;
+  long long num_slots;
+  int T, H, Hkv, chunks, log_page, max_pos, heads_per_group;
+};
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// The code of x: its 32-bit quotient t is off by less than 30 x 3 x 2^-24 < 1e-5 (the difference, the reciprocal and the product
+// each round once, and t <= 30 where s is a subnormal), so a nearest integer of distance below 0.4999 is the right one.  The
+// test fails too where the difference or the reciprocal overflows.
+__device__ __forceinline__ int code_of(float x, float m, float s, float inv) {
+  const float t = (x - m) * inv;
+  float c = rintf(t);
+  if (!(fabsf(t - c) < 0.4999f)) c = (float)rint(((double)x - (double)m) / (double)s);
+  return (int)fminf(c, 15.f);
+}
+
+// Eight values of this thread's group -> their word of codes, the group's (s, m) (the same in its four threads).
+template <typename T>
+__device__ __forceinline__ uint32_t quantize8(uint4 x, uint32_t* params) {
+  const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = Codes4<T>::value((uint16_t)(u[i >> 1] >> (i & 1) * 16));
+  float lo = f[0], hi = f[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    lo = min_nan(lo, f[i]);
+    hi = max_nan(hi, f[i]);
+  }
+#pragma unroll
+  for (int d = 1; d < 4; d *= 2) {
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+  }
+  lo += 0.f;  // (-0 becomes 0)
+  const bool finite = lo > -INFINITY && hi < INFINITY;
+  const uint16_t s16 = Codes4<T>::down(((double)hi - (double)lo) / 15.0);
+  const float s = Codes4<T>::value(s16), inv = 1.f / s;
+  uint32_t w = 0;
+  if (finite && s > 0.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= (uint32_t)code_of(f[i], lo, s, inv) << (4 * (i >> 1) + 16 * (i & 1));
+  }
+  *params = finite ? (uint32_t)s16 | (uint32_t)Codes4<T>::nearest(lo) << 16 : Codes4<T>::NaN2;
+  return w;
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 turn8_exact(uint4 x, const float4& c, const float4& s) {
+  const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+  const float cf[4] = {c.x, c.y, c.z, c.w}, sf[4] = {s.x, s.y, s.z, s.w};
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const double a = Codes4<T>::value((uint16_t)u[i]), b = Codes4<T>::value((uint16_t)(u[i] >> 16));
+    // (products of 11 and 24 bits are exact)
+    r[i] = Codes4<T>::nearest(a * cf[i] - b * sf[i]) | (uint32_t)Codes4<T>::nearest(a * sf[i] + b * cf[i]) << 16;
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <typename T, typename T2>
+__global__ void __launch_bounds__(kRopeThreads) rope_paged_write_int4_kernel(const __grid_constant__ Rope4Args a) {
+  pdl_launch_dependents();
+  pdl_wait_primary();
+  const long long i = (long long)blockIdx.x * kRopeThreads + threadIdx.x;
+  const bool mine = i / a.chunks < a.T;  // (the others go along: a group's threads talk to one another)
+  const long long t = mine ? i / a.chunks : a.T - 1;
+  const int chunk = (int)(i % a.chunks), d = chunk * 8;
+  int pos = a.positions[t];
+  const long long slot = a.slots[t];
+  if (slot >= a.num_slots || (slot >= 0 && (pos < 0 || pos >= a.max_pos))) atomicOr(&g_paged_device_error, 128u);
+  pos = max(0, min(pos, a.max_pos - 1));
+  const bool keep = mine && slot >= 0 && slot < a.num_slots;
+  const long long page = keep ? slot >> a.log_page : 0, row = keep ? slot & ((1 << a.log_page) - 1) : 0;
+  const float4 c = *reinterpret_cast<const float4*>(a.cos + (long long)pos * a.srope + d / 2);
+  const float4 s = *reinterpret_cast<const float4*>(a.sin + (long long)pos * a.srope + d / 2);
+  const int h0 = blockIdx.y * a.heads_per_group, h1 = min(a.H + 2 * a.Hkv, h0 + a.heads_per_group);
+  for_heads(h0, min(h1, a.H), a.q + t * a.sqt + d, a.sqh, [&](int h, uint4 x) {
+    if (mine) *reinterpret_cast<uint4*>(a.q_out + t * a.sqot + (long long)h * a.sqoh + d) = turn8<T2>(x, c, s);
+  });
+  auto put = [&](const li4_int4_pages& p, int h, uint4 x, uint16_t* held) {
+    uint32_t params;
+    const uint32_t w = quantize8<T>(x, &params);
+    if (keep) {
+      uint8_t* codes = static_cast<uint8_t*>(p.codes) + page * p.stride_cp + row * p.stride_ct + (long long)h * p.stride_ch;
+      *reinterpret_cast<uint32_t*>(codes + chunk * 4) = w;
+      if ((chunk & 3) == 0)
+        static_cast<uint32_t*>(p.params)[page * p.stride_pp + row * p.stride_pt + (long long)h * p.stride_ph + chunk / 4] = params;
+    }
+    if (held && mine) {
+      uint32_t u[4];
+      values8<T>(w, both_low(params), both_high(params), u);
+      *reinterpret_cast<uint4*>(held) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+  };
+  for_heads(max(h0 - a.H, 0), min(h1 - a.H, a.Hkv), a.k + t * a.skt + d, a.skh, [&](int h, uint4 x) {
+    put(a.ck, h, turn8_exact<T>(x, c, s), a.k_out ? a.k_out + t * a.skot + (long long)h * a.skoh + d : nullptr);
+  });
+  for_heads(max(h0 - a.H - a.Hkv, 0), h1 - a.H - a.Hkv, a.v + t * a.svt + d, a.svh, [&](int h, uint4 x) {
+    put(a.cv, h, x, a.v_out ? a.v_out + t * a.svot + (long long)h * a.svoh + d : nullptr);
+  });
+}
+
 template <typename KernelT, typename ArgsT>
 static int launch_pdl(KernelT kernel, const ArgsT& a, dim3 grid, int threads, size_t smem, int cluster,
                       cudaStream_t stream, const char* what) {
@@ -332,6 +467,16 @@ static int launch_pdl(KernelT kernel, const ArgsT& a, dim3 grid, int threads, si
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, a), what);
+}
+
+// Heads per thread: all of them when the tokens alone fill the GPU, else as few as keeps it busy.
+static void rope_grid(int T, int chunks, int heads, long long* blocks, long long* groups, int* heads_per_group) {
+  *blocks = ((long long)T * chunks + kRopeThreads - 1) / kRopeThreads;
+  const long long want = 4LL * current_sm_count();
+  *groups = *blocks >= want ? 1 : (want + *blocks - 1) / *blocks;
+  if (*groups > heads) *groups = heads;
+  *heads_per_group = (int)((heads + *groups - 1) / *groups);
+  *groups = (heads + *heads_per_group - 1) / *heads_per_group;
 }
 
 template <int THREADS, int TOK>
@@ -479,14 +624,8 @@ extern "C" int li4_rope_paged_write(const void* q, const void* k, const void* v,
   a.Hkv = (int)n_kv_heads;
   a.chunks = (int)(head_dim / 8);
   a.max_pos = (int)max_pos;
-  // heads per thread: all of them when the tokens alone fill the GPU, else as few as keeps it busy
-  const int heads = a.H + 2 * a.Hkv;
-  const long long blocks = ((long long)a.T * a.chunks + kRopeThreads - 1) / kRopeThreads;
-  const long long want = 4LL * current_sm_count();
-  long long groups = blocks >= want ? 1 : (want + blocks - 1) / blocks;
-  if (groups > heads) groups = heads;
-  a.heads_per_group = (int)((heads + groups - 1) / groups);
-  groups = (heads + a.heads_per_group - 1) / a.heads_per_group;
+  long long blocks, groups;
+  rope_grid(a.T, a.chunks, a.H + 2 * a.Hkv, &blocks, &groups, &a.heads_per_group);
   const dim3 grid((unsigned)blocks, (unsigned)groups, 1);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int rc = dtype == LI4_F16
@@ -494,6 +633,85 @@ extern "C" int li4_rope_paged_write(const void* q, const void* k, const void* v,
                                   "rope_paged_write: kernel launch")
                      : launch_pdl(rope_paged_write_kernel<__nv_bfloat162>, a, grid, kRopeThreads, 0, 1, s,
                                   "rope_paged_write: kernel launch");
+  if (rc == LI4_OK) clear_error();
+  return rc;
+}
+
+extern "C" int li4_rope_paged_write_int4(const void* q, const void* k, const void* v, int dtype, int64_t n_tokens,
+                                         int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, const int64_t* strides,
+                                         const float* rope_cos, const float* rope_sin, int64_t rope_stride,
+                                         int64_t max_pos, const int32_t* positions, const int64_t* slots, void* q_out,
+                                         void* k_out, void* v_out, const li4_int4_pages* cache_k,
+                                         const li4_int4_pages* cache_v, int64_t num_pages, int64_t page_size,
+                                         void* stream) {
+  using namespace li4;
+  const char* what = "rope_paged_write_int4";
+  if (dtype != LI4_F16 && dtype != LI4_BF16)
+    return set_error(LI4_ERR_UNSUPPORTED, "%s: dtype %d (LI4_F16 or LI4_BF16)", what, dtype);
+  if (n_tokens < 0 || n_heads < 0 || n_kv_heads < 0 || num_pages < 0 || max_pos < 0 || n_tokens > (1 << 30) ||
+      n_heads > 65535 || n_kv_heads > 65535 || n_heads + 2 * n_kv_heads > 65535 || max_pos > (1 << 30) ||
+      num_pages > (1LL << 31) - 1)
+    return set_error(LI4_ERR_INVALID_ARG, "%s: n_tokens=%lld n_heads=%lld n_kv_heads=%lld num_pages=%lld max_pos=%lld",
+                     what, (long long)n_tokens, (long long)n_heads, (long long)n_kv_heads, (long long)num_pages,
+                     (long long)max_pos);
+  if (head_dim < kGroup4 || head_dim > 128 || head_dim % kGroup4 != 0)
+    return set_error(LI4_ERR_UNSUPPORTED, "%s: head_dim=%lld (a multiple of %d up to 128)", what, (long long)head_dim,
+                     kGroup4);
+  if (!is_pow2(page_size) || page_size < 8 || page_size > 1024)
+    return set_error(LI4_ERR_UNSUPPORTED, "%s: page_size=%lld (a power of two from 8 to 1024)", what,
+                     (long long)page_size);
+  if (n_tokens == 0 || n_heads + n_kv_heads == 0) {
+    clear_error();
+    return LI4_OK;
+  }
+  if (max_pos < 1)
+    return set_error(LI4_ERR_INVALID_ARG, "%s: max_pos=%lld (tokens need a table row)", what, (long long)max_pos);
+  if (!strides || !rope_cos || !rope_sin || !positions || !slots || !cache_k || !cache_v ||
+      (n_heads > 0 && (!q || !q_out)) || (n_kv_heads > 0 && (!k || !v)) ||
+      (n_kv_heads > 0 && num_pages > 0 && (!cache_k->codes || !cache_k->params || !cache_v->codes || !cache_v->params)))
+    return set_error(LI4_ERR_INVALID_ARG, "%s: null pointer", what);
+  bool aligned = aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out) && aligned16(k_out) &&
+                 aligned16(v_out) && aligned16(rope_cos) && aligned16(rope_sin) && rope_stride % 4 == 0 &&
+                 int4_pages_aligned(*cache_k) && int4_pages_aligned(*cache_v);
+  for (int i = 0; i < 12; ++i) aligned = aligned && strides[i] % 8 == 0;
+  if (!aligned)
+    return set_error(LI4_ERR_ALIGNMENT, "%s: rows and codes must start on 16-byte boundaries, params on 4-byte ones", what);
+  if (rope_stride < head_dim / 2)
+    return set_error(LI4_ERR_INVALID_ARG, "%s: table rows of %lld for head_dim %lld", what, (long long)rope_stride,
+                     (long long)head_dim);
+  Rope4Args a;
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.q_out = static_cast<uint16_t*>(q_out);
+  a.k_out = static_cast<uint16_t*>(k_out);
+  a.v_out = static_cast<uint16_t*>(v_out);
+  a.sqt = strides[0], a.sqh = strides[1], a.skt = strides[2], a.skh = strides[3], a.svt = strides[4],
+  a.svh = strides[5], a.sqot = strides[6], a.sqoh = strides[7], a.skot = strides[8], a.skoh = strides[9],
+  a.svot = strides[10], a.svoh = strides[11];
+  a.cos = rope_cos;
+  a.sin = rope_sin;
+  a.srope = rope_stride;
+  a.positions = positions;
+  a.slots = reinterpret_cast<const long long*>(slots);
+  a.ck = *cache_k;
+  a.cv = *cache_v;
+  a.log_page = ilog2(page_size);
+  a.num_slots = num_pages << a.log_page;
+  a.T = (int)n_tokens;
+  a.H = (int)n_heads;
+  a.Hkv = (int)n_kv_heads;
+  a.chunks = (int)(head_dim / 8);
+  a.max_pos = (int)max_pos;
+  long long blocks, groups;
+  rope_grid(a.T, a.chunks, a.H + 2 * a.Hkv, &blocks, &groups, &a.heads_per_group);
+  const dim3 grid((unsigned)blocks, (unsigned)groups, 1);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int rc = dtype == LI4_F16
+                     ? launch_pdl(rope_paged_write_int4_kernel<__half, __half2>, a, grid, kRopeThreads, 0, 1, s,
+                                  "rope_paged_write_int4: kernel launch")
+                     : launch_pdl(rope_paged_write_int4_kernel<__nv_bfloat16, __nv_bfloat162>, a, grid, kRopeThreads, 0,
+                                  1, s, "rope_paged_write_int4: kernel launch");
   if (rc == LI4_OK) clear_error();
   return rc;
 }

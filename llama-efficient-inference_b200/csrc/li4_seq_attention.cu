@@ -27,6 +27,7 @@
 
 #include "li4_attention_args.cuh"
 #include "li4_gemv_device.cuh"
+#include "li4_int4_pages.cuh"
 
 namespace li4 {
 
@@ -39,9 +40,27 @@ constexpr int kSeqStages = 3;   // stages per warp
 // starts an item the other's copies go on: one CTA of 32-key stages at 128 dims, 32 requests of 1000-8000 tokens 81 us
 // instead of 75).
 __host__ __device__ constexpr int seq_keys(int D) { return 32 * 64 / D; }
-__host__ __device__ constexpr int seq_unit(int D) { return kSeqWarps * seq_keys(D); }  // keys per unit
+__host__ __device__ constexpr int seq_unit(int D, bool q4) { return kSeqWarps * (q4 ? 32 : seq_keys(D)); }  // keys per unit
 __host__ __device__ constexpr int seq_stage_bytes(int D) { return 2 * seq_keys(D) * D * 2; }
-__host__ __device__ constexpr int seq_smem_bytes(int D) { return kSeqWarps * kSeqStages * seq_stage_bytes(D); }
+
+// A cache in 4 bits (Q4): stages of 32 keys hold codes and params as they are, unpacked on the way to the products.
+template <typename ArgsT>
+constexpr bool kIsInt4 = __is_same(ArgsT, Seq4Args);
+constexpr int kSeq4Keys = 32;
+__host__ __device__ constexpr int seq4_stages(int D) { return D == 64 ? 6 : 4; }
+__host__ __device__ constexpr int seq4_stage_bytes(int D) { return 2 * kSeq4Keys * (D / 2 + D / kGroup4 * 4); }
+
+__host__ __device__ constexpr int seq_stage_keys(int D, bool q4) { return q4 ? kSeq4Keys : seq_keys(D); }
+__host__ __device__ constexpr int seq_stage_count(int D, bool q4) { return q4 ? seq4_stages(D) : kSeqStages; }
+__host__ __device__ constexpr int seq_stage_size(int D, bool q4) { return q4 ? seq4_stage_bytes(D) : seq_stage_bytes(D); }
+// outputs of the warps and one part of them, in the ring's place
+__host__ __device__ constexpr int seq_join_bytes(int D, int NT) {
+  return (kSeqWarps * 8 * NT * (D + 8) + 8 * NT * (D + 2)) * 4;
+}
+__host__ __device__ constexpr int seq_ring_bytes(int D, int NT, bool q4) {
+  const int ring = kSeqWarps * seq_stage_count(D, q4) * seq_stage_size(D, q4);
+  return ring > seq_join_bytes(D, NT) ? ring : seq_join_bytes(D, NT);
+}
 // floats of one partial result: 8 NT rows of D outputs, then (maximum, sum) per row
 __host__ __device__ constexpr int seq_part_floats(int D, int NT) { return 8 * NT * (D + 2); }
 
@@ -56,16 +75,16 @@ struct Line {
 __device__ __forceinline__ long long share(const Line& l, int g) { return l.total * g / l.active; }
 
 // Key units of an item and the units that a sequence takes.
-template <int D, int NT>
+template <int D, int NT, bool Q4>
 __device__ __forceinline__ long long seq_units(const SeqAttnArgs& a, const Seq& s, int* tiles, int* per) {
   *tiles = (int)(((long long)s.n * a.rep + 8 * NT - 1) / (8 * NT));
-  *per = max(1, (s.len + seq_unit(D) - 1) / seq_unit(D));
+  *per = max(1, (s.len + seq_unit(D, Q4) - 1) / seq_unit(D, Q4));
   return (long long)*tiles * (*per + kItemUnits) * a.Hkv;
 }
 
 // Finds the sequence that holds unit share(g): each thread sums a slice of the sequences.  Every thread
 // returns the line, the sequence and the units before it (b = -1: no share).
-template <int D, int NT, bool PAGED>
+template <int D, int NT, bool PAGED, bool Q4>
 __device__ Line find_share(const SeqAttnArgs& a, int g, int* b_out, long long* before) {
   __shared__ long long s_sum[kSeqWarps];
   __shared__ int s_b;
@@ -75,7 +94,7 @@ __device__ Line find_share(const SeqAttnArgs& a, int g, int* b_out, long long* b
   const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
   long long mine = 0;
   int tiles, units;
-  for (int b = b0; b < b1; ++b) mine += seq_units<D, NT>(a, load_seq<PAGED>(a, b), &tiles, &units);
+  for (int b = b0; b < b1; ++b) mine += seq_units<D, NT, Q4>(a, load_seq<PAGED>(a, b), &tiles, &units);
   long long incl = mine;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -99,7 +118,7 @@ __device__ Line find_share(const SeqAttnArgs& a, int g, int* b_out, long long* b
     long long excl = incl - mine;
     if (at >= excl && at < incl) {
       for (int b = b0; b < b1; ++b) {
-        const long long u = seq_units<D, NT>(a, load_seq<PAGED>(a, b), &tiles, &units);
+        const long long u = seq_units<D, NT, Q4>(a, load_seq<PAGED>(a, b), &tiles, &units);
         if (at < excl + u) {
           s_b = b;
           s_before = excl;
@@ -202,20 +221,159 @@ __device__ __forceinline__ void load_stage(const SeqAttnArgs& a, const KeyPages<
   }
 }
 
+// ---- a cache in 4 bits
+// The page of one key (a stage has a key per lane); -1: past the end or outside the cache.
+__device__ __forceinline__ int key_page4(const Seq4Args& a, int b, int j, int end) {
+  if (j >= end) return -1;
+  const int page = a.tables[(long long)b * a.table_stride + (j >> a.log_page)];
+  return (unsigned)page < (unsigned)a.num_pages ? page : -1;
+}
+
+// A stage: codes of the keys' and the values' rows, then their params.  Row r's 16-byte chunks of codes stand at c ^ swizzle(r).
+// Rows of no page are zeros.
+template <int D>
+__device__ __forceinline__ int swizzle4(int r) { return D == 128 ? r & 2 : 0; }
+
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async8z(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(have ? 8 : 0) : "memory");
+}
+
+template <int D>
+__device__ __forceinline__ void load_stage4(const Seq4Args& a, int my_page, int kvh, int j0, int end, uint32_t stage) {
+  constexpr int CH = D / 32, RPI = 32 / CH, G = D / kGroup4;
+  const int lane = threadIdx.x & 31, c = lane % CH, mask = (1 << a.log_page) - 1;
+  const uint8_t* kc = static_cast<const uint8_t*>(a.k4.codes) + kvh * a.k4.stride_ch + c * 16;
+  const uint8_t* vc = static_cast<const uint8_t*>(a.v4.codes) + kvh * a.v4.stride_ch + c * 16;
+  const bool in_head = c * 32 < a.hd;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int r = i * RPI + lane / CH, row = (j0 + r) & mask;
+    const long long page = __shfl_sync(0xffffffffu, my_page, r);
+    const bool ok = page >= 0 && in_head;
+    const uint32_t at = stage + r * (D / 2) + ((c ^ swizzle4<D>(r)) << 4);
+    cp_async16z(at, ok ? kc + page * a.k4.stride_cp + row * a.k4.stride_ct : static_cast<const void*>(a.q), ok);
+    cp_async16z(at + kSeq4Keys * (D / 2), ok ? vc + page * a.v4.stride_cp + row * a.v4.stride_ct : static_cast<const void*>(a.q), ok);
+  }
+  {
+    const int row = (j0 + lane) & mask;
+    const bool ok = my_page >= 0;
+    const uint32_t* kp = static_cast<const uint32_t*>(a.k4.params) + my_page * a.k4.stride_pp + row * a.k4.stride_pt + kvh * a.k4.stride_ph;
+    const uint32_t* vp = static_cast<const uint32_t*>(a.v4.params) + my_page * a.v4.stride_pp + row * a.v4.stride_pt + kvh * a.v4.stride_ph;
+    const uint32_t at = stage + kSeq4Keys * D + lane * (G * 4);
+    const void* none = a.q;  // (not read)
+    if (a.wide_params) {
+      if constexpr (D == 64) {
+        cp_async8z(at, ok ? kp : none, ok);
+        cp_async8z(at + kSeq4Keys * G * 4, ok ? vp : none, ok);
+      } else {
+        cp_async16z(at, ok ? kp : none, ok);
+        cp_async16z(at + kSeq4Keys * G * 4, ok ? vp : none, ok);
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const bool have = ok && g * kGroup4 < a.hd;
+        cp_async_small(at + g * 4, have ? kp + g : none, have);
+        cp_async_small(at + kSeq4Keys * G * 4 + g * 4, have ? vp + g : none, have);
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ bool params_not_finite(uint32_t p) {
+  return Type16<T>::not_finite((uint16_t)p) || Type16<T>::not_finite((uint16_t)(p >> 16));
+}
+
+// Which of 8 keys is row r of a tile of keys.  Any order serves, as both products use the same one; this one lets the 4 threads
+// of a quad, each with two neighbouring rows, and 8 threads of neighbouring rows read words of different banks.
+__device__ __forceinline__ int key_of_row(int r) { return r & 1 ? 7 - (r >> 1) : r >> 1; }
+
+// 16 keys as A fragments: this thread's keys are key and key + 8, its dims D / 4 in a row.
+template <typename T, int D>
+__device__ __forceinline__ void key_fragments4(const uint8_t* stage, int key, uint32_t kf[][4]) {
+  constexpr int G = D / kGroup4;
+  const int t = threadIdx.x & 3;
+  const uint32_t* kp = reinterpret_cast<const uint32_t*>(stage + kSeq4Keys * D);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = key + 8 * h;
+    const uint8_t* row = stage + r * (D / 2);
+    uint32_t w[D / 32];
+    if constexpr (D == 64) {
+      const uint2 x = *reinterpret_cast<const uint2*>(row + t * 8);
+      w[0] = x.x, w[1] = x.y;
+    } else {
+      const uint4 x = *reinterpret_cast<const uint4*>(row + ((t ^ swizzle4<D>(r)) << 4));
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    }
+    const uint32_t p = kp[r * G + t * G / 4], s2 = both_low(p), m2 = both_high(p);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      uint32_t u[4];
+      values8<T>(w[i], s2, m2, u);
+      kf[2 * i][h] = u[0], kf[2 * i][2 + h] = u[1];
+      kf[2 * i + 1][h] = u[2], kf[2 * i + 1][2 + h] = u[3];
+    }
+  }
+}
+
+// 16 keys' values, dims by keys, as A fragments: this thread's keys are key = 16 mt + t and 7 - t, and each + 8; its dims
+// D / 8 in a row: fragment dt's rows are dims (D / 8) (lane / 4) + 2 dt and the next.
+template <typename T, int D>
+__device__ __forceinline__ void value_fragments4(const uint8_t* stage, int key, uint32_t vf[][4]) {
+  constexpr int G = D / kGroup4, W = D / 64;
+  const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+  const uint8_t* codes = stage + kSeq4Keys * (D / 2);
+  const uint32_t* vp = reinterpret_cast<const uint32_t*>(stage + kSeq4Keys * D) + kSeq4Keys * G;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int ra = key + 8 * h, rb = key - t + 7 - t + 8 * h;
+    uint32_t wa[W], wb[W];
+    if constexpr (D == 64) {
+      wa[0] = *reinterpret_cast<const uint32_t*>(codes + ra * 32 + g * 4);
+      wb[0] = *reinterpret_cast<const uint32_t*>(codes + rb * 32 + g * 4);
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(codes + ra * 64 + (((g >> 1) ^ swizzle4<D>(ra)) << 4) + (g & 1) * 8);
+      const uint2 y = *reinterpret_cast<const uint2*>(codes + rb * 64 + (((g >> 1) ^ swizzle4<D>(rb)) << 4) + (g & 1) * 8);
+      wa[0] = x.x, wb[0] = y.x;
+      wa[W - 1] = x.y, wb[W - 1] = y.y;
+    }
+    const uint32_t pa = vp[ra * G + g * G / 8], pb = vp[rb * G + g * G / 8];
+    const uint32_t s2 = __byte_perm(pa, pb, 0x5410), m2 = __byte_perm(pa, pb, 0x7632);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      uint32_t even[4], odd[4];  // dims 0, 2, 4, 6 and 1, 3, 5, 7 of the word, a key in each half
+      values8<T>(__byte_perm(wa[i], wb[i], 0x5410), s2, m2, even);
+      values8<T>(__byte_perm(wa[i], wb[i], 0x7632), s2, m2, odd);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        vf[4 * i + e][2 * h] = even[e];
+        vf[4 * i + e][2 * h + 1] = odd[e];
+      }
+    }
+  }
+}
+
 // CL: few requests of short contexts.  A cluster of CTAs takes all keys of a (request, KV head) and joins its parts through
 // distributed shared memory, so there is no second launch (see seq_cluster).
-template <typename T, int D, int NT, bool PAGED, bool CL>
-__global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid_constant__ SeqAttnArgs a) {
+template <typename T, int D, int NT, bool PAGED, bool CL, typename ArgsT>
+__global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid_constant__ ArgsT a) {
+  constexpr bool Q4 = kIsInt4<ArgsT>;
   constexpr int RT = 8 * NT;
   constexpr int KS = D / 16;  // k steps of K Q^T
   constexpr int DT = D / 16;  // 16-dim tiles of the output
-  constexpr int KW = seq_keys(D), KT = KW / 16, UNIT = seq_unit(D);  // a warp's keys per stage, their 16-key tiles
+  constexpr int KW = seq_stage_keys(D, Q4), KT = KW / 16, UNIT = seq_unit(D, Q4);  // a warp's keys per stage, their 16-key tiles
+  constexpr int STAGES = seq_stage_count(D, Q4), STAGE = seq_stage_size(D, Q4);
   constexpr int LD = D + 8;   // floats per row of the warps' outputs in shared memory
-  static_assert((kSeqWarps * RT * LD + RT * (D + 2)) * 4 <= seq_smem_bytes(D), "outputs and a part fit the ring");
+  static_assert(Q4 || seq_join_bytes(D, NT) <= kSeqWarps * STAGES * STAGE, "outputs and a part fit the ring");
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ float s_ml[kSeqWarps][RT][2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t ring = smem_addr(smem) + warp * kSeqStages * seq_stage_bytes(D);
+  const uint32_t ring = smem_addr(smem) + warp * STAGES * STAGE;
   pdl_launch_dependents();
   pdl_wait_primary();
 
@@ -229,18 +387,18 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
   if constexpr (CL) {
     b = g / ranks / a.Hkv;
     s = load_seq<PAGED>(a, b);
-    seq_units<D, NT>(a, s, &tiles, &per);
+    seq_units<D, NT, Q4>(a, s, &tiles, &per);
     left = tiles;
     rem = 0;
   } else {
     long long before;
-    const Line line = find_share<D, NT, PAGED>(a, g, &b, &before);
+    const Line line = find_share<D, NT, PAGED, Q4>(a, g, &b, &before);
     if (b < 0) return;
     const long long at0 = share(line, g);
     left = share(line, g + 1) - at0;
     rem = at0 - before;
     s = load_seq<PAGED>(a, b);
-    seq_units<D, NT>(a, s, &tiles, &per);
+    seq_units<D, NT, Q4>(a, s, &tiles, &per);
   }
 
   while (left > 0) {
@@ -268,15 +426,23 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
     // ---- the warp's keys: k0 + KW warp + UNIT i, their first stages under way
     const int w0 = k0 + warp * KW;
     const int steps = w0 < k1 ? (k1 - w0 + UNIT - 1) / UNIT : 0;
-    KeyPages<D> pages[kSeqStages];
+    auto pages_of = [&](int j0) {
+      if constexpr (Q4) return key_page4(a, b, j0 + lane, k1);
+      else return key_pages<D, PAGED>(a, b, j0, k1);
+    };
+    auto load = [&](const auto& page, int j0, uint32_t stage) {
+      if constexpr (Q4) load_stage4<D>(a, page, kvh, j0, k1, stage);
+      else load_stage<D, PAGED>(a, page, s, kvh, j0, k1, stage);
+    };
+    decltype(pages_of(0)) pages[STAGES];
 #pragma unroll
-    for (int i = 0; i < kSeqStages; ++i) pages[i] = key_pages<D, PAGED>(a, b, w0 + i * UNIT, k1);
+    for (int i = 0; i < STAGES; ++i) pages[i] = pages_of(w0 + i * UNIT);
 #pragma unroll
-    for (int i = 0; i < kSeqStages - 1; ++i) {
-      if (i < steps) load_stage<D, PAGED>(a, pages[i], s, kvh, w0 + i * UNIT, k1, ring + i * seq_stage_bytes(D));
+    for (int i = 0; i < STAGES - 1; ++i) {
+      if (i < steps) load(pages[i], w0 + i * UNIT, ring + i * STAGE);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    KeyPages<D> next_pages = pages[kSeqStages - 1];
+    auto next_pages = pages[STAGES - 1];
 
     // ---- queries as B fragments (n = row, k = dim); rows past the tile are zero rows
     uint32_t qf[NT][KS][2];
@@ -290,7 +456,8 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int d = ks * 16 + c * 8 + (lane & 3) * 2;
+          // (of a 4-bit key a thread unpacks D / 4 dims in a row, four per step)
+          const int d = Q4 ? (lane & 3) * (D / 4) + ks * 4 + c * 2 : ks * 16 + c * 8 + (lane & 3) * 2;
           qf[nt][ks][c] = valid && d < a.hd ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
         }
     }
@@ -312,19 +479,19 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
 
     int slot = 0;
     for (int i = 0; i < steps; ++i) {
-      const int ahead = i + kSeqStages - 1;
-      int next = slot + kSeqStages - 1;
-      if (next >= kSeqStages) next -= kSeqStages;
+      const int ahead = i + STAGES - 1;
+      int next = slot + STAGES - 1;
+      if (next >= STAGES) next -= STAGES;
       __syncwarp();
-      if (ahead < steps)
-        load_stage<D, PAGED>(a, next_pages, s, kvh, w0 + ahead * UNIT, k1, ring + next * seq_stage_bytes(D));
+      if (ahead < steps) load(next_pages, w0 + ahead * UNIT, ring + next * STAGE);
       asm volatile("cp.async.commit_group;" ::: "memory");
-      next_pages = key_pages<D, PAGED>(a, b, w0 + (ahead + 1) * UNIT, k1);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kSeqStages - 1) : "memory");
+      next_pages = pages_of(w0 + (ahead + 1) * UNIT);
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
       __syncwarp();
-      const uint32_t ks_at = ring + slot * seq_stage_bytes(D), vs_at = ks_at + KW * D * 2;
+      const uint32_t ks_at = ring + slot * STAGE, vs_at = ks_at + KW * D * 2;
+      const uint8_t* const stage4 = smem + (ks_at - smem_addr(smem));
       const int j0 = w0 + i * UNIT;
-      slot = slot + 1 == kSeqStages ? 0 : slot + 1;
+      slot = slot + 1 == STAGES ? 0 : slot + 1;
 
       // S^T: KW keys x 8 NT rows
       float sc[KT][NT][4];
@@ -332,13 +499,22 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
       for (int mt = 0; mt < KT; ++mt) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
+        if constexpr (Q4) {
+          uint32_t kf[KS][4];
+          key_fragments4<T, D>(stage4, mt * 16 + key_of_row(lane / 4), kf);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {  // 16 keys x 16 dims: four 8x8 matrices
-          uint32_t kf[4];
-          const int r = mt * 16 + (lane & 15), c = ks * 2 + (lane >> 4);
-          ldmatrix_x4(kf, ks_at + r * (D * 2) + ((c ^ (r & 7)) << 4));
+          for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[mt][nt], kf, qf[nt][ks][0], qf[nt][ks][1]);
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[mt][nt], kf[ks], qf[nt][ks][0], qf[nt][ks][1]);
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {  // 16 keys x 16 dims: four 8x8 matrices
+            uint32_t kf[4];
+            const int r = mt * 16 + (lane & 15), c = ks * 2 + (lane >> 4);
+            ldmatrix_x4(kf, ks_at + r * (D * 2) + ((c ^ (r & 7)) << 4));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[mt][nt], kf, qf[nt][ks][0], qf[nt][ks][1]);
+          }
         }
       }
       if (j0 + KW - 1 > first_lim || j0 + KW > k1) {  // some key of them is hidden from some row
@@ -348,7 +524,7 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int j = j0 + mt * 16 + (e >> 1) * 8 + lane / 4;
+              const int j = j0 + mt * 16 + (e >> 1) * 8 + (Q4 ? key_of_row(lane / 4) : lane / 4);
               sc[mt][nt][e] = j > lim[nt][e & 1] || j >= k1 ? -INFINITY : sc[mt][nt][e] * a.scale_log2;
             }
       } else {
@@ -394,7 +570,36 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
           pf[mt][nt][1] = transpose8(Type16<T>::pack(sc[mt][nt][2], sc[mt][nt][3]));
         }
       }
-      if (j0 + KW - 1 > first_lim) {
+      if constexpr (Q4) {
+        if (j0 + KW - 1 > first_lim) {
+          uint32_t* vp = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(stage4) + kSeq4Keys * D) + kSeq4Keys * (D / kGroup4);
+          constexpr int G = D / kGroup4;
+          bool odd = false;  // lane's key is hidden from some row and has a group that is not finite
+#pragma unroll
+          for (int g = 0; g < G; ++g) odd |= params_not_finite<T>(vp[lane * G + g]);
+          unsigned bad = __ballot_sync(0xffffffffu, odd && j0 + lane > first_lim);
+          for (unsigned rest = bad; rest != 0; rest &= rest - 1) {
+            const int r = __ffs(rest) - 1;
+            if (params_not_finite<T>(vp[r * G + (lane / 4) * G / 8])) {  // this thread's dims lie in one group
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (j0 + r <= lim[nt][e]) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) o[dt][nt][e] = o[dt][nt][2 + e] = NAN;
+                  }
+            }
+          }
+          __syncwarp();
+          if (odd && j0 + lane > first_lim) {
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+              if (params_not_finite<T>(vp[lane * G + g])) vp[lane * G + g] = 0u;
+          }
+          __syncwarp();
+        }
+      } else if (j0 + KW - 1 > first_lim) {
         uint8_t* vs = smem + (vs_at - smem_addr(smem));
         unsigned bad = 0;  // hidden keys of the stage with a value that is not finite
         constexpr int CH = D / 8;
@@ -434,15 +639,25 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
       }
       // O^T += V^T P^T: 16 dims x 16 keys by four transposed 8x8 matrices
 #pragma unroll
-      for (int mt = 0; mt < KT; ++mt)
+      for (int mt = 0; mt < KT; ++mt) {
+        if constexpr (Q4) {
+          uint32_t vf[DT][4];
+          value_fragments4<T, D>(stage4, mt * 16 + (lane & 3), vf);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          uint32_t vf[4];
-          const int r = mt * 16 + (lane >> 4) * 8 + (lane & 7), c = dt * 2 + ((lane >> 3) & 1);
-          ldmatrix_x4_trans(vf, vs_at + r * (D * 2) + ((c ^ (r & 7)) << 4));
+          for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[dt][nt], vf, pf[mt][nt][0], pf[mt][nt][1]);
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[dt][nt], vf[dt], pf[mt][nt][0], pf[mt][nt][1]);
+        } else {
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            uint32_t vf[4];
+            const int r = mt * 16 + (lane >> 4) * 8 + (lane & 7), c = dt * 2 + ((lane >> 3) & 1);
+            ldmatrix_x4_trans(vf, vs_at + r * (D * 2) + ((c ^ (r & 7)) << 4));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[dt][nt], vf, pf[mt][nt][0], pf[mt][nt][1]);
+          }
         }
+      }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();  // every warp is done with its ring: the outputs may use it
@@ -464,8 +679,8 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
         }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          so[r * LD + dt * 16 + lane / 4] = o[dt][nt][e];
-          so[r * LD + dt * 16 + 8 + lane / 4] = o[dt][nt][e + 2];
+          so[r * LD + (Q4 ? lane / 4 * (D / 8) + dt * 2 : dt * 16 + lane / 4)] = o[dt][nt][e];
+          so[r * LD + (Q4 ? lane / 4 * (D / 8) + dt * 2 + 1 : dt * 16 + 8 + lane / 4)] = o[dt][nt][e + 2];
         }
       }
     __syncthreads();
@@ -539,7 +754,7 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
     while (left > 0 && rem >= (long long)tiles * (per + kItemUnits) * a.Hkv) {
       rem -= (long long)tiles * (per + kItemUnits) * a.Hkv;
       s = load_seq<PAGED>(a, ++b);
-      seq_units<D, NT>(a, s, &tiles, &per);
+      seq_units<D, NT, Q4>(a, s, &tiles, &per);
     }
   }
 }
@@ -548,8 +763,9 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid
 // first boundary inside that item; blockIdx.y takes a share of its outputs.  The parts' weights come first, all loads in
 // flight together, then the outputs.
 constexpr int kJoinShares = 4;
-template <typename T, int D, int NT, bool PAGED>
-__global__ void __launch_bounds__(kSeqThreads) seq_attention_join_kernel(const __grid_constant__ SeqAttnArgs a) {
+template <typename T, int D, int NT, bool PAGED, typename ArgsT>
+__global__ void __launch_bounds__(kSeqThreads) seq_attention_join_kernel(const __grid_constant__ ArgsT a) {
+  constexpr bool Q4 = kIsInt4<ArgsT>;
   constexpr int RT = 8 * NT;
   extern __shared__ float s_w[];  // [parts][RT] weight of a part in a row's output
   pdl_launch_dependents();
@@ -557,11 +773,11 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_join_kernel(const _
   const int g = blockIdx.x + 1;
   int b;
   long long before;
-  const Line line = find_share<D, NT, PAGED>(a, g, &b, &before);
+  const Line line = find_share<D, NT, PAGED, Q4>(a, g, &b, &before);
   if (b < 0) return;
   const Seq s = load_seq<PAGED>(a, b);
   int tiles, per;
-  seq_units<D, NT>(a, s, &tiles, &per);
+  seq_units<D, NT, Q4>(a, s, &tiles, &per);
   const long long rem = share(line, g) - before;
   const int span = per + kItemUnits, item = (int)(rem / span);
   const long long start = before + (long long)item * span, end = start + span;
@@ -613,9 +829,8 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_join_kernel(const _
   }
 }
 
-template <typename KernelT>
-static int launch_attn_grid(KernelT kernel, const SeqAttnArgs& a, dim3 grid, size_t smem, int cluster,
-                            cudaStream_t stream) {
+template <typename KernelT, typename ArgsT>
+static int launch_attn_grid(KernelT kernel, const ArgsT& a, dim3 grid, size_t smem, int cluster, cudaStream_t stream) {
   if (smem > 40 * 1024) {  // (the table is by kernel: instantiations of one signature share this function)
     static std::mutex mu;
     static std::vector<std::pair<int, const void*>> raised;
@@ -659,22 +874,22 @@ static int seq_cluster(const SeqAttnArgs& a) {
   return c > 1 && a.max_keys <= 1024LL * c ? c : 1;
 }
 
-template <typename T, int D, int NT, bool PAGED>
-static int launch_seq(const SeqAttnArgs& a, cudaStream_t stream) {
+template <typename T, int D, int NT, bool PAGED, typename ArgsT>
+static int launch_seq(const ArgsT& a, cudaStream_t stream) {
   const int c = seq_cluster(a);
+  const size_t smem = seq_ring_bytes(D, NT, kIsInt4<ArgsT>);
   if (c > 1)
-    return launch_attn_grid(seq_attention_kernel<T, D, NT, PAGED, true>, a, dim3((unsigned)(a.B * a.Hkv * c)),
-                            seq_smem_bytes(D), c, stream);
-  int rc = launch_attn_grid(seq_attention_kernel<T, D, NT, PAGED, false>, a, dim3((unsigned)a.grid), seq_smem_bytes(D), 1,
-                            stream);
+    return launch_attn_grid(seq_attention_kernel<T, D, NT, PAGED, true, ArgsT>, a, dim3((unsigned)(a.B * a.Hkv * c)), smem,
+                            c, stream);
+  int rc = launch_attn_grid(seq_attention_kernel<T, D, NT, PAGED, false, ArgsT>, a, dim3((unsigned)a.grid), smem, 1, stream);
   if (rc == LI4_OK)
-    rc = launch_attn_grid(seq_attention_join_kernel<T, D, NT, PAGED>, a, dim3((unsigned)a.grid - 1, kJoinShares),
+    rc = launch_attn_grid(seq_attention_join_kernel<T, D, NT, PAGED, ArgsT>, a, dim3((unsigned)a.grid - 1, kJoinShares),
                           (size_t)a.grid * 8 * NT * sizeof(float), 1, stream);
   return rc;
 }
 
-template <typename T, bool PAGED>
-static int launch_seq_d(const SeqAttnArgs& a, int nt, cudaStream_t stream) {
+template <typename T, bool PAGED, typename ArgsT>
+static int launch_seq_d(const ArgsT& a, int nt, cudaStream_t stream) {
   if (a.hd <= 64)
     return nt == 1   ? launch_seq<T, 64, 1, PAGED>(a, stream)
            : nt == 2 ? launch_seq<T, 64, 2, PAGED>(a, stream)
@@ -700,6 +915,13 @@ int launch_seq_attention(const SeqAttnArgs& args, bool paged, int dtype, int max
   return paged ? launch_seq_d<__nv_bfloat16, true>(a, nt, stream) : launch_seq_d<__nv_bfloat16, false>(a, nt, stream);
 }
 
+int launch_seq_attention_int4(const Seq4Args& args, int dtype, int max_rows, cudaStream_t stream) {
+  Seq4Args a = args;
+  a.grid = seq_grid(current_sm_count());
+  const int nt = seq_nt(max_rows);
+  return dtype == LI4_F16 ? launch_seq_d<__half, true>(a, nt, stream) : launch_seq_d<__nv_bfloat16, true>(a, nt, stream);
+}
+
 // Rows (queries x heads of a KV head) up to which a sequence is streamed: where no sequence has more the streaming
 // kernel runs alone, with tiles of 8, 16 or 32 rows; beside longer ones it takes those of one 8-row tile.  Beside a chunk
 // of 512 tokens, 31 requests of 200-6000 tokens each, with the limit at 8 / 16 / 32 rows and tiles as high (us):
@@ -712,7 +934,12 @@ constexpr int kFewRows = 32, kFewRowsBeside = 8;
 
 constexpr int64_t kAttentionMost = 1 << 30;  // rows of a sequence, keys: what is claimed above it counts as it
 
-static int check_attention(const li4_attention* p, bool paged, const char* what) {
+struct Int4Pages {
+  const li4_int4_pages *k, *v;
+};
+
+// int4: not null for a cache in 4 bits.
+static int check_attention(const li4_attention* p, bool paged, const Int4Pages* int4, const char* what) {
   if (!p) return set_error(LI4_ERR_INVALID_ARG, "%s: null arguments", what);
   if (p->dtype != LI4_F16 && p->dtype != LI4_BF16)
     return set_error(LI4_ERR_UNSUPPORTED, "%s: dtype %d (LI4_F16 or LI4_BF16)", what, p->dtype);
@@ -724,6 +951,10 @@ static int check_attention(const li4_attention* p, bool paged, const char* what)
   if (p->head_dim < 8 || p->head_dim > 128 || p->head_dim % 8 != 0)
     return set_error(LI4_ERR_UNSUPPORTED, "%s: head_dim=%lld (a multiple of 8 up to 128)", what,
                      (long long)p->head_dim);
+  if (int4 && p->head_dim % kGroup4 != 0)
+    return set_error(LI4_ERR_UNSUPPORTED, "%s: head_dim=%lld (a multiple of %d up to 128)", what, (long long)p->head_dim,
+                     kGroup4);
+  if (int4 && (!int4->k || !int4->v)) return set_error(LI4_ERR_INVALID_ARG, "%s: null pointer", what);
   if (p->n_heads / p->n_kv_heads > 128 || p->n_heads > 65535 || p->n_seqs > (1 << 24) ||
       p->n_tokens > (1LL << 30) / p->n_heads)
     return set_error(LI4_ERR_UNSUPPORTED, "%s: n_seqs=%lld n_tokens=%lld n_heads=%lld too large", what,
@@ -740,20 +971,30 @@ static int check_attention(const li4_attention* p, bool paged, const char* what)
                        (long long)p->num_pages, (long long)p->table_width, (long long)p->table_stride);
   }
   if (p->n_seqs == 0 || p->n_tokens == 0) return LI4_OK;
-  if (!p->q || !p->out || !p->cu_seqlens || ((!p->k || !p->v) && !(paged && p->num_pages == 0)) ||
+  const bool no_keys = int4 ? !int4->k->codes || !int4->k->params || !int4->v->codes || !int4->v->params : !p->k || !p->v;
+  if (!p->q || !p->out || !p->cu_seqlens || (no_keys && !(paged && p->num_pages == 0)) ||
       (paged && (!p->kv_lens || (!p->block_tables && p->table_width > 0))))
     return set_error(LI4_ERR_INVALID_ARG, "%s: null pointer", what);
   const int64_t st[] = {p->stride_qt, p->stride_qh, p->stride_ot, p->stride_oh, p->stride_kt, p->stride_kh,
                         p->stride_vt, p->stride_vh, paged ? p->stride_kp : 0, paged ? p->stride_vp : 0};
-  bool aligned = aligned16(p->q) && aligned16(p->k) && aligned16(p->v) && aligned16(p->out);
+  bool aligned = aligned16(p->q) && aligned16(p->out);
+  if (int4) aligned = aligned && int4_pages_aligned(*int4->k) && int4_pages_aligned(*int4->v);
+  else aligned = aligned && aligned16(p->k) && aligned16(p->v);
   const int64_t rep = p->n_heads / p->n_kv_heads;
   const int64_t size[] = {p->n_tokens, p->n_heads, p->n_tokens, p->n_heads, paged ? p->page_size : p->n_tokens,
                           p->n_kv_heads, paged ? p->page_size : p->n_tokens, p->n_kv_heads, p->num_pages, p->num_pages};
-  for (int i = 0; i < 10; ++i)  // (the stride of a dimension of one element is not used)
+  for (int i = 0; i < (int4 ? 4 : 10); ++i)  // (the stride of a dimension of one element is not used)
     aligned = aligned && st[i] % 8 == 0 && (st[i] > 0 || (st[i] == 0 && (size[i] <= 1 || (!paged && i >= 8))));
   if (!aligned || rep < 1)
     return set_error(LI4_ERR_ALIGNMENT, "%s: every row must start on a 16-byte boundary, at a positive stride", what);
   return LI4_OK;
+}
+
+// Whether the rows' params can be copied in one piece each (head_dim 64 or 128).
+static bool wide_params(const li4_int4_pages& p, int hd) {
+  const int64_t pairs = hd / kGroup4;
+  return (hd == 64 || hd == 128) && reinterpret_cast<uintptr_t>(p.params) % (pairs * 4) == 0 &&
+         p.stride_pp % pairs == 0 && p.stride_pt % pairs == 0 && p.stride_ph % pairs == 0;
 }
 
 static int attention_rows(const li4_attention* p) {
@@ -768,19 +1009,19 @@ static int64_t attention_keys(const li4_attention* p) {
   return p->table_width > kAttentionMost / p->page_size ? kAttentionMost : p->table_width * p->page_size;
 }
 
-static int run_attention(const li4_attention* p, bool paged, void* workspace, size_t workspace_bytes, void* stream,
-                         const char* what) {
-  int rc = check_attention(p, paged, what);
+static int run_attention(const li4_attention* p, bool paged, const Int4Pages* int4, void* workspace,
+                         size_t workspace_bytes, void* stream, const char* what) {
+  int rc = check_attention(p, paged, int4, what);
   if (rc != LI4_OK) return rc;
   if (p->n_seqs == 0 || p->n_tokens == 0) {
     clear_error();
     return LI4_OK;
   }
-  const size_t need = li4_attention_workspace_bytes(p);
+  const size_t need = int4 ? li4_attention_int4_workspace_bytes(p) : li4_attention_workspace_bytes(p);
   if (workspace_bytes < need || (need && !workspace) || !aligned16(workspace))
     return set_error(LI4_ERR_WORKSPACE, "%s: %zu bytes of 16-byte aligned workspace needed, %zu given", what, need,
                      workspace_bytes);
-  SeqAttnArgs a = {};
+  Seq4Args a = {};
   a.q = static_cast<const uint16_t*>(p->q);
   a.k = static_cast<const uint16_t*>(p->k);
   a.v = static_cast<const uint16_t*>(p->v);
@@ -811,6 +1052,16 @@ static int run_attention(const li4_attention* p, bool paged, void* workspace, si
   const bool tiles = rows > kFewRows && a.scale_log2 > 0.f && !(paged && p->num_pages == 0);
   const bool both = tiles && paged && p->n_seqs > 1;
   rc = LI4_OK;
+  if (int4) {
+    a.k4 = *int4->k;
+    a.v4 = *int4->v;
+    a.wide_params = wide_params(*int4->k, a.hd) && wide_params(*int4->v, a.hd);
+    a.small_rows = 0;
+    a.big_rows = 0x7fffffff;
+    rc = launch_seq_attention_int4(a, p->dtype, rows, st);
+    if (rc == LI4_OK) clear_error();
+    return rc;
+  }
   if (!tiles || both) {
     a.small_rows = 0;
     a.big_rows = both ? kFewRowsBeside : 0x7fffffff;
@@ -841,9 +1092,18 @@ extern "C" size_t li4_attention_workspace_bytes(const li4_attention* p) {
 }
 
 extern "C" int li4_prompt_attention(const li4_attention* args, void* workspace, size_t workspace_bytes, void* stream) {
-  return li4::run_attention(args, false, workspace, workspace_bytes, stream, "prompt_attention");
+  return li4::run_attention(args, false, nullptr, workspace, workspace_bytes, stream, "prompt_attention");
 }
 
 extern "C" int li4_paged_attention(const li4_attention* args, void* workspace, size_t workspace_bytes, void* stream) {
-  return li4::run_attention(args, true, workspace, workspace_bytes, stream, "paged_attention");
+  return li4::run_attention(args, true, nullptr, workspace, workspace_bytes, stream, "paged_attention");
+}
+
+extern "C" size_t li4_attention_int4_workspace_bytes(const li4_attention* p) { return li4_attention_workspace_bytes(p); }
+
+extern "C" int li4_paged_attention_int4(const li4_attention* args, const li4_int4_pages* cache_k,
+                                        const li4_int4_pages* cache_v, void* workspace, size_t workspace_bytes,
+                                        void* stream) {
+  const li4::Int4Pages pages = {cache_k, cache_v};
+  return li4::run_attention(args, true, &pages, workspace, workspace_bytes, stream, "paged_attention_int4");
 }

@@ -97,6 +97,14 @@ class Attention(ctypes.Structure):
         [(name, ctypes.c_int64) for name in ("table_stride", "table_width", "num_pages", "page_size")]
 
 
+class Int4Pages(ctypes.Structure):
+    """struct li4_int4_pages (include/llama_int4_b200.h): keys or values of a paged cache in 4 bits."""
+
+    _fields_ = [("codes", ctypes.c_void_p), ("params", ctypes.c_void_p)] + \
+        [(name, ctypes.c_int64) for name in ("stride_cp", "stride_ct", "stride_ch", "stride_pp", "stride_pt",
+                                             "stride_ph")]
+
+
 # name -> (restype, argtypes); mirrors include/llama_int4_b200.h
 SIGNATURES = {
     "li4_version": (_INT, []),
@@ -149,6 +157,16 @@ SIGNATURES = {
     "li4_attention_workspace_bytes": (_SZ, [ctypes.POINTER(Attention)]),
     "li4_prompt_attention": (_INT, [ctypes.POINTER(Attention), _P, _SZ, _P]),
     "li4_paged_attention": (_INT, [ctypes.POINTER(Attention), _P, _SZ, _P]),
+    "li4_rope_paged_write_int4": (_INT, [_P, _P, _P, _INT, _I64, _I64, _I64, _I64, ctypes.POINTER(_I64), _P, _P, _I64,
+                                         _I64, _P, _P, _P, _P, _P, ctypes.POINTER(Int4Pages),
+                                         ctypes.POINTER(Int4Pages), _I64, _I64, _P]),
+    "li4_attention_int4_workspace_bytes": (_SZ, [ctypes.POINTER(Attention)]),
+    "li4_paged_attention_int4": (_INT, [ctypes.POINTER(Attention), ctypes.POINTER(Int4Pages),
+                                        ctypes.POINTER(Int4Pages), _P, _SZ, _P]),
+    "li4_paged_fork_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "li4_paged_fork": (_INT, [_P, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, ctypes.POINTER(_P),
+                              ctypes.POINTER(_I64), ctypes.POINTER(_I64), _I64, _P, _SZ, _P]),
+    "li4_token_logprobs": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _P]),
     "li4_dequantize": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
     "li4_quantize": (_INT, [_P, _INT, _P, _P, _P, _I64, _I64, _I64, _I64, _P]),
 }
@@ -186,7 +204,8 @@ def lib() -> ctypes.CDLL:
 
 
 def ext():
-    """The paged-cache entry points on torch tensors (csrc/li4_torch.cpp), loaded once after the library."""
+    """The paged-cache entry points and token_logprobs on torch tensors (csrc/li4_torch.cpp), loaded once after the
+    library."""
     global _ext
     if _ext is None:
         lib()

@@ -12,6 +12,9 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from .logprobs import token_logprobs
+from .paged import hidden_paged
+
 
 class DecodeGraph:
     """Greedy decode steps replayed from one CUDA graph.
@@ -193,37 +196,60 @@ class Generation(nn.Module):
 
     @torch.no_grad()
     def generate_paged(self, tokenizer, prompts, max_gen_len, temperature, top_p, device, page_size=16,
-                       cuda_graph=False):
+                       cuda_graph=False, samples=1, kv_bits=16, logprobs=None):
         """generate() over a paged KV cache (llama.paged), without padding: the prompts run packed as one step, then
         every unfinished request gets a token per step, and a finished one returns its pages at once.
         cuda_graph=True (greedy only) replays one captured step for all requests until max_gen_len and cuts the
-        answers at eos afterwards."""
+        answers at eos afterwards.
+
+        samples: answers per prompt, one after another in the results; they share the prompt's full pages
+        (PagedKVCache.fork).  kv_bits=4 keeps the cache in 4 bits.  logprobs=k adds "logprobs" to each result: the answer's
+        tokens, their log probabilities under the model (before temperature and top_p), the entropies and the k likeliest
+        (token, log probability) pairs (llama.logprobs)."""
         if cuda_graph and temperature > 0:
             raise ValueError("cuda_graph decode needs greedy sampling (temperature 0)")
+        if samples < 1:
+            raise ValueError(f"generate_paged: {samples} samples")
         encoded = [tokenizer.encode(text, bos=True, eos=False) for text in prompts]
-        n, lengths = len(encoded), [len(t) for t in encoded]
-        if n == 0 or min(lengths) < 1:
+        lengths = [len(t) for t in encoded]
+        if not encoded or min(lengths) < 1:
             raise ValueError("generate_paged: every prompt needs a token")
+        n = len(encoded) * samples  # requests: a prompt's answers stand together, the first has its tokens
         total = max(lengths) + max_gen_len
-        pages = sum(-(-(l + max_gen_len) // page_size) for l in lengths)
-        cache = self.paged_cache(pages, page_size, max_requests=n, max_len=total)
+        pages = sum(samples * (-(-(l + max_gen_len) // page_size)) - (samples - 1) * (l // page_size) for l in lengths)
+        cache = self.paged_cache(pages, page_size, max_requests=n, max_len=total, bits=kv_bits)
 
         def pick(logits):
             if temperature > 0:
                 return sample_top_p(torch.softmax(logits / temperature, dim=-1), top_p).view(-1)
             return logits.argmax(dim=-1)
 
+        costs = []  # by step: what token_logprobs says of all requests
+
+        def note(logits, choice):
+            if logprobs is not None:
+                costs.append(token_logprobs(logits, choice, logprobs))
+
         answers = [[] for _ in range(n)]
         if max_gen_len > 0:
             packed = torch.tensor([t for toks in encoded for t in toks], dtype=torch.long, device=device)
-            step = cache.append(torch.tensor(lengths, dtype=torch.int32, device=device), sum(lengths))
-            choice = pick(self.forward_paged(packed, step, cache, max(lengths), whole_prompts=True))
+            new = [0] * n
+            new[::samples] = lengths
+            step = cache.append(torch.tensor(new, dtype=torch.int32, device=device), sum(lengths))
+            logits = self.forward_paged(packed, step, cache, max(lengths), whole_prompts=True)
+            if samples > 1:
+                first = torch.arange(n, dtype=torch.int32, device=device) // samples * samples
+                cache.fork(first)
+                logits = logits.index_select(0, first)
+            choice = pick(logits)
+            note(logits, choice)
             if cuda_graph:
                 graph = PagedDecodeGraph(self, cache, choice)
                 chosen = [choice]
                 for _ in range(max_gen_len - 1):
                     graph.replay()
                     chosen.append(graph.tok.clone())
+                    note(graph.logits, graph.tok)
                 if not bool(graph.granted.all()):
                     raise RuntimeError("generate_paged: a request was refused a token")
                 answers = torch.stack(chosen, 1).tolist()
@@ -242,13 +268,50 @@ class Generation(nn.Module):
                         break
                     new = torch.tensor([int(g) for g in going], dtype=torch.int32, device=device)
                     fed = torch.tensor([answers[r][-1] for r in range(n) if going[r]], dtype=torch.long, device=device)
-                    choice = pick(self.forward_paged(fed, cache.append(new, fed.shape[0]), cache, 1))
+                    logits = self.forward_paged(fed, cache.append(new, fed.shape[0]), cache, 1)
+                    choice = pick(logits)
+                    note(logits, choice)
+        costs = [[None if t is None else t.tolist() for t in c] for c in costs]
         results = []
-        for gen in answers:
+        for row, gen in enumerate(answers):
             if tokenizer.eos_id in gen:
                 gen = gen[:gen.index(tokenizer.eos_id)]
             results.append({"generation": tokenizer.decode(gen)})
+            if logprobs is not None:
+                results[-1]["logprobs"] = _costs_of(gen, row, costs[:len(gen)])
         return results
+
+    @torch.no_grad()
+    def score_paged(self, tokenizer, texts, device, page_size=16, kv_bits=16, top=0, rows=1024):
+        """What the model gives the tokens of each text after its first one: [{"tokens", "logprobs", "entropy", "top"}]
+        (see generate_paged's logprobs).  The texts run packed as one step; their logits are made `rows` tokens at a
+        time, so all of them never exist at once."""
+        encoded = [tokenizer.encode(text, bos=True, eos=False) for text in texts]
+        lengths = [len(t) for t in encoded]
+        if not encoded or min(lengths) < 1:
+            raise ValueError("score_paged: every text needs a token")
+        cache = self.paged_cache(sum(-(-l // page_size) for l in lengths), page_size, max_requests=len(encoded),
+                                 max_len=max(lengths), bits=kv_bits)
+        packed = torch.tensor([t for toks in encoded for t in toks], dtype=torch.long, device=device)
+        step = cache.append(torch.tensor(lengths, dtype=torch.int32, device=device), packed.shape[0])
+        h = hidden_paged(self, packed, step, cache, max(lengths), whole_prompts=True)
+        nexts = torch.cat([packed[1:], packed[:1]])  # (of a text's last token: not used)
+        costs = []
+        for at in range(0, packed.shape[0], rows):
+            some = token_logprobs(self._logits(self.norm(h[at:at + rows])), nexts[at:at + rows], top)
+            costs += zip(*([None] * some.logprobs.shape[0] if t is None else t.tolist() for t in some))
+        results, at = [], 0
+        for toks in encoded:
+            each = [[None if t is None else [t] for t in c] for c in costs[at:at + len(toks) - 1]]
+            results.append(_costs_of(toks[1:], 0, each))
+            at += len(toks)
+        return results
+
+
+def _costs_of(tokens, row, costs):
+    """Request `row` of each step's (logprobs, entropy, top_tokens, top_logprobs) beside its tokens."""
+    return {"tokens": list(tokens), "logprobs": [c[0][row] for c in costs], "entropy": [c[1][row] for c in costs],
+            "top": [[] if c[2] is None else list(zip(c[2][row], c[3][row])) for c in costs]}
 
 
 def sample_top_p(probs, p):

@@ -339,9 +339,9 @@ class Llama(Generation):
         return self
 
     def paged_cache(self, num_pages: int, page_size: int = 16, max_requests: Optional[int] = None,
-                    max_len: Optional[int] = None):
-        """A PagedKVCache (llama.paged) for this model's layers, type and device.  max_len (default
-        max_seq_len) is at most the RoPE table's 2 * max_seq_len positions."""
+                    max_len: Optional[int] = None, bits: int = 16):
+        """A PagedKVCache (llama.paged) for this model's layers, type and device, of 16 or 4 bits a value.
+        max_len (default max_seq_len) is at most the RoPE table's 2 * max_seq_len positions."""
         from .paged import PagedKVCache
 
         p, att, w = self.params, self.layers[0].attention, self.tok_embeddings.weight
@@ -349,7 +349,8 @@ class Llama(Generation):
         if max_len > self.freqs_cis.shape[0]:
             raise ValueError(f"max_len {max_len} exceeds the {self.freqs_cis.shape[0]} positions of the RoPE table")
         return PagedKVCache(p.n_layers, num_pages, page_size, att.n_local_kv_heads, att.head_dim,
-                            p.max_batch_size if max_requests is None else max_requests, max_len, w.dtype, w.device)
+                            p.max_batch_size if max_requests is None else max_requests, max_len, w.dtype, w.device,
+                            bits=bits)
 
     @torch.no_grad()
     def forward_paged(self, tokens: torch.Tensor, step, cache, max_new: int, whole_prompts: bool = False):

@@ -11,6 +11,11 @@ block tables name per request, and a step's new tokens of all requests stand one
     prompt_attention   whole prompts, from the packed keys and values              (li4_prompt_attention)
     paged_attention    anything else, from the cache                               (li4_paged_attention)
 
+With PagedKVCache(bits=4) the cache holds keys and values in 4 bits (5 with their parameters): rope_paged_write_int4 and
+paged_attention_int4 (li4_rope_paged_write_int4, li4_paged_attention_int4) take the places of their 16-bit forms, and
+whole prompts attend to the values that the cache holds.  Requests go on from one another's tokens, sharing full pages, and
+end by paged_fork (li4_paged_fork): several answers to a prompt, the steps of a search, PagedKVCache.release.
+
 The lengths live on the GPU: no call reads them on the host, so a step can be captured in a CUDA graph
 and replayed while the requests grow.  PagedKVCache holds the pool, Llama.forward_paged runs the model's
 blocks over it, Generation.generate_paged is the loop around them.
@@ -22,7 +27,7 @@ and calls under a tracer are refused.
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -38,6 +43,43 @@ class PagedStep(NamedTuple):
     kv_lens: torch.Tensor     # int32 [requests], the step's tokens included
     n_free: torch.Tensor      # int32 [1]
     granted: torch.Tensor     # bool [requests]
+
+
+class PagedFork(NamedTuple):
+    """What paged_fork leaves (all on the GPU)."""
+
+    kv_lens: torch.Tensor  # int32 [requests]
+    n_free: torch.Tensor   # int32 [1]
+    granted: torch.Tensor  # bool [requests]
+
+
+class Int4Pages(NamedTuple):
+    """Keys or values of a paged cache in 4 bits: groups of 32 dims with a scale s and an offset m stand for c s + m,
+    rounded to the type of s and m."""
+
+    codes: torch.Tensor   # uint8 [pages, page_size, kv_heads, head_dim / 2], see pack_codes
+    params: torch.Tensor  # float16 or bfloat16 [pages, page_size, kv_heads, head_dim / 32, 2]: (s, m)
+
+    def values(self) -> torch.Tensor:
+        """The 16-bit values [pages, page_size, kv_heads, head_dim] (plain tensor operations: for looking, not for steps)."""
+        c = unpack_codes(self.codes).unflatten(-1, (-1, 32)).double()
+        p = self.params.double()
+        return (c * p[..., 0:1] + p[..., 1:2]).to(self.params.dtype).flatten(-2)
+
+
+_CODE_BITS = (0, 16, 4, 20, 8, 24, 12, 28)  # where in its 32-bit word the code of dim 0 .. 7 begins
+
+
+def pack_codes(codes: torch.Tensor) -> torch.Tensor:
+    """Codes 0 .. 15 [..., head_dim] as the cache holds them, uint8 [..., head_dim / 2]."""
+    at = torch.tensor(_CODE_BITS, dtype=torch.int32, device=codes.device)
+    return (codes.to(torch.int32).unflatten(-1, (-1, 8)) << at).sum(-1, dtype=torch.int32).view(torch.uint8)
+
+
+def unpack_codes(packed: torch.Tensor) -> torch.Tensor:
+    """The codes [..., head_dim] (int32) of packed rows [..., head_dim / 2]."""
+    at = torch.tensor(_CODE_BITS, dtype=torch.int32, device=packed.device)
+    return ((packed.contiguous().view(torch.int32).unsqueeze(-1) >> at) & 15).flatten(-2)
 
 
 def _done(what: str, result):
@@ -105,25 +147,76 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
                                                                  max_new, scale, out))
 
 
+def rope_paged_write_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                          positions: torch.Tensor, slots: torch.Tensor, cache_k: Int4Pages, cache_v: Int4Pages,
+                          q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+                          v_out: Optional[torch.Tensor] = None,
+                          need_kv: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """rope_paged_write into a cache in 4 bits (li4_rope_paged_write_int4); head_dim a multiple of 32 up to 128.
+
+    A group of 32 values x gets m = the smallest, s = (the largest - m) / 15 rounded towards zero to the type, and codes
+    min(15, (x - m) / s to the nearest, ties to even), 0 where s is 0; a key is turned in 64 bits and rounded first, so
+    the codes are a function of the inputs alone.  A group with a value that is not finite reads as NaN.
+    Returns (turned q, k, v): k and v packed, as the cache holds them, for prompt_attention.  need_kv = False leaves them
+    out (None).  q_out / k_out / v_out may be q / k / v themselves and overlap nothing else."""
+    return _done("rope_paged_write_int4", native.ext().rope_paged_write_int4(
+        q, k, v, cos, sin, positions, slots, cache_k, cache_v, q_out, k_out, v_out, need_kv))
+
+
+def paged_attention_int4(q: torch.Tensor, cache_k: Int4Pages, cache_v: Int4Pages, block_tables: torch.Tensor,
+                         kv_lens: torch.Tensor, cu_seqlens: torch.Tensor, max_new: int, scale: Optional[float] = None,
+                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_attention over a cache in 4 bits (li4_paged_attention_int4): the same function of the 16-bit values that
+    the cache stands for, with the same arguments; cache_k / cache_v are Int4Pages (or pairs) of q's type."""
+    return _done("paged_attention_int4", native.ext().paged_attention_int4(
+        q, cache_k, cache_v, block_tables, kv_lens, cu_seqlens, max_new, scale, out))
+
+
+def paged_fork(kv_lens: torch.Tensor, block_tables: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor,
+               parents: torch.Tensor, page_size: int, pools: Sequence[torch.Tensor] = (),
+               kv_lens_out: Optional[torch.Tensor] = None, n_free_out: Optional[torch.Tensor] = None) -> PagedFork:
+    """Requests that go on from others, and that end (li4_paged_fork): parents int32 [requests] names for each request
+    itself (it stays), another (it holds that one's tokens from now on, as they were before the call) or -1 (it ends).
+
+    Full pages are shared, a last page that is not full is copied into one from the top of the free stack, in every tensor
+    of pools ([pages, ...], each page one block of memory).  A request whose copy finds no page, or whose parent is none,
+    stays as it was (granted False).  Pages that no request holds any more go back on the stack, in the order of requests
+    and blocks.  block_tables and free_pages are updated in place; kv_lens_out / n_free_out may be kv_lens / n_free (in
+    place), by default they are new tensors.  Sharing is read off the tables: append and this are all there is to call."""
+    return PagedFork._make(_done("paged_fork", native.ext().paged_fork(
+        kv_lens, block_tables, free_pages, n_free, parents, page_size, pools, kv_lens_out, n_free_out)))
+
+
 class PagedKVCache:
     """Pages, block tables and lengths of up to max_requests requests of up to max_len tokens each.
 
-    k[i] / v[i] are layer i's pages [num_pages, page_size, kv_heads, head_dim]; each (page, head) is contiguous in
-    memory, so the rows a KV head reads of a page are one run.  Request r is row r of block_tables and kv_lens for as
-    long as it lives; release() returns its pages."""
+    k[i] / v[i] are layer i's pages [num_pages, page_size, kv_heads, head_dim], or with bits = 4 its Int4Pages; each
+    (page, head) is contiguous in memory, so the rows a KV head reads of a page are one run.  Request r is row r of
+    block_tables and kv_lens for as long as it lives; fork() lets it go on from another, release() returns its pages."""
 
     def __init__(self, n_layers: int, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
-                 max_requests: int, max_len: int, dtype: torch.dtype = torch.float16, device="cuda"):
+                 max_requests: int, max_len: int, dtype: torch.dtype = torch.float16, device="cuda", bits: int = 16):
         if page_size < 8 or page_size > 1024 or page_size & (page_size - 1):
             raise ValueError(f"page_size {page_size}: a power of two from 8 to 1024")
         if dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"cache dtype {dtype}: float16 or bfloat16")
         if head_dim % 8 or not 8 <= head_dim <= 128:
             raise ValueError(f"head_dim {head_dim}: a multiple of 8 up to 128")
-        self.page_size, self.max_len = page_size, max_len
-        shape = (n_layers, num_pages, n_kv_heads, page_size, head_dim)
-        self.k = [t.transpose(1, 2) for t in torch.zeros(shape, dtype=dtype, device=device)]
-        self.v = [t.transpose(1, 2) for t in torch.zeros(shape, dtype=dtype, device=device)]
+        if bits not in (4, 16) or (bits == 4 and head_dim % 32):
+            raise ValueError(f"a cache of {bits} bits with head_dim {head_dim}: 16, or 4 with head_dim a multiple of 32")
+        self.page_size, self.max_len, self.bits = page_size, max_len, bits
+
+        def pages(row, kind):  # a layer's after another
+            return [t.transpose(1, 2)
+                    for t in torch.zeros(n_layers, num_pages, n_kv_heads, page_size, *row, dtype=kind, device=device)]
+
+        if bits == 16:
+            self.k, self.v = pages([head_dim], dtype), pages([head_dim], dtype)
+            self.pools = self.k + self.v  # all tensors of pages
+        else:
+            self.k, self.v = ([Int4Pages(c, p) for c, p in zip(pages([head_dim // 2], torch.uint8),
+                                                               pages([head_dim // 32, 2], dtype))] for _ in range(2))
+            self.pools = [t for pair in self.k + self.v for t in pair]
         i32 = dict(dtype=torch.int32, device=device)
         self.block_tables = torch.zeros(max_requests, -(-max_len // page_size), **i32)
         self.kv_lens = torch.zeros(max_requests, **i32)
@@ -139,9 +232,21 @@ class PagedKVCache:
         return paged_append(self.kv_lens, new_lens, self.block_tables, self.free_pages, self.n_free, self.page_size,
                             num_tokens, kv_lens_out=self.kv_lens, n_free_out=self.n_free, max_len=self.max_len)
 
+    def fork(self, parents: torch.Tensor) -> torch.Tensor:
+        """Every request r goes on from request parents[r] (int32 [max_requests]): itself, another, or none (-1: it ends);
+        see paged_fork.  Updates lengths, tables, free pages and the copied pages in place; returns granted
+        bool [max_requests].  No host synchronisation."""
+        return paged_fork(self.kv_lens, self.block_tables, self.free_pages, self.n_free, parents, self.page_size,
+                          self.pools, kv_lens_out=self.kv_lens, n_free_out=self.n_free).granted
+
     def release(self, finished: torch.Tensor) -> None:
-        """Returns the pages of the requests flagged in finished (bool [max_requests]) and sets their lengths to 0.
-        No host synchronisation."""
+        """Returns the pages of the requests flagged in finished (bool [max_requests]), those that no other request
+        shares, and sets their lengths to 0.  No host synchronisation."""
+        if self.kv_lens.is_cuda:
+            stay = torch.arange(finished.shape[0], dtype=torch.int32, device=finished.device)
+            self.fork(stay.masked_fill_(finished, -1))
+            return
+        # (index arithmetic; nothing forks off the GPU, so no page is shared)
         held = torch.div(self.kv_lens + (self.page_size - 1), self.page_size, rounding_mode="floor")
         block = torch.arange(self.block_tables.shape[1], device=self.kv_lens.device)
         back = (finished[:, None] & (block < held[:, None])).flatten()
@@ -168,6 +273,14 @@ def forward_paged(model, tokens: torch.Tensor, step: PagedStep, cache: PagedKVCa
                   whole_prompts: bool = False) -> torch.Tensor:
     """fp32 logits [requests, vocab] of each request's last token of the step (rows of requests without new tokens
     hold another token's): see Llama.forward_paged."""
+    h = hidden_paged(model, tokens, step, cache, max_new, whole_prompts)
+    last = (step.cu_seqlens[1:].long() - 1).clamp(0, max(tokens.shape[0] - 1, 0))
+    return model._logits(model.norm(h.index_select(0, last)))
+
+
+def hidden_paged(model, tokens: torch.Tensor, step: PagedStep, cache: PagedKVCache, max_new: int,
+                 whole_prompts: bool = False) -> torch.Tensor:
+    """The blocks' outputs [tokens, dim], before the last norm: forward_paged without its logits."""
     if tokens.dim() != 1 or tokens.shape[0] == 0:
         raise ValueError(f"forward_paged: a step has at least one token, tokens [T]; got {list(tokens.shape)}")
     cos, sin = rope_tables(model)
@@ -179,13 +292,18 @@ def forward_paged(model, tokens: torch.Tensor, step: PagedStep, cache: PagedKVCa
         q = att.wq(x).view(T, att.n_local_heads, att.head_dim)
         k = att.wk(x).view(T, att.n_local_kv_heads, att.head_dim)
         v = att.wv(x).view(T, att.n_local_kv_heads, att.head_dim)
-        q, k = rope_paged_write(q, k, v, cos, sin, step.positions, step.slots, cache.k[i], cache.v[i], q_out=q,
-                                k_out=k if whole_prompts else None, need_k=whole_prompts)
+        if cache.bits == 4:
+            q, k, v = rope_paged_write_int4(q, k, v, cos, sin, step.positions, step.slots, cache.k[i], cache.v[i], q_out=q,
+                                            k_out=k if whole_prompts else None, v_out=v if whole_prompts else None,
+                                            need_kv=whole_prompts)
+        else:
+            q, k = rope_paged_write(q, k, v, cos, sin, step.positions, step.slots, cache.k[i], cache.v[i], q_out=q,
+                                    k_out=k if whole_prompts else None, need_k=whole_prompts)
         if whole_prompts:
             o = prompt_attention(q, k, v, step.cu_seqlens, max_new)
         else:
-            o = paged_attention(q, cache.k[i], cache.v[i], cache.block_tables, step.kv_lens, step.cu_seqlens, max_new)
+            attention = paged_attention_int4 if cache.bits == 4 else paged_attention
+            o = attention(q, cache.k[i], cache.v[i], cache.block_tables, step.kv_lens, step.cu_seqlens, max_new)
         h = h + att._reduce(att.wo(o.view(T, -1)))
         h = h + layer.feed_forward(layer.ffn_norm(h))
-    last = (step.cu_seqlens[1:].long() - 1).clamp(0, max(T - 1, 0))
-    return model._logits(model.norm(h.index_select(0, last)))
+    return h
