@@ -1056,21 +1056,17 @@ static int run_attention(const li4_attention* p, bool paged, const Int4Pages* in
     a.k4 = *int4->k;
     a.v4 = *int4->v;
     a.wide_params = wide_params(*int4->k, a.hd) && wide_params(*int4->v, a.hd);
-    a.small_rows = 0;
-    a.big_rows = 0x7fffffff;
-    rc = launch_seq_attention_int4(a, p->dtype, rows, st);
-    if (rc == LI4_OK) clear_error();
-    return rc;
   }
   if (!tiles || both) {
     a.small_rows = 0;
     a.big_rows = both ? kFewRowsBeside : 0x7fffffff;
-    rc = launch_seq_attention(a, paged, p->dtype, both ? kFewRowsBeside : rows, st);
+    const int most = both ? kFewRowsBeside : rows;
+    rc = int4 ? launch_seq_attention_int4(a, p->dtype, most, st) : launch_seq_attention(a, paged, p->dtype, most, st);
   }
   if (rc == LI4_OK && tiles) {
     a.small_rows = both ? kFewRowsBeside : 0;
     a.big_rows = 0x7fffffff;
-    rc = launch_tile_attention(a, paged, p->dtype, st);
+    rc = int4 ? launch_tile_attention_int4(a, p->dtype, st) : launch_tile_attention(a, paged, p->dtype, st);
   }
   if (rc == LI4_OK) clear_error();
   return rc;

@@ -13,6 +13,7 @@
 //   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a row (tensor-memory lane) and needs no exchange;
 //                   writes P in the 16-bit type
 //   warp 10         the CTA's next item, when the present one nears its end
+// Over a cache in 4 bits warps 8 and 11 unpack half of each key and value tile into its slot instead (unpack_tiles).
 //
 // Prompts of 8192 tokens (32 / 8 heads, fp16), 128 dims: 463 us in a burst (1.19 PFLOP/s, 0.72 of cuBLAS's burst rate);
 // call after call for seconds 530 us (1.04 PFLOP/s, 0.75 of its sustained rate), as the power limit brings the clock to
@@ -43,6 +44,7 @@
 
 #include "li4_attention_args.cuh"
 #include "li4_gemv_device.cuh"
+#include "li4_int4_pages.cuh"
 
 namespace li4 {
 
@@ -82,6 +84,13 @@ struct TileArgs {
   int box_rows;         // key rows of one copy
   unsigned wait_limit;  // polls of a wait
 };
+
+// Over a cache in 4 bits (Q4): k, v and box_rows are not used.
+struct Tile4Args : TileArgs {
+  li4_int4_pages k4, v4;
+};
+template <typename ArgsT>
+constexpr bool kTileInt4 = __is_same(ArgsT, Tile4Args);
 
 // ---- mbarriers, tensor memory ----
 // A converged warp waits for a phase, at most `limit` polls; a wait that runs out leaves limit = 1, which makes every later
@@ -410,11 +419,72 @@ __device__ __noinline__ void put_back(uint32_t o_at, const int* first, int last)
   tmem_st_wait();
 }
 
-template <typename T, int D, bool PAGED>
+// ---- a cache in 4 bits: half of a tile (64 rows) by a warp.  In its turn i a lane holds the group of 32 dims c = (lane & 1) +
+// 2 (i % SUB) of row lane / 2 + 16 (i / SUB): 8 neighbouring lanes then store to all eight 16-byte places of a swizzled row.
+template <int D>
+struct HalfTile4 {
+  static constexpr int SUB = D / 64, TURNS = 4 * SUB;
+  uint4 codes[TURNS];
+  uint32_t params[TURNS];
+};
+
+// The pages of the half tile's keys key0 + lane and key0 + 32 + lane; -1: past the end or outside the cache.
+struct Pages4 {
+  int at[2];
+};
+__device__ __forceinline__ Pages4 half_pages4(const SeqAttnArgs& a, const TileWork& w, int key0) {
+  Pages4 p;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int key = key0 + 32 * h + (threadIdx.x & 31);
+    int page = -1;
+    if (key < w.len) page = a.tables[(long long)w.b * a.table_stride + (key >> a.log_page)];
+    p.at[h] = (unsigned)page < (unsigned)a.num_pages ? page : -1;
+  }
+  return p;
+}
+
+// Turn i's loads; what does not exist reads as zero codes and parameters, which make zeros.
+template <int D>
+__device__ __forceinline__ void load_turn4(HalfTile4<D>& h, int i, const SeqAttnArgs& a, const li4_int4_pages& pages, const Pages4& p,
+                                           int kvh, int key0) {
+  constexpr int SUB = HalfTile4<D>::SUB;
+  const int lane = threadIdx.x & 31, c = (lane & 1) + 2 * (i % SUB);
+  const int page = __shfl_sync(0xffffffffu, p.at[(i / SUB) >> 1], lane / 2 + 16 * ((i / SUB) & 1));
+  const int row = (key0 + lane / 2 + 16 * (i / SUB)) & ((1 << a.log_page) - 1);
+  h.codes[i] = make_uint4(0, 0, 0, 0);
+  h.params[i] = 0;
+  if (page >= 0 && c * kGroup4 < a.hd) {
+    h.codes[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pages.codes) + page * pages.stride_cp +
+                                                 row * pages.stride_ct + kvh * pages.stride_ch + c * 16);
+    h.params[i] = static_cast<const uint32_t*>(pages.params)[page * pages.stride_pp + row * pages.stride_pt +
+                                                             kvh * pages.stride_ph + c];
+  }
+}
+
+// Turn i's values to their places of the tile; row0: the half's first row.
+template <typename T, int D>
+__device__ __forceinline__ void store_turn4(const HalfTile4<D>& h, int i, uint8_t* tile, int row0) {
+  constexpr int SUB = HalfTile4<D>::SUB;
+  const int lane = threadIdx.x & 31, r = row0 + lane / 2 + 16 * (i / SUB);
+  uint8_t* at = tile + (i % SUB) * (tile_bytes(D) / SUB) + r * 128;
+  const uint32_t s2 = both_low(h.params[i]), m2 = both_high(h.params[i]);
+  const uint32_t w[4] = {h.codes[i].x, h.codes[i].y, h.codes[i].z, h.codes[i].w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t u[4];
+    values8<T>(w[e], s2, m2, u);
+    *reinterpret_cast<uint4*>(at + (((4 * (lane & 1) + e) ^ (r & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+
+template <typename T, int D, bool PAGED, typename ArgsT>
 __global__ void __launch_bounds__(kTileThreads, 1)
-    tile_attention_kernel(const __grid_constant__ TileArgs a, const __grid_constant__ CUtensorMap map_q,
+    tile_attention_kernel(const __grid_constant__ ArgsT a, const __grid_constant__ CUtensorMap map_q,
                           const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   constexpr int NS = tile_slots(D), TB = tile_bytes(D), SUB = D / 64;
+  constexpr bool Q4 = kTileInt4<ArgsT>;
+  constexpr int kUnpackWarp = kTmaWarp + 3;  // Q4: the second half of each tile
   constexpr int TYPE = __is_same(T, __half) ? 0 : 1;
   // Tensor-memory columns: S_i at 128 i, O_i at 256 + D i.  At 64 dims there is room for P_i beside them (64 columns
   // each), so S_i of the next step is computed as soon as the softmax has read the last one; at 128 dims P_i lies in
@@ -440,18 +510,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* replied = work_empty + 2;    // the reply is there
   uint64_t* ending = replied + 1;        // the products are near the item's end
   uint64_t* taken_out = ending + 1;      // [2] an item's infinities and NaNs are noted (items taken with care alone)
-  TileWork* work = reinterpret_cast<TileWork*>(taken_out + 2);  // [2]
+  uint64_t* noted = taken_out + 2;       // Q4: the notes of an item taken with care are clear
+  TileWork* work = reinterpret_cast<TileWork*>(noted + 1);  // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(work + 2);
   volatile int* again = reinterpret_cast<int*>(tmem_holder + 1);  // [2] by item parity: one to run again
   volatile int* gave_up = again + 2;             // [2] a wait of the usual pass, of the one with care ran out
   int* first_bad = const_cast<int*>(again) + 4;  // [2][2][D] of items taken with care: see take_out
-  static_assert(16 + (2 * NS + 22) * 8 + 2 * sizeof(TileWork) + 20 <= 512, "what lies behind the tiles fits");
+  static_assert(16 + (2 * NS + 23) * 8 + 2 * sizeof(TileWork) + 20 <= 512, "what lies behind the tiles fits");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_full[i], Q4 ? 2 : 1);
       mbar_init(&kv_empty[i], 1);
     }
     mbar_init(q_full, 1);
@@ -463,14 +534,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&o_done[i], 1);
       mbar_init(&s_free[i], 4);
       mbar_init(&work_full[i], 1);
-      mbar_init(&work_empty[i], 10);
+      mbar_init(&work_empty[i], Q4 ? 11 : 10);
     }
     mbar_init(v_tail, 1);
     mbar_init(drained, 1);
     mbar_init(replied, 1);
     mbar_init(ending, 1);
-    mbar_init(&taken_out[0], 1);
-    mbar_init(&taken_out[1], 1);
+    mbar_init(&taken_out[0], Q4 ? 2 : 1);
+    mbar_init(&taken_out[1], Q4 ? 2 : 1);
+    if (Q4) mbar_init(noted, 1);
     again[0] = again[1] = gave_up[0] = gave_up[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -525,7 +597,98 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   // (2 x 128 x 208 + 128 x 80 <= 384 x 168)
   if (warp >= kTmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == kTmaWarp) {
+    if (Q4 && (warp == kTmaWarp || warp == kUnpackWarp)) {
+      // ---- queries (warp 8), and this warp's half of the key and value tiles unpacked into their slots
+      if constexpr (Q4) {
+        const int half = warp == kTmaWarp ? 0 : 1;
+        int k = 0;
+        unsigned base = 0, qn = 0;
+        for (bool care = false;; care = true) {
+          unsigned cares = 0;
+          for (;;) {
+            const TileWork w = next_work(k++);
+            if (w.b < 0) break;
+            const int nk = max(w.steps[0], w.steps[1]);
+            if (nk == 0) continue;
+            const int at0 = w.first * kTileKeys + half * (kTileKeys / 2);  // the half's first key of key tile 0
+            Pages4 next = half_pages4(a.s, w, at0), now = next, last = next;
+            HalfTile4<D> h;
+#pragma unroll
+            for (int i = 0; i < HalfTile4<D>::TURNS; ++i) load_turn4<D>(h, i, a.s, a.k4, next, w.kvh, at0);
+            if (nk > 1) next = half_pages4(a.s, w, at0 + kTileKeys);
+            if (half == 0) {
+              if (qn > 0) tile_wait(q_empty, (qn - 1) & 1, limit);
+              if (lane == 0 && limit != 1) {
+                const int lo = w.steps[0] > 0 ? 0 : 1, hi = w.steps[1] > 0 ? 2 : 1;
+                mbar_arrive_expect_tx(q_full, (hi - lo) * SUB * TPT * a.s.rep * 128);
+                for (int i = lo; i < hi; ++i)
+                  for (int c = 0; c < SUB; ++c)
+                    tma_load4(smem_addr(smem + i * TB + c * (TB / SUB)), &map_q, q_full, c * 64, 0, w.kvh,
+                              w.start + w.tok0 + i * TPT);
+              }
+              ++qn;
+            }
+            const int care_from = care ? masked_from(w) : nk;
+            int* bad = first_bad + (cares & 1) * 2 * D;
+            if (care && half == 0) {
+              for (int e = lane; e < 2 * D; e += 32) bad[e] = kUnseen;
+              __syncwarp();
+              if (lane == 0) mbar_arrive(noted);
+            } else if (care) {
+              tile_wait(noted, cares & 1, limit);
+            }
+            auto value_at_turn = [&](int n) { return !EARLY ? (n & 1) != 0 : n == 2 * nk - 1 || (n > 0 && !(n & 1)); };
+            auto tile_at_turn = [&](int n) {
+              return !EARLY ? n / 2 : n == 2 * nk - 1 ? nk - 1 : value_at_turn(n) ? n / 2 - 1 : (n + 1) / 2;
+            };
+#pragma unroll 1
+            for (int n = 0; n < 2 * nk; ++n) {
+              const unsigned g = base + n, slot = g % NS;
+              // the next tile: a key tile takes the pages asked for a tile ahead, a value tile those of its keys
+              const bool more = n + 1 < 2 * nk, next_value = more && value_at_turn(n + 1);
+              const int j1 = more ? tile_at_turn(n + 1) : 0;
+              if (more && !next_value) {
+                last = now;
+                now = next;
+                if (j1 + 1 < nk) next = half_pages4(a.s, w, at0 + (j1 + 1) * kTileKeys);
+              }
+              const Pages4 pages = next_value && EARLY && j1 < nk - 1 ? last : now;
+              if (g >= NS) tile_wait(&kv_empty[slot], ((g / NS) - 1) & 1, limit);
+              if (ran_out()) continue;
+              uint8_t* tile = ring + slot * TB;
+#pragma unroll
+              for (int i = 0; i < HalfTile4<D>::TURNS; ++i) {
+                store_turn4<T, D>(h, i, tile, half * (kTileKeys / 2));
+                if (more) load_turn4<D>(h, i, a.s, next_value ? a.v4 : a.k4, pages, w.kvh, at0 + j1 * kTileKeys);
+              }
+              const int j = tile_at_turn(n);
+              if (value_at_turn(n) && j >= care_from) {
+                __syncwarp();
+                take_out<T, D>(tile, half * (kTileKeys / 2), (half + 1) * (kTileKeys / 2), (w.first + j) * kTileKeys, bad);
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&kv_full[slot]);
+            }
+            if (care) {
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&taken_out[cares & 1]);
+              ++cares;
+            }
+            base += 2 * nk;
+          }
+          if (ran_out() && qn > 0) {  // the queries' copies land before the memory goes
+            unsigned more = kTileWaitLimit;
+            tile_wait(q_full, (qn - 1) & 1, more);
+          }
+          if (care) {
+            end_care();
+            break;
+          }
+          if (!go_again()) break;
+        }
+      }
+    } else if (warp == kTmaWarp) {
       // ---- copies
       int k = 0;
       unsigned base = 0, issued = 0, qn = 0, tails = 0;  // ring tiles of earlier items, all issued; queries; mended tiles
@@ -1019,8 +1182,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 }
 
 // Joins the ranges of keys of an item, 32 of its rows per CTA; returns at once where the launch did not split.
-template <typename T, int D, bool PAGED>
-__global__ void __launch_bounds__(256) tile_join_kernel(const __grid_constant__ TileArgs a) {
+template <typename T, int D, bool PAGED, typename ArgsT>
+__global__ void __launch_bounds__(256) tile_join_kernel(const __grid_constant__ ArgsT a) {
   __shared__ TileWork s_work;
   __shared__ int s_splits;
   pdl_launch_dependents();
@@ -1117,8 +1280,8 @@ static int make_map(CUtensorMap* map, int dtype, const void* base, int64_t d, in
   return LI4_OK;
 }
 
-template <typename T, int D, bool PAGED>
-static int launch_tile(const TileArgs& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+template <typename T, int D, bool PAGED, typename ArgsT>
+static int launch_tile(const ArgsT& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                        unsigned grid, cudaStream_t stream) {
   static std::mutex mu;
   static std::vector<int> done_dev;  // of this kernel
@@ -1129,7 +1292,7 @@ static int launch_tile(const TileArgs& a, const CUtensorMap& q, const CUtensorMa
     bool seen = false;
     for (int d : done_dev) seen |= (d == dev);
     if (!seen) {
-      const int rc = check_cuda(cudaFuncSetAttribute(tile_attention_kernel<T, D, PAGED>,
+      const int rc = check_cuda(cudaFuncSetAttribute(tile_attention_kernel<T, D, PAGED, ArgsT>,
                                                      cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem_bytes(D)),
                                 "attention: shared memory limit");
       if (rc != LI4_OK) return rc;
@@ -1146,13 +1309,13 @@ static int launch_tile(const TileArgs& a, const CUtensorMap& q, const CUtensorMa
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  int rc = check_cuda(cudaLaunchKernelEx(&cfg, tile_attention_kernel<T, D, PAGED>, a, q, k, v),
+  int rc = check_cuda(cudaLaunchKernelEx(&cfg, tile_attention_kernel<T, D, PAGED, ArgsT>, a, q, k, v),
                       "attention: kernel launch");
   if (rc != LI4_OK || a.part_slots == 0) return rc;
   cfg.gridDim = dim3((unsigned)a.part_slots / 2, 2 * kTileRows / 32, 1);  // (a split item has two parts at least)
   cfg.blockDim = dim3(256, 1, 1);
   cfg.dynamicSmemBytes = 0;
-  return check_cuda(cudaLaunchKernelEx(&cfg, tile_join_kernel<T, D, PAGED>, a), "attention: kernel launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, tile_join_kernel<T, D, PAGED, ArgsT>, a), "attention: kernel launch");
 }
 
 // Items whose partial results the workspace has room for: one per SM, where the pairs of tiles that the tokens alone
@@ -1174,31 +1337,40 @@ int tile_set_wait_limit(unsigned polls) {
   return LI4_OK;
 }
 
-int launch_tile_attention(const SeqAttnArgs& args, bool paged, int dtype, cudaStream_t stream) {
-  TileArgs a;
-  a.s = args;
-  const int rep = args.rep, page = 1 << args.log_page;
+// What both launches share: queries' map, work limits; the grid, or 0 and a status.
+static int plan_tiles(TileArgs& a, bool paged, int dtype, CUtensorMap* q, unsigned* grid_out) {
+  const SeqAttnArgs& args = a.s;
+  const int rep = args.rep;
   a.tokens_per_tile = kTileRows / rep;
-  a.box_rows = paged ? (page < kTileKeys ? page : kTileKeys) : kTileKeys;
-  CUtensorMap q, k, v;
   // queries [token][KV head][head of the group][d]: a box is the rep rows of tokens_per_tile tokens
-  int rc = make_map(&q, dtype, args.q, args.hd, rep, args.sqh, args.Hkv, args.sqh * rep, args.T, args.sqt, rep,
-                    a.tokens_per_tile);
-  const int64_t y = paged ? page : args.T, w = paged ? args.num_pages : 1;
-  if (rc == LI4_OK)
-    rc = make_map(&k, dtype, args.k, args.hd, y, args.skt, args.Hkv, args.skh, w, args.skp, a.box_rows, 1);
-  if (rc == LI4_OK)
-    rc = make_map(&v, dtype, args.v, args.hd, y, args.svt, args.Hkv, args.svh, w, args.svp, a.box_rows, 1);
+  const int rc = make_map(q, dtype, args.q, args.hd, rep, args.sqh, args.Hkv, args.sqh * rep, args.T, args.sqt, rep,
+                          a.tokens_per_tile);
   if (rc != LI4_OK) return rc;
-  const int sm = current_sm_count();
-  a.part_slots = tile_part_slots(rep, args.T, args.Hkv, args.max_keys, sm);
+  a.part_slots = tile_part_slots(rep, args.T, args.Hkv, args.max_keys, current_sm_count());
   const unsigned polls = g_tile_wait_polls.load();
   a.wait_limit = polls != 0 ? polls : kTileWaitLimit + kTileWaitStep * (unsigned)((paged ? args.max_keys : args.T) / kTileKeys);
   const int64_t pairs = args.T / (2 * a.tokens_per_tile) + args.B;  // at least the sequences' pairs of tiles
   int64_t grid = pairs * args.Hkv;
   if (grid < a.part_slots) grid = a.part_slots;
   if (grid > 0x7fffffff) return set_error(LI4_ERR_UNSUPPORTED, "attention: too many items");
-  const unsigned g = (unsigned)grid;
+  *grid_out = (unsigned)grid;
+  return LI4_OK;
+}
+
+int launch_tile_attention(const SeqAttnArgs& args, bool paged, int dtype, cudaStream_t stream) {
+  TileArgs a;
+  a.s = args;
+  const int page = 1 << args.log_page;
+  a.box_rows = paged ? (page < kTileKeys ? page : kTileKeys) : kTileKeys;
+  CUtensorMap q, k, v;
+  unsigned g = 0;
+  int rc = plan_tiles(a, paged, dtype, &q, &g);
+  const int64_t y = paged ? page : args.T, w = paged ? args.num_pages : 1;
+  if (rc == LI4_OK)
+    rc = make_map(&k, dtype, args.k, args.hd, y, args.skt, args.Hkv, args.skh, w, args.skp, a.box_rows, 1);
+  if (rc == LI4_OK)
+    rc = make_map(&v, dtype, args.v, args.hd, y, args.svt, args.Hkv, args.svh, w, args.svp, a.box_rows, 1);
+  if (rc != LI4_OK) return rc;
   const bool half = dtype == LI4_F16;
   if (args.hd <= 64) {
     if (paged) return half ? launch_tile<__half, 64, true>(a, q, k, v, g, stream) : launch_tile<__nv_bfloat16, 64, true>(a, q, k, v, g, stream);
@@ -1206,6 +1378,22 @@ int launch_tile_attention(const SeqAttnArgs& args, bool paged, int dtype, cudaSt
   }
   if (paged) return half ? launch_tile<__half, 128, true>(a, q, k, v, g, stream) : launch_tile<__nv_bfloat16, 128, true>(a, q, k, v, g, stream);
   return half ? launch_tile<__half, 128, false>(a, q, k, v, g, stream) : launch_tile<__nv_bfloat16, 128, false>(a, q, k, v, g, stream);
+}
+
+int launch_tile_attention_int4(const Seq4Args& args, int dtype, cudaStream_t stream) {
+  Tile4Args a;
+  a.s = args;
+  a.box_rows = 0;
+  a.k4 = args.k4;
+  a.v4 = args.v4;
+  CUtensorMap q;
+  unsigned g = 0;
+  const int rc = plan_tiles(a, true, dtype, &q, &g);
+  if (rc != LI4_OK) return rc;
+  const bool half = dtype == LI4_F16;  // (no maps of keys and values: the queries' stands in their places)
+  if (args.hd <= 64)
+    return half ? launch_tile<__half, 64, true>(a, q, q, q, g, stream) : launch_tile<__nv_bfloat16, 64, true>(a, q, q, q, g, stream);
+  return half ? launch_tile<__half, 128, true>(a, q, q, q, g, stream) : launch_tile<__nv_bfloat16, 128, true>(a, q, q, q, g, stream);
 }
 
 }  // namespace li4
