@@ -13,7 +13,8 @@
 //   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a row (tensor-memory lane) and needs no exchange;
 //                   writes P in the 16-bit type
 //   warp 10         the CTA's next item, when the present one nears its end
-// Over a cache in 4 bits warps 8 and 11 unpack half of each key and value tile into its slot instead (unpack_tiles).
+// Over a cache in 4 bits a fourth group of warps, 12 to 15, unpacks a quarter each of every key and value tile into its
+// slot instead; warp 8 copies the queries alone.
 //
 // Prompts of 8192 tokens (32 / 8 heads, fp16), 128 dims: 463 us in a burst (1.19 PFLOP/s, 0.72 of cuBLAS's burst rate);
 // call after call for seconds 530 us (1.04 PFLOP/s, 0.75 of its sustained rate), as the power limit brings the clock to
@@ -62,7 +63,8 @@ int tile_device_errors(unsigned* flags, bool reset) {
 constexpr int kTileRows = 128;       // rows of a tile: tensor-memory lanes
 constexpr int kTileKeys = 128;       // keys of a step
 constexpr int kTileThreads = 384;    // 8 softmax warps, the TMA, MMA and item warps, one that only fills its group
-constexpr int kTmaWarp = 8, kMmaWarp = 9;
+constexpr int kTmaWarp = 8, kMmaWarp = 9, kUnpackWarp = 12;
+constexpr int kTile4Threads = 512;   // over a cache in 4 bits: and 4 unpacking warps
 constexpr unsigned kTileWaitLimit = 1u << 24;  // polls, about half a second; and for each key tile that an item may have,
 constexpr unsigned kTileWaitStep = 1u << 8;    // as some waits last an item (a step of 2900 cycles is some 60 polls)
 constexpr int kTileMinSteps = 8;     // key tiles below which a range is not cut
@@ -419,38 +421,31 @@ __device__ __noinline__ void put_back(uint32_t o_at, const int* first, int last)
   tmem_st_wait();
 }
 
-// ---- a cache in 4 bits: half of a tile (64 rows) by a warp.  In its turn i a lane holds the group of 32 dims c = (lane & 1) +
-// 2 (i % SUB) of row lane / 2 + 16 (i / SUB): 8 neighbouring lanes then store to all eight 16-byte places of a swizzled row.
+// ---- a cache in 4 bits: a quarter of a tile (32 rows) by a warp.  In its turn i a lane holds the group of 32 dims c =
+// (lane & 1) + 2 (i % SUB) of row lane / 2 + 16 (i / SUB): 8 neighbouring lanes then store to all eight 16-byte places of
+// swizzled rows.
 template <int D>
-struct HalfTile4 {
-  static constexpr int SUB = D / 64, TURNS = 4 * SUB;
+struct Quarter4 {
+  static constexpr int SUB = D / 64, TURNS = 2 * SUB;
   uint4 codes[TURNS];
   uint32_t params[TURNS];
 };
 
-// The pages of the half tile's keys key0 + lane and key0 + 32 + lane; -1: past the end or outside the cache.
-struct Pages4 {
-  int at[2];
-};
-__device__ __forceinline__ Pages4 half_pages4(const SeqAttnArgs& a, const TileWork& w, int key0) {
-  Pages4 p;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int key = key0 + 32 * h + (threadIdx.x & 31);
-    int page = -1;
-    if (key < w.len) page = a.tables[(long long)w.b * a.table_stride + (key >> a.log_page)];
-    p.at[h] = (unsigned)page < (unsigned)a.num_pages ? page : -1;
-  }
-  return p;
+// The page of key key0 + lane; -1: past the end or outside the cache.
+__device__ __forceinline__ int quarter_page4(const SeqAttnArgs& a, const TileWork& w, int key0) {
+  const int key = key0 + (threadIdx.x & 31);
+  int page = -1;
+  if (key < w.len) page = a.tables[(long long)w.b * a.table_stride + (key >> a.log_page)];
+  return (unsigned)page < (unsigned)a.num_pages ? page : -1;
 }
 
 // Turn i's loads; what does not exist reads as zero codes and parameters, which make zeros.
 template <int D>
-__device__ __forceinline__ void load_turn4(HalfTile4<D>& h, int i, const SeqAttnArgs& a, const li4_int4_pages& pages, const Pages4& p,
+__device__ __forceinline__ void load_turn4(Quarter4<D>& h, int i, const SeqAttnArgs& a, const li4_int4_pages& pages, int my_page,
                                            int kvh, int key0) {
-  constexpr int SUB = HalfTile4<D>::SUB;
+  constexpr int SUB = Quarter4<D>::SUB;
   const int lane = threadIdx.x & 31, c = (lane & 1) + 2 * (i % SUB);
-  const int page = __shfl_sync(0xffffffffu, p.at[(i / SUB) >> 1], lane / 2 + 16 * ((i / SUB) & 1));
+  const int page = __shfl_sync(0xffffffffu, my_page, lane / 2 + 16 * (i / SUB));
   const int row = (key0 + lane / 2 + 16 * (i / SUB)) & ((1 << a.log_page) - 1);
   h.codes[i] = make_uint4(0, 0, 0, 0);
   h.params[i] = 0;
@@ -462,10 +457,10 @@ __device__ __forceinline__ void load_turn4(HalfTile4<D>& h, int i, const SeqAttn
   }
 }
 
-// Turn i's values to their places of the tile; row0: the half's first row.
+// Turn i's values to their places of the tile; row0: the quarter's first row.
 template <typename T, int D>
-__device__ __forceinline__ void store_turn4(const HalfTile4<D>& h, int i, uint8_t* tile, int row0) {
-  constexpr int SUB = HalfTile4<D>::SUB;
+__device__ __forceinline__ void store_turn4(const Quarter4<D>& h, int i, uint8_t* tile, int row0) {
+  constexpr int SUB = Quarter4<D>::SUB;
   const int lane = threadIdx.x & 31, r = row0 + lane / 2 + 16 * (i / SUB);
   uint8_t* at = tile + (i % SUB) * (tile_bytes(D) / SUB) + r * 128;
   const uint32_t s2 = both_low(h.params[i]), m2 = both_high(h.params[i]);
@@ -479,12 +474,11 @@ __device__ __forceinline__ void store_turn4(const HalfTile4<D>& h, int i, uint8_
 }
 
 template <typename T, int D, bool PAGED, typename ArgsT>
-__global__ void __launch_bounds__(kTileThreads, 1)
+__global__ void __launch_bounds__(kTileInt4<ArgsT> ? kTile4Threads : kTileThreads, 1)
     tile_attention_kernel(const __grid_constant__ ArgsT a, const __grid_constant__ CUtensorMap map_q,
                           const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   constexpr int NS = tile_slots(D), TB = tile_bytes(D), SUB = D / 64;
   constexpr bool Q4 = kTileInt4<ArgsT>;
-  constexpr int kUnpackWarp = kTmaWarp + 3;  // Q4: the second half of each tile
   constexpr int TYPE = __is_same(T, __half) ? 0 : 1;
   // Tensor-memory columns: S_i at 128 i, O_i at 256 + D i.  At 64 dims there is room for P_i beside them (64 columns
   // each), so S_i of the next step is computed as soon as the softmax has read the last one; at 128 dims P_i lies in
@@ -506,23 +500,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* v_tail = s_free + 2;         // the last value tile's rows are there, its missing rows not yet zeros
   uint64_t* drained = v_tail + 1;        // a wait ran out: the MMAs issued so far have finished
   uint64_t* work_full = drained + 1;     // [2] work[i] names an item
-  uint64_t* work_empty = work_full + 2;  // [2] the 10 working warps have read it
+  uint64_t* work_empty = work_full + 2;  // [2] the working warps have read it (Q4: 14 of them)
   uint64_t* replied = work_empty + 2;    // the reply is there
   uint64_t* ending = replied + 1;        // the products are near the item's end
   uint64_t* taken_out = ending + 1;      // [2] an item's infinities and NaNs are noted (items taken with care alone)
   uint64_t* noted = taken_out + 2;       // Q4: the notes of an item taken with care are clear
-  TileWork* work = reinterpret_cast<TileWork*>(noted + 1);  // [2]
+  uint64_t* notes_read = noted + 1;      // [2] the 8 softmax warps have read an item's notes
+  TileWork* work = reinterpret_cast<TileWork*>(notes_read + 2);  // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(work + 2);
   volatile int* again = reinterpret_cast<int*>(tmem_holder + 1);  // [2] by item parity: one to run again
   volatile int* gave_up = again + 2;             // [2] a wait of the usual pass, of the one with care ran out
   int* first_bad = const_cast<int*>(again) + 4;  // [2][2][D] of items taken with care: see take_out
-  static_assert(16 + (2 * NS + 23) * 8 + 2 * sizeof(TileWork) + 20 <= 512, "what lies behind the tiles fits");
+  static_assert(16 + (2 * NS + 25) * 8 + 2 * sizeof(TileWork) + 20 <= 512, "what lies behind the tiles fits");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&kv_full[i], Q4 ? 2 : 1);
+      mbar_init(&kv_full[i], Q4 ? 4 : 1);
       mbar_init(&kv_empty[i], 1);
     }
     mbar_init(q_full, 1);
@@ -534,15 +529,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&o_done[i], 1);
       mbar_init(&s_free[i], 4);
       mbar_init(&work_full[i], 1);
-      mbar_init(&work_empty[i], Q4 ? 11 : 10);
+      mbar_init(&work_empty[i], Q4 ? 14 : 10);
     }
     mbar_init(v_tail, 1);
     mbar_init(drained, 1);
     mbar_init(replied, 1);
     mbar_init(ending, 1);
-    mbar_init(&taken_out[0], Q4 ? 2 : 1);
-    mbar_init(&taken_out[1], Q4 ? 2 : 1);
+    mbar_init(&taken_out[0], Q4 ? 4 : 1);
+    mbar_init(&taken_out[1], Q4 ? 4 : 1);
     if (Q4) mbar_init(noted, 1);
+    mbar_init(&notes_read[0], 8);
+    mbar_init(&notes_read[1], 8);
     again[0] = again[1] = gave_up[0] = gave_up[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -595,98 +592,115 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   // 384 threads x 168 registers at the launch: the softmax's two groups take 208 each, the third keeps 80
   // (2 x 128 x 208 + 128 x 80 <= 384 x 168)
-  if (warp >= kTmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (Q4 && (warp == kTmaWarp || warp == kUnpackWarp)) {
-      // ---- queries (warp 8), and this warp's half of the key and value tiles unpacked into their slots
-      if constexpr (Q4) {
-        const int half = warp == kTmaWarp ? 0 : 1;
-        int k = 0;
-        unsigned base = 0, qn = 0;
-        for (bool care = false;; care = true) {
-          unsigned cares = 0;
-          for (;;) {
-            const TileWork w = next_work(k++);
-            if (w.b < 0) break;
-            const int nk = max(w.steps[0], w.steps[1]);
-            if (nk == 0) continue;
-            const int at0 = w.first * kTileKeys + half * (kTileKeys / 2);  // the half's first key of key tile 0
-            Pages4 next = half_pages4(a.s, w, at0), now = next, last = next;
-            HalfTile4<D> h;
+  // Q4: 512 threads x 128, 200 each for the softmax, 48 for the third group, 64 for the unpacking warps
+  // (2 x 128 x 200 + 128 x 48 + 128 x 64 = 512 x 128)
+  if (Q4 && warp >= kUnpackWarp) {
+    if constexpr (Q4) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+      // ---- this warp's quarter of the key and value tiles
+      const int row0 = (warp - kUnpackWarp) * (kTileKeys / 4);
+      int k = 0;
+      unsigned base = 0;
+      for (bool care = false;; care = true) {
+        unsigned cares = 0;
+        for (;;) {
+          const TileWork w = next_work(k++);
+          if (w.b < 0) break;
+          const int nk = max(w.steps[0], w.steps[1]);
+          if (nk == 0) continue;
+          const int at0 = w.first * kTileKeys + row0;  // the quarter's first key of key tile 0
+          int next = quarter_page4(a.s, w, at0), now = next, last = next;  // pages of the key tile ahead, of this, of the one before
+          Quarter4<D> h;
 #pragma unroll
-            for (int i = 0; i < HalfTile4<D>::TURNS; ++i) load_turn4<D>(h, i, a.s, a.k4, next, w.kvh, at0);
-            if (nk > 1) next = half_pages4(a.s, w, at0 + kTileKeys);
-            if (half == 0) {
-              if (qn > 0) tile_wait(q_empty, (qn - 1) & 1, limit);
-              if (lane == 0 && limit != 1) {
-                const int lo = w.steps[0] > 0 ? 0 : 1, hi = w.steps[1] > 0 ? 2 : 1;
-                mbar_arrive_expect_tx(q_full, (hi - lo) * SUB * TPT * a.s.rep * 128);
-                for (int i = lo; i < hi; ++i)
-                  for (int c = 0; c < SUB; ++c)
-                    tma_load4(smem_addr(smem + i * TB + c * (TB / SUB)), &map_q, q_full, c * 64, 0, w.kvh,
-                              w.start + w.tok0 + i * TPT);
-              }
-              ++qn;
-            }
-            const int care_from = care ? masked_from(w) : nk;
-            int* bad = first_bad + (cares & 1) * 2 * D;
-            if (care && half == 0) {
-              for (int e = lane; e < 2 * D; e += 32) bad[e] = kUnseen;
-              __syncwarp();
-              if (lane == 0) mbar_arrive(noted);
-            } else if (care) {
-              tile_wait(noted, cares & 1, limit);
-            }
-            auto value_at_turn = [&](int n) { return !EARLY ? (n & 1) != 0 : n == 2 * nk - 1 || (n > 0 && !(n & 1)); };
-            auto tile_at_turn = [&](int n) {
-              return !EARLY ? n / 2 : n == 2 * nk - 1 ? nk - 1 : value_at_turn(n) ? n / 2 - 1 : (n + 1) / 2;
-            };
+          for (int i = 0; i < Quarter4<D>::TURNS; ++i) load_turn4<D>(h, i, a.s, a.k4, next, w.kvh, at0);
+          if (nk > 1) next = quarter_page4(a.s, w, at0 + kTileKeys);
+          const int care_from = care ? masked_from(w) : nk;
+          int* bad = first_bad + (cares & 1) * 2 * D;
+          if (care) tile_wait(noted, cares & 1, limit);
+          auto is_value = [&](int n) { return !EARLY ? (n & 1) != 0 : n == 2 * nk - 1 || (n > 0 && !(n & 1)); };
+          auto tile_of = [&](int n) { return !EARLY ? n / 2 : n == 2 * nk - 1 ? nk - 1 : is_value(n) ? n / 2 - 1 : (n + 1) / 2; };
 #pragma unroll 1
-            for (int n = 0; n < 2 * nk; ++n) {
-              const unsigned g = base + n, slot = g % NS;
-              // the next tile: a key tile takes the pages asked for a tile ahead, a value tile those of its keys
-              const bool more = n + 1 < 2 * nk, next_value = more && value_at_turn(n + 1);
-              const int j1 = more ? tile_at_turn(n + 1) : 0;
-              if (more && !next_value) {
-                last = now;
-                now = next;
-                if (j1 + 1 < nk) next = half_pages4(a.s, w, at0 + (j1 + 1) * kTileKeys);
-              }
-              const Pages4 pages = next_value && EARLY && j1 < nk - 1 ? last : now;
-              if (g >= NS) tile_wait(&kv_empty[slot], ((g / NS) - 1) & 1, limit);
-              if (ran_out()) continue;
-              uint8_t* tile = ring + slot * TB;
+          for (int n = 0; n < 2 * nk; ++n) {
+            const unsigned g = base + n, slot = g % NS;
+            // the next tile: a key tile takes the pages asked for a tile ahead, a value tile those of its keys
+            const bool more = n + 1 < 2 * nk, next_value = more && is_value(n + 1);
+            const int j1 = more ? tile_of(n + 1) : 0;
+            if (more && !next_value) {
+              last = now;
+              now = next;
+              if (j1 + 1 < nk) next = quarter_page4(a.s, w, at0 + (j1 + 1) * kTileKeys);
+            }
+            const int page = next_value && EARLY && j1 < nk - 1 ? last : now;
+            if (g >= NS) tile_wait(&kv_empty[slot], ((g / NS) - 1) & 1, limit);
+            if (ran_out()) continue;
+            uint8_t* tile = ring + slot * TB;
 #pragma unroll
-              for (int i = 0; i < HalfTile4<D>::TURNS; ++i) {
-                store_turn4<T, D>(h, i, tile, half * (kTileKeys / 2));
-                if (more) load_turn4<D>(h, i, a.s, next_value ? a.v4 : a.k4, pages, w.kvh, at0 + j1 * kTileKeys);
-              }
-              const int j = tile_at_turn(n);
-              if (value_at_turn(n) && j >= care_from) {
-                __syncwarp();
-                take_out<T, D>(tile, half * (kTileKeys / 2), (half + 1) * (kTileKeys / 2), (w.first + j) * kTileKeys, bad);
-              }
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&kv_full[slot]);
+            for (int i = 0; i < Quarter4<D>::TURNS; ++i) {
+              store_turn4<T, D>(h, i, tile, row0);
+              if (more) load_turn4<D>(h, i, a.s, next_value ? a.v4 : a.k4, page, w.kvh, at0 + j1 * kTileKeys);
             }
-            if (care) {
+            const int j = tile_of(n);
+            if (is_value(n) && j >= care_from) {
               __syncwarp();
-              if (lane == 0) mbar_arrive(&taken_out[cares & 1]);
-              ++cares;
+              take_out<T, D>(tile, row0, row0 + kTileKeys / 4, (w.first + j) * kTileKeys, bad);
             }
-            base += 2 * nk;
-          }
-          if (ran_out() && qn > 0) {  // the queries' copies land before the memory goes
-            unsigned more = kTileWaitLimit;
-            tile_wait(q_full, (qn - 1) & 1, more);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&kv_full[slot]);
           }
           if (care) {
-            end_care();
-            break;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&taken_out[cares & 1]);
+            ++cares;
           }
-          if (!go_again()) break;
+          base += 2 * nk;
         }
+        if (care) {
+          end_care();
+          break;
+        }
+        if (!go_again()) break;
+      }
+    }
+  } else if (warp >= kTmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q4 ? 48 : 80));
+    if (Q4 && warp == kTmaWarp) {
+      // ---- queries
+      int k = 0;
+      unsigned qn = 0;
+      for (bool care = false;; care = true) {
+        unsigned cares = 0;
+        for (;;) {
+          const TileWork w = next_work(k++);
+          if (w.b < 0) break;
+          if (max(w.steps[0], w.steps[1]) == 0) continue;
+          if (qn > 0) tile_wait(q_empty, (qn - 1) & 1, limit);
+          if (lane == 0 && limit != 1) {
+            const int lo = w.steps[0] > 0 ? 0 : 1, hi = w.steps[1] > 0 ? 2 : 1;
+            mbar_arrive_expect_tx(q_full, (hi - lo) * SUB * TPT * a.s.rep * 128);
+            for (int i = lo; i < hi; ++i)
+              for (int c = 0; c < SUB; ++c)
+                tma_load4(smem_addr(smem + i * TB + c * (TB / SUB)), &map_q, q_full, c * 64, 0, w.kvh,
+                          w.start + w.tok0 + i * TPT);
+          }
+          if (!ran_out()) ++qn;
+          if (care) {
+            if (cares > 1) tile_wait(&notes_read[cares & 1], ((cares >> 1) - 1) & 1, limit);
+            for (int e = lane; e < 2 * D; e += 32) first_bad[(cares & 1) * 2 * D + e] = kUnseen;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(noted);
+            ++cares;
+          }
+        }
+        if (ran_out() && qn > 0) {  // the copies land before the memory goes
+          unsigned more = kTileWaitLimit;
+          tile_wait(q_full, (qn - 1) & 1, more);
+        }
+        if (care) {
+          end_care();
+          break;
+        }
+        if (!go_again()) break;
       }
     } else if (warp == kTmaWarp) {
       // ---- copies
@@ -715,6 +729,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           const int care_from = with_care ? masked_from(w) : nk;
           int* bad = first_bad + (cares & 1) * 2 * D;
           if (with_care) {
+            if (cares > 1) tile_wait(&notes_read[cares & 1], ((cares >> 1) - 1) & 1, limit);
             for (int e = lane; e < 2 * D; e += 32) bad[e] = kUnseen;
             __syncwarp();
           }
@@ -978,7 +993,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       end_care();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q4 ? 200 : 208));
     // ---- softmax of tile i: this thread's row
     const int i = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
@@ -1113,6 +1128,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (CARE && max(item.steps[0], item.steps[1]) > 0) {
           tile_wait(&taken_out[cares & 1], cares >> 1 & 1, limit);
           if (my_steps > 0) put_back<D>(o_at, first_bad + (cares & 1) * 2 * D, lim);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&notes_read[cares & 1]);
           ++cares;
         }
         // a row's outputs go out a 32-byte sector at a time where they start on one (16 prompts of 15001 tokens together:
@@ -1301,7 +1318,7 @@ static int launch_tile(const ArgsT& a, const CUtensorMap& q, const CUtensorMap& 
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(kTileThreads, 1, 1);
+  cfg.blockDim = dim3(kTileInt4<ArgsT> ? kTile4Threads : kTileThreads, 1, 1);
   cfg.dynamicSmemBytes = tile_smem_bytes(D);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
