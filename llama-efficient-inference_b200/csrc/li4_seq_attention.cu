@@ -222,11 +222,11 @@ __device__ __forceinline__ void load_stage(const SeqAttnArgs& a, const KeyPages<
 }
 
 // ---- a cache in 4 bits
-// The page of one key (a stage has a key per lane); -1: past the end or outside the cache.
+// The page of one key (a stage has a key per lane), -1 past the end; asked for a stage ahead of its use, like key_pages.
 __device__ __forceinline__ int key_page4(const Seq4Args& a, int b, int j, int end) {
-  if (j >= end) return -1;
-  const int page = a.tables[(long long)b * a.table_stride + (j >> a.log_page)];
-  return (unsigned)page < (unsigned)a.num_pages ? page : -1;
+  int page = -1;
+  if (j < end) page = a.tables[(long long)b * a.table_stride + (j >> a.log_page)];
+  return page;
 }
 
 // A stage: codes of the keys' and the values' rows, then their params.  Row r's 16-byte chunks of codes stand at c ^ swizzle(r).
@@ -252,14 +252,14 @@ __device__ __forceinline__ void load_stage4(const Seq4Args& a, int my_page, int 
   for (int i = 0; i < CH; ++i) {
     const int r = i * RPI + lane / CH, row = (j0 + r) & mask;
     const long long page = __shfl_sync(0xffffffffu, my_page, r);
-    const bool ok = page >= 0 && in_head;
+    const bool ok = (unsigned long long)page < (unsigned)a.num_pages && in_head;
     const uint32_t at = stage + r * (D / 2) + ((c ^ swizzle4<D>(r)) << 4);
     cp_async16z(at, ok ? kc + page * a.k4.stride_cp + row * a.k4.stride_ct : static_cast<const void*>(a.q), ok);
     cp_async16z(at + kSeq4Keys * (D / 2), ok ? vc + page * a.v4.stride_cp + row * a.v4.stride_ct : static_cast<const void*>(a.q), ok);
   }
   {
     const int row = (j0 + lane) & mask;
-    const bool ok = my_page >= 0;
+    const bool ok = (unsigned)my_page < (unsigned)a.num_pages;
     const uint32_t* kp = static_cast<const uint32_t*>(a.k4.params) + my_page * a.k4.stride_pp + row * a.k4.stride_pt + kvh * a.k4.stride_ph;
     const uint32_t* vp = static_cast<const uint32_t*>(a.v4.params) + my_page * a.v4.stride_pp + row * a.v4.stride_pt + kvh * a.v4.stride_ph;
     const uint32_t at = stage + kSeq4Keys * D + lane * (G * 4);

@@ -421,55 +421,57 @@ __device__ __noinline__ void put_back(uint32_t o_at, const int* first, int last)
   tmem_st_wait();
 }
 
-// ---- a cache in 4 bits: a quarter of a tile (32 rows) by a warp.  In its turn i a lane holds the group of 32 dims c =
-// (lane & 1) + 2 (i % SUB) of row lane / 2 + 16 (i / SUB): 8 neighbouring lanes then store to all eight 16-byte places of
-// swizzled rows.
+// ---- a cache in 4 bits: a quarter of a tile (32 rows) by a warp, a row per lane: one address per row, and 8 neighbouring
+// lanes store to all eight 16-byte places of swizzled rows.  (Two lanes per row and 16 rows per turn, with an address and a
+// shuffle for each turn: a chunk of 2048 tokens over 8000 at 64 dims 410 us.)
 template <int D>
-struct Quarter4 {
-  static constexpr int SUB = D / 64, TURNS = 2 * SUB;
-  uint4 codes[TURNS];
-  uint32_t params[TURNS];
+struct Row4 {
+  uint4 codes[D / 32];
+  uint32_t params[D / 32];
 };
 
-// The page of key key0 + lane; -1: past the end or outside the cache.
-__device__ __forceinline__ int quarter_page4(const SeqAttnArgs& a, const TileWork& w, int key0) {
-  const int key = key0 + (threadIdx.x & 31);
+// The page of key `key`, -1 past the end.  (Whether it lies in the cache is asked where it is used: the answer of the
+// table takes a trip to L2.)
+__device__ __forceinline__ int row_page4(const SeqAttnArgs& a, const TileWork& w, int key) {
   int page = -1;
   if (key < w.len) page = a.tables[(long long)w.b * a.table_stride + (key >> a.log_page)];
-  return (unsigned)page < (unsigned)a.num_pages ? page : -1;
+  return page;
 }
 
-// Turn i's loads; what does not exist reads as zero codes and parameters, which make zeros.
+// The row of this lane's key; what does not exist reads as zero codes and parameters, which make zeros.  codes, params: of
+// the item's KV head.
 template <int D>
-__device__ __forceinline__ void load_turn4(Quarter4<D>& h, int i, const SeqAttnArgs& a, const li4_int4_pages& pages, int my_page,
-                                           int kvh, int key0) {
-  constexpr int SUB = Quarter4<D>::SUB;
-  const int lane = threadIdx.x & 31, c = (lane & 1) + 2 * (i % SUB);
-  const int page = __shfl_sync(0xffffffffu, my_page, lane / 2 + 16 * (i / SUB));
-  const int row = (key0 + lane / 2 + 16 * (i / SUB)) & ((1 << a.log_page) - 1);
-  h.codes[i] = make_uint4(0, 0, 0, 0);
-  h.params[i] = 0;
-  if (page >= 0 && c * kGroup4 < a.hd) {
-    h.codes[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pages.codes) + page * pages.stride_cp +
-                                                 row * pages.stride_ct + kvh * pages.stride_ch + c * 16);
-    h.params[i] = static_cast<const uint32_t*>(pages.params)[page * pages.stride_pp + row * pages.stride_pt +
-                                                             kvh * pages.stride_ph + c];
+__device__ __forceinline__ void load_row4(Row4<D>& h, const SeqAttnArgs& a, const li4_int4_pages& pages, const uint8_t* codes,
+                                          const uint32_t* params, int page, int key) {
+  const int row = key & ((1 << a.log_page) - 1);
+  const bool ok = (unsigned)page < (unsigned)a.num_pages;
+  const uint4* c = reinterpret_cast<const uint4*>(codes + page * pages.stride_cp + row * pages.stride_ct);
+  const uint32_t* p = params + page * pages.stride_pp + row * pages.stride_pt;
+#pragma unroll
+  for (int g = 0; g < D / 32; ++g) {
+    h.codes[g] = make_uint4(0, 0, 0, 0);
+    h.params[g] = 0;
+    if (ok && g * kGroup4 < a.hd) {
+      h.codes[g] = c[g];
+      h.params[g] = p[g];
+    }
   }
 }
 
-// Turn i's values to their places of the tile; row0: the quarter's first row.
+// The row's values to row r of the tile.
 template <typename T, int D>
-__device__ __forceinline__ void store_turn4(const Quarter4<D>& h, int i, uint8_t* tile, int row0) {
-  constexpr int SUB = Quarter4<D>::SUB;
-  const int lane = threadIdx.x & 31, r = row0 + lane / 2 + 16 * (i / SUB);
-  uint8_t* at = tile + (i % SUB) * (tile_bytes(D) / SUB) + r * 128;
-  const uint32_t s2 = both_low(h.params[i]), m2 = both_high(h.params[i]);
-  const uint32_t w[4] = {h.codes[i].x, h.codes[i].y, h.codes[i].z, h.codes[i].w};
+__device__ __forceinline__ void store_row4(const Row4<D>& h, uint8_t* tile, int r) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    uint32_t u[4];
-    values8<T>(w[e], s2, m2, u);
-    *reinterpret_cast<uint4*>(at + (((4 * (lane & 1) + e) ^ (r & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+  for (int g = 0; g < D / 32; ++g) {
+    uint8_t* at = tile + (g >> 1) * (tile_bytes(D) * 64 / D) + r * 128;
+    const uint32_t s2 = both_low(h.params[g]), m2 = both_high(h.params[g]);
+    const uint32_t w[4] = {h.codes[g].x, h.codes[g].y, h.codes[g].z, h.codes[g].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t u[4];
+      values8<T>(w[e], s2, m2, u);
+      *reinterpret_cast<uint4*>(at + (((4 * (g & 1) + e) ^ (r & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
   }
 }
 
@@ -596,7 +598,7 @@ __global__ void __launch_bounds__(kTileInt4<ArgsT> ? kTile4Threads : kTileThread
   // (2 x 128 x 200 + 128 x 48 + 128 x 64 = 512 x 128)
   if (Q4 && warp >= kUnpackWarp) {
     if constexpr (Q4) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
       // ---- this warp's quarter of the key and value tiles
       const int row0 = (warp - kUnpackWarp) * (kTileKeys / 4);
       int k = 0;
@@ -608,46 +610,49 @@ __global__ void __launch_bounds__(kTileInt4<ArgsT> ? kTile4Threads : kTileThread
           if (w.b < 0) break;
           const int nk = max(w.steps[0], w.steps[1]);
           if (nk == 0) continue;
-          const int at0 = w.first * kTileKeys + row0;  // the quarter's first key of key tile 0
-          int next = quarter_page4(a.s, w, at0), now = next, last = next;  // pages of the key tile ahead, of this, of the one before
-          Quarter4<D> h;
-#pragma unroll
-          for (int i = 0; i < Quarter4<D>::TURNS; ++i) load_turn4<D>(h, i, a.s, a.k4, next, w.kvh, at0);
-          if (nk > 1) next = quarter_page4(a.s, w, at0 + kTileKeys);
+          const int key0 = w.first * kTileKeys + row0 + lane;  // this lane's key of key tile 0
+          const uint8_t* kc = static_cast<const uint8_t*>(a.k4.codes) + w.kvh * a.k4.stride_ch;
+          const uint8_t* vc = static_cast<const uint8_t*>(a.v4.codes) + w.kvh * a.v4.stride_ch;
+          const uint32_t* kp = static_cast<const uint32_t*>(a.k4.params) + w.kvh * a.k4.stride_ph;
+          const uint32_t* vp = static_cast<const uint32_t*>(a.v4.params) + w.kvh * a.v4.stride_ph;
+          // rows of the next key and the next value tile, and pages of the key tile after that one
+          Row4<D> hk, hv;
+          int page = row_page4(a.s, w, key0), page_v = page;
+          load_row4<D>(hk, a.s, a.k4, kc, kp, page, key0);
+          load_row4<D>(hv, a.s, a.v4, vc, vp, page, key0);
+          page = row_page4(a.s, w, key0 + kTileKeys);
           const int care_from = care ? masked_from(w) : nk;
           int* bad = first_bad + (cares & 1) * 2 * D;
           if (care) tile_wait(noted, cares & 1, limit);
-          auto is_value = [&](int n) { return !EARLY ? (n & 1) != 0 : n == 2 * nk - 1 || (n > 0 && !(n & 1)); };
-          auto tile_of = [&](int n) { return !EARLY ? n / 2 : n == 2 * nk - 1 ? nk - 1 : is_value(n) ? n / 2 - 1 : (n + 1) / 2; };
-#pragma unroll 1
-          for (int n = 0; n < 2 * nk; ++n) {
-            const unsigned g = base + n, slot = g % NS;
-            // the next tile: a key tile takes the pages asked for a tile ahead, a value tile those of its keys
-            const bool more = n + 1 < 2 * nk, next_value = more && is_value(n + 1);
-            const int j1 = more ? tile_of(n + 1) : 0;
-            if (more && !next_value) {
-              last = now;
-              now = next;
-              if (j1 + 1 < nk) next = quarter_page4(a.s, w, at0 + (j1 + 1) * kTileKeys);
-            }
-            const int page = next_value && EARLY && j1 < nk - 1 ? last : now;
+          unsigned g = base;
+          // one tile into the ring; its row of the same tile a step on is asked for at once
+          auto put = [&](Row4<D>& h, bool value, int j, int page_next) {
+            const unsigned slot = g % NS;
             if (g >= NS) tile_wait(&kv_empty[slot], ((g / NS) - 1) & 1, limit);
-            if (ran_out()) continue;
+            ++g;
+            if (ran_out()) return;
             uint8_t* tile = ring + slot * TB;
-#pragma unroll
-            for (int i = 0; i < Quarter4<D>::TURNS; ++i) {
-              store_turn4<T, D>(h, i, tile, row0);
-              if (more) load_turn4<D>(h, i, a.s, next_value ? a.v4 : a.k4, page, w.kvh, at0 + j1 * kTileKeys);
-            }
-            const int j = tile_of(n);
-            if (is_value(n) && j >= care_from) {
+            store_row4<T, D>(h, tile, row0 + lane);
+            const int key = key0 + (j + 1) * kTileKeys;
+            if (value) load_row4<D>(h, a.s, a.v4, vc, vp, page_next, key);
+            else load_row4<D>(h, a.s, a.k4, kc, kp, page_next, key);
+            if (value && j >= care_from) {
               __syncwarp();
               take_out<T, D>(tile, row0, row0 + kTileKeys / 4, (w.first + j) * kTileKeys, bad);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&kv_full[slot]);
+          };
+#pragma unroll 1
+          for (int j = 0; j < nk; ++j) {
+            put(hk, false, j, page);
+            if (EARLY && j > 0) put(hv, true, j - 1, page_v);
+            page_v = page;  // of key tile j + 1
+            page = row_page4(a.s, w, key0 + (j + 2) * kTileKeys);
+            if (!EARLY) put(hv, true, j, page_v);
           }
+          if (EARLY) put(hv, true, nk - 1, -1);
           if (care) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&taken_out[cares & 1]);
@@ -993,7 +998,7 @@ __global__ void __launch_bounds__(kTileInt4<ArgsT> ? kTile4Threads : kTileThread
       end_care();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q4 ? 200 : 208));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q4 ? 192 : 208));
     // ---- softmax of tile i: this thread's row
     const int i = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
