@@ -98,5 +98,6 @@ int launch_tile_attention(const SeqAttnArgs& a, bool paged, int dtype, cudaStrea
 int launch_tile_attention_int4(const Seq4Args& a, int dtype, cudaStream_t stream);
 size_t tile_attention_part_bytes(int hd, int rep, int64_t tokens, int64_t kv_heads, int64_t max_keys, int sm);
 size_t seq_attention_part_bytes(int hd, int max_rows, int sm);
+size_t seq_attention_int4_part_bytes(int hd, int max_rows, int sm);
 
 }  // namespace li4

@@ -47,7 +47,9 @@ __host__ __device__ constexpr int seq_stage_bytes(int D) { return 2 * seq_keys(D
 template <typename ArgsT>
 constexpr bool kIsInt4 = __is_same(ArgsT, Seq4Args);
 constexpr int kSeq4Keys = 32;
-__host__ __device__ constexpr int seq4_stages(int D) { return D == 64 ? 6 : 4; }
+__host__ __device__ constexpr int seq4_stages(int D) { return D == 64 ? 5 : 3; }
+// CTAs per SM: unpacking is work that more warps hide better.
+__host__ __device__ constexpr int seq4_ctas(int D, int NT) { return NT > 1 ? 2 : D == 64 ? 4 : 3; }
 __host__ __device__ constexpr int seq4_stage_bytes(int D) { return 2 * kSeq4Keys * (D / 2 + D / kGroup4 * 4); }
 
 __host__ __device__ constexpr int seq_stage_keys(int D, bool q4) { return q4 ? kSeq4Keys : seq_keys(D); }
@@ -361,7 +363,8 @@ __device__ __forceinline__ void value_fragments4(const uint8_t* stage, int key, 
 // CL: few requests of short contexts.  A cluster of CTAs takes all keys of a (request, KV head) and joins its parts through
 // distributed shared memory, so there is no second launch (see seq_cluster).
 template <typename T, int D, int NT, bool PAGED, bool CL, typename ArgsT>
-__global__ void __launch_bounds__(kSeqThreads) seq_attention_kernel(const __grid_constant__ ArgsT a) {
+__global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT) : 1)
+    seq_attention_kernel(const __grid_constant__ ArgsT a) {
   constexpr bool Q4 = kIsInt4<ArgsT>;
   constexpr int RT = 8 * NT;
   constexpr int KS = D / 16;  // k steps of K Q^T
@@ -875,7 +878,9 @@ static int seq_cluster(const SeqAttnArgs& a) {
 }
 
 template <typename T, int D, int NT, bool PAGED, typename ArgsT>
-static int launch_seq(const ArgsT& a, cudaStream_t stream) {
+static int launch_seq(const ArgsT& args, cudaStream_t stream) {
+  ArgsT a = args;
+  if constexpr (kIsInt4<ArgsT>) a.grid = seq4_ctas(D, NT) * current_sm_count();
   const int c = seq_cluster(a);
   const size_t smem = seq_ring_bytes(D, NT, kIsInt4<ArgsT>);
   if (c > 1)
@@ -906,6 +911,11 @@ size_t seq_attention_part_bytes(int hd, int max_rows, int sm) {
   return (size_t)2 * seq_grid(sm) * seq_part_floats(hd <= 64 ? 64 : 128, seq_nt(max_rows)) * sizeof(float);
 }
 
+size_t seq_attention_int4_part_bytes(int hd, int max_rows, int sm) {
+  const int D = hd <= 64 ? 64 : 128, nt = seq_nt(max_rows);
+  return (size_t)2 * seq4_ctas(D, nt) * sm * seq_part_floats(D, nt) * sizeof(float);
+}
+
 int launch_seq_attention(const SeqAttnArgs& args, bool paged, int dtype, int max_rows, cudaStream_t stream) {
   SeqAttnArgs a = args;
   a.grid = seq_grid(current_sm_count());
@@ -916,10 +926,8 @@ int launch_seq_attention(const SeqAttnArgs& args, bool paged, int dtype, int max
 }
 
 int launch_seq_attention_int4(const Seq4Args& args, int dtype, int max_rows, cudaStream_t stream) {
-  Seq4Args a = args;
-  a.grid = seq_grid(current_sm_count());
   const int nt = seq_nt(max_rows);
-  return dtype == LI4_F16 ? launch_seq_d<__half, true>(a, nt, stream) : launch_seq_d<__nv_bfloat16, true>(a, nt, stream);
+  return dtype == LI4_F16 ? launch_seq_d<__half, true>(args, nt, stream) : launch_seq_d<__nv_bfloat16, true>(args, nt, stream);
 }
 
 // Rows (queries x heads of a KV head) up to which a sequence is streamed: where no sequence has more the streaming
@@ -1072,19 +1080,25 @@ static int run_attention(const li4_attention* p, bool paged, const Int4Pages* in
   return rc;
 }
 
-}  // namespace li4
-
-extern "C" size_t li4_attention_workspace_bytes(const li4_attention* p) {
-  using namespace li4;
+// Streamed parts' bytes by (head_dim, most rows, SMs).
+static size_t attention_workspace(const li4_attention* p, size_t (*seq_bytes)(int, int, int)) {
   if (!p || p->n_seqs <= 0 || p->n_tokens <= 0 || p->n_kv_heads < 1 || p->max_queries < 0) return 0;
   const int64_t rep = p->n_heads / p->n_kv_heads;
   if (rep < 1 || rep > 128) return 0;
-  const size_t seq = seq_attention_part_bytes((int)p->head_dim, attention_rows(p), current_sm_count());
-  const size_t tile = attention_rows(p) > kFewRows ? tile_attention_part_bytes((int)p->head_dim, (int)rep, p->n_tokens,
-                                                                               p->n_kv_heads, attention_keys(p),
-                                                                               current_sm_count())
-                                                   : 0;
+  const int sm = current_sm_count(), rows = attention_rows(p);
+  // (beside longer ones sequences of one tile of 8 rows are streamed)
+  const size_t alone = seq_bytes((int)p->head_dim, rows, sm), beside = seq_bytes((int)p->head_dim, kFewRowsBeside, sm);
+  const size_t seq = alone > beside ? alone : beside;
+  const size_t tile = rows > kFewRows ? tile_attention_part_bytes((int)p->head_dim, (int)rep, p->n_tokens, p->n_kv_heads,
+                                                                  attention_keys(p), sm)
+                                      : 0;
   return seq > tile ? seq : tile;  // (the two kernels run one after the other)
+}
+
+}  // namespace li4
+
+extern "C" size_t li4_attention_workspace_bytes(const li4_attention* p) {
+  return li4::attention_workspace(p, li4::seq_attention_part_bytes);
 }
 
 extern "C" int li4_prompt_attention(const li4_attention* args, void* workspace, size_t workspace_bytes, void* stream) {
@@ -1095,7 +1109,9 @@ extern "C" int li4_paged_attention(const li4_attention* args, void* workspace, s
   return li4::run_attention(args, true, nullptr, workspace, workspace_bytes, stream, "paged_attention");
 }
 
-extern "C" size_t li4_attention_int4_workspace_bytes(const li4_attention* p) { return li4_attention_workspace_bytes(p); }
+extern "C" size_t li4_attention_int4_workspace_bytes(const li4_attention* p) {
+  return li4::attention_workspace(p, li4::seq_attention_int4_part_bytes);
+}
 
 extern "C" int li4_paged_attention_int4(const li4_attention* args, const li4_int4_pages* cache_k,
                                         const li4_int4_pages* cache_v, void* workspace, size_t workspace_bytes,

@@ -422,13 +422,11 @@ __device__ __noinline__ void put_back(uint32_t o_at, const int* first, int last)
 }
 
 // ---- a cache in 4 bits: a quarter of a tile (32 rows) by a warp, a row per lane: one address per row, and 8 neighbouring
-// lanes store to all eight 16-byte places of swizzled rows.  (Two lanes per row and 16 rows per turn, with an address and a
-// shuffle for each turn: a chunk of 2048 tokens over 8000 at 64 dims 410 us.)
-template <int D>
-struct Row4 {
-  uint4 codes[D / 32];
-  uint32_t params[D / 32];
-};
+// lanes store to all eight 16-byte places of swizzled rows.  A lane's row of the next key and of the next value tile waits in
+// shared memory of its own (2048 tokens over 8000 at 128 dims: two lanes per row, an address and a shuffle for each turn
+// of 16 rows 741 us, rows kept in registers 461 us).
+__host__ __device__ constexpr int row4_bytes(int D) { return D / 2 + D / kGroup4 * 4; }
+__host__ __device__ constexpr int rows4_bytes(int D) { return 2 * kTileKeys * row4_bytes(D); }  // of the four warps
 
 // The page of key `key`, -1 past the end.  (Whether it lies in the cache is asked where it is used: the answer of the
 // table takes a trip to L2.)
@@ -438,34 +436,43 @@ __device__ __forceinline__ int row_page4(const SeqAttnArgs& a, const TileWork& w
   return page;
 }
 
-// The row of this lane's key; what does not exist reads as zero codes and parameters, which make zeros.  codes, params: of
-// the item's KV head.
+// Asks for the row of this lane's key; what does not exist becomes zero codes and parameters, which make zeros.  to: the
+// warp's rows, 16-byte pieces of codes of all lanes after one another, then their parameters; kvh: the item's KV head.
 template <int D>
-__device__ __forceinline__ void load_row4(Row4<D>& h, const SeqAttnArgs& a, const li4_int4_pages& pages, const uint8_t* codes,
-                                          const uint32_t* params, int page, int key) {
-  const int row = key & ((1 << a.log_page) - 1);
+__device__ __forceinline__ void load_row4(uint32_t to, const SeqAttnArgs& a, const li4_int4_pages& pages, int kvh, int page,
+                                          int key) {
+  const int lane = threadIdx.x & 31, row = key & ((1 << a.log_page) - 1);
   const bool ok = (unsigned)page < (unsigned)a.num_pages;
-  const uint4* c = reinterpret_cast<const uint4*>(codes + page * pages.stride_cp + row * pages.stride_ct);
-  const uint32_t* p = params + page * pages.stride_pp + row * pages.stride_pt;
+  const uint8_t* c = static_cast<const uint8_t*>(pages.codes) + page * pages.stride_cp + row * pages.stride_ct + kvh * pages.stride_ch;
+  const uint32_t* p = static_cast<const uint32_t*>(pages.params) + page * pages.stride_pp + row * pages.stride_pt + kvh * pages.stride_ph;
+  if (!ok) {  // (addresses are not read then)
+    c = reinterpret_cast<const uint8_t*>(a.q);
+    p = reinterpret_cast<const uint32_t*>(a.q);
+  }
 #pragma unroll
   for (int g = 0; g < D / 32; ++g) {
-    h.codes[g] = make_uint4(0, 0, 0, 0);
-    h.params[g] = 0;
-    if (ok && g * kGroup4 < a.hd) {
-      h.codes[g] = c[g];
-      h.params[g] = p[g];
-    }
+    const bool have = ok && g * kGroup4 < a.hd;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + g * 512 + lane * 16), "l"(have ? c + g * 16 : c),
+                 "r"(have ? 16 : 0)
+                 : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 16 * D + g * 128 + lane * 4), "l"(have ? p + g : p),
+                 "r"(have ? 4 : 0)
+                 : "memory");
   }
+  asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
 // The row's values to row r of the tile.
 template <typename T, int D>
-__device__ __forceinline__ void store_row4(const Row4<D>& h, uint8_t* tile, int r) {
+__device__ __forceinline__ void store_row4(const uint8_t* from, uint8_t* tile, int r) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int g = 0; g < D / 32; ++g) {
+    const uint4 c = *reinterpret_cast<const uint4*>(from + g * 512 + lane * 16);
+    const uint32_t p = *reinterpret_cast<const uint32_t*>(from + 16 * D + g * 128 + lane * 4);
     uint8_t* at = tile + (g >> 1) * (tile_bytes(D) * 64 / D) + r * 128;
-    const uint32_t s2 = both_low(h.params[g]), m2 = both_high(h.params[g]);
-    const uint32_t w[4] = {h.codes[g].x, h.codes[g].y, h.codes[g].z, h.codes[g].w};
+    const uint32_t s2 = both_low(p), m2 = both_high(p);
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       uint32_t u[4];
@@ -601,6 +608,7 @@ __global__ void __launch_bounds__(kTileInt4<ArgsT> ? kTile4Threads : kTileThread
       asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
       // ---- this warp's quarter of the key and value tiles
       const int row0 = (warp - kUnpackWarp) * (kTileKeys / 4);
+      uint8_t* const rows = reinterpret_cast<uint8_t*>(reply) + 512 + 16 * D + (warp - kUnpackWarp) * 64 * row4_bytes(D);  // keys', values'
       int k = 0;
       unsigned base = 0;
       for (bool care = false;; care = true) {
@@ -611,31 +619,27 @@ __global__ void __launch_bounds__(kTileInt4<ArgsT> ? kTile4Threads : kTileThread
           const int nk = max(w.steps[0], w.steps[1]);
           if (nk == 0) continue;
           const int key0 = w.first * kTileKeys + row0 + lane;  // this lane's key of key tile 0
-          const uint8_t* kc = static_cast<const uint8_t*>(a.k4.codes) + w.kvh * a.k4.stride_ch;
-          const uint8_t* vc = static_cast<const uint8_t*>(a.v4.codes) + w.kvh * a.v4.stride_ch;
-          const uint32_t* kp = static_cast<const uint32_t*>(a.k4.params) + w.kvh * a.k4.stride_ph;
-          const uint32_t* vp = static_cast<const uint32_t*>(a.v4.params) + w.kvh * a.v4.stride_ph;
-          // rows of the next key and the next value tile, and pages of the key tile after that one
-          Row4<D> hk, hv;
           int page = row_page4(a.s, w, key0), page_v = page;
-          load_row4<D>(hk, a.s, a.k4, kc, kp, page, key0);
-          load_row4<D>(hv, a.s, a.v4, vc, vp, page, key0);
-          page = row_page4(a.s, w, key0 + kTileKeys);
+          load_row4<D>(smem_addr(rows), a.s, a.k4, w.kvh, page, key0);
+          load_row4<D>(smem_addr(rows + 32 * row4_bytes(D)), a.s, a.v4, w.kvh, page, key0);
+          page = row_page4(a.s, w, key0 + kTileKeys);  // pages of the key tile that is asked for next
           const int care_from = care ? masked_from(w) : nk;
           int* bad = first_bad + (cares & 1) * 2 * D;
           if (care) tile_wait(noted, cares & 1, limit);
           unsigned g = base;
-          // one tile into the ring; its row of the same tile a step on is asked for at once
-          auto put = [&](Row4<D>& h, bool value, int j, int page_next) {
+          // one tile into the ring; its row of the same kind of tile a step on is asked for at once
+          auto put = [&](bool value, int j, int page_next) {
             const unsigned slot = g % NS;
+            uint8_t* const tile = ring + slot * TB;
+            uint8_t* const mine = rows + (value ? 32 * row4_bytes(D) : 0);
             if (g >= NS) tile_wait(&kv_empty[slot], ((g / NS) - 1) & 1, limit);
             ++g;
+            // (the row was the last request but one, or the last: the second key tile's and the last value tile's, 64 dims)
+            if (EARLY && j == (value ? nk - 1 : 1)) asm volatile("cp.async.wait_group 0;" ::: "memory");
+            else asm volatile("cp.async.wait_group 1;" ::: "memory");
             if (ran_out()) return;
-            uint8_t* tile = ring + slot * TB;
-            store_row4<T, D>(h, tile, row0 + lane);
-            const int key = key0 + (j + 1) * kTileKeys;
-            if (value) load_row4<D>(h, a.s, a.v4, vc, vp, page_next, key);
-            else load_row4<D>(h, a.s, a.k4, kc, kp, page_next, key);
+            store_row4<T, D>(mine, tile, row0 + lane);
+            load_row4<D>(smem_addr(mine), a.s, value ? a.v4 : a.k4, w.kvh, page_next, key0 + (j + 1) * kTileKeys);
             if (value && j >= care_from) {
               __syncwarp();
               take_out<T, D>(tile, row0, row0 + kTileKeys / 4, (w.first + j) * kTileKeys, bad);
@@ -646,13 +650,14 @@ __global__ void __launch_bounds__(kTileInt4<ArgsT> ? kTile4Threads : kTileThread
           };
 #pragma unroll 1
           for (int j = 0; j < nk; ++j) {
-            put(hk, false, j, page);
-            if (EARLY && j > 0) put(hv, true, j - 1, page_v);
+            put(false, j, page);
+            if (EARLY && j > 0) put(true, j - 1, page_v);
             page_v = page;  // of key tile j + 1
             page = row_page4(a.s, w, key0 + (j + 2) * kTileKeys);
-            if (!EARLY) put(hv, true, j, page_v);
+            if (!EARLY) put(true, j, page_v);
           }
-          if (EARLY) put(hv, true, nk - 1, -1);
+          if (EARLY) put(true, nk - 1, -1);
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
           if (care) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&taken_out[cares & 1]);
@@ -1305,6 +1310,7 @@ static int make_map(CUtensorMap* map, int dtype, const void* base, int64_t d, in
 template <typename T, int D, bool PAGED, typename ArgsT>
 static int launch_tile(const ArgsT& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                        unsigned grid, cudaStream_t stream) {
+  const int smem = tile_smem_bytes(D) + (kTileInt4<ArgsT> ? rows4_bytes(D) : 0);
   static std::mutex mu;
   static std::vector<int> done_dev;  // of this kernel
   int dev = 0;
@@ -1315,7 +1321,7 @@ static int launch_tile(const ArgsT& a, const CUtensorMap& q, const CUtensorMap& 
     for (int d : done_dev) seen |= (d == dev);
     if (!seen) {
       const int rc = check_cuda(cudaFuncSetAttribute(tile_attention_kernel<T, D, PAGED, ArgsT>,
-                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem_bytes(D)),
+                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
                                 "attention: shared memory limit");
       if (rc != LI4_OK) return rc;
       done_dev.push_back(dev);
@@ -1324,7 +1330,7 @@ static int launch_tile(const ArgsT& a, const CUtensorMap& q, const CUtensorMap& 
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, 1, 1);
   cfg.blockDim = dim3(kTileInt4<ArgsT> ? kTile4Threads : kTileThreads, 1, 1);
-  cfg.dynamicSmemBytes = tile_smem_bytes(D);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
