@@ -231,56 +231,62 @@ __device__ __forceinline__ int key_page4(const Seq4Args& a, int b, int j, int en
   return page;
 }
 
-// A stage: codes of the keys' and the values' rows, then their params.  Row r's 16-byte chunks of codes stand at c ^ swizzle(r).
-// Rows of no page are zeros.
-template <int D>
-__device__ __forceinline__ int swizzle4(int r) { return D == 128 ? r & 2 : 0; }
-
-__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool have) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have ? 4 : 0) : "memory");
+// Keys or values of one KV head; offsets of codes in 16 bytes and of params in pairs fit 32 bits (int4_offsets_fit), so an
+// address is two multiply-adds and a wide one.
+struct Head4 {
+  const uint8_t* codes;
+  const uint32_t* params;
+  uint32_t cp, ct, pp, pt;
+};
+__device__ __forceinline__ Head4 head4(const li4_int4_pages& p, int kvh) {
+  return {static_cast<const uint8_t*>(p.codes) + kvh * p.stride_ch, static_cast<const uint32_t*>(p.params) + kvh * p.stride_ph,
+          (uint32_t)(p.stride_cp >> 4), (uint32_t)(p.stride_ct >> 4), (uint32_t)p.stride_pp, (uint32_t)p.stride_pt};
 }
-__device__ __forceinline__ void cp_async8z(uint32_t dst, const void* src, bool have) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(have ? 8 : 0) : "memory");
+
+__device__ __forceinline__ void cp_async4z(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async8z(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async16n(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
+// A stage: codes of the keys' and the values' rows, then their params.  Rows of no page are zeros (page 0 is not read).
 template <int D>
-__device__ __forceinline__ void load_stage4(const Seq4Args& a, int my_page, int kvh, int j0, int end, uint32_t stage) {
+__device__ __forceinline__ void load_stage4(const Seq4Args& a, const Head4& k, const Head4& v, int my_page, int j0, uint32_t stage) {
   constexpr int CH = D / 32, RPI = 32 / CH, G = D / kGroup4;
   const int lane = threadIdx.x & 31, c = lane % CH, mask = (1 << a.log_page) - 1;
-  const uint8_t* kc = static_cast<const uint8_t*>(a.k4.codes) + kvh * a.k4.stride_ch + c * 16;
-  const uint8_t* vc = static_cast<const uint8_t*>(a.v4.codes) + kvh * a.v4.stride_ch + c * 16;
-  const bool in_head = c * 32 < a.hd;
+  if ((unsigned)my_page >= (unsigned)a.num_pages) my_page = -1;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int r = i * RPI + lane / CH, row = (j0 + r) & mask;
-    const long long page = __shfl_sync(0xffffffffu, my_page, r);
-    const bool ok = (unsigned long long)page < (unsigned)a.num_pages && in_head;
-    const uint32_t at = stage + r * (D / 2) + ((c ^ swizzle4<D>(r)) << 4);
-    cp_async16z(at, ok ? kc + page * a.k4.stride_cp + row * a.k4.stride_ct : static_cast<const void*>(a.q), ok);
-    cp_async16z(at + kSeq4Keys * (D / 2), ok ? vc + page * a.v4.stride_cp + row * a.v4.stride_ct : static_cast<const void*>(a.q), ok);
+    const int r = i * RPI + lane / CH;
+    const uint32_t row = (j0 + r) & mask;
+    const int page = __shfl_sync(0xffffffffu, my_page, r);
+    const uint32_t bytes = page >= 0 && c * 32 < a.hd ? 16 : 0, pg = max(page, 0);
+    const uint32_t at = stage + r * (D / 2) + c * 16;
+    cp_async16n(at, k.codes + (uint64_t)(pg * k.cp + row * k.ct + c) * 16, bytes);
+    cp_async16n(at + kSeq4Keys * (D / 2), v.codes + (uint64_t)(pg * v.cp + row * v.ct + c) * 16, bytes);
   }
-  {
-    const int row = (j0 + lane) & mask;
-    const bool ok = (unsigned)my_page < (unsigned)a.num_pages;
-    const uint32_t* kp = static_cast<const uint32_t*>(a.k4.params) + my_page * a.k4.stride_pp + row * a.k4.stride_pt + kvh * a.k4.stride_ph;
-    const uint32_t* vp = static_cast<const uint32_t*>(a.v4.params) + my_page * a.v4.stride_pp + row * a.v4.stride_pt + kvh * a.v4.stride_ph;
-    const uint32_t at = stage + kSeq4Keys * D + lane * (G * 4);
-    const void* none = a.q;  // (not read)
-    if (a.wide_params) {
-      if constexpr (D == 64) {
-        cp_async8z(at, ok ? kp : none, ok);
-        cp_async8z(at + kSeq4Keys * G * 4, ok ? vp : none, ok);
-      } else {
-        cp_async16z(at, ok ? kp : none, ok);
-        cp_async16z(at + kSeq4Keys * G * 4, ok ? vp : none, ok);
-      }
+  const uint32_t row = (j0 + lane) & mask, pg = max(my_page, 0), all = my_page >= 0 ? G * 4 : 0;
+  const uint32_t* kp = k.params + (pg * k.pp + row * k.pt);
+  const uint32_t* vp = v.params + (pg * v.pp + row * v.pt);
+  const uint32_t at = stage + kSeq4Keys * D + lane * (G * 4);
+  if (a.wide_params) {
+    if constexpr (D == 64) {
+      cp_async8z(at, kp, all);
+      cp_async8z(at + kSeq4Keys * G * 4, vp, all);
     } else {
+      cp_async16n(at, kp, all);
+      cp_async16n(at + kSeq4Keys * G * 4, vp, all);
+    }
+  } else {
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const bool have = ok && g * kGroup4 < a.hd;
-        cp_async_small(at + g * 4, have ? kp + g : none, have);
-        cp_async_small(at + kSeq4Keys * G * 4 + g * 4, have ? vp + g : none, have);
-      }
+    for (int g = 0; g < G; ++g) {
+      const bool have = g * kGroup4 < a.hd;
+      cp_async4z(at + g * 4, have ? kp + g : kp, have ? all / G : 0);
+      cp_async4z(at + kSeq4Keys * G * 4 + g * 4, have ? vp + g : vp, have ? all / G : 0);
     }
   }
 }
@@ -309,7 +315,7 @@ __device__ __forceinline__ void key_fragments4(const uint8_t* stage, int key, ui
       const uint2 x = *reinterpret_cast<const uint2*>(row + t * 8);
       w[0] = x.x, w[1] = x.y;
     } else {
-      const uint4 x = *reinterpret_cast<const uint4*>(row + ((t ^ swizzle4<D>(r)) << 4));
+      const uint4 x = *reinterpret_cast<const uint4*>(row + t * 16);
       w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
     }
     const uint32_t p = kp[r * G + t * G / 4], s2 = both_low(p), m2 = both_high(p);
@@ -339,8 +345,8 @@ __device__ __forceinline__ void value_fragments4(const uint8_t* stage, int key, 
       wa[0] = *reinterpret_cast<const uint32_t*>(codes + ra * 32 + g * 4);
       wb[0] = *reinterpret_cast<const uint32_t*>(codes + rb * 32 + g * 4);
     } else {
-      const uint2 x = *reinterpret_cast<const uint2*>(codes + ra * 64 + (((g >> 1) ^ swizzle4<D>(ra)) << 4) + (g & 1) * 8);
-      const uint2 y = *reinterpret_cast<const uint2*>(codes + rb * 64 + (((g >> 1) ^ swizzle4<D>(rb)) << 4) + (g & 1) * 8);
+      const uint2 x = *reinterpret_cast<const uint2*>(codes + ra * 64 + g * 8);
+      const uint2 y = *reinterpret_cast<const uint2*>(codes + rb * 64 + g * 8);
       wa[0] = x.x, wb[0] = y.x;
       wa[W - 1] = x.y, wb[W - 1] = y.y;
     }
@@ -356,6 +362,84 @@ __device__ __forceinline__ void value_fragments4(const uint8_t* stage, int key, 
         vf[4 * i + e][2 * h] = even[e];
         vf[4 * i + e][2 * h + 1] = odd[e];
       }
+    }
+  }
+}
+
+// The softmax's step over the raw scores sc of keys j0 .. (4-bit cache): probabilities 2^(scale s - m) as B fragments, with a
+// maximum m that may lag up to 2^8 behind (as in li4_tile_attention.cu), so that the usual step needs neither the warp's
+// maximum nor a rescaled output.  A scale below zero turns the scores' signs, one of zero makes
+// them zeros.
+template <typename T, int D, int NT, int KT>
+__device__ __forceinline__ void lazy_softmax(float (&sc)[KT][NT][4], float scale, int j0, bool some_hidden, const int (&lim)[NT][2],
+                                             int end, float (&m)[NT][2], float (&l)[NT][2], float (&o)[D / 16][NT][4],
+                                             uint32_t (&pf)[KT][NT][2]) {
+  const int lane = threadIdx.x & 31;
+  const float c = scale == 0.f ? 1.f : fabsf(scale), sign = scale < 0.f ? -1.f : 0.f;
+  if (scale <= 0.f) {
+#pragma unroll
+    for (int mt = 0; mt < KT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[mt][nt][e] *= sign;
+  }
+  if (some_hidden) {
+#pragma unroll
+    for (int mt = 0; mt < KT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + mt * 16 + (e >> 1) * 8 + key_of_row(lane / 4);
+          if (j > lim[nt][e & 1] || j >= end) sc[mt][nt][e] = -INFINITY;
+        }
+  }
+  float top[NT][2];
+  bool move = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float mx = fmaxf(sc[0][nt][e], sc[0][nt][e + 2]);
+#pragma unroll
+      for (int mt = 1; mt < KT; ++mt) mx = fmaxf(mx, fmaxf(sc[mt][nt][e], sc[mt][nt][e + 2]));
+      top[nt][e] = mx;
+      move = move || fmaf(mx, c, -m[nt][e]) > 8.f;  // (no move for two infinities of one sign, whose difference is NaN)
+    }
+  if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = top[nt][e];
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float mn = fmaxf(m[nt][e], mx * c), keep = m[nt][e] == mn ? 1.f : exp2_fast(m[nt][e] - mn);
+        m[nt][e] = mn;
+        l[nt][e] *= keep;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+          o[dt][nt][e] *= keep;
+          o[dt][nt][e + 2] *= keep;
+        }
+      }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float base[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) base[e] = m[nt][e] == -INFINITY ? 0.f : -m[nt][e];  // nothing seen: every probability is 0
+#pragma unroll
+    for (int mt = 0; mt < KT; ++mt) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sc[mt][nt][e] = exp2_fast(fmaf(sc[mt][nt][e], c, base[e & 1]));
+        l[nt][e & 1] += sc[mt][nt][e];
+      }
+      pf[mt][nt][0] = transpose8(Type16<T>::pack(sc[mt][nt][0], sc[mt][nt][1]));
+      pf[mt][nt][1] = transpose8(Type16<T>::pack(sc[mt][nt][2], sc[mt][nt][3]));
     }
   }
 }
@@ -429,12 +513,14 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
     // ---- the warp's keys: k0 + KW warp + UNIT i, their first stages under way
     const int w0 = k0 + warp * KW;
     const int steps = w0 < k1 ? (k1 - w0 + UNIT - 1) / UNIT : 0;
+    [[maybe_unused]] Head4 k4, v4;
+    if constexpr (Q4) k4 = head4(a.k4, kvh), v4 = head4(a.v4, kvh);
     auto pages_of = [&](int j0) {
       if constexpr (Q4) return key_page4(a, b, j0 + lane, k1);
       else return key_pages<D, PAGED>(a, b, j0, k1);
     };
     auto load = [&](const auto& page, int j0, uint32_t stage) {
-      if constexpr (Q4) load_stage4<D>(a, page, kvh, j0, k1, stage);
+      if constexpr (Q4) load_stage4<D>(a, k4, v4, page, j0, stage);
       else load_stage<D, PAGED>(a, page, s, kvh, j0, k1, stage);
     };
     decltype(pages_of(0)) pages[STAGES];
@@ -520,6 +606,10 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
           }
         }
       }
+      uint32_t pf[KT][NT][2];
+      if constexpr (Q4) {
+        lazy_softmax<T, D, NT, KT>(sc, a.scale_log2, j0, j0 + KW - 1 > first_lim || j0 + KW > k1, lim, k1, m, l, o, pf);
+      } else {
       if (j0 + KW - 1 > first_lim || j0 + KW > k1) {  // some key of them is hidden from some row
 #pragma unroll
         for (int mt = 0; mt < KT; ++mt)
@@ -527,7 +617,7 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int j = j0 + mt * 16 + (e >> 1) * 8 + (Q4 ? key_of_row(lane / 4) : lane / 4);
+              const int j = j0 + mt * 16 + (e >> 1) * 8 + lane / 4;
               sc[mt][nt][e] = j > lim[nt][e & 1] || j >= k1 ? -INFINITY : sc[mt][nt][e] * a.scale_log2;
             }
       } else {
@@ -538,7 +628,6 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[mt][nt][e] *= a.scale_log2;
       }
-      uint32_t pf[KT][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float base[2], keep[2];
@@ -572,6 +661,7 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
           pf[mt][nt][0] = transpose8(Type16<T>::pack(sc[mt][nt][0], sc[mt][nt][1]));
           pf[mt][nt][1] = transpose8(Type16<T>::pack(sc[mt][nt][2], sc[mt][nt][3]));
         }
+      }
       }
       if constexpr (Q4) {
         if (j0 + KW - 1 > first_lim) {
@@ -942,6 +1032,16 @@ constexpr int kFewRows = 32, kFewRowsBeside = 8;
 
 constexpr int64_t kAttentionMost = 1 << 30;  // rows of a sequence, keys: what is claimed above it counts as it
 
+// Whether an offset of a head's codes in 16 bytes, and of its params in pairs, fits 32 bits.
+static bool int4_offsets_fit(const li4_int4_pages& p, int64_t pages, int64_t page_size) {
+  const int64_t most = 1LL << 32;
+  auto fits = [&](int64_t page, int64_t row, int64_t unit) {
+    return page / unit <= most && row / unit <= most &&
+           (double)page / unit * (double)(pages - 1) + (double)row / unit * (double)(page_size - 1) + 8 < (double)most;
+  };
+  return fits(p.stride_cp, p.stride_ct, 16) && fits(p.stride_pp, p.stride_pt, 1);
+}
+
 struct Int4Pages {
   const li4_int4_pages *k, *v;
 };
@@ -963,6 +1063,8 @@ static int check_attention(const li4_attention* p, bool paged, const Int4Pages* 
     return set_error(LI4_ERR_UNSUPPORTED, "%s: head_dim=%lld (a multiple of %d up to 128)", what, (long long)p->head_dim,
                      kGroup4);
   if (int4 && (!int4->k || !int4->v)) return set_error(LI4_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (int4 && p->num_pages > 0 && (!int4_offsets_fit(*int4->k, p->num_pages, p->page_size) || !int4_offsets_fit(*int4->v, p->num_pages, p->page_size)))
+    return set_error(LI4_ERR_UNSUPPORTED, "%s: codes of a head spread over more than 64 GB, or params over more than 16 GB", what);
   if (p->n_heads / p->n_kv_heads > 128 || p->n_heads > 65535 || p->n_seqs > (1 << 24) ||
       p->n_tokens > (1LL << 30) / p->n_heads)
     return set_error(LI4_ERR_UNSUPPORTED, "%s: n_seqs=%lld n_tokens=%lld n_heads=%lld too large", what,
@@ -983,6 +1085,11 @@ static int check_attention(const li4_attention* p, bool paged, const Int4Pages* 
   if (!p->q || !p->out || !p->cu_seqlens || (no_keys && !(paged && p->num_pages == 0)) ||
       (paged && (!p->kv_lens || (!p->block_tables && p->table_width > 0))))
     return set_error(LI4_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (int4)
+    for (const li4_int4_pages* g : {int4->k, int4->v})  // (strides of one element are not used)
+      if ((p->num_pages > 1 && (g->stride_cp <= 0 || g->stride_pp <= 0)) || g->stride_ct <= 0 || g->stride_pt <= 0 ||
+          (p->n_kv_heads > 1 && (g->stride_ch <= 0 || g->stride_ph <= 0)))
+        return set_error(LI4_ERR_ALIGNMENT, "%s: rows of the cache must lie at positive strides", what);
   const int64_t st[] = {p->stride_qt, p->stride_qh, p->stride_ot, p->stride_oh, p->stride_kt, p->stride_kh,
                         p->stride_vt, p->stride_vh, paged ? p->stride_kp : 0, paged ? p->stride_vp : 0};
   bool aligned = aligned16(p->q) && aligned16(p->out);
