@@ -40,19 +40,20 @@ constexpr int kSeqStages = 3;   // stages per warp
 // starts an item the other's copies go on: one CTA of 32-key stages at 128 dims, 32 requests of 1000-8000 tokens 81 us
 // instead of 75).
 __host__ __device__ constexpr int seq_keys(int D) { return 32 * 64 / D; }
-__host__ __device__ constexpr int seq_unit(int D, bool q4) { return kSeqWarps * (q4 ? 32 : seq_keys(D)); }  // keys per unit
+// (of a 4-bit cache: 5 KB)
+__host__ __device__ constexpr int seq4_keys(int D) { return D == 64 ? 64 : 32; }
+__host__ __device__ constexpr int seq_unit(int D, bool q4) { return kSeqWarps * (q4 ? seq4_keys(D) : seq_keys(D)); }  // keys per unit
 __host__ __device__ constexpr int seq_stage_bytes(int D) { return 2 * seq_keys(D) * D * 2; }
 
-// A cache in 4 bits (Q4): stages of 32 keys hold codes and params as they are, unpacked on the way to the products.
+// A cache in 4 bits (Q4): stages hold codes and params as they are, unpacked on the way to the products.
 template <typename ArgsT>
 constexpr bool kIsInt4 = __is_same(ArgsT, Seq4Args);
-constexpr int kSeq4Keys = 32;
-__host__ __device__ constexpr int seq4_stages(int D) { return D == 64 ? 5 : 3; }
+__host__ __device__ constexpr int seq4_stages(int D) { return D == 64 ? 2 : 3; }
 // CTAs per SM: unpacking is work that more warps hide better.
 __host__ __device__ constexpr int seq4_ctas(int D, int NT) { return NT > 1 ? 2 : D == 64 ? 4 : 3; }
-__host__ __device__ constexpr int seq4_stage_bytes(int D) { return 2 * kSeq4Keys * (D / 2 + D / kGroup4 * 4); }
+__host__ __device__ constexpr int seq4_stage_bytes(int D) { return 2 * seq4_keys(D) * (D / 2 + D / kGroup4 * 4); }
 
-__host__ __device__ constexpr int seq_stage_keys(int D, bool q4) { return q4 ? kSeq4Keys : seq_keys(D); }
+__host__ __device__ constexpr int seq_stage_keys(int D, bool q4) { return q4 ? seq4_keys(D) : seq_keys(D); }
 __host__ __device__ constexpr int seq_stage_count(int D, bool q4) { return q4 ? seq4_stages(D) : kSeqStages; }
 __host__ __device__ constexpr int seq_stage_size(int D, bool q4) { return q4 ? seq4_stage_bytes(D) : seq_stage_bytes(D); }
 // outputs of the warps and one part of them, in the ring's place
@@ -224,11 +225,20 @@ __device__ __forceinline__ void load_stage(const SeqAttnArgs& a, const KeyPages<
 }
 
 // ---- a cache in 4 bits
-// The page of one key (a stage has a key per lane), -1 past the end; asked for a stage ahead of its use, like key_pages.
-__device__ __forceinline__ int key_page4(const Seq4Args& a, int b, int j, int end) {
-  int page = -1;
-  if (j < end) page = a.tables[(long long)b * a.table_stride + (j >> a.log_page)];
-  return page;
+// The pages of the lane's keys (j, and j + 32 in a stage of 64), -1 past the end; asked for a stage ahead of its use, like key_pages.
+template <int D>
+struct KeyPages4 {
+  int page[seq4_keys(D) / 32];
+};
+template <int D>
+__device__ __forceinline__ KeyPages4<D> key_pages4(const Seq4Args& a, int b, int j, int end) {
+  KeyPages4<D> k;
+#pragma unroll
+  for (int h = 0; h < seq4_keys(D) / 32; ++h) {
+    k.page[h] = -1;
+    if (j + 32 * h < end) k.page[h] = a.tables[(long long)b * a.table_stride + ((j + 32 * h) >> a.log_page)];
+  }
+  return k;
 }
 
 // Keys or values of one KV head; offsets of codes in 16 bytes and of params in pairs fit 32 bits (int4_offsets_fit), so an
@@ -255,38 +265,42 @@ __device__ __forceinline__ void cp_async16n(uint32_t dst, const void* src, uint3
 
 // A stage: codes of the keys' and the values' rows, then their params.  Rows of no page are zeros (page 0 is not read).
 template <int D>
-__device__ __forceinline__ void load_stage4(const Seq4Args& a, const Head4& k, const Head4& v, int my_page, int j0, uint32_t stage) {
-  constexpr int CH = D / 32, RPI = 32 / CH, G = D / kGroup4;
+__device__ __forceinline__ void load_stage4(const Seq4Args& a, const Head4& k, const Head4& v, KeyPages4<D> pages, int j0, uint32_t stage) {
+  constexpr int CH = D / 32, RPI = 32 / CH, G = D / kGroup4, KK = seq4_keys(D);
   const int lane = threadIdx.x & 31, c = lane % CH, mask = (1 << a.log_page) - 1;
-  if ((unsigned)my_page >= (unsigned)a.num_pages) my_page = -1;
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    const int r = i * RPI + lane / CH;
-    const uint32_t row = (j0 + r) & mask;
-    const int page = __shfl_sync(0xffffffffu, my_page, r);
-    const uint32_t bytes = page >= 0 && c * 32 < a.hd ? 16 : 0, pg = max(page, 0);
-    const uint32_t at = stage + r * (D / 2) + c * 16;
-    cp_async16n(at, k.codes + (uint64_t)(pg * k.cp + row * k.ct + c) * 16, bytes);
-    cp_async16n(at + kSeq4Keys * (D / 2), v.codes + (uint64_t)(pg * v.cp + row * v.ct + c) * 16, bytes);
-  }
-  const uint32_t row = (j0 + lane) & mask, pg = max(my_page, 0), all = my_page >= 0 ? G * 4 : 0;
-  const uint32_t* kp = k.params + (pg * k.pp + row * k.pt);
-  const uint32_t* vp = v.params + (pg * v.pp + row * v.pt);
-  const uint32_t at = stage + kSeq4Keys * D + lane * (G * 4);
-  if (a.wide_params) {
-    if constexpr (D == 64) {
-      cp_async8z(at, kp, all);
-      cp_async8z(at + kSeq4Keys * G * 4, vp, all);
-    } else {
-      cp_async16n(at, kp, all);
-      cp_async16n(at + kSeq4Keys * G * 4, vp, all);
+  for (int h = 0; h < KK / 32; ++h) {
+    int my_page = pages.page[h];
+    if ((unsigned)my_page >= (unsigned)a.num_pages) my_page = -1;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int r = i * RPI + lane / CH;
+      const uint32_t row = (j0 + 32 * h + r) & mask;
+      const int page = __shfl_sync(0xffffffffu, my_page, r);
+      const uint32_t bytes = page >= 0 && c * 32 < a.hd ? 16 : 0, pg = max(page, 0);
+      const uint32_t at = stage + (32 * h + r) * (D / 2) + c * 16;
+      cp_async16n(at, k.codes + (uint64_t)(pg * k.cp + row * k.ct + c) * 16, bytes);
+      cp_async16n(at + KK * (D / 2), v.codes + (uint64_t)(pg * v.cp + row * v.ct + c) * 16, bytes);
     }
-  } else {
+    const uint32_t row = (j0 + 32 * h + lane) & mask, pg = max(my_page, 0), all = my_page >= 0 ? G * 4 : 0;
+    const uint32_t* kp = k.params + (pg * k.pp + row * k.pt);
+    const uint32_t* vp = v.params + (pg * v.pp + row * v.pt);
+    const uint32_t at = stage + KK * D + (32 * h + lane) * (G * 4);
+    if (a.wide_params) {
+      if constexpr (D == 64) {
+        cp_async8z(at, kp, all);
+        cp_async8z(at + KK * G * 4, vp, all);
+      } else {
+        cp_async16n(at, kp, all);
+        cp_async16n(at + KK * G * 4, vp, all);
+      }
+    } else {
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const bool have = g * kGroup4 < a.hd;
-      cp_async4z(at + g * 4, have ? kp + g : kp, have ? all / G : 0);
-      cp_async4z(at + kSeq4Keys * G * 4 + g * 4, have ? vp + g : vp, have ? all / G : 0);
+      for (int g = 0; g < G; ++g) {
+        const bool have = g * kGroup4 < a.hd;
+        cp_async4z(at + g * 4, have ? kp + g : kp, have ? all / G : 0);
+        cp_async4z(at + KK * G * 4 + g * 4, have ? vp + g : vp, have ? all / G : 0);
+      }
     }
   }
 }
@@ -305,7 +319,7 @@ template <typename T, int D>
 __device__ __forceinline__ void key_fragments4(const uint8_t* stage, int key, uint32_t kf[][4]) {
   constexpr int G = D / kGroup4;
   const int t = threadIdx.x & 3;
-  const uint32_t* kp = reinterpret_cast<const uint32_t*>(stage + kSeq4Keys * D);
+  const uint32_t* kp = reinterpret_cast<const uint32_t*>(stage + seq4_keys(D) * D);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int r = key + 8 * h;
@@ -335,8 +349,8 @@ template <typename T, int D>
 __device__ __forceinline__ void value_fragments4(const uint8_t* stage, int key, uint32_t vf[][4]) {
   constexpr int G = D / kGroup4, W = D / 64;
   const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
-  const uint8_t* codes = stage + kSeq4Keys * (D / 2);
-  const uint32_t* vp = reinterpret_cast<const uint32_t*>(stage + kSeq4Keys * D) + kSeq4Keys * G;
+  const uint8_t* codes = stage + seq4_keys(D) * (D / 2);
+  const uint32_t* vp = reinterpret_cast<const uint32_t*>(stage + seq4_keys(D) * D) + seq4_keys(D) * G;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int ra = key + 8 * h, rb = key - t + 7 - t + 8 * h;
@@ -516,7 +530,7 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
     [[maybe_unused]] Head4 k4, v4;
     if constexpr (Q4) k4 = head4(a.k4, kvh), v4 = head4(a.v4, kvh);
     auto pages_of = [&](int j0) {
-      if constexpr (Q4) return key_page4(a, b, j0 + lane, k1);
+      if constexpr (Q4) return key_pages4<D>(a, b, j0 + lane, k1);
       else return key_pages<D, PAGED>(a, b, j0, k1);
     };
     auto load = [&](const auto& page, int j0, uint32_t stage) {
@@ -665,30 +679,33 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
       }
       if constexpr (Q4) {
         if (j0 + KW - 1 > first_lim) {
-          uint32_t* vp = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(stage4) + kSeq4Keys * D) + kSeq4Keys * (D / kGroup4);
           constexpr int G = D / kGroup4;
-          bool odd = false;  // lane's key is hidden from some row and has a group that is not finite
+          uint32_t* vp = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(stage4) + KW * D) + KW * G;
+#pragma unroll 1
+          for (int r0 = 0; r0 < KW; r0 += 32) {
+            bool odd = false;  // lane's key is hidden from some row and has a group that is not finite
 #pragma unroll
-          for (int g = 0; g < G; ++g) odd |= params_not_finite<T>(vp[lane * G + g]);
-          unsigned bad = __ballot_sync(0xffffffffu, odd && j0 + lane > first_lim);
-          for (unsigned rest = bad; rest != 0; rest &= rest - 1) {
-            const int r = __ffs(rest) - 1;
-            if (params_not_finite<T>(vp[r * G + (lane / 4) * G / 8])) {  // this thread's dims lie in one group
+            for (int g = 0; g < G; ++g) odd |= params_not_finite<T>(vp[(r0 + lane) * G + g]);
+            odd = odd && j0 + r0 + lane > first_lim;
+            for (unsigned rest = __ballot_sync(0xffffffffu, odd); rest != 0; rest &= rest - 1) {
+              const int r = r0 + __ffs(rest) - 1;
+              if (params_not_finite<T>(vp[r * G + (lane / 4) * G / 8])) {  // this thread's dims lie in one group
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                  if (j0 + r <= lim[nt][e]) {
+                  for (int e = 0; e < 2; ++e)
+                    if (j0 + r <= lim[nt][e]) {
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) o[dt][nt][e] = o[dt][nt][2 + e] = NAN;
-                  }
+                      for (int dt = 0; dt < DT; ++dt) o[dt][nt][e] = o[dt][nt][2 + e] = NAN;
+                    }
+              }
             }
-          }
-          __syncwarp();
-          if (odd && j0 + lane > first_lim) {
+            __syncwarp();
+            if (odd) {
 #pragma unroll
-            for (int g = 0; g < G; ++g)
-              if (params_not_finite<T>(vp[lane * G + g])) vp[lane * G + g] = 0u;
+              for (int g = 0; g < G; ++g)
+                if (params_not_finite<T>(vp[(r0 + lane) * G + g])) vp[(r0 + lane) * G + g] = 0u;
+            }
           }
           __syncwarp();
         }
