@@ -5,12 +5,13 @@
 // in one pass: a thread's base moves with its largest value, once per tile of 32 values, and sums with different bases join as
 // S' = f S, W' = f (W + d S), d = (b - b') log2(e), f = 2^d.
 //
-// The likeliest tokens: the threads are cut into 32 groups, and the top-th largest of the groups' maxima so far bounds
-// the top-th largest value of the row from below.  Values that reach the bound are set aside: of a row of V
-// values in random order some 32 ln(32 / (32 - top)) by the first tile and fewer by every later one (20 of 128256: about a
-// hundred).  Their order decides at the end: 64-bit keys of (value's order, inverted index), ranked by counting.
-// A bound may be old: it only has to be one.  A row whose values rise or are equal can set aside more than there is room
-// for; its likeliest are then found one after the other, a pass over the row each.
+// The likeliest tokens: a thread keeps the largest values of its two best tiles, which tiles these were, and the largest of its
+// other tiles.  At the end, of each warp's 32 largest values the j-th, and of these the c-th largest among the warps, j c >= top, bounds
+// the top-th largest of all from below.  The few threads whose largest reaches the bound read that tile again, and the
+// second (a warp reads all tiles of a thread where a third reaches it) and set such values aside; 64-bit keys of (value's order, inverted index) give their
+// order, ranked by counting.  (Values set aside tile by tile, against a bound that grows: 2047 rows of 128256 fp16 values, 8
+// likeliest, 148 us, one fp32 row, 20 likeliest, 12.2 us.)  A row whose values are equal can have more of them than there is
+// room for; its likeliest are then found one after the other, a pass over the row each.
 //
 // A cluster of 1, 2, 4 or 8 CTAs takes a row.  Bound by the bytes of the logits where there are many rows, by two trips to memory and
 // the cluster's join where there are few.
@@ -25,8 +26,11 @@ namespace cg = cooperative_groups;
 
 constexpr int kLogThreads = 256;
 constexpr int kLogWarps = kLogThreads / 32;
-constexpr int kLogValues = 32;   // of a thread in a tile
-constexpr int kLogTile = kLogThreads * kLogValues;
+// 16-byte loads of a thread in a tile, CTAs per SM: 16 values either way, and as many CTAs as their registers allow (2047 rows of
+// 128256 fp16 values, 8 likeliest: 126 us, with four loads and three CTAs 141; 1023 rows of fp32: 92 us, with two and five 108).
+__host__ __device__ constexpr int log_loads(int bytes) { return bytes == 4 ? 4 : 2; }
+__host__ __device__ constexpr int log_ctas(int bytes) { return bytes == 4 ? 4 : 5; }
+constexpr int kLogTile = kLogThreads * 16;  // values
 constexpr int kLogAside = 2048;  // keys set aside per CTA
 constexpr int kMaxTop = LI4_MAX_TOP;
 constexpr int kLogCluster = 8;
@@ -81,6 +85,38 @@ __device__ __forceinline__ float t_of(float x, float b) { return maxn((x - b) * 
 struct Sums {
   float b, s, w;  // base, sum 2^t, sum 2^t t
 };
+
+// Two fp32 lanes at once.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float max_of3(float a, float b, float c) {  // (drops NaN)
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ Sums join(const Sums& x, const Sums& y) {
   const float b = fmaxf(x.b, y.b);
   // (a base of -infinity: nothing but -infinity seen, sums of 0)
@@ -89,71 +125,152 @@ __device__ __forceinline__ Sums join(const Sums& x, const Sums& y) {
   return {b, fx * x.s + fy * y.s, fx * (x.w + dx * x.s) + fy * (y.w + dy * y.s)};
 }
 
-// The bound: values x with !(x <= bound) are set aside.  The top-th largest of 32 maxima less one step (equal values
-// belong to those set aside), or -infinity itself.
-__device__ __forceinline__ float bound_of(float group_max, int top) {
+// The j-th largest of a warp's values (j from 1 to 4), on every lane.
+__device__ __forceinline__ float warp_largest(float x, int j) {
   const int lane = threadIdx.x & 31;
+  if (j == 1) {
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    return x;
+  }
+#pragma unroll
+  for (int k = 2; k <= 32; k *= 2)  // a sorting network, the largest on lane 0
+#pragma unroll
+    for (int d = k / 2; d > 0; d /= 2) {
+      const float y = __shfl_xor_sync(0xffffffffu, x, d);
+      x = ((lane & d) == 0) == ((lane & k) == 0) ? fmaxf(x, y) : fminf(x, y);
+    }
+  return __shfl_sync(0xffffffffu, x, j - 1);
+}
+
+// Values x with !(x <= bound) are set aside.  The c-th largest of the warps' values less one step (equal values belong to
+// those set aside), or -infinity itself.
+__device__ __forceinline__ float bound_of(const float* of_warp, int c) {
+  const float x = of_warp[threadIdx.x % kLogWarps];
   int above = 0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const float v = __shfl_sync(0xffffffffu, group_max, i);
-    above += v > group_max || (v == group_max && i < lane) ? 1 : 0;
+  for (int w = 0; w < kLogWarps; ++w) {
+    const float y = __shfl_sync(0xffffffffu, x, w);
+    above += y > x || (y == x && w < (int)threadIdx.x % kLogWarps) ? 1 : 0;
   }
-  const unsigned at = __ballot_sync(0xffffffffu, above == top - 1);
-  const float x = __shfl_sync(0xffffffffu, group_max, __ffs(at) - 1);
-  return x == -INFINITY ? x : nextafterf(x, -INFINITY);
+  const unsigned at = __ballot_sync(0xffffffffu, above == c - 1);
+  const float v = __shfl_sync(0xffffffffu, x, __ffs(at) - 1);
+  const unsigned u = __float_as_uint(v + 0.f);  // one step down: towards 0 above it, away from it below
+  return v == -INFINITY ? v : __uint_as_float(v > 0.f ? u - 1 : u == 0 ? 0x80000001u : u + 1);
+}
+
+// Sixteen bytes of logits: their largest value (NaN dropped), pair e of them.
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static __device__ __forceinline__ float largest(const uint4& r) {
+    return max_of3(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), __uint_as_float(r.z), __uint_as_float(r.w));
+  }
+  static __device__ __forceinline__ float2 two(const uint4& r, int e) {
+    return e == 0 ? make_float2(__uint_as_float(r.x), __uint_as_float(r.y)) : make_float2(__uint_as_float(r.z), __uint_as_float(r.w));
+  }
+};
+__device__ __forceinline__ uint32_t word(const uint4& r, int e) { return e == 0 ? r.x : e == 1 ? r.y : e == 2 ? r.z : r.w; }
+template <>
+struct Vec<__half> {
+  static __device__ __forceinline__ float largest(const uint4& r) {
+    const __half2 m = __hmax2(__hmax2(u32_as_h2(r.x), u32_as_h2(r.y)), __hmax2(u32_as_h2(r.z), u32_as_h2(r.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ float2 two(const uint4& r, int e) { return __half22float2(u32_as_h2(word(r, e))); }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static __device__ __forceinline__ __nv_bfloat162 b2(uint32_t u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); }
+  static __device__ __forceinline__ float largest(const uint4& r) {
+    const __nv_bfloat162 m = __hmax2(__hmax2(b2(r.x), b2(r.y)), __hmax2(b2(r.z), b2(r.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ float2 two(const uint4& r, int e) {
+    const uint32_t w = word(r, e);  // (a bf16 is the high half of its fp32)
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+};
+
+// Joins a Sums of each of the lowest N lanes, on lane 0.
+template <int N>
+__device__ __forceinline__ Sums join_lanes(Sums x) {
+#pragma unroll
+  for (int d = 1; d < N; d *= 2)
+    x = join(x, {__shfl_xor_sync(0xffffffffu, x.b, d), __shfl_xor_sync(0xffffffffu, x.s, d), __shfl_xor_sync(0xffffffffu, x.w, d)});
+  return x;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLogThreads, 4) token_logprobs_kernel(const __grid_constant__ LogArgs a) {
-  constexpr int VEC = 16 / sizeof(T), LOADS = kLogValues / VEC;
-  __shared__ unsigned long long s_aside[kLogAside];
-  __shared__ unsigned long long s_top[kMaxTop];                 // the CTA's likeliest, in order
-  __shared__ unsigned long long s_all[kLogCluster * kMaxTop];   // rank 0: every CTA's
+__global__ void __launch_bounds__(kLogThreads, log_ctas(sizeof(T))) token_logprobs_kernel(const __grid_constant__ LogArgs a) {
+  constexpr int VEC = 16 / sizeof(T), kLogLoads = log_loads(sizeof(T)), STEP = kLogThreads * kLogLoads;
+  __shared__ __align__(16) unsigned long long s_aside[kLogAside];
+  __shared__ __align__(16) unsigned long long s_top[kMaxTop];                // the CTA's likeliest, in order
+  __shared__ __align__(16) unsigned long long s_all[kLogCluster * kMaxTop];  // rank 0: every CTA's
   __shared__ unsigned long long s_best[kLogWarps];
-  __shared__ float s_group[32];
+  __shared__ float s_warp[kLogWarps];  // each warp's j-th largest
   __shared__ Sums s_sums[kLogWarps];
-  __shared__ Sums s_row;        // the CTA's
-  __shared__ float s_bound;
+  __shared__ Sums s_row;               // the CTA's
   __shared__ int s_n;
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = (int)cluster.block_rank(), C = (int)cluster.num_blocks();
   const long long r = blockIdx.x / C;
   const int V = a.cols, top = a.top;
+  const int j = (top + kLogWarps - 1) / kLogWarps, c = j > 0 ? (top + j - 1) / j : 0;
   pdl_launch_dependents();
+  if (tid == 0) s_n = 0;  // (counted in after a barrier)
   pdl_wait_primary();
 
   const T* row = static_cast<const T*>(a.logits) + r * a.stride;
   // vector v of the row: values VEC v - off .. VEC v - off + VEC - 1, on 16-byte boundaries
   const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+  const uint4* vec = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row) & ~uintptr_t(15));
   const int vectors = (int)(((long long)V + off + VEC - 1) / VEC);
   const int v0 = (int)((long long)vectors * rank / C), v1 = (int)((long long)vectors * (rank + 1) / C);
-  if (tid == 0) s_n = 0;
+  // vectors that lie wholly in the row, of this CTA
+  const int c0 = max(v0, off > 0 ? 1 : 0), c1 = min(v1, (int)(((long long)V + off) / VEC));
+  auto clean = [&](int t0) { return t0 >= c0 && t0 + STEP <= c1; };
 
   Sums sum = {-INFINITY, 0.f, 0.f};
-  float group_max = -INFINITY, bound = -INFINITY;
-  bool first = true;
-  for (int t0 = v0; t0 < v1; t0 += kLogThreads * LOADS) {
-    float x[kLogValues];
+  float most = -INFINITY, second = -INFINITY, other = -INFINITY;  // of the thread's tiles: the two best, the best of the rest
+  int most_at = v0, second_at = v0;
+  uint4 raw[kLogLoads], next[kLogLoads];
+  auto load = [&](uint4* to, int t0) {
 #pragma unroll
-    for (int l = 0; l < LOADS; ++l) {
-      const int v = t0 + l * kLogThreads + tid;
-      const long long e0 = (long long)v * VEC - off;
-      if (v < v1 && e0 >= 0 && e0 + VEC <= V) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(row + e0);
-        const T* p = reinterpret_cast<const T*>(&raw);
+    for (int l = 0; l < kLogLoads; ++l) to[l] = __ldg(vec + t0 + l * kLogThreads + tid);
+  };
+  if (clean(v0)) load(next, v0);
+  for (int t0 = v0; t0 < v1; t0 += STEP) {
+    if (clean(t0)) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) x[l * VEC + e] = logit<T>(p[e]);
-      } else {
+      for (int l = 0; l < kLogLoads; ++l) raw[l] = next[l];
+    } else {
+      constexpr uint32_t LOW = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;  // -infinity
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          x[l * VEC + e] = v < v1 && e0 + e >= 0 && e0 + e < V ? logit<T>(row[e0 + e]) : -INFINITY;
+      for (int l = 0; l < kLogLoads; ++l) {
+        const int v = t0 + l * kLogThreads + tid;
+        raw[l] = make_uint4(LOW, LOW, LOW, LOW);
+        if (v >= c0 && v < c1) {
+          raw[l] = __ldg(vec + v);
+        } else if (v < v1) {  // a vector that the row's end cuts, value by value; -infinity beside them
+          uint32_t u[4] = {LOW, LOW, LOW, LOW};
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const long long at = (long long)v * VEC - off + e;
+            if (at < 0 || at >= V) continue;
+            if constexpr (sizeof(T) == 4) u[e] = reinterpret_cast<const uint32_t*>(row)[at];
+            else u[e >> 1] = __byte_perm(u[e >> 1], reinterpret_cast<const uint16_t*>(row)[at], e & 1 ? 0x5410 : 0x3254);
+          }
+          raw[l] = make_uint4(u[0], u[1], u[2], u[3]);
+        }
       }
     }
-    float m = x[0];
+    if (t0 + STEP < v1 && clean(t0 + STEP)) load(next, t0 + STEP);
+    float m = Vec<T>::largest(raw[0]);
 #pragma unroll
-    for (int e = 1; e < kLogValues; ++e) m = fmaxf(m, x[e]);
+    for (int l = 1; l < kLogLoads; ++l) m = fmaxf(m, Vec<T>::largest(raw[l]));
     if (m > sum.b) {
       const float d = sum.b == -INFINITY ? 0.f : t_of(sum.b, m), f = ex2(d);
       sum.w = f * (sum.w + d * sum.s);
@@ -161,67 +278,111 @@ __global__ void __launch_bounds__(kLogThreads, 4) token_logprobs_kernel(const __
       sum.b = m;
     }
     const float base = sum.b == -INFINITY ? 0.f : sum.b;
-    float s = 0.f, w = 0.f;
+    const uint64_t nb = pair(-base, -base), l2e = pair(kLog2e, kLog2e);
+    uint64_t s2 = 0, w2 = 0;
 #pragma unroll
-    for (int e = 0; e < kLogValues; ++e) {
-      const float t = t_of(x[e], base);
-      const float p = ex2(t);
-      s += p;
-      w = fmaf(p, t, w);
+    for (int l = 0; l < kLogLoads; ++l)
+#pragma unroll
+      for (int e = 0; e < VEC / 2; ++e) {
+        const float2 x = Vec<T>::two(raw[l], e);
+        const uint64_t t = mul_pair(add_pair(pair(x.x, x.y), nb), l2e);
+        const float2 tf = halves(t);
+        const uint64_t p = pair(ex2(tf.x), ex2(tf.y));
+        s2 = add_pair(s2, p);
+        w2 = fma_pair(p, t, w2);
+      }
+    const float2 ss = halves(s2), ww = halves(w2);
+    const float s = ss.x + ss.y;
+    float w = ww.x + ww.y;
+    if (w != w) {  // 0 x -infinity: values of probability 0 add 0 (a NaN stays one)
+      w = 0.f;
+#pragma unroll
+      for (int l = 0; l < kLogLoads; ++l)
+#pragma unroll
+        for (int e = 0; e < VEC / 2; ++e) {
+          const float2 x = Vec<T>::two(raw[l], e);
+          const float t = t_of(x.x, base), u = t_of(x.y, base);
+          w = fmaf(ex2(u), u, fmaf(ex2(t), t, w));
+        }
     }
     sum.s += s;
     sum.w += w;
-    if (top > 0) {
-      // groups of 8 threads
-      group_max = fmaxf(group_max, m);
-      float g = group_max;
-#pragma unroll
-      for (int d = 1; d < 8; d *= 2) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, d));
-      if ((lane & 7) == 0) *const_cast<volatile float*>(&s_group[tid / 8]) = g;
-      if (first) {
-        __syncthreads();
-        bound = bound_of(s_group[lane], top);
-        if (tid == 0) *const_cast<volatile float*>(&s_bound) = bound;
-        __syncthreads();
-      } else {
-        bound = *const_cast<volatile float*>(&s_bound);
-        if (warp == 0) {  // (the other groups' maxima may be of this tile or the last: a bound either way)
-          bound = bound_of(*const_cast<volatile float*>(&s_group[lane]), top);
-          if (lane == 0) *const_cast<volatile float*>(&s_bound) = bound;
-        }
-      }
-      first = false;
-      if (!(m <= bound) || s != s) {
-#pragma unroll
-        for (int e = 0; e < kLogValues; ++e)
-          if (!(x[e] <= bound)) {
-            const int at = atomicAdd(&s_n, 1);
-            const long long index = (long long)(t0 + e / VEC * kLogThreads + tid) * VEC - off + e % VEC;
-            if (at < kLogAside) s_aside[at] = key_of(x[e], (int)index);
-          }
-      }
+    other = fmaxf(other, fminf(m, second));
+    if (m > second) {
+      const bool best = m > most;
+      second_at = best ? most_at : t0;
+      second = best ? most : m;
+      most_at = best ? t0 : most_at;
+      most = best ? m : most;
     }
   }
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2)
-    sum = join(sum, {__shfl_xor_sync(0xffffffffu, sum.b, d), __shfl_xor_sync(0xffffffffu, sum.s, d),
-                     __shfl_xor_sync(0xffffffffu, sum.w, d)});
+  const bool nan = sum.s != sum.s;  // (or an infinity: either way every value is looked at)
+  sum = join_lanes<32>(sum);
   if (lane == 0) s_sums[warp] = sum;
+  if (top > 0) {
+    const float g = warp_largest(most, j);
+    if (lane == 0) s_warp[warp] = g;
+    if (tid < kMaxTop) s_top[tid] = 0;
+  }
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kLogWarps; ++w) sum = join(sum, s_sums[w]);
-    s_row = sum;
+  if (warp == kLogWarps - 1) {
+    sum = join_lanes<kLogWarps>(s_sums[lane % kLogWarps]);
+    if (lane == 0) s_row = sum;
   }
   // ---- the CTA's likeliest, in order; places that no value fills have key 0
   if (top > 0) {
-    const int n = s_n;
-    if (tid < kMaxTop) s_top[tid] = 0;
+    const float bound = bound_of(s_warp, c);
+    // sets aside what reaches the bound of the values of thread `who` in the tile at t0
+    auto take = [&](int t0, int who) {
+      unsigned mine = 0;  // a bit per value
+#pragma unroll
+      for (int l = 0; l < kLogLoads; ++l) {
+        const int v = t0 + l * kLogThreads + who;
+        const long long e0 = (long long)v * VEC - off;
+        if (v >= c0 && v < c1) {
+          const uint4 again = __ldg(vec + v);
+#pragma unroll
+          for (int e = 0; e < VEC; e += 2) {
+            const float2 x = Vec<T>::two(again, e / 2);
+            mine |= (x.x <= bound ? 0u : 1u << (l * VEC + e)) | (x.y <= bound ? 0u : 2u << (l * VEC + e));
+          }
+        } else if (v < v1) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (e0 + e >= 0 && e0 + e < V && !(logit<T>(row[e0 + e]) <= bound)) mine |= 1u << (l * VEC + e);
+        }
+      }
+      if (mine != 0) {
+        int at = atomicAdd(&s_n, __popc(mine));
+        for (; mine != 0; mine &= mine - 1, ++at) {
+          const int b = __ffs(mine) - 1;
+          const long long index = (long long)(t0 + b / VEC * kLogThreads + who) * VEC - off + b % VEC;
+          if (at < kLogAside) s_aside[at] = key_of(logit<T>(row[index]), (int)index);
+        }
+      }
+    };
+    const int tiles = (v1 - v0 + STEP - 1) / STEP;
+    if (nan) {
+      for (int i = 0; i < tiles; ++i) take(v0 + i * STEP, tid);
+    } else if (most > bound && !(other > bound)) {
+      take(most_at, tid);
+      if (second > bound) take(second_at, tid);
+    }
+    // a thread whose third tile reaches the bound: the warp reads all of that thread's, a tile per lane
+    for (unsigned whole = __ballot_sync(0xffffffffu, !nan && other > bound); whole != 0; whole &= whole - 1)
+      for (int i = lane; i < tiles; i += 32) take(v0 + i * STEP, warp * 32 + __ffs(whole) - 1);
     __syncthreads();
+    const int n = s_n;
     if (n <= kLogAside) {
       for (int i = tid; i < n; i += kLogThreads) {
         const unsigned long long key = s_aside[i];
-        int above = 0;
-        for (int j = 0; j < n; ++j) above += s_aside[j] > key ? 1 : 0;
+        int above = 0, k = 0;
+#pragma unroll 4
+        for (; k + 2 <= n; k += 2) {
+          const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(s_aside + k);
+          above += (two.x > key ? 1 : 0) + (two.y > key ? 1 : 0);
+        }
+        if (k < n) above += s_aside[k] > key ? 1 : 0;
         if (above < top) s_top[above] = key;
       }
     } else {
@@ -247,23 +408,27 @@ __global__ void __launch_bounds__(kLogThreads, 4) token_logprobs_kernel(const __
       }
     }
   }
-  cluster.sync();
+  if (C > 1) cluster.sync();
+  else __syncthreads();
   // ---- the row's
   if (rank == 0) {
-    if (tid < C * kMaxTop && top > 0)
-      s_all[tid] = tid % kMaxTop < top ? cluster.map_shared_rank(s_top, tid / kMaxTop)[tid % kMaxTop] : 0ull;
-    Sums all = s_row;
-    for (int c = 1; c < C; ++c) all = join(all, *cluster.map_shared_rank(&s_row, c));
-    const float l2 = all.b == -INFINITY ? NAN : log2f(all.s), base = all.b;
+    if (tid < C * top) s_all[tid] = cluster.map_shared_rank(s_top, tid / top)[tid % top];
+    if (C > 1 && warp == kLogWarps - 1) {
+      sum = join_lanes<kLogCluster>(lane < C ? *cluster.map_shared_rank(&s_row, lane) : Sums{-INFINITY, 0.f, 0.f});
+      if (lane == 0) s_sums[0] = sum;
+    }
     __syncthreads();
+    const Sums all = C > 1 ? s_sums[0] : s_row;
+    const float l2 = all.b == -INFINITY ? NAN : log2f(all.s), base = all.b;
     auto logprob = [&](float x) { return (x - base) - kLn2 * l2; };
     if (top > 0) {
-      const unsigned long long key = tid < C * kMaxTop ? s_all[tid] : 0;
-      int above = 0, values = 0;
-      for (int j = 0; j < C * kMaxTop; ++j) {
-        above += s_all[j] > key ? 1 : 0;
-        values += s_all[j] != 0 ? 1 : 0;
-      }
+      const unsigned long long key = tid < C * top ? s_all[tid] : 0;
+      const int values = __syncthreads_count(key != 0);
+      int above = 0;
+      if (C == 1) above = tid;
+      else if (key != 0)
+#pragma unroll 4
+        for (int k = 0; k < C * top; ++k) above += s_all[k] > key ? 1 : 0;
       if (key != 0 && above < top) {
         a.top_ids[r * top + above] = index_of(key);
         a.top_logprobs[r * top + above] = logprob(value_of(key));
@@ -291,7 +456,7 @@ __global__ void __launch_bounds__(kLogThreads, 4) token_logprobs_kernel(const __
       if (a.entropy) a.entropy[r] = kLn2 * (l2 - all.w / all.s);
     }
   }
-  cluster.sync();  // (the shared memory of every CTA is read until here)
+  if (C > 1) cluster.sync();  // (the shared memory of every CTA is read until here)
 }
 
 template <typename T>
