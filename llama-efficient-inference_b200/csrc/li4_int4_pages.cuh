@@ -33,9 +33,8 @@ struct Codes4<__half> {
   static __device__ __forceinline__ uint16_t nearest(double x) {
     return __half_as_ushort(__float2half_rn(__double2float_rn(x)));  // (by way of 32 bits)
   }
-  static __device__ __forceinline__ uint16_t down(double x) {  // towards zero; x >= 0
-    return __half_as_ushort(__float2half_rz(__double2float_rz(x)));
-  }
+  static __device__ __forceinline__ uint16_t cut(float x) { return __half_as_ushort(__float2half_rz(x)); }  // towards zero
+  static __device__ __forceinline__ uint16_t down(double x) { return cut(__double2float_rz(x)); }          // x >= 0
 };
 template <>
 struct Codes4<__nv_bfloat16> {
@@ -57,9 +56,8 @@ struct Codes4<__nv_bfloat16> {
   static __device__ __forceinline__ uint16_t nearest(double x) {
     return __bfloat16_as_ushort(__float2bfloat16_rn(__double2float_rn(x)));
   }
-  static __device__ __forceinline__ uint16_t down(double x) {
-    return __bfloat16_as_ushort(__float2bfloat16_rz(__double2float_rz(x)));
-  }
+  static __device__ __forceinline__ uint16_t cut(float x) { return __bfloat16_as_ushort(__float2bfloat16_rz(x)); }
+  static __device__ __forceinline__ uint16_t down(double x) { return cut(__double2float_rz(x)); }
 };
 
 // (s, s) and (m, m) of a pair of parameters.

@@ -2,7 +2,7 @@
 //
 // With t_j = (x_j - b) log2(e) for a base b, the largest value, S = sum 2^t_j and W = sum 2^t_j t_j give
 //   log p_j = x_j - b - ln 2 log2 S,   entropy = ln 2 (log2 S - W / S)
-// in one pass: a thread's base moves with its largest value, once per tile of 32 values, and sums with different bases join as
+// in one pass: a thread's base moves with its largest value, once per tile of 16 values, and sums with different bases join as
 // S' = f S, W' = f (W + d S), d = (b - b') log2(e), f = 2^d.
 //
 // The likeliest tokens: a thread keeps the largest values of its two best tiles, which tiles these were, and the largest of its

@@ -319,8 +319,9 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_write_kernel(const __
 // ---------------------------------------------------------------------------
 // RoPE and the write into a cache in 4 bits.  A thread owns 8 dims of one token as above, so four neighbouring threads
 // hold a group of 32: its smallest and largest value cross them by two shuffles each, and every thread packs its eight codes
-// into one word.  Whatever decides a code is exact or in 64 bits: a key is turned in 64 bits, the scale
-// is a 64-bit quotient cut to the type, and a code whose 32-bit quotient lies near a border is found again in 64 bits.
+// into one word.  The codes are those of arithmetic in 64 bits, which 32 bits nearly always decide: a turned key, a scale and
+// a code are computed in 32 bits with a bound on their error, and found again in 64 where a border of the result's type or between
+// two codes lies within it.  (All in 64 bits, 16381 tokens of 8 KV heads of 128 dims took 139 us.)  Bound by HBM.
 // ---------------------------------------------------------------------------
 struct Rope4Args {
   const uint16_t* q;
@@ -351,14 +352,31 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+__device__ __noinline__ float code_exact(float x, float m, float s) {
+  return (float)rint(((double)x - (double)m) / (double)s);
+}
 // The code of x: its 32-bit quotient t is off by less than 30 x 3 x 2^-24 < 1e-5 (the difference, the reciprocal and the product
 // each round once, and t <= 30 where s is a subnormal), so a nearest integer of distance below 0.4999 is the right one.  The
 // test fails too where the difference or the reciprocal overflows.
 __device__ __forceinline__ int code_of(float x, float m, float s, float inv) {
   const float t = (x - m) * inv;
   float c = rintf(t);
-  if (!(fabsf(t - c) < 0.4999f)) c = (float)rint(((double)x - (double)m) / (double)s);
+  if (!(fabsf(t - c) < 0.4999f)) c = code_exact(x, m, s);
   return (int)fminf(c, 15.f);
+}
+
+// (hi - lo) / 15 cut to the type.  In 32 bits it is off by less than 3 x 2^-24 of itself; where the cut is the same a little below
+// and above, it is the right one.
+template <typename T>
+__device__ __noinline__ uint16_t scale_exact(float lo, float hi) {
+  return Codes4<T>::down(((double)hi - (double)lo) / 15.0);
+}
+template <typename T>
+__device__ __forceinline__ uint16_t scale_of(float lo, float hi) {
+  if (hi == lo) return 0;
+  const float q = (hi - lo) * (1.f / 15.f);
+  const uint16_t below = Codes4<T>::cut(q * (1.f - 0x1p-21f)), above = Codes4<T>::cut(q * (1.f + 0x1p-21f));
+  return below == above && q < 1e37f && q > 1e-30f ? below : scale_exact<T>(lo, hi);
 }
 
 // Eight values of this thread's group -> their word of codes, the group's (s, m) (the same in its four threads).
@@ -381,7 +399,7 @@ __device__ __forceinline__ uint32_t quantize8(uint4 x, uint32_t* params) {
   }
   lo += 0.f;  // (-0 becomes 0)
   const bool finite = lo > -INFINITY && hi < INFINITY;
-  const uint16_t s16 = Codes4<T>::down(((double)hi - (double)lo) / 15.0);
+  const uint16_t s16 = scale_of<T>(lo, hi);
   const float s = Codes4<T>::value(s16), inv = 1.f / s;
   uint32_t w = 0;
   if (finite && s > 0.f) {
@@ -393,21 +411,34 @@ __device__ __forceinline__ uint32_t quantize8(uint4 x, uint32_t* params) {
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 turn8_exact(uint4 x, const float4& c, const float4& s) {
+__device__ __noinline__ uint32_t turn_exact(uint32_t u, float c, float s) {
+  const double a = Codes4<T>::value((uint16_t)u), b = Codes4<T>::value((uint16_t)(u >> 16));
+  // (products of 11 and 24 bits are exact)
+  return Codes4<T>::nearest(a * c - b * s) | (uint32_t)Codes4<T>::nearest(a * s + b * c) << 16;
+}
+
+// Keys turned as in 64 bits.  A product's rounding is taken off again, so a turned value v is off by less than 2^-22 |v| in 32
+// bits; where the values a little below and above round to the same, that is it (of fp16 keys all but one in a thousand).
+template <typename T, typename T2>
+__device__ __forceinline__ uint4 turn8_keys(uint4 x, const float4& c, const float4& s) {
   const uint32_t u[4] = {x.x, x.y, x.z, x.w};
   const float cf[4] = {c.x, c.y, c.z, c.w}, sf[4] = {s.x, s.y, s.z, s.w};
   uint32_t r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const double a = Codes4<T>::value((uint16_t)u[i]), b = Codes4<T>::value((uint16_t)(u[i] >> 16));
-    // (products of 11 and 24 bits are exact)
-    r[i] = Codes4<T>::nearest(a * cf[i] - b * sf[i]) | (uint32_t)Codes4<T>::nearest(a * sf[i] + b * cf[i]) << 16;
+    const float2 p = Pair<T2>::load(u[i]);
+    const float ys = p.y * sf[i], yc = p.y * cf[i];
+    const float v0 = fmaf(p.x, cf[i], -ys) - fmaf(p.y, sf[i], -ys), v1 = fmaf(p.x, sf[i], yc) + fmaf(p.y, cf[i], -yc);
+    r[i] = Pair<T2>::store(v0 - 0x1p-22f * v0, v1 - 0x1p-22f * v1);
+    // (below 2^-100 the products' roundings may not be numbers any more)
+    const bool tiny = (fabsf(v0) < 0x1p-100f || fabsf(v1) < 0x1p-100f) && u[i] != 0;
+    if (tiny || r[i] != Pair<T2>::store(v0 + 0x1p-22f * v0, v1 + 0x1p-22f * v1)) r[i] = turn_exact<T>(u[i], cf[i], sf[i]);
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
 template <typename T, typename T2>
-__global__ void __launch_bounds__(kRopeThreads) rope_paged_write_int4_kernel(const __grid_constant__ Rope4Args a) {
+__global__ void __launch_bounds__(kRopeThreads, 4) rope_paged_write_int4_kernel(const __grid_constant__ Rope4Args a) {
   pdl_launch_dependents();
   pdl_wait_primary();
   const long long i = (long long)blockIdx.x * kRopeThreads + threadIdx.x;
@@ -442,7 +473,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_write_int4_kernel(con
     }
   };
   for_heads(max(h0 - a.H, 0), min(h1 - a.H, a.Hkv), a.k + t * a.skt + d, a.skh, [&](int h, uint4 x) {
-    put(a.ck, h, turn8_exact<T>(x, c, s), a.k_out ? a.k_out + t * a.skot + (long long)h * a.skoh + d : nullptr);
+    put(a.ck, h, turn8_keys<T, T2>(x, c, s), a.k_out ? a.k_out + t * a.skot + (long long)h * a.skoh + d : nullptr);
   });
   for_heads(max(h0 - a.H - a.Hkv, 0), h1 - a.H - a.Hkv, a.v + t * a.svt + d, a.svh, [&](int h, uint4 x) {
     put(a.cv, h, x, a.v_out ? a.v_out + t * a.svot + (long long)h * a.svoh + d : nullptr);
