@@ -269,15 +269,15 @@ __device__ __forceinline__ uint4 turn8(uint4 x, const float4& c, const float4& s
                     Pair<T2>::store(e.x * c.w - e.y * s.w, e.x * s.w + e.y * c.w));
 }
 
-template <typename F>
+template <int N = 4, typename F>
 __device__ __forceinline__ void for_heads(int h0, int h1, const uint16_t* src, long long stride, F&& put) {
-  for (int h = h0; h < h1; h += 4) {
-    uint4 x[4];
+  for (int h = h0; h < h1; h += N) {
+    uint4 x[N];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < N; ++i)
       if (h + i < h1) x[i] = *reinterpret_cast<const uint4*>(src + (long long)(h + i) * stride);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < N; ++i)
       if (h + i < h1) put(h + i, x[i]);
   }
 }
@@ -341,28 +341,49 @@ struct Rope4Args {
   int T, H, Hkv, chunks, log_page, max_pos, heads_per_group;
 };
 
-__device__ __forceinline__ float min_nan(float a, float b) {
+// (NaN where one of them is)
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
   float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
 __device__ __noinline__ float code_exact(float x, float m, float s) {
-  return (float)rint(((double)x - (double)m) / (double)s);
+  const double c = rint(((double)x - (double)m) / (double)s);
+  return c < 15.0 ? (float)c : 15.f;
 }
-// The code of x: its 32-bit quotient t is off by less than 30 x 3 x 2^-24 < 1e-5 (the difference, the reciprocal and the product
-// each round once, and t <= 30 where s is a subnormal), so a nearest integer of distance below 0.4999 is the right one.  The
-// test fails too where the difference or the reciprocal overflows.
-__device__ __forceinline__ int code_of(float x, float m, float s, float inv) {
-  const float t = (x - m) * inv;
-  float c = rintf(t);
-  if (!(fabsf(t - c) < 0.4999f)) c = code_exact(x, m, s);
-  return (int)fminf(c, 15.f);
+// The code c of x beside a border: d = x - m and r = d - c s, both rounded.  Where the difference is exact so is r (of few digits),
+// and says which side the border lies on; equal distances go to the even code.
+__device__ __noinline__ float code_beside(float x, float m, float s, float c, float d) {
+  const float back = d - x, lost = (x - (d - back)) - (m + back);  // what d's rounding has lost
+  const float r = fmaf(-c, s, d), half = 0.5f * s;
+  if (lost != 0.f || !(c <= 15.f) || !(half > 0x1p-120f) || !(fabsf(d) < 1e37f)) return code_exact(x, m, s);
+  const bool odd = (__float_as_uint(c + 12582912.f) & 1u) != 0;
+  if (fabsf(r) > half || (fabsf(r) == half && odd)) c += copysignf(1.f, r);
+  return fminf(c, 15.f);
+}
+// The word of eight codes.  In 32 bits a code c is the nearest integer of a quotient; r = x - m - c s, off by less than 2^-20 s
+// (x - m rounds once, below 16 s), shows that no other is nearer, or that the border is near (of 16-bit types with few digits
+// often: quotients halfway between two integers).  Adding 1.5 x 2^23 rounds to an integer; the codes are put together as numbers,
+// four at a time below 2^16.
+__device__ __forceinline__ uint32_t codes_of(const float f[8], float m, float s) {
+  constexpr float kRound = 12582912.f;
+  const float inv = 1.f / s, near = s * (0.5f - 0x1p-18f);
+  float c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float d = f[i] - m;
+    c[i] = (d * inv + kRound) - kRound;
+    if (!(fabsf(fmaf(-c[i], s, d)) < near) || !(c[i] <= 15.f)) c[i] = code_beside(f[i], m, s, c[i], d);
+  }
+  const float even = fmaf(fmaf(fmaf(c[6], 16.f, c[4]), 16.f, c[2]), 16.f, c[0]) + 8388608.f;
+  const float odd = fmaf(fmaf(fmaf(c[7], 16.f, c[5]), 16.f, c[3]), 16.f, c[1]) + 8388608.f;
+  return __byte_perm(__float_as_uint(even), __float_as_uint(odd), 0x5410);
 }
 
 // (hi - lo) / 15 cut to the type.  In 32 bits it is off by less than 3 x 2^-24 of itself; where the cut is the same a little below
@@ -386,54 +407,55 @@ __device__ __forceinline__ uint32_t quantize8(uint4 x, uint32_t* params) {
   float f[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = Codes4<T>::value((uint16_t)(u[i >> 1] >> (i & 1) * 16));
-  float lo = f[0], hi = f[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = min_nan(lo, f[i]);
-    hi = max_nan(hi, f[i]);
-  }
-#pragma unroll
-  for (int d = 1; d < 4; d *= 2) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-  }
+  float lo = min_nan(f[0], f[1], f[2]), hi = max_nan(f[0], f[1], f[2]);
+  lo = min_nan(lo, f[3], f[4]), hi = max_nan(hi, f[3], f[4]);
+  lo = min_nan(lo, f[5], f[6]), hi = max_nan(hi, f[5], f[6]);
+  lo = min_nan(lo, f[7], __shfl_xor_sync(0xffffffffu, min_nan(lo, f[7], f[7]), 1));
+  hi = max_nan(hi, f[7], __shfl_xor_sync(0xffffffffu, max_nan(hi, f[7], f[7]), 1));
+  lo = min_nan(lo, lo, __shfl_xor_sync(0xffffffffu, lo, 2));
+  hi = max_nan(hi, hi, __shfl_xor_sync(0xffffffffu, hi, 2));
   lo += 0.f;  // (-0 becomes 0)
   const bool finite = lo > -INFINITY && hi < INFINITY;
   const uint16_t s16 = scale_of<T>(lo, hi);
-  const float s = Codes4<T>::value(s16), inv = 1.f / s;
-  uint32_t w = 0;
-  if (finite && s > 0.f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w |= (uint32_t)code_of(f[i], lo, s, inv) << (4 * (i >> 1) + 16 * (i & 1));
-  }
+  const float s = Codes4<T>::value(s16);
+  const uint32_t w = finite && s > 0.f ? codes_of(f, lo, s) : 0u;
   *params = finite ? (uint32_t)s16 | (uint32_t)Codes4<T>::nearest(lo) << 16 : Codes4<T>::NaN2;
   return w;
 }
 
 template <typename T>
-__device__ __noinline__ uint32_t turn_exact(uint32_t u, float c, float s) {
-  const double a = Codes4<T>::value((uint16_t)u), b = Codes4<T>::value((uint16_t)(u >> 16));
-  // (products of 11 and 24 bits are exact)
-  return Codes4<T>::nearest(a * c - b * s) | (uint32_t)Codes4<T>::nearest(a * s + b * c) << 16;
-}
-
-// Keys turned as in 64 bits.  A product's rounding is taken off again, so a turned value v is off by less than 2^-22 |v| in 32
-// bits; where the values a little below and above round to the same, that is it (of fp16 keys all but one in a thousand).
-template <typename T, typename T2>
-__device__ __forceinline__ uint4 turn8_keys(uint4 x, const float4& c, const float4& s) {
+__device__ __noinline__ uint4 turn8_exact(uint4 x, float4 c, float4 s) {
   const uint32_t u[4] = {x.x, x.y, x.z, x.w};
   const float cf[4] = {c.x, c.y, c.z, c.w}, sf[4] = {s.x, s.y, s.z, s.w};
   uint32_t r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    const double a = Codes4<T>::value((uint16_t)u[i]), b = Codes4<T>::value((uint16_t)(u[i] >> 16));
+    // (products of 11 and 24 bits are exact)
+    r[i] = Codes4<T>::nearest(a * cf[i] - b * sf[i]) | (uint32_t)Codes4<T>::nearest(a * sf[i] + b * cf[i]) << 16;
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// Keys turned as in 64 bits.  A product's rounding is taken off again, so a turned value v is off by less than 2^-23 |v| in 32
+// bits; where the values a little below and above round to the same, that is it (of fp16 keys all but one in a thousand).
+// Below 2^-100 the products' roundings may not be numbers any more.
+template <typename T, typename T2>
+__device__ __forceinline__ uint4 turn8_keys(uint4 x, const float4& c, const float4& s) {
+  const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+  const float cf[4] = {c.x, c.y, c.z, c.w}, sf[4] = {s.x, s.y, s.z, s.w};
+  uint32_t r[4], differ = 0;
+  float least = 1.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
     const float2 p = Pair<T2>::load(u[i]);
     const float ys = p.y * sf[i], yc = p.y * cf[i];
     const float v0 = fmaf(p.x, cf[i], -ys) - fmaf(p.y, sf[i], -ys), v1 = fmaf(p.x, sf[i], yc) + fmaf(p.y, cf[i], -yc);
-    r[i] = Pair<T2>::store(v0 - 0x1p-22f * v0, v1 - 0x1p-22f * v1);
-    // (below 2^-100 the products' roundings may not be numbers any more)
-    const bool tiny = (fabsf(v0) < 0x1p-100f || fabsf(v1) < 0x1p-100f) && u[i] != 0;
-    if (tiny || r[i] != Pair<T2>::store(v0 + 0x1p-22f * v0, v1 + 0x1p-22f * v1)) r[i] = turn_exact<T>(u[i], cf[i], sf[i]);
+    r[i] = Pair<T2>::store(fmaf(v0, -0x1p-22f, v0), fmaf(v1, -0x1p-22f, v1));
+    differ |= r[i] ^ Pair<T2>::store(fmaf(v0, 0x1p-22f, v0), fmaf(v1, 0x1p-22f, v1));
+    least = fminf(least, fminf(fabsf(v0), fabsf(v1)));
   }
+  if (differ != 0 || !(least > 0x1p-100f)) return turn8_exact<T>(x, c, s);
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
@@ -472,10 +494,10 @@ __global__ void __launch_bounds__(kRopeThreads, 4) rope_paged_write_int4_kernel(
       *reinterpret_cast<uint4*>(held) = make_uint4(u[0], u[1], u[2], u[3]);
     }
   };
-  for_heads(max(h0 - a.H, 0), min(h1 - a.H, a.Hkv), a.k + t * a.skt + d, a.skh, [&](int h, uint4 x) {
+  for_heads<1>(max(h0 - a.H, 0), min(h1 - a.H, a.Hkv), a.k + t * a.skt + d, a.skh, [&](int h, uint4 x) {
     put(a.ck, h, turn8_keys<T, T2>(x, c, s), a.k_out ? a.k_out + t * a.skot + (long long)h * a.skoh + d : nullptr);
   });
-  for_heads(max(h0 - a.H - a.Hkv, 0), h1 - a.H - a.Hkv, a.v + t * a.svt + d, a.svh, [&](int h, uint4 x) {
+  for_heads<1>(max(h0 - a.H - a.Hkv, 0), h1 - a.H - a.Hkv, a.v + t * a.svt + d, a.svh, [&](int h, uint4 x) {
     put(a.cv, h, x, a.v_out ? a.v_out + t * a.svot + (long long)h * a.svoh + d : nullptr);
   });
 }
