@@ -1,17 +1,18 @@
 // li4_fork.cu -- requests of a paged KV cache that go on from others, or end: tables, free pages, page copies, sm_100a.
 //
 // Which pages come back is a question about all tables at once: a page that a request lets go may be held by another, before
-// the call and after it.  One cluster answers it in four passes over the lines of held pages (a line: the pages of
-// all requests, request after request, as prefix sums of their counts number them; a warp takes a run of a line):
-//   1  owner[page] = none, for every page that some request lets go
+// the call and after it.  One cluster answers it in passes over the lines of held pages (a line: the pages of all requests,
+// request after request, as prefix sums of their counts number them; a warp takes a run of a line):
+//   1  owner[page] = none, everywhere, while the requests are read and their needs summed
 //   2  owner[page] = 0 for every page that some request holds after the call, the least 1 + place on the line among
 //      the requests that let it go otherwise (a minimum, so the order of threads does not matter); the entries that
 //      requests take over are set aside, since the rows they come from may be written
 //   3  a let-go entry whose place stands in owner is where a page comes back: counted, and by the warps' counts
 //      before it numbered
-//   4  those pages go on the stack, and then the rows are written
-// A second launch copies the pages that are not full.  The tables cost a few trips to L2 and cluster barriers between
-// them, the copies their bytes.
+//   4  those pages go on the stack, and the rows are written
+// Bound by latency: trips to L2 one after another and cluster barriers between them.  A warp keeps its entries from pass 2 on
+// where its run is short (kForkKept); otherwise it reads them again.
+// A second launch copies the pages that are not full, bound by their bytes.
 #include <cooperative_groups.h>
 
 #include "li4_common.cuh"
@@ -25,6 +26,7 @@ constexpr int kForkMaxRequests = 8192;
 constexpr int kForkThreads = 512;
 constexpr int kForkWarps = kForkThreads / 32;
 constexpr int kForkCtas = 8;
+constexpr int kForkKept = 4;  // groups of 32 entries of the line that a warp keeps
 constexpr int kCopyThreads = 256;
 constexpr int kCopyBytes = 8192;  // of a page that a CTA copies at a time
 
@@ -52,6 +54,7 @@ struct ForkShared {
   int* old_at;  // [B + 1] first place on the line of pages held before
   int* take_at; // [B + 1] and on that of pages taken over
   int* fresh;   // [B] number of its page for the part of a page; -1: none
+  int* len;     // [B] tokens it holds after the call
 };
 
 // Exclusive sums of three counts over the CTA's threads.
@@ -122,6 +125,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const __grid_c
   s.old_at = s.source + a.B;
   s.take_at = s.old_at + a.B + 1;
   s.fresh = s.take_at + a.B + 1;
+  s.len = s.fresh + a.B;
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, rank = (int)cluster.block_rank(), C = (int)cluster.num_blocks();
   const int warp = rank * kForkWarps + (tid >> 5), warps = C * kForkWarps;
@@ -129,39 +133,40 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const __grid_c
   pdl_launch_dependents();
   pdl_wait_primary();
 
+  // ---- 1: no owner yet
+  for (int p = rank * kForkThreads + tid; p < a.capacity; p += C * kForkThreads) a.owner[p] = 0xffffffffu;
+  cluster.barrier_arrive();
   // ---- what happens to each request (every CTA works it out for itself)
   const int n_free = max(0, min(*a.n_free, a.capacity));
   const int per = (a.B + kForkThreads - 1) / kForkThreads;
   const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
-  auto asks = [&](int b, int* parent, int* from_len) {  // whether the request takes tokens over, and from whom
-    const int p = a.parents[b];
-    *parent = p;
-    *from_len = 0;
-    if (p < 0 || p == b || p >= a.B) return false;
-    *from_len = a.kv_lens[p];
-    return fits(a, *from_len);
-  };
   Counts3 sum = {0, 0, 0};
   for (int b = b0; b < b1; ++b) {
-    int p, len;
-    if (asks(b, &p, &len) && (len & (page - 1)) != 0) ++sum.a;
+    const int p = a.parents[b], own = a.kv_lens[b];
+    const bool other = p >= 0 && p != b && p < a.B;
+    const int len = other ? a.kv_lens[p] : p == b ? own : 0;
+    const bool none = p < -1 || p >= a.B || (other && !fits(a, len));  // no request to go on from
+    s.source[b] = none ? -2 : p;
+    s.len[b] = len;
+    s.old_at[b] = own;
+    if (other && !none && (len & (page - 1)) != 0) ++sum.a;
   }
   Counts3 total;
   int wanted = block_scan3(sum, warp_sums, &total).a;  // pages asked for before this thread's requests
   sum = {0, 0, 0};
   for (int b = b0; b < b1; ++b) {
-    int p, len;
-    const bool comes = asks(b, &p, &len);
+    const int p = s.source[b], len = s.len[b], own = s.old_at[b];
+    const bool comes = p >= 0 && p != b;
     const bool part = comes && (len & (page - 1)) != 0;
-    const bool ok = comes ? !part || wanted + 1 <= n_free : p == b || p == -1;
+    const bool ok = comes ? !part || wanted + 1 <= n_free : p != -2;
     s.source[b] = ok ? p : b;
     s.fresh[b] = ok && part ? wanted : -1;
+    s.len[b] = ok ? len : own;
     if (part) ++wanted;
-    const int old = held_pages(a, a.kv_lens[b]);
-    s.old_at[b] = old;
+    s.old_at[b] = held_pages(a, own);
     s.take_at[b] = ok && comes ? held_pages(a, len) : 0;
     if (rank == 0) a.granted[b] = ok ? 1 : 0;
-    sum.a += old;
+    sum.a += s.old_at[b];
     sum.b += s.take_at[b];
     sum.c += s.fresh[b] >= 0 ? 1 : 0;
   }
@@ -181,24 +186,29 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const __grid_c
     s.take_at[a.B] = total.b;
   }
   const int taken = total.c;  // fresh pages: numbers 0 .. taken - 1 from the top of the stack
+  const bool kept = total.a <= (long long)warps * kForkKept * 32 - warps;  // (the same for every warp)
   __syncthreads();
+  cluster.barrier_wait();
 
   auto entry = [&](int r, int j) { return a.tables[(long long)r * a.table_stride + j]; };
   auto is_page = [&](int p) { return (unsigned)p < (unsigned)a.capacity; };
-  // ---- 1: no owner yet
-  for_line(s.old_at, a.B, warp, warps, [&](int r, int j, int) {
-    if (r < 0 || s.source[r] == r) return;
-    const int p = entry(r, j);
-    if (is_page(p)) a.owner[p] = 0xffffffffu;
-  });
-  cluster.sync();
   // ---- 2: owners; what is taken over is set aside
+  int mine[kForkKept];  // this lane's entries of requests that let them go; -1: none
+#pragma unroll
+  for (int i = 0; i < kForkKept; ++i) mine[i] = -1;
+  const int run0 = (int)((long long)total.a * warp / warps);
   for_line(s.old_at, a.B, warp, warps, [&](int r, int j, int place) {
     if (r < 0) return;
     const int p = entry(r, j);
     if (!is_page(p)) return;
-    if (s.source[r] == r) a.owner[p] = 0;  // (no minimum is less)
-    else atomicMin(a.owner + p, (unsigned)place + 1u);
+    if (s.source[r] == r) {
+      a.owner[p] = 0;  // (no minimum is less)
+    } else {
+      atomicMin(a.owner + p, (unsigned)place + 1u);
+#pragma unroll
+      for (int i = 0; i < kForkKept; ++i)
+        if ((place - run0) >> 5 == i) mine[i] = p;
+    }
   });
   for_line(s.take_at, a.B, warp, warps, [&](int r, int j, int place) {
     if (r < 0) return;
@@ -213,10 +223,6 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const __grid_c
       if (is_page(p)) a.owner[p] = 0;
     }
   });
-  // (the lengths may be overwritten: every CTA has read them before the first barrier, this one reads the parents' here)
-  int new_len[(kForkMaxRequests + kForkThreads - 1) / kForkThreads];
-#pragma unroll 1
-  for (int b = b0, i = 0; rank == 0 && b < b1; ++b, ++i) new_len[i] = s.source[b] < 0 ? 0 : a.kv_lens[s.source[b]];
   cluster.sync();
   // ---- 3: how many come back in this warp's run
   auto comes_back = [&](int r, int j, int place) {
@@ -224,14 +230,21 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const __grid_c
     const int p = entry(r, j);
     return is_page(p) && a.owner[p] == (unsigned)place + 1u ? p : -1;
   };
-  int mine = 0;
-  for_line(s.old_at, a.B, warp, warps,
-           [&](int r, int j, int place) { mine += __popc(__ballot_sync(0xffffffffu, comes_back(r, j, place) >= 0)); });
-  if (lane == 0) a.counts[warp] = mine;
-  if (rank == 0) {
-#pragma unroll 1
-    for (int b = b0, i = 0; b < b1; ++b, ++i) a.kv_out[b] = new_len[i];
+  int back = 0;
+  if (kept) {
+    unsigned owner[kForkKept];
+#pragma unroll
+    for (int i = 0; i < kForkKept; ++i) owner[i] = mine[i] >= 0 ? a.owner[mine[i]] : 0u;
+#pragma unroll
+    for (int i = 0; i < kForkKept; ++i) {
+      if (owner[i] != (unsigned)(run0 + 32 * i + lane) + 1u) mine[i] = -1;
+      back += __popc(__ballot_sync(0xffffffffu, mine[i] >= 0));
+    }
+  } else {
+    for_line(s.old_at, a.B, warp, warps,
+             [&](int r, int j, int place) { back += __popc(__ballot_sync(0xffffffffu, comes_back(r, j, place) >= 0)); });
   }
+  if (lane == 0) a.counts[warp] = back;
   cluster.sync();
   // ---- 4: onto the stack, in the line's order; then the rows
   int ahead = 0, all = 0;
@@ -243,20 +256,29 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const __grid_c
   ahead = __reduce_add_sync(0xffffffffu, ahead);
   all = __reduce_add_sync(0xffffffffu, all);
   int height = n_free - taken + ahead;
-  for_line(s.old_at, a.B, warp, warps, [&](int r, int j, int place) {
-    const int p = comes_back(r, j, place);
-    const unsigned back = __ballot_sync(0xffffffffu, p >= 0);
-    const int at = height + __popc(back & ((1u << lane) - 1u));
+  auto put = [&](int p) {
+    const unsigned hit = __ballot_sync(0xffffffffu, p >= 0);
+    const int at = height + __popc(hit & ((1u << lane) - 1u));
     if (p >= 0 && at < a.capacity) a.free_pages[at] = p;  // (a page on the stack twice is the caller's mistake)
-    height += __popc(back);
-  });
-  cluster.sync();
+    height += __popc(hit);
+  };
+  if (kept) {
+#pragma unroll
+    for (int i = 0; i < kForkKept; ++i) put(mine[i]);
+  } else {
+    for_line(s.old_at, a.B, warp, warps, [&](int r, int j, int place) { put(comes_back(r, j, place)); });
+    cluster.sync();  // the rows have been read
+  }
   for_line(s.take_at, a.B, warp, warps, [&](int r, int j, int place) {
     if (r >= 0) a.tables[(long long)r * a.table_stride + j] = a.aside[place];
   });
-  if (rank == 0 && tid == 0) {
-    *a.n_free_out = min(a.capacity, n_free - taken + all);
-    *a.n_copies = taken;
+  if (rank == 0) {
+    // (the lengths and the stack's height may be overwritten: every CTA has read them before the first barrier's end)
+    for (int b = tid; b < a.B; b += kForkThreads) a.kv_out[b] = s.len[b];
+    if (tid == 0) {
+      *a.n_free_out = min(a.capacity, n_free - taken + all);
+      *a.n_copies = taken;
+    }
   }
 }
 
@@ -320,7 +342,7 @@ static int launch_fork(KernelT kernel, const ArgsT& a, unsigned grid, int thread
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, a), "paged_fork: kernel launch");
 }
 
-static size_t fork_shared_bytes(int64_t B) { return (size_t)(4 * B + 2) * sizeof(int); }
+static size_t fork_shared_bytes(int64_t B) { return (size_t)(5 * B + 2) * sizeof(int); }
 
 // Workspace: copies, owner, aside, counts and the number of copies.
 struct ForkSpace {

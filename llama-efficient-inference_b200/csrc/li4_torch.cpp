@@ -639,10 +639,11 @@ PyObject* paged_fork(PyObject* const* v) {
   std::vector<void*> pools(n_pools);
   std::vector<int64_t> strides(n_pools), bytes(n_pools);
   for (int64_t i = 0; i < n_pools; ++i) {
-    const std::string name = c10::str("pools[", i, "]");
-    const Tensor t = tensor(what, name.c_str(), PySequence_Fast_GET_ITEM(seq, i));
-    d.add(name.c_str(), t);
-    if (t.dim() < 1 || t.size(0) < capacity) fail(what, name, " must have ", capacity, " pages at least, got ", t.sizes());
+    const char* name = "a tensor of pools";
+    const Tensor t = tensor(what, name, PySequence_Fast_GET_ITEM(seq, i));
+    d.add(name, t);
+    if (t.dim() < 1 || t.size(0) < capacity)
+      fail(what, "pools[", i, "] must have ", capacity, " pages at least, got ", t.sizes());
     // a page is one block of memory, in whatever order of its dimensions
     int64_t block = 1, left = 1;
     for (int64_t k = 1; k < t.dim(); ++k) left *= t.size(k);
@@ -658,7 +659,7 @@ PyObject* paged_fork(PyObject* const* v) {
     }
     const int64_t size = t.element_size();
     if (block != values || values < 1 || (t.size(0) > 1 && t.stride(0) < values))
-      fail(what, name, ": a page must be one block of memory, apart from the others");
+      fail(what, "pools[", i, "]: a page must be one block of memory, apart from the others");
     pools[i] = t.data_ptr();
     bytes[i] = values * size;
     strides[i] = t.size(0) > 1 ? t.stride(0) * size : values * size;
