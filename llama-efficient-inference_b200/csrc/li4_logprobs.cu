@@ -1,8 +1,8 @@
 // li4_logprobs.cu -- log probabilities of given tokens, entropy and the likeliest tokens of rows of logits, sm_100a.
 //
-// With t_j = (x_j - b) log2(e) for a base b, the largest value, S = sum 2^t_j and W = sum 2^t_j t_j give
+// With t_j = (x_j - b) log2(e) for a base b near the largest value, S = sum 2^t_j and W = sum 2^t_j t_j give
 //   log p_j = x_j - b - ln 2 log2 S,   entropy = ln 2 (log2 S - W / S)
-// in one pass: a thread's base moves with its largest value, once per tile of 16 values, and sums with different bases join as
+// in one pass: a thread's base follows its largest value, at a distance of up to 4, and sums with different bases join as
 // S' = f S, W' = f (W + d S), d = (b - b') log2(e), f = 2^d.
 //
 // The likeliest tokens: a thread keeps the largest values of its two best tiles, which tiles these were, and the largest of its
@@ -26,14 +26,17 @@ namespace cg = cooperative_groups;
 
 constexpr int kLogThreads = 256;
 constexpr int kLogWarps = kLogThreads / 32;
-// 16-byte loads of a thread in a tile, CTAs per SM: 16 values either way, and as many CTAs as their registers allow (2047 rows of
-// 128256 fp16 values, 8 likeliest: 126 us, with four loads and three CTAs 141; 1023 rows of fp32: 92 us, with two and five 108).
+// Of a type's values: 16-byte loads of a thread under way at a time, how many such steps make a tile.  16 values a step; the larger
+// tile halves the bookkeeping beside 16-bit values, whose exponentials and unpacking bound (2047 rows of 128256 fp16 values, 8
+// likeliest: 121 us; tiles of one step 126 us, of one step of four loads 141 us), fp32 rows want the smaller one (one row, 20
+// likeliest: 10.3 us, with tiles of two steps 12.1 us).  Four CTAs per SM, five for bf16 (130 us instead of 147).
 __host__ __device__ constexpr int log_loads(int bytes) { return bytes == 4 ? 4 : 2; }
-__host__ __device__ constexpr int log_ctas(int bytes) { return bytes == 4 ? 4 : 5; }
+__host__ __device__ constexpr int log_steps(int bytes) { return bytes == 4 ? 1 : 2; }
 constexpr int kLogTile = kLogThreads * 16;  // values
 constexpr int kLogAside = 2048;  // keys set aside per CTA
 constexpr int kMaxTop = LI4_MAX_TOP;
 constexpr int kLogCluster = 8;
+constexpr float kLag = 4.f;  // how far a thread's base may lag behind its largest value: 2^t <= e^4
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct LogArgs {
@@ -203,8 +206,9 @@ __device__ __forceinline__ Sums join_lanes(Sums x) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLogThreads, log_ctas(sizeof(T))) token_logprobs_kernel(const __grid_constant__ LogArgs a) {
+__global__ void __launch_bounds__(kLogThreads, __is_same(T, __nv_bfloat16) ? 5 : 4) token_logprobs_kernel(const __grid_constant__ LogArgs a) {
   constexpr int VEC = 16 / sizeof(T), kLogLoads = log_loads(sizeof(T)), STEP = kLogThreads * kLogLoads;
+  constexpr int STEPS = log_steps(sizeof(T)), TILE = STEPS * STEP;
   __shared__ __align__(16) unsigned long long s_aside[kLogAside];
   __shared__ __align__(16) unsigned long long s_top[kMaxTop];                // the CTA's likeliest, in order
   __shared__ __align__(16) unsigned long long s_all[kLogCluster * kMaxTop];  // rank 0: every CTA's
@@ -233,7 +237,6 @@ __global__ void __launch_bounds__(kLogThreads, log_ctas(sizeof(T))) token_logpro
   const int c0 = max(v0, off > 0 ? 1 : 0), c1 = min(v1, (int)(((long long)V + off) / VEC));
   auto clean = [&](int t0) { return t0 >= c0 && t0 + STEP <= c1; };
 
-  Sums sum = {-INFINITY, 0.f, 0.f};
   float most = -INFINITY, second = -INFINITY, other = -INFINITY;  // of the thread's tiles: the two best, the best of the rest
   int most_at = v0, second_at = v0;
   uint4 raw[kLogLoads], next[kLogLoads];
@@ -242,80 +245,91 @@ __global__ void __launch_bounds__(kLogThreads, log_ctas(sizeof(T))) token_logpro
     for (int l = 0; l < kLogLoads; ++l) to[l] = __ldg(vec + t0 + l * kLogThreads + tid);
   };
   if (clean(v0)) load(next, v0);
-  for (int t0 = v0; t0 < v1; t0 += STEP) {
-    if (clean(t0)) {
+  uint64_t run_s = 0, run_w = 0;  // pairs of sums against base b
+  float b = -INFINITY, nb = 0.f;  // the base, which may lag behind the largest value by kLag; minus it, or 0
+  for (int t0 = v0; t0 < v1; t0 += TILE) {
+    float best = -INFINITY;
 #pragma unroll
-      for (int l = 0; l < kLogLoads; ++l) raw[l] = next[l];
-    } else {
-      constexpr uint32_t LOW = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;  // -infinity
+    for (int h = 0; h < STEPS; ++h) {
+      const int at = t0 + h * STEP;
+      if (at >= v1) break;
+      if (clean(at)) {
 #pragma unroll
-      for (int l = 0; l < kLogLoads; ++l) {
-        const int v = t0 + l * kLogThreads + tid;
-        raw[l] = make_uint4(LOW, LOW, LOW, LOW);
-        if (v >= c0 && v < c1) {
-          raw[l] = __ldg(vec + v);
-        } else if (v < v1) {  // a vector that the row's end cuts, value by value; -infinity beside them
-          uint32_t u[4] = {LOW, LOW, LOW, LOW};
+        for (int l = 0; l < kLogLoads; ++l) raw[l] = next[l];
+      } else {
+        constexpr uint32_t LOW = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;  // -infinity
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const long long at = (long long)v * VEC - off + e;
-            if (at < 0 || at >= V) continue;
-            if constexpr (sizeof(T) == 4) u[e] = reinterpret_cast<const uint32_t*>(row)[at];
-            else u[e >> 1] = __byte_perm(u[e >> 1], reinterpret_cast<const uint16_t*>(row)[at], e & 1 ? 0x5410 : 0x3254);
+        for (int l = 0; l < kLogLoads; ++l) {
+          const int v = at + l * kLogThreads + tid;
+          raw[l] = make_uint4(LOW, LOW, LOW, LOW);
+          if (v >= c0 && v < c1) {
+            raw[l] = __ldg(vec + v);
+          } else if (v < v1) {  // a vector that the row's end cuts, value by value; -infinity beside them
+            uint32_t u[4] = {LOW, LOW, LOW, LOW};
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const long long at = (long long)v * VEC - off + e;
+              if (at < 0 || at >= V) continue;
+              if constexpr (sizeof(T) == 4) u[e] = reinterpret_cast<const uint32_t*>(row)[at];
+              else u[e >> 1] = __byte_perm(u[e >> 1], reinterpret_cast<const uint16_t*>(row)[at], e & 1 ? 0x5410 : 0x3254);
+            }
+            raw[l] = make_uint4(u[0], u[1], u[2], u[3]);
           }
-          raw[l] = make_uint4(u[0], u[1], u[2], u[3]);
         }
       }
-    }
-    if (t0 + STEP < v1 && clean(t0 + STEP)) load(next, t0 + STEP);
-    float m = Vec<T>::largest(raw[0]);
+      if (at + STEP < v1 && clean(at + STEP)) load(next, at + STEP);
+      float m = Vec<T>::largest(raw[0]);
 #pragma unroll
-    for (int l = 1; l < kLogLoads; ++l) m = fmaxf(m, Vec<T>::largest(raw[l]));
-    if (m > sum.b) {
-      const float d = sum.b == -INFINITY ? 0.f : t_of(sum.b, m), f = ex2(d);
-      sum.w = f * (sum.w + d * sum.s);
-      sum.s *= f;
-      sum.b = m;
-    }
-    const float base = sum.b == -INFINITY ? 0.f : sum.b;
-    const uint64_t nb = pair(-base, -base), l2e = pair(kLog2e, kLog2e);
-    uint64_t s2 = 0, w2 = 0;
-#pragma unroll
-    for (int l = 0; l < kLogLoads; ++l)
-#pragma unroll
-      for (int e = 0; e < VEC / 2; ++e) {
-        const float2 x = Vec<T>::two(raw[l], e);
-        const uint64_t t = mul_pair(add_pair(pair(x.x, x.y), nb), l2e);
-        const float2 tf = halves(t);
-        const uint64_t p = pair(ex2(tf.x), ex2(tf.y));
-        s2 = add_pair(s2, p);
-        w2 = fma_pair(p, t, w2);
+      for (int l = 1; l < kLogLoads; ++l) m = fmaxf(m, Vec<T>::largest(raw[l]));
+      best = fmaxf(best, m);
+      if (m - kLag > b) {
+        const float d = b == -INFINITY ? 0.f : t_of(b, m), f = ex2(d);
+        const float2 ss = halves(run_s), ww = halves(run_w);
+        run_s = pair(f * ss.x, f * ss.y);
+        run_w = pair(f * fmaf(d, ss.x, ww.x), f * fmaf(d, ss.y, ww.y));
+        b = m;
+        nb = -m;
       }
-    const float2 ss = halves(s2), ww = halves(w2);
-    const float s = ss.x + ss.y;
-    float w = ww.x + ww.y;
-    if (w != w) {  // 0 x -infinity: values of probability 0 add 0 (a NaN stays one)
-      w = 0.f;
+      const uint64_t nb2 = pair(nb, nb), l2e = pair(kLog2e, kLog2e);
+      uint64_t s2 = 0, w2 = 0;
 #pragma unroll
       for (int l = 0; l < kLogLoads; ++l)
 #pragma unroll
         for (int e = 0; e < VEC / 2; ++e) {
           const float2 x = Vec<T>::two(raw[l], e);
-          const float t = t_of(x.x, base), u = t_of(x.y, base);
-          w = fmaf(ex2(u), u, fmaf(ex2(t), t, w));
+          const uint64_t t = mul_pair(add_pair(pair(x.x, x.y), nb2), l2e);
+          const float2 tf = halves(t);
+          const uint64_t p = pair(ex2(tf.x), ex2(tf.y));
+          s2 = add_pair(s2, p);
+          w2 = fma_pair(p, t, w2);
         }
+      const float2 ww = halves(w2);
+      if (!(ww.x + ww.y == ww.x + ww.y)) {  // 0 x -infinity: values of probability 0 add 0 (a NaN stays one)
+        float w = 0.f;
+#pragma unroll
+        for (int l = 0; l < kLogLoads; ++l)
+#pragma unroll
+          for (int e = 0; e < VEC / 2; ++e) {
+            const float2 x = Vec<T>::two(raw[l], e);
+            const float t = t_of(x.x, -nb), u = t_of(x.y, -nb);
+            w = fmaf(ex2(u), u, fmaf(ex2(t), t, w));
+          }
+        w2 = pair(w, 0.f);
+      }
+      run_s = add_pair(run_s, s2);
+      run_w = add_pair(run_w, w2);
     }
-    sum.s += s;
-    sum.w += w;
-    other = fmaxf(other, fminf(m, second));
-    if (m > second) {
-      const bool best = m > most;
-      second_at = best ? most_at : t0;
-      second = best ? most : m;
-      most_at = best ? t0 : most_at;
-      most = best ? m : most;
+    other = fmaxf(other, fminf(best, second));
+    if (best > second) {
+      const bool first = best > most;
+      second_at = first ? most_at : t0;
+      second = first ? most : best;
+      most_at = first ? t0 : most_at;
+      most = first ? best : most;
     }
   }
+  const float2 ss = halves(run_s), ww = halves(run_w);
+  Sums sum = {b, ss.x + ss.y, ww.x + ww.y};
   const bool nan = sum.s != sum.s;  // (or an infinity: either way every value is looked at)
   sum = join_lanes<32>(sum);
   if (lane == 0) s_sums[warp] = sum;
@@ -336,7 +350,7 @@ __global__ void __launch_bounds__(kLogThreads, log_ctas(sizeof(T))) token_logpro
     auto take = [&](int t0, int who) {
       unsigned mine = 0;  // a bit per value
 #pragma unroll
-      for (int l = 0; l < kLogLoads; ++l) {
+      for (int l = 0; l < STEPS * kLogLoads; ++l) {
         const int v = t0 + l * kLogThreads + who;
         const long long e0 = (long long)v * VEC - off;
         if (v >= c0 && v < c1) {
@@ -361,16 +375,16 @@ __global__ void __launch_bounds__(kLogThreads, log_ctas(sizeof(T))) token_logpro
         }
       }
     };
-    const int tiles = (v1 - v0 + STEP - 1) / STEP;
+    const int tiles = (v1 - v0 + TILE - 1) / TILE;
     if (nan) {
-      for (int i = 0; i < tiles; ++i) take(v0 + i * STEP, tid);
+      for (int i = 0; i < tiles; ++i) take(v0 + i * TILE, tid);
     } else if (most > bound && !(other > bound)) {
       take(most_at, tid);
       if (second > bound) take(second_at, tid);
     }
     // a thread whose third tile reaches the bound: the warp reads all of that thread's, a tile per lane
     for (unsigned whole = __ballot_sync(0xffffffffu, !nan && other > bound); whole != 0; whole &= whole - 1)
-      for (int i = lane; i < tiles; i += 32) take(v0 + i * STEP, warp * 32 + __ffs(whole) - 1);
+      for (int i = lane; i < tiles; i += 32) take(v0 + i * TILE, warp * 32 + __ffs(whole) - 1);
     __syncthreads();
     const int n = s_n;
     if (n <= kLogAside) {

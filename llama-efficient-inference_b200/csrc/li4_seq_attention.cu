@@ -50,7 +50,7 @@ template <typename ArgsT>
 constexpr bool kIsInt4 = __is_same(ArgsT, Seq4Args);
 __host__ __device__ constexpr int seq4_stages(int D) { return D == 64 ? 2 : 3; }
 // CTAs per SM: unpacking is work that more warps hide better.
-__host__ __device__ constexpr int seq4_ctas(int D, int NT) { return NT > 1 ? 2 : D == 64 ? 4 : 3; }
+__host__ __device__ constexpr int seq4_ctas(int D, int NT) { return NT > 2 ? 2 : NT > 1 ? (D == 64 ? 3 : 2) : D == 64 ? 4 : 3; }
 __host__ __device__ constexpr int seq4_stage_bytes(int D) { return 2 * seq4_keys(D) * (D / 2 + D / kGroup4 * 4); }
 
 __host__ __device__ constexpr int seq_stage_keys(int D, bool q4) { return q4 ? seq4_keys(D) : seq_keys(D); }

@@ -1,10 +1,11 @@
 """token_logprobs on the GPU against 64 bits.
 
 Tolerance (u = 2^-24).  t = (x - b) log2(e) carries three roundings, the constant's among them: 3 u |t| absolute; a
-2^t the unit's 2^-22 and ln 2 x 3 u |t|.  With E = sum p |ln p'| (p' against the largest) the sum S is off by
-  d = 2^-22 + 3 u E + n u,   n = 32 + V / 8192 + 32 the longest chain of additions (a tile's values, tiles, joins),
-relatively, log p by d + 3 u (|x - b| + log S), and the entropy, whose W = sum 2^t t meets the same errors in weights of
-|t|, by d (1 + 2 E) + 2 sum p ln^2 p' 3 u + 3 u (log S + E)."""
+2^t the unit's 2^-22 and ln 2 x 3 u |t|.  The base b lies up to 4 below the largest value.  With E = 4 + sum p |ln p'| (p' against
+the largest) the sum S is off by
+  d = 2^-22 + 3 u E + n u,   n = 8 + V / 4096 + 24 the longest chain of additions (a tile's values, tiles, joins),
+relatively, log p by d + 3 u (|x - b| + log S + 4), and the entropy, whose W = sum 2^t t meets the same errors in weights of
+|t|, by d (1 + 2 E) + 2 sum p (|ln p'| + 4)^2 3 u + 3 u (log S + E)."""
 import math
 
 import pytest
@@ -37,10 +38,10 @@ def check(logprobs, x, tokens, top):
     b = d.amax(1)
     away = (b[:, None] - d).clamp(max=1e6)
     weight = p.exp()
-    E, E2 = (weight * away).sum(1), (weight * away * away).sum(1)
+    E, E2 = (weight * away).sum(1) + 4, (weight * (away + 4) ** 2).sum(1)
     u = 2.0 ** -24
-    off = 2.0 ** -22 + 3 * u * E + (64 + V / 8192) * u
-    log_s = torch.logsumexp(d, 1) - b
+    off = 2.0 ** -22 + 3 * u * E + (32 + V / 4096) * u
+    log_s = torch.logsumexp(d, 1) - b + 4
     if tokens is not None:
         at = tokens.clamp(0, V - 1)[:, None]
         want = p.gather(1, at).view(-1)
