@@ -41,27 +41,29 @@ constexpr int kSeqStages = 3;   // stages per warp
 // instead of 75).
 __host__ __device__ constexpr int seq_keys(int D) { return 32 * 64 / D; }
 // (of a 4-bit cache: 5 KB)
-__host__ __device__ constexpr int seq4_keys(int D) { return D == 64 ? 64 : 32; }
-__host__ __device__ constexpr int seq_unit(int D, bool q4) { return kSeqWarps * (q4 ? seq4_keys(D) : seq_keys(D)); }  // keys per unit
+// (a cluster's stages hold fewer keys, so that short contexts reach all of its warps: one request of 576 tokens 5.7 us,
+// 6.7 us with 64)
+__host__ __device__ constexpr int seq4_keys(int D, bool cl) { return D == 64 && !cl ? 64 : 32; }
+__host__ __device__ constexpr int seq_unit(int D, bool q4, bool cl) { return kSeqWarps * (q4 ? seq4_keys(D, cl) : seq_keys(D)); }  // keys per unit
 __host__ __device__ constexpr int seq_stage_bytes(int D) { return 2 * seq_keys(D) * D * 2; }
 
 // A cache in 4 bits (Q4): stages hold codes and params as they are, unpacked on the way to the products.
 template <typename ArgsT>
 constexpr bool kIsInt4 = __is_same(ArgsT, Seq4Args);
-__host__ __device__ constexpr int seq4_stages(int D) { return D == 64 ? 2 : 3; }
-// CTAs per SM: unpacking is work that more warps hide better.
+__host__ __device__ constexpr int seq4_stages(int D, bool cl) { return D != 64 ? 3 : cl ? 4 : 2; }
+// CTAs per SM: unpacking is work that more warps hide better (64 requests of 300-16000 tokens at 64 dims: two 80 us, four 76 us).
 __host__ __device__ constexpr int seq4_ctas(int D, int NT) { return NT > 2 ? 2 : NT > 1 ? (D == 64 ? 3 : 2) : D == 64 ? 4 : 3; }
-__host__ __device__ constexpr int seq4_stage_bytes(int D) { return 2 * seq4_keys(D) * (D / 2 + D / kGroup4 * 4); }
+__host__ __device__ constexpr int seq4_stage_bytes(int D, bool cl) { return 2 * seq4_keys(D, cl) * (D / 2 + D / kGroup4 * 4); }
 
-__host__ __device__ constexpr int seq_stage_keys(int D, bool q4) { return q4 ? seq4_keys(D) : seq_keys(D); }
-__host__ __device__ constexpr int seq_stage_count(int D, bool q4) { return q4 ? seq4_stages(D) : kSeqStages; }
-__host__ __device__ constexpr int seq_stage_size(int D, bool q4) { return q4 ? seq4_stage_bytes(D) : seq_stage_bytes(D); }
+__host__ __device__ constexpr int seq_stage_keys(int D, bool q4, bool cl) { return q4 ? seq4_keys(D, cl) : seq_keys(D); }
+__host__ __device__ constexpr int seq_stage_count(int D, bool q4, bool cl) { return q4 ? seq4_stages(D, cl) : kSeqStages; }
+__host__ __device__ constexpr int seq_stage_size(int D, bool q4, bool cl) { return q4 ? seq4_stage_bytes(D, cl) : seq_stage_bytes(D); }
 // outputs of the warps and one part of them, in the ring's place
 __host__ __device__ constexpr int seq_join_bytes(int D, int NT) {
   return (kSeqWarps * 8 * NT * (D + 8) + 8 * NT * (D + 2)) * 4;
 }
-__host__ __device__ constexpr int seq_ring_bytes(int D, int NT, bool q4) {
-  const int ring = kSeqWarps * seq_stage_count(D, q4) * seq_stage_size(D, q4);
+__host__ __device__ constexpr int seq_ring_bytes(int D, int NT, bool q4, bool cl) {
+  const int ring = kSeqWarps * seq_stage_count(D, q4, cl) * seq_stage_size(D, q4, cl);
   return ring > seq_join_bytes(D, NT) ? ring : seq_join_bytes(D, NT);
 }
 // floats of one partial result: 8 NT rows of D outputs, then (maximum, sum) per row
@@ -69,8 +71,10 @@ __host__ __device__ constexpr int seq_part_floats(int D, int NT) { return 8 * NT
 
 // The line of units.  An item takes kItemUnits more than its keys do: starting it and joining its warps cost about that
 // much time (256 requests of 100-4000 tokens: 143 us without, 108 with 4, 107 with 2, 109 with 6; 64 of
-// 300-16000 tokens 81, 77, 79, 78 us).
-constexpr int kItemUnits = 4;
+// 300-16000 tokens 81, 77, 79, 78 us; over a 4-bit cache, whose units are of more keys, 256 requests 84 us with 4, 81 with 2, 32 of
+// 4 new tokens 47 and 44 us).
+template <bool Q4>
+constexpr int kItemUnits = Q4 ? 2 : 4;
 struct Line {
   long long total;
   int active;  // CTAs that get a share
@@ -78,11 +82,11 @@ struct Line {
 __device__ __forceinline__ long long share(const Line& l, int g) { return l.total * g / l.active; }
 
 // Key units of an item and the units that a sequence takes.
-template <int D, int NT, bool Q4>
+template <int D, int NT, bool Q4, bool CL = false>
 __device__ __forceinline__ long long seq_units(const SeqAttnArgs& a, const Seq& s, int* tiles, int* per) {
   *tiles = (int)(((long long)s.n * a.rep + 8 * NT - 1) / (8 * NT));
-  *per = max(1, (s.len + seq_unit(D, Q4) - 1) / seq_unit(D, Q4));
-  return (long long)*tiles * (*per + kItemUnits) * a.Hkv;
+  *per = max(1, (s.len + seq_unit(D, Q4, CL) - 1) / seq_unit(D, Q4, CL));
+  return (long long)*tiles * (*per + kItemUnits<Q4>) * a.Hkv;
 }
 
 // Finds the sequence that holds unit share(g): each thread sums a slice of the sequences.  Every thread
@@ -226,15 +230,15 @@ __device__ __forceinline__ void load_stage(const SeqAttnArgs& a, const KeyPages<
 
 // ---- a cache in 4 bits
 // The pages of the lane's keys (j, and j + 32 in a stage of 64), -1 past the end; asked for a stage ahead of its use, like key_pages.
-template <int D>
+template <int KW>
 struct KeyPages4 {
-  int page[seq4_keys(D) / 32];
+  int page[KW / 32];
 };
-template <int D>
-__device__ __forceinline__ KeyPages4<D> key_pages4(const Seq4Args& a, int b, int j, int end) {
-  KeyPages4<D> k;
+template <int KW>
+__device__ __forceinline__ KeyPages4<KW> key_pages4(const Seq4Args& a, int b, int j, int end) {
+  KeyPages4<KW> k;
 #pragma unroll
-  for (int h = 0; h < seq4_keys(D) / 32; ++h) {
+  for (int h = 0; h < KW / 32; ++h) {
     k.page[h] = -1;
     if (j + 32 * h < end) k.page[h] = a.tables[(long long)b * a.table_stride + ((j + 32 * h) >> a.log_page)];
   }
@@ -264,9 +268,9 @@ __device__ __forceinline__ void cp_async16n(uint32_t dst, const void* src, uint3
 }
 
 // A stage: codes of the keys' and the values' rows, then their params.  Rows of no page are zeros (page 0 is not read).
-template <int D>
-__device__ __forceinline__ void load_stage4(const Seq4Args& a, const Head4& k, const Head4& v, KeyPages4<D> pages, int j0, uint32_t stage) {
-  constexpr int CH = D / 32, RPI = 32 / CH, G = D / kGroup4, KK = seq4_keys(D);
+template <int D, int KK>
+__device__ __forceinline__ void load_stage4(const Seq4Args& a, const Head4& k, const Head4& v, KeyPages4<KK> pages, int j0, uint32_t stage) {
+  constexpr int CH = D / 32, RPI = 32 / CH, G = D / kGroup4;
   const int lane = threadIdx.x & 31, c = lane % CH, mask = (1 << a.log_page) - 1;
 #pragma unroll
   for (int h = 0; h < KK / 32; ++h) {
@@ -315,11 +319,11 @@ __device__ __forceinline__ bool params_not_finite(uint32_t p) {
 __device__ __forceinline__ int key_of_row(int r) { return r & 1 ? 7 - (r >> 1) : r >> 1; }
 
 // 16 keys as A fragments: this thread's keys are key and key + 8, its dims D / 4 in a row.
-template <typename T, int D>
+template <typename T, int D, int KK>
 __device__ __forceinline__ void key_fragments4(const uint8_t* stage, int key, uint32_t kf[][4]) {
   constexpr int G = D / kGroup4;
   const int t = threadIdx.x & 3;
-  const uint32_t* kp = reinterpret_cast<const uint32_t*>(stage + seq4_keys(D) * D);
+  const uint32_t* kp = reinterpret_cast<const uint32_t*>(stage + KK * D);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int r = key + 8 * h;
@@ -345,12 +349,12 @@ __device__ __forceinline__ void key_fragments4(const uint8_t* stage, int key, ui
 
 // 16 keys' values, dims by keys, as A fragments: this thread's keys are key = 16 mt + t and 7 - t, and each + 8; its dims
 // D / 8 in a row: fragment dt's rows are dims (D / 8) (lane / 4) + 2 dt and the next.
-template <typename T, int D>
+template <typename T, int D, int KK>
 __device__ __forceinline__ void value_fragments4(const uint8_t* stage, int key, uint32_t vf[][4]) {
   constexpr int G = D / kGroup4, W = D / 64;
   const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
-  const uint8_t* codes = stage + seq4_keys(D) * (D / 2);
-  const uint32_t* vp = reinterpret_cast<const uint32_t*>(stage + seq4_keys(D) * D) + seq4_keys(D) * G;
+  const uint8_t* codes = stage + KK * (D / 2);
+  const uint32_t* vp = reinterpret_cast<const uint32_t*>(stage + KK * D) + KK * G;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int ra = key + 8 * h, rb = key - t + 7 - t + 8 * h;
@@ -467,8 +471,8 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
   constexpr int RT = 8 * NT;
   constexpr int KS = D / 16;  // k steps of K Q^T
   constexpr int DT = D / 16;  // 16-dim tiles of the output
-  constexpr int KW = seq_stage_keys(D, Q4), KT = KW / 16, UNIT = seq_unit(D, Q4);  // a warp's keys per stage, their 16-key tiles
-  constexpr int STAGES = seq_stage_count(D, Q4), STAGE = seq_stage_size(D, Q4);
+  constexpr int KW = seq_stage_keys(D, Q4, CL), KT = KW / 16, UNIT = seq_unit(D, Q4, CL);  // a warp's keys per stage, their 16-key tiles
+  constexpr int STAGES = seq_stage_count(D, Q4, CL), STAGE = seq_stage_size(D, Q4, CL);
   constexpr int LD = D + 8;   // floats per row of the warps' outputs in shared memory
   static_assert(Q4 || seq_join_bytes(D, NT) <= kSeqWarps * STAGES * STAGE, "outputs and a part fit the ring");
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -488,7 +492,7 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
   if constexpr (CL) {
     b = g / ranks / a.Hkv;
     s = load_seq<PAGED>(a, b);
-    seq_units<D, NT, Q4>(a, s, &tiles, &per);
+    seq_units<D, NT, Q4, CL>(a, s, &tiles, &per);
     left = tiles;
     rem = 0;
   } else {
@@ -510,11 +514,11 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
       u0 = per * rank / ranks;
       u1 = per * (rank + 1) / ranks;
     } else {
-      const int span = per + kItemUnits, item = (int)(rem / span);
+      const int span = per + kItemUnits<Q4>, item = (int)(rem / span);
       r0 = (int)(rem - (long long)item * span);
       r1 = (int)min((long long)span, r0 + left);
-      u0 = max(0, r0 - kItemUnits);
-      u1 = max(0, r1 - kItemUnits);
+      u0 = max(0, r0 - kItemUnits<Q4>);
+      u1 = max(0, r1 - kItemUnits<Q4>);
       kvh = item % a.Hkv;
       tile = item / a.Hkv;
     }
@@ -530,11 +534,11 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
     [[maybe_unused]] Head4 k4, v4;
     if constexpr (Q4) k4 = head4(a.k4, kvh), v4 = head4(a.v4, kvh);
     auto pages_of = [&](int j0) {
-      if constexpr (Q4) return key_pages4<D>(a, b, j0 + lane, k1);
+      if constexpr (Q4) return key_pages4<KW>(a, b, j0 + lane, k1);
       else return key_pages<D, PAGED>(a, b, j0, k1);
     };
     auto load = [&](const auto& page, int j0, uint32_t stage) {
-      if constexpr (Q4) load_stage4<D>(a, k4, v4, page, j0, stage);
+      if constexpr (Q4) load_stage4<D, KW>(a, k4, v4, page, j0, stage);
       else load_stage<D, PAGED>(a, page, s, kvh, j0, k1, stage);
     };
     decltype(pages_of(0)) pages[STAGES];
@@ -604,7 +608,7 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
         for (int nt = 0; nt < NT; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
         if constexpr (Q4) {
           uint32_t kf[KS][4];
-          key_fragments4<T, D>(stage4, mt * 16 + key_of_row(lane / 4), kf);
+          key_fragments4<T, D, KW>(stage4, mt * 16 + key_of_row(lane / 4), kf);
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -752,7 +756,7 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
       for (int mt = 0; mt < KT; ++mt) {
         if constexpr (Q4) {
           uint32_t vf[DT][4];
-          value_fragments4<T, D>(stage4, mt * 16 + (lane & 3), vf);
+          value_fragments4<T, D, KW>(stage4, mt * 16 + (lane & 3), vf);
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -794,7 +798,7 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
         }
       }
     __syncthreads();
-    const bool whole = !CL && r0 == 0 && r1 == per + kItemUnits;
+    const bool whole = !CL && r0 == 0 && r1 == per + kItemUnits<Q4>;
     // where a part of the item's result goes: the workspace, or this CTA's shared memory past the warps' outputs
     float* part = CL ? reinterpret_cast<float*>(smem) + kSeqWarps * RT * LD
                      : a.part + (size_t)(2 * g + (r0 == 0 ? 1 : 0)) * seq_part_floats(D, NT);
@@ -861,8 +865,8 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
     }
     left -= r1 - r0;
     rem += r1 - r0;
-    while (left > 0 && rem >= (long long)tiles * (per + kItemUnits) * a.Hkv) {
-      rem -= (long long)tiles * (per + kItemUnits) * a.Hkv;
+    while (left > 0 && rem >= (long long)tiles * (per + kItemUnits<Q4>) * a.Hkv) {
+      rem -= (long long)tiles * (per + kItemUnits<Q4>) * a.Hkv;
       s = load_seq<PAGED>(a, ++b);
       seq_units<D, NT, Q4>(a, s, &tiles, &per);
     }
@@ -889,7 +893,7 @@ __global__ void __launch_bounds__(kSeqThreads) seq_attention_join_kernel(const _
   int tiles, per;
   seq_units<D, NT, Q4>(a, s, &tiles, &per);
   const long long rem = share(line, g) - before;
-  const int span = per + kItemUnits, item = (int)(rem / span);
+  const int span = per + kItemUnits<Q4>, item = (int)(rem / span);
   const long long start = before + (long long)item * span, end = start + span;
   if (start == share(line, g) || share(line, g - 1) > start) return;
   // the parts are CTAs g - 1 (from the item's start) and g .. last, the last CTA with share(last) < end
@@ -989,7 +993,7 @@ static int launch_seq(const ArgsT& args, cudaStream_t stream) {
   ArgsT a = args;
   if constexpr (kIsInt4<ArgsT>) a.grid = seq4_ctas(D, NT) * current_sm_count();
   const int c = seq_cluster(a);
-  const size_t smem = seq_ring_bytes(D, NT, kIsInt4<ArgsT>);
+  const size_t smem = seq_ring_bytes(D, NT, kIsInt4<ArgsT>, c > 1);
   if (c > 1)
     return launch_attn_grid(seq_attention_kernel<T, D, NT, PAGED, true, ArgsT>, a, dim3((unsigned)(a.B * a.Hkv * c)), smem,
                             c, stream);
