@@ -480,7 +480,8 @@ typedef struct li4_int4_pages {
  * gets s = m = NaN and reads as NaN.  k_out and v_out (each may be null, and may be k, v): the turned keys and the values
  * as the cache holds them, c s + m, packed like k and v.
  * strides: 12 element strides -- q, k, v, q_out, k_out, v_out: token, head -- multiples of 8.  head_dim: a multiple of 32
- * up to 128.  Bit 7 of li4_device_errors as there. */
+ * up to 128.  Bit 7 of li4_device_errors as there, and tokens that share a slot are the caller's mistake: their codes and
+ * parameters mix. */
 int li4_rope_paged_write_int4(const void* q, const void* k, const void* v, int dtype, int64_t n_tokens, int64_t n_heads,
                               int64_t n_kv_heads, int64_t head_dim, const int64_t* strides, const float* rope_cos,
                               const float* rope_sin, int64_t rope_stride, int64_t max_pos, const int32_t* positions,
@@ -489,7 +490,8 @@ int li4_rope_paged_write_int4(const void* q, const void* k, const void* v, int d
                               int64_t page_size, void* stream);
 
 /* li4_paged_attention over such a cache: the same function of the values that the cache stands for.  args: as there,
- * its k, v and their strides unused; head_dim a multiple of 32.  A group of not finite parameters reads as NaN, and as in
+ * its k, v and their strides unused; head_dim a multiple of 32.  A head's codes may spread over up to 64 GB of memory, its
+ * params over up to 16 GB (larger tensors are refused).  A group of not finite parameters reads as NaN, and as in
  * li4_paged_attention reaches only queries that see it. */
 size_t li4_attention_int4_workspace_bytes(const li4_attention* args);
 int li4_paged_attention_int4(const li4_attention* args, const li4_int4_pages* cache_k, const li4_int4_pages* cache_v,

@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kLogThreads, __is_same(T, __nv_bfloat16) ? 5 :
   uint4 raw[kLogLoads], next[kLogLoads];
   auto load = [&](uint4* to, int t0) {
 #pragma unroll
-    for (int l = 0; l < kLogLoads; ++l) to[l] = __ldg(vec + t0 + l * kLogThreads + tid);
+    for (int l = 0; l < kLogLoads; ++l) to[l] = __ldcg(vec + t0 + l * kLogThreads + tid);
   };
   if (clean(v0)) load(next, v0);
   uint64_t run_s = 0, run_w = 0;  // pairs of sums against base b
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(kLogThreads, __is_same(T, __nv_bfloat16) ? 5 :
           const int v = at + l * kLogThreads + tid;
           raw[l] = make_uint4(LOW, LOW, LOW, LOW);
           if (v >= c0 && v < c1) {
-            raw[l] = __ldg(vec + v);
+            raw[l] = __ldcg(vec + v);
           } else if (v < v1) {  // a vector that the row's end cuts, value by value; -infinity beside them
             uint32_t u[4] = {LOW, LOW, LOW, LOW};
 #pragma unroll
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kLogThreads, __is_same(T, __nv_bfloat16) ? 5 :
         const int v = t0 + l * kLogThreads + who;
         const long long e0 = (long long)v * VEC - off;
         if (v >= c0 && v < c1) {
-          const uint4 again = __ldg(vec + v);
+          const uint4 again = __ldcg(vec + v);
 #pragma unroll
           for (int e = 0; e < VEC; e += 2) {
             const float2 x = Vec<T>::two(again, e / 2);

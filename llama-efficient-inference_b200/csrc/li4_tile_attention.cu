@@ -424,7 +424,7 @@ __device__ __noinline__ void put_back(uint32_t o_at, const int* first, int last)
 // ---- a cache in 4 bits: a quarter of a tile (32 rows) by a warp, a row per lane: one address per row, and 8 neighbouring
 // lanes store to all eight 16-byte places of swizzled rows.  A lane's row of the next key and of the next value tile waits in
 // shared memory of its own (2048 tokens over 8000 at 128 dims: two lanes per row, an address and a shuffle for each turn
-// of 16 rows 741 us, rows kept in registers 461 us).
+// of 16 rows 741 us, rows kept in registers 461 us, like this 369 us; the 16-bit cache 270 us).
 __host__ __device__ constexpr int row4_bytes(int D) { return D / 2 + D / kGroup4 * 4; }
 __host__ __device__ constexpr int rows4_bytes(int D) { return 2 * kTileKeys * row4_bytes(D); }  // of the four warps
 
@@ -601,8 +601,8 @@ __global__ void __launch_bounds__(kTileInt4<ArgsT> ? kTile4Threads : kTileThread
 
   // 384 threads x 168 registers at the launch: the softmax's two groups take 208 each, the third keeps 80
   // (2 x 128 x 208 + 128 x 80 <= 384 x 168)
-  // Q4: 512 threads x 128, 200 each for the softmax, 48 for the third group, 64 for the unpacking warps
-  // (2 x 128 x 200 + 128 x 48 + 128 x 64 = 512 x 128)
+  // Q4: 512 threads x 128 at the launch: 192 each for the softmax, 48 for the third group, 80 for the unpacking warps
+  // (2 x 128 x 192 + 128 x 48 + 128 x 80 = 512 x 128; 192 / 64 / 64: 2048 tokens over 8000 at 128 dims 555 us instead of 461)
   if (Q4 && warp >= kUnpackWarp) {
     if constexpr (Q4) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");

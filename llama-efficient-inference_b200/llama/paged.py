@@ -284,6 +284,7 @@ def hidden_paged(model, tokens: torch.Tensor, step: PagedStep, cache: PagedKVCac
     if tokens.dim() != 1 or tokens.shape[0] == 0:
         raise ValueError(f"forward_paged: a step has at least one token, tokens [T]; got {list(tokens.shape)}")
     cos, sin = rope_tables(model)
+    bits = getattr(cache, "bits", 16)
     h = model.tok_embeddings(tokens)
     T = tokens.shape[0]
     for i, layer in enumerate(model.layers):
@@ -292,7 +293,7 @@ def hidden_paged(model, tokens: torch.Tensor, step: PagedStep, cache: PagedKVCac
         q = att.wq(x).view(T, att.n_local_heads, att.head_dim)
         k = att.wk(x).view(T, att.n_local_kv_heads, att.head_dim)
         v = att.wv(x).view(T, att.n_local_kv_heads, att.head_dim)
-        if cache.bits == 4:
+        if bits == 4:
             q, k, v = rope_paged_write_int4(q, k, v, cos, sin, step.positions, step.slots, cache.k[i], cache.v[i], q_out=q,
                                             k_out=k if whole_prompts else None, v_out=v if whole_prompts else None,
                                             need_kv=whole_prompts)
@@ -302,7 +303,7 @@ def hidden_paged(model, tokens: torch.Tensor, step: PagedStep, cache: PagedKVCac
         if whole_prompts:
             o = prompt_attention(q, k, v, step.cu_seqlens, max_new)
         else:
-            attention = paged_attention_int4 if cache.bits == 4 else paged_attention
+            attention = paged_attention_int4 if bits == 4 else paged_attention
             o = attention(q, cache.k[i], cache.v[i], cache.block_tables, step.kv_lens, step.cu_seqlens, max_new)
         h = h + att._reduce(att.wo(o.view(T, -1)))
         h = h + layer.feed_forward(layer.ffn_norm(h))
