@@ -394,7 +394,7 @@ extern "C" int li4_paged_fork(const int32_t* kv_lens, const int32_t* parents, in
       (n_pools > 0 && (!pools || !pool_strides || !pool_bytes)))
     return set_error(LI4_ERR_INVALID_ARG, "%s: null pointer", what);
   for (int64_t i = 0; i < n_pools; ++i) {
-    if (!pools[i] || !aligned16(pools[i]) || pool_bytes[i] % 16 != 0 || pool_strides[i] % 16 != 0)
+    if ((!pools[i] && free_capacity > 0) || !aligned16(pools[i]) || pool_bytes[i] % 16 != 0 || pool_strides[i] % 16 != 0)
       return set_error(LI4_ERR_ALIGNMENT, "%s: pool %lld: pages must start on 16-byte boundaries, of a multiple of 16 bytes",
                        what, (long long)i);
     if (pool_bytes[i] < 0 || pool_bytes[i] > (1 << 30) || (pool_strides[i] < pool_bytes[i] && free_capacity > 1))

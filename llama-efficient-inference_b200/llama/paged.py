@@ -27,7 +27,7 @@ and calls under a tracer are refused.
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -180,7 +180,8 @@ def paged_fork(kv_lens: torch.Tensor, block_tables: torch.Tensor, free_pages: to
 
     Full pages are shared, a last page that is not full is copied into one from the top of the free stack, in every tensor
     of pools ([pages, ...], each page one block of memory).  A request whose copy finds no page, or whose parent is none,
-    stays as it was (granted False).  Pages that no request holds any more go back on the stack, in the order of requests
+    stays as it was (granted False).  Pages are 0 .. len(free_pages) - 1; other entries of block_tables count as no page and
+    are not copied.  Pages that no request holds any more go back on the stack, in the order of requests
     and blocks.  block_tables and free_pages are updated in place; kv_lens_out / n_free_out may be kv_lens / n_free (in
     place), by default they are new tensors.  Sharing is read off the tables: append and this are all there is to call."""
     return PagedFork._make(_done("paged_fork", native.ext().paged_fork(
@@ -212,11 +213,9 @@ class PagedKVCache:
 
         if bits == 16:
             self.k, self.v = pages([head_dim], dtype), pages([head_dim], dtype)
-            self.pools = self.k + self.v  # all tensors of pages
         else:
             self.k, self.v = ([Int4Pages(c, p) for c, p in zip(pages([head_dim // 2], torch.uint8),
                                                                pages([head_dim // 32, 2], dtype))] for _ in range(2))
-            self.pools = [t for pair in self.k + self.v for t in pair]
         i32 = dict(dtype=torch.int32, device=device)
         self.block_tables = torch.zeros(max_requests, -(-max_len // page_size), **i32)
         self.kv_lens = torch.zeros(max_requests, **i32)
@@ -224,6 +223,11 @@ class PagedKVCache:
         self._stack = torch.cat([torch.arange(num_pages - 1, -1, -1, **i32), torch.zeros(1, **i32)])
         self.free_pages = self._stack[:num_pages]
         self.n_free = torch.full((1,), num_pages, **i32)
+
+    @property
+    def pools(self) -> List[torch.Tensor]:
+        """All tensors of pages."""
+        return self.k + self.v if self.bits == 16 else [t for pair in self.k + self.v for t in pair]
 
     def append(self, new_lens: torch.Tensor, num_tokens: int) -> PagedStep:
         """Takes pages for new_lens[r] more tokens of every request r (int32 [max_requests], zeros for idle rows);

@@ -211,6 +211,27 @@ def test_cache_fork_append_release(paged):
         assert cache.n_free.item() == 120 and sorted(cache.free_pages.tolist()) == list(range(120))
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+def test_cache_without_pages(paged, bits):
+    """Nothing is granted, and ending requests that hold nothing is no error."""
+    cache = paged.PagedKVCache(1, 0, 8, 2, 32, max_requests=3, max_len=16, bits=bits)
+    assert not cache.append(i32([1, 0, 2]), 3).granted[0]
+    cache.release(torch.ones(3, dtype=torch.bool, device="cuda"))
+    assert cache.fork(i32([1, 1, -1])).tolist() == [True] * 3
+    assert cache.n_free.item() == 0 and cache.kv_lens.tolist() == [0, 0, 0]
+
+
+def test_cache_whose_tensors_are_replaced(paged):
+    """fork copies in the tensors that the cache holds when it is called."""
+    cache = paged.PagedKVCache(1, 4, 8, 1, 32, max_requests=2, max_len=16)
+    cache.append(i32([3, 0]), 3)
+    cache.k[0] = torch.full_like(cache.k[0], 2.0)
+    cache.k[0][cache.block_tables[0, 0].long()] = 5.0
+    cache.fork(i32([0, 0]))
+    assert (cache.k[0][cache.block_tables[1, 0].long()] == 5.0).all()
+    assert (cache.k[0] == 5.0).sum().item() == 2 * 8 * 32
+
+
 def test_refusals(paged):
     kv, bt, free, n_free, parents = i32([1, 2]), i32([[0], [1]]), i32([2, 3, 0, 0]), i32([2]), i32([0, 0])
     pool = torch.zeros(4, 16, device="cuda")
