@@ -1061,8 +1061,10 @@ __global__ void __launch_bounds__(kTileInt4<ArgsT> ? kTile4Threads : kTileThread
           // (asked here, used a little later: the answer takes a while)
           [[maybe_unused]] const bool o_here = !EARLY || j == 0 || mbar_test_wait(&o_done[i], (done + j - 1) & 1);
           const float top = max2(max3(mx[0], mx[1], mx[2]), mx[3]);
-          // (the difference is NaN for two infinities of one sign and beside a NaN score: no move)
-          if (__any_sync(0xffffffffu, (top - m) * c > kLazyLog2)) {
+          // (the difference is NaN for two infinities of one sign and beside a NaN score: no move.  A tile's rows past its
+          // queries hold other requests' queries or what shared memory held before: they have no say in when the others'
+          // sums are rounded anew)
+          if (__any_sync(0xffffffffu, lim >= 0 && (top - m) * c > kLazyLog2)) {
             const float mn = fmaxf(m, top);
             const float nb = mn == -INFINITY ? 0.f : mn * c;
             const float f = m == -INFINITY ? 0.f : exp2_fast(m * c - nb);
