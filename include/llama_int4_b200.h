@@ -416,8 +416,10 @@ int li4_rope_paged_write(const void* q, const void* k, const void* v, int dtype,
  * cu_seqlens[b + 1] - 1 of q [n_tokens, n_heads, head_dim]; query i of n sees keys 0 .. L - n + i of its
  * sequence's L.  A query that sees no key gives zeros; rows past cu_seqlens[n_seqs] are left as they
  * were.  Scores, softmax statistics and sums in fp32; probabilities rounded to the type for the second
- * product; one rounding at the end.  A value row's NaN or infinity reaches only queries that see it (a call that
- * meets one takes up to three times as long); a NaN or infinite score makes its query's outputs NaN. */
+ * product; one rounding at the end.  The sums are of values times 2^t exp(x - max), t up to 8, divided at the end: for
+ * bf16 values near the type's largest such a sum can pass fp32's largest, and the output is then not finite.  A value
+ * row's NaN or infinity reaches only queries that see it (a call that meets one takes up to three times as long); a NaN or
+ * infinite score makes its query's outputs NaN. */
 typedef struct li4_attention {
   const void* q;
   const void* k;                /* prompt: [n_tokens, n_kv_heads, head_dim]; paged: the cache's pages */
@@ -491,8 +493,8 @@ int li4_rope_paged_write_int4(const void* q, const void* k, const void* v, int d
 
 /* li4_paged_attention over such a cache: the same function of the values that the cache stands for.  args: as there,
  * its k, v and their strides unused; head_dim a multiple of 32.  A head's codes may spread over up to 64 GB of memory, its
- * params over up to 16 GB (larger tensors are refused).  A group of not finite parameters reads as NaN, and as in
- * li4_paged_attention reaches only queries that see it. */
+ * params over up to 16 GB (larger tensors are refused).  What is not finite among the values c s + m of any
+ * parameters reaches, as in li4_paged_attention, only queries that see it. */
 size_t li4_attention_int4_workspace_bytes(const li4_attention* args);
 int li4_paged_attention_int4(const li4_attention* args, const li4_int4_pages* cache_k, const li4_int4_pages* cache_v,
                              void* workspace, size_t workspace_bytes, void* stream);

@@ -309,9 +309,11 @@ __device__ __forceinline__ void load_stage4(const Seq4Args& a, const Head4& k, c
   }
 }
 
+// Whether a group of these parameters can hold a value that is not finite: its values lie between those of the codes 0 and 15.
 template <typename T>
-__device__ __forceinline__ bool params_not_finite(uint32_t p) {
-  return Type16<T>::not_finite((uint16_t)p) || Type16<T>::not_finite((uint16_t)(p >> 16));
+__device__ __forceinline__ bool not_finite4(uint32_t p) {
+  const uint32_t last = Codes4<T>::fma(Codes4<T>::template codes<0>(0x000F000Fu), both_low(p), both_high(p));
+  return Type16<T>::not_finite((uint16_t)p) || Type16<T>::not_finite((uint16_t)(p >> 16)) || Type16<T>::not_finite((uint16_t)last);
 }
 
 // Which of 8 keys is row r of a tile of keys.  Any order serves, as both products use the same one; this one lets the 4 threads
@@ -379,6 +381,46 @@ __device__ __forceinline__ void value_fragments4(const uint8_t* stage, int key, 
       for (int e = 0; e < 4; ++e) {
         vf[4 * i + e][2 * h] = even[e];
         vf[4 * i + e][2 * h + 1] = odd[e];
+      }
+    }
+  }
+}
+
+// Key r of the stage, p the parameters of this thread's dims: where they make values that are not finite, the group's are added
+// here to the rows that see the key -- the finite ones by the row's probability, the others as they are (a sum with what is
+// not finite does not depend on its weight) -- and the caller makes the group's parameters zeros before the product.
+template <typename T, int D, int NT, int KT>
+__device__ __forceinline__ void add_key4(const uint8_t* stage, int r, uint32_t p, int j, const int (&lim)[NT][2],
+                                         const uint32_t (&pf)[KT][NT][2], float (&o)[D / 16][NT][4]) {
+  const int lane = threadIdx.x & 31, k = r & 7;
+  const int at = k < 4 ? 2 * k : 15 - 2 * k;  // key_of_row's row
+  const bool mine = not_finite4<T>(p);        // (the dims of a thread lie in one group)
+  const uint8_t* codes = stage + KT * 16 * (D / 2) + r * (D / 2) + (lane / 4) * (D / 16);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    uint32_t of_rows = 0;  // the fragment of this key's eight
+#pragma unroll
+    for (int h = 0; h < 2 * KT; ++h)  // (in C++ this becomes an index, and pf an array in memory)
+      asm("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, %2;\n\tselp.b32 %0, %3, %0, p;\n\t}"
+          : "+r"(of_rows)
+          : "r"(h), "r"(r >> 3), "r"(pf[h >> 1][nt][h & 1]));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t two = __shfl_sync(0xffffffffu, of_rows, ((lane & 3) * 2 + e) * 4 + (at >> 1));
+      const float2 pp = Type16<T>::unpack(two);
+      const float prob = at & 1 ? pp.y : pp.x;
+      if (!mine || j > lim[nt][e]) continue;
+#pragma unroll
+      for (int w = 0; w < D / 64; ++w) {
+        uint32_t u[4];
+        values8<T>(*reinterpret_cast<const uint32_t*>(codes + 4 * w), both_low(p), both_high(p), u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = Type16<T>::unpack(u[i]);
+          float(&to)[4] = o[4 * w + i][nt];
+          to[e] = isfinite(x.x) ? fmaf(prob, x.x, to[e]) : to[e] + x.x;
+          to[2 + e] = isfinite(x.y) ? fmaf(prob, x.y, to[2 + e]) : to[2 + e] + x.y;
+        }
       }
     }
   }
@@ -687,28 +729,19 @@ __global__ void __launch_bounds__(kSeqThreads, kIsInt4<ArgsT> ? seq4_ctas(D, NT)
           uint32_t* vp = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(stage4) + KW * D) + KW * G;
 #pragma unroll 1
           for (int r0 = 0; r0 < KW; r0 += 32) {
-            bool odd = false;  // lane's key is hidden from some row and has a group that is not finite
+            bool odd = false;  // lane's key is hidden from some row and has a group that may hold a value that is not finite
 #pragma unroll
-            for (int g = 0; g < G; ++g) odd |= params_not_finite<T>(vp[(r0 + lane) * G + g]);
+            for (int g = 0; g < G; ++g) odd |= not_finite4<T>(vp[(r0 + lane) * G + g]);
             odd = odd && j0 + r0 + lane > first_lim;
             for (unsigned rest = __ballot_sync(0xffffffffu, odd); rest != 0; rest &= rest - 1) {
               const int r = r0 + __ffs(rest) - 1;
-              if (params_not_finite<T>(vp[r * G + (lane / 4) * G / 8])) {  // this thread's dims lie in one group
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e)
-                    if (j0 + r <= lim[nt][e]) {
-#pragma unroll
-                      for (int dt = 0; dt < DT; ++dt) o[dt][nt][e] = o[dt][nt][2 + e] = NAN;
-                    }
-              }
+              add_key4<T, D, NT, KT>(stage4, r, vp[r * G + (lane / 4) * G / 8], j0 + r, lim, pf, o);
             }
             __syncwarp();
             if (odd) {
 #pragma unroll
               for (int g = 0; g < G; ++g)
-                if (params_not_finite<T>(vp[(r0 + lane) * G + g])) vp[(r0 + lane) * G + g] = 0u;
+                if (not_finite4<T>(vp[(r0 + lane) * G + g])) vp[(r0 + lane) * G + g] = 0u;
             }
           }
           __syncwarp();
