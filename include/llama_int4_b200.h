@@ -515,6 +515,8 @@ int li4_paged_attention_int4(const li4_attention* args, const li4_int4_pages* ca
  *   granted       [n_requests]
  *   pools         in each of n_pools memory blocks of pages (pools[i] + page * pool_strides[i] bytes: pool_bytes[i] bytes, all
  *                 multiples of 16), the pages of the parts that were copied
+ * Arrays that the call writes overlap no other argument (kv_lens_out may be kv_lens, n_free_out n_free); two pools may be
+ * interleaved, or hold the same pages, but no page of one overlaps a page of another number of the other.
  * pools, pool_strides and pool_bytes are host arrays.  Pages are 0 .. free_capacity - 1; other entries of the tables count as no page.
  * At most 8192 requests, and n_requests * table_width below 2^31.  Two or more launches: the tables, then the copies, up to
  * LI4_FORK_POOLS pools each.  No counterpart in the reference, which decodes each prompt once. */

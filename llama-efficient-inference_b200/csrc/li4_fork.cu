@@ -15,6 +15,9 @@
 // A second launch copies the pages that are not full, bound by their bytes.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+#include <vector>
+
 #include "li4_common.cuh"
 #include "li4_internal.h"
 
@@ -358,6 +361,71 @@ static ForkSpace fork_space(int64_t B, int64_t width, int64_t capacity) {
   return s;
 }
 
+// ---- memory that a call may not name twice
+// rows of `bytes` bytes, `stride` apart
+struct Region {
+  const char* name;
+  uintptr_t at;
+  int64_t rows, stride, bytes;
+};
+static Region region(const char* name, const void* p, int64_t bytes, int64_t rows = 1, int64_t stride = 0) {
+  return {name, reinterpret_cast<uintptr_t>(p), bytes > 0 ? rows : 0, stride, bytes};
+}
+static int64_t span(const Region& r) { return r.rows > 0 ? (r.rows - 1) * r.stride + r.bytes : 0; }
+
+// Whether one of a's rows meets b's span.
+static bool meet(const Region& a, const Region& b) {
+  if (a.rows <= 0 || b.rows <= 0) return false;
+  const int64_t off = (int64_t)(b.at - a.at), n = span(b);  // b from a's start
+  if (off + n <= 0 || off >= span(a)) return false;
+  if (off < 0 || a.rows == 1) return true;
+  const int64_t row = off / a.stride;
+  return off - row * a.stride < a.bytes || (row + 1 < a.rows && off + n > (row + 1) * a.stride);
+}
+
+// Whether a page of one pool lies over a page of another number of another pool: a copy into one would then change the
+// other.  (The same pages named twice are copied twice.)  The ranges are sorted; those that meet have to be interleaved: of one
+// stride, and modulo it apart or at the same page.
+static bool pools_meet(void* const* pools, const int64_t* strides, const int64_t* bytes, int64_t n_pools, int64_t pages) {
+  struct Pool {
+    uintptr_t at;
+    int64_t stride, bytes;
+    uintptr_t end(int64_t n) const { return at + (uintptr_t)((n - 1) * stride + bytes); }
+  };
+  std::vector<Pool> all;
+  all.reserve((size_t)n_pools);
+  for (int64_t i = 0; i < n_pools; ++i)
+    if (bytes[i] > 0) all.push_back({reinterpret_cast<uintptr_t>(pools[i]), strides[i], bytes[i]});
+  std::sort(all.begin(), all.end(), [](const Pool& a, const Pool& b) { return a.at < b.at; });
+  struct Piece {
+    int64_t at, end, page;
+  };
+  std::vector<Piece> pieces;
+  for (size_t i = 0, next; i < all.size(); i = next) {
+    uintptr_t end = all[i].end(pages);
+    for (next = i + 1; next < all.size() && all[next].at < end; ++next) {
+      if (all[next].stride != all[i].stride) return true;
+      end = std::max(end, all[next].end(pages));
+    }
+    if (next == i + 1) continue;
+    // two strides' worth: every pool's page `page` of the first stride and the page after it in the second
+    const int64_t stride = all[i].stride;
+    pieces.clear();
+    for (size_t k = i; k < next; ++k) {
+      const int64_t off = (int64_t)(all[k].at - all[i].at), at = off % stride;
+      for (int lap = 0; lap < 2; ++lap)
+        pieces.push_back({at + lap * stride, at + lap * stride + all[k].bytes, lap - off / stride});
+    }
+    std::sort(pieces.begin(), pieces.end(), [](const Piece& a, const Piece& b) { return a.at < b.at; });
+    Piece last = pieces[0];
+    for (const Piece& p : pieces) {
+      if (p.at < last.end && p.page != last.page) return true;
+      if (p.end > last.end) last = p;
+    }
+  }
+  return false;
+}
+
 }  // namespace li4
 
 extern "C" size_t li4_paged_fork_workspace_bytes(int64_t n_requests, int64_t table_width, int64_t free_capacity) {
@@ -375,7 +443,9 @@ extern "C" int li4_paged_fork(const int32_t* kv_lens, const int32_t* parents, in
                               void* stream) {
   using namespace li4;
   const char* what = "paged_fork";
-  if (n_requests < 0 || table_width < 0 || free_capacity < 0 || table_stride < table_width || n_pools < 0)
+  constexpr int64_t kMostBytes = 1LL << 60;  // (so that no span of a table or pool overflows)
+  if (n_requests < 0 || table_width < 0 || free_capacity < 0 || table_stride < table_width || n_pools < 0 ||
+      (n_requests > 1 && table_stride > kMostBytes / 4 / n_requests))
     return set_error(LI4_ERR_INVALID_ARG,
                      "%s: n_requests=%lld table_width=%lld table_stride=%lld free_capacity=%lld n_pools=%lld", what,
                      (long long)n_requests, (long long)table_width, (long long)table_stride, (long long)free_capacity,
@@ -397,7 +467,8 @@ extern "C" int li4_paged_fork(const int32_t* kv_lens, const int32_t* parents, in
     if ((!pools[i] && free_capacity > 0) || !aligned16(pools[i]) || pool_bytes[i] % 16 != 0 || pool_strides[i] % 16 != 0)
       return set_error(LI4_ERR_ALIGNMENT, "%s: pool %lld: pages must start on 16-byte boundaries, of a multiple of 16 bytes",
                        what, (long long)i);
-    if (pool_bytes[i] < 0 || pool_bytes[i] > (1 << 30) || (pool_strides[i] < pool_bytes[i] && free_capacity > 1))
+    if (pool_bytes[i] < 0 || pool_bytes[i] > (1 << 30) || (pool_strides[i] < pool_bytes[i] && free_capacity > 1) ||
+        (free_capacity > 1 && pool_strides[i] > kMostBytes / free_capacity))
       return set_error(LI4_ERR_INVALID_ARG, "%s: pool %lld: pages of %lld bytes, %lld apart", what, (long long)i,
                        (long long)pool_bytes[i], (long long)pool_strides[i]);
   }
@@ -415,6 +486,34 @@ extern "C" int li4_paged_fork(const int32_t* kv_lens, const int32_t* parents, in
   if (!workspace || workspace_bytes < space.bytes || !aligned16(workspace))
     return set_error(LI4_ERR_WORKSPACE, "%s: %zu bytes of 16-byte aligned workspace needed, %zu given", what, space.bytes,
                      workspace_bytes);
+  const Region tables = region("block_tables", block_tables, table_width * 4, n_requests, table_stride * 4);
+  const Region written[5] = {tables, region("free_pages", free_pages, free_capacity * 4), region("kv_lens_out", kv_lens_out, n_requests * 4),
+                             region("n_free_out", n_free_out, 4), region("granted", granted, n_requests)};
+  const Region read[3] = {region("kv_lens", kv_lens, n_requests * 4), region("parents", parents, n_requests * 4),
+                          region("n_free", n_free, 4)};
+  for (int i = 0; i < 5; ++i) {
+    for (int k = i + 1; k < 5; ++k)
+      if (meet(written[i], written[k]))
+        return set_error(LI4_ERR_INVALID_ARG, "%s: %s must not overlap %s", what, written[k].name, written[i].name);
+    for (int k = 0; k < 3; ++k)
+      if (meet(written[i], read[k]) && !(read[k].at == written[i].at && ((i == 2 && k == 0) || (i == 3 && k == 2))))
+        return set_error(LI4_ERR_INVALID_ARG, "%s: %s must not overlap %s", what, written[i].name, read[k].name);
+  }
+  if (free_capacity > 0) {
+    for (int64_t p = 0; p < n_pools; ++p) {
+      const Region pool = region("a pool", pools[p], pool_bytes[p], free_capacity, pool_strides[p]);
+      for (int i = 0; i < 8; ++i) {
+        const Region& other = i < 5 ? written[i] : read[i - 5];
+        if (meet(pool, other)) return set_error(LI4_ERR_INVALID_ARG, "%s: pool %lld must not overlap %s", what, (long long)p, other.name);
+      }
+    }
+    try {
+      if (pools_meet(pools, pool_strides, pool_bytes, n_pools, free_capacity))
+        return set_error(LI4_ERR_INVALID_ARG, "%s: pages of one pool must not overlap other pages of another", what);
+    } catch (...) {  // (no exception leaves a C function)
+      return set_error(LI4_ERR_INVALID_ARG, "%s: no host memory for %lld pools", what, (long long)n_pools);
+    }
+  }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   ForkArgs a;
   a.kv_lens = kv_lens;

@@ -183,7 +183,8 @@ def paged_fork(kv_lens: torch.Tensor, block_tables: torch.Tensor, free_pages: to
     stays as it was (granted False).  Pages are 0 .. len(free_pages) - 1; other entries of block_tables count as no page and
     are not copied.  Pages that no request holds any more go back on the stack, in the order of requests
     and blocks.  block_tables and free_pages are updated in place; kv_lens_out / n_free_out may be kv_lens / n_free (in
-    place), by default they are new tensors.  Sharing is read off the tables: append and this are all there is to call."""
+    place), by default they are new tensors; what is written overlaps nothing else, and pools overlap one another at most in
+    the same pages.  Sharing is read off the tables: append and this are all there is to call."""
     return PagedFork._make(_done("paged_fork", native.ext().paged_fork(
         kv_lens, block_tables, free_pages, n_free, parents, page_size, pools, kv_lens_out, n_free_out)))
 
