@@ -635,15 +635,17 @@ PyObject* paged_fork(PyObject* const* v) {
     PyObject* o;
     ~Drop() { Py_DECREF(o); }
   } drop{seq};
-  const int64_t n_pools = PySequence_Fast_GET_SIZE(seq);
-  std::vector<void*> pools(n_pools);
-  std::vector<int64_t> strides(n_pools), bytes(n_pools);
-  for (int64_t i = 0; i < n_pools; ++i) {
+  const int64_t given = PySequence_Fast_GET_SIZE(seq);
+  std::vector<void*> pools;
+  std::vector<int64_t> strides, bytes;
+  pools.reserve(given), strides.reserve(given), bytes.reserve(given);
+  for (int64_t i = 0; i < given; ++i) {
     const char* name = "a tensor of pools";
     const Tensor t = tensor(what, name, PySequence_Fast_GET_ITEM(seq, i));
     d.add(name, t);
     if (t.dim() < 1 || t.size(0) < capacity)
       fail(what, "pools[", i, "] must have ", capacity, " pages at least, got ", t.sizes());
+    if (capacity == 0) continue;  // (no page to copy, whatever the strides of an empty tensor are)
     // a page is one block of memory, in whatever order of its dimensions
     int64_t block = 1, left = 1;
     for (int64_t k = 1; k < t.dim(); ++k) left *= t.size(k);
@@ -660,10 +662,11 @@ PyObject* paged_fork(PyObject* const* v) {
     const int64_t size = t.element_size();
     if (block != values || values < 1 || (t.size(0) > 1 && t.stride(0) < values))
       fail(what, "pools[", i, "]: a page must be one block of memory, apart from the others");
-    pools[i] = t.data_ptr();
-    bytes[i] = values * size;
-    strides[i] = t.size(0) > 1 ? t.stride(0) * size : values * size;
+    pools.push_back(t.data_ptr());
+    bytes.push_back(values * size);
+    strides.push_back(t.size(0) > 1 ? t.stride(0) * size : values * size);
   }
+  const int64_t n_pools = (int64_t)pools.size();
   const c10::cuda::CUDAGuard guard(d.dev);
   const Tensor kc = kv.contiguous(), pc = parents.contiguous();
   auto result = [&](const char* name, PyObject* o, const Tensor& like) {

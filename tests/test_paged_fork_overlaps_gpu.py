@@ -65,3 +65,11 @@ def test_refusals(paged):  # noqa: F811
         with pytest.raises(RuntimeError, match="overlap"):
             paged.paged_fork(**{**s, **kw})
     assert s["kv_lens"].tolist() == [20, 9, 0] and s["n_free"].item() == 3 and s["free_pages"].tolist() == [7, 3, 6, 0, 0, 0, 0, 0]
+
+
+def test_pools_without_pages(paged):  # noqa: F811
+    """Without pages there is nothing to copy, whatever the strides of the empty tensors say."""
+    empty = torch.zeros(0, dtype=torch.int32, device="cuda")
+    odd = torch.zeros(1, 1, 1, device="cuda").expand(1, 3, 8)[:0]
+    got = paged.paged_fork(i32([0, 0]), torch.zeros(2, 0, dtype=torch.int32, device="cuda"), empty, i32([0]), i32([1, -1]), 8, [odd, odd[:, ::2]])
+    assert got.granted.tolist() == [True, True] and got.n_free.item() == 0
