@@ -30,6 +30,7 @@ from __future__ import annotations
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
+from torch.utils._python_dispatch import is_in_torch_dispatch_mode
 
 from . import _native as native
 
@@ -80,6 +81,15 @@ def unpack_codes(packed: torch.Tensor) -> torch.Tensor:
     """The codes [..., head_dim] (int32) of packed rows [..., head_dim / 2]."""
     at = torch.tensor(_CODE_BITS, dtype=torch.int32, device=packed.device)
     return ((packed.contiguous().view(torch.int32).unsqueeze(-1) >> at) & 15).flatten(-2)
+
+
+MAX_FORK_REQUESTS = 8192  # li4_paged_fork's
+
+
+def _runs_now(*tensors: torch.Tensor) -> bool:
+    """Whether a call on these tensors is made at once on the GPU: plain CUDA tensors, outside of any tracing."""
+    return not torch.compiler.is_compiling() and not torch.jit.is_tracing() and not is_in_torch_dispatch_mode() and \
+        all(type(t) is torch.Tensor and t.is_cuda for t in tensors)
 
 
 def _done(what: str, result):
@@ -247,16 +257,29 @@ class PagedKVCache:
     def release(self, finished: torch.Tensor) -> None:
         """Returns the pages of the requests flagged in finished (bool [max_requests]), those that no other request
         shares, and sets their lengths to 0.  No host synchronisation."""
-        if self.kv_lens.is_cuda:
-            stay = torch.arange(finished.shape[0], dtype=torch.int32, device=finished.device)
-            self.fork(stay.masked_fill_(finished, -1))
-            return
-        # (index arithmetic; nothing forks off the GPU, so no page is shared)
+        n = self.kv_lens.shape[0]
+        if _runs_now(self.kv_lens, self.block_tables, self.free_pages, self.n_free, finished) and n <= MAX_FORK_REQUESTS:
+            parents = torch.arange(n, dtype=torch.int32, device=self.kv_lens.device).masked_fill_(finished, -1)
+            paged_fork(self.kv_lens, self.block_tables, self.free_pages, self.n_free, parents, self.page_size,
+                       kv_lens_out=self.kv_lens, n_free_out=self.n_free)  # (nothing is copied: no pools)
+        else:
+            self._release_by_index(finished)
+
+    def _release_by_index(self, finished: torch.Tensor) -> None:
+        """release() in tensor operations, for what paged_fork refuses: off the GPU, fake tensors, tracers, more requests."""
+        table, pages = self.block_tables, self.free_pages.shape[0]
         held = torch.div(self.kv_lens + (self.page_size - 1), self.page_size, rounding_mode="floor")
-        block = torch.arange(self.block_tables.shape[1], device=self.kv_lens.device)
-        back = (finished[:, None] & (block < held[:, None])).flatten()
+        block = torch.arange(table.shape[1], device=table.device)
+        held = (block < held[:, None]) & (table >= 0) & (table < pages)
+        page = torch.where(held, table, pages).flatten().long()  # (pages: none)
+        # by page the first entry that lets it go, or -1 where a request keeps it
+        entry = torch.arange(table.numel(), device=table.device)
+        goes = (finished[:, None] & held).flatten()
+        first = torch.full((pages + 1,), table.numel(), device=table.device).scatter_reduce_(
+            0, page, torch.where(goes, entry, -1), "amin")
+        back = goes & (first[page] == entry)
         place = torch.where(back, self.n_free + back.cumsum(0) - 1, self._stack.numel() - 1)
-        self._stack.scatter_(0, place, self.block_tables.flatten())
+        self._stack.scatter_(0, place, table.flatten())
         self.n_free.add_(back.sum().to(torch.int32))
         self.kv_lens.masked_fill_(finished, 0)
 
