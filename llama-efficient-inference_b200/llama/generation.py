@@ -239,7 +239,8 @@ class Generation(nn.Module):
             logits = self.forward_paged(packed, step, cache, max(lengths), whole_prompts=True)
             if samples > 1:
                 first = torch.arange(n, dtype=torch.int32, device=device) // samples * samples
-                cache.fork(first)
+                if not bool(cache.fork(first).all()):
+                    raise RuntimeError("generate_paged: a sample was refused its prompt")
                 logits = logits.index_select(0, first)
             choice = pick(logits)
             note(logits, choice)
