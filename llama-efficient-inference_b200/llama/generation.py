@@ -291,6 +291,8 @@ class Generation(nn.Module):
         lengths = [len(t) for t in encoded]
         if not encoded or min(lengths) < 1:
             raise ValueError("score_paged: every text needs a token")
+        if rows < 1:
+            raise ValueError(f"score_paged: {rows} rows of logits at a time")
         cache = self.paged_cache(sum(-(-l // page_size) for l in lengths), page_size, max_requests=len(encoded),
                                  max_len=max(lengths), bits=kv_bits)
         packed = torch.tensor([t for toks in encoded for t in toks], dtype=torch.long, device=device)

@@ -50,3 +50,11 @@ def test_a_refused_sample_is_an_error():
     with pytest.raises(RuntimeError, match="refused"):
         Model(refused=4).generate_paged(*args, samples=3)
     assert len(Model(refused=1).generate_paged(*args)) == 2  # (one answer per prompt forks nothing)
+
+
+@pytest.mark.parametrize("rows", [0, -1, -1024])
+def test_no_rows_of_logits(rows, monkeypatch):
+    """(They gave results without log probabilities.)"""
+    monkeypatch.setattr("llama.generation.hidden_paged", lambda *a, **k: torch.zeros(2, 4))
+    with pytest.raises(ValueError, match="rows"):
+        Model().score_paged(Letters(), ["a"], "cpu", rows=rows)
