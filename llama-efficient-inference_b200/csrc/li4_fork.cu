@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const __grid_c
     if (r >= 0) a.tables[(long long)r * a.table_stride + j] = a.aside[place];
   });
   if (rank == 0) {
-    // (the lengths and the stack's height may be overwritten: every CTA has read them before the first barrier's end)
+    // (kv_out and n_free_out may be the inputs: every CTA has read those before it arrived at the barrier that ends pass 2)
     for (int b = tid; b < a.B; b += kForkThreads) a.kv_out[b] = s.len[b];
     if (tid == 0) {
       *a.n_free_out = min(a.capacity, n_free - taken + all);

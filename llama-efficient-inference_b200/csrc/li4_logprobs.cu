@@ -11,7 +11,9 @@
 // second (a warp reads all tiles of a thread where a third reaches it) and set such values aside; 64-bit keys of (value's order, inverted index) give their
 // order, ranked by counting.  (Values set aside tile by tile, against a bound that grows: 2047 rows of 128256 fp16 values, 8
 // likeliest, 148 us, one fp32 row, 20 likeliest, 12.2 us.)  A row whose values are equal can have more of them than there is
-// room for; its likeliest are then found one after the other, a pass over the row each.
+// room for; its likeliest are then found one after the other, a pass over the row each.  So rows with fewer allowed tokens than
+// likeliest asked for want -infinity in the other places, not the type's lowest value (2047 fp16 rows with three tokens
+// allowed, 8 / 32 likeliest: 150 / 151 us with -infinity, 7200 / 27000 us with the lowest value; one row 8 / 10 and 64 / 193).
 //
 // A cluster of 1, 2, 4 or 8 CTAs takes a row.  Bound by the bytes of the logits where there are many rows, by two trips to memory and
 // the cluster's join where there are few.
@@ -26,13 +28,14 @@ namespace cg = cooperative_groups;
 
 constexpr int kLogThreads = 256;
 constexpr int kLogWarps = kLogThreads / 32;
-// Of a type's values: 16-byte loads of a thread under way at a time, how many such steps make a tile.  16 values a step; the larger
-// tile halves the bookkeeping beside 16-bit values, whose exponentials and unpacking bound (2047 rows of 128256 fp16 values, 8
-// likeliest: 121 us; tiles of one step 126 us, of one step of four loads 141 us), fp32 rows want the smaller one (one row, 20
-// likeliest: 10.3 us, with tiles of two steps 12.1 us).  Four CTAs per SM, five for bf16 (130 us instead of 147).
+// Of a type's values: 16-byte loads of a thread under way at a time, how many such steps make a tile.  16 values a step for 16-bit
+// types (2047 rows of 128256 values, 8 likeliest: fp16 122 us, of four loads a step 131; bf16 127 and 209).  A tile of two steps
+// halves the bookkeeping, but with the loads as they are now tiles of one step would do for 16-bit types too (117 and 110 us);
+// fp32 rows want them (one row, 20 likeliest: 10.3 us, with tiles of two steps 12.3 us).  Four CTAs per SM, five for bf16 (127
+// us instead of 148).
 __host__ __device__ constexpr int log_loads(int bytes) { return bytes == 4 ? 4 : 2; }
 __host__ __device__ constexpr int log_steps(int bytes) { return bytes == 4 ? 1 : 2; }
-constexpr int kLogTile = kLogThreads * 16;  // values
+constexpr int kLogStep = kLogThreads * 16;  // values of a step
 constexpr int kLogAside = 2048;  // keys set aside per CTA
 constexpr int kMaxTop = LI4_MAX_TOP;
 constexpr int kLogCluster = 8;
@@ -524,9 +527,10 @@ extern "C" int li4_token_logprobs(const void* logits, int dtype, int64_t rows, i
   a.entropy = entropy;
   a.top_ids = reinterpret_cast<long long*>(top_ids);
   a.top_logprobs = top_logprobs;
-  // CTAs per row: as many as keep the SMs busy, a tile each at least
+  // CTAs per row: as many as keep the SMs busy, a step's values each at least (64 fp32 rows of 128256, 5 likeliest: one
+  // CTA each 25.8 us, 2 17.6, 4 14.5, 8 13.5; without the likeliest 23.0, 14.5, 11.4, 9.7)
   int c = 1;
-  while (c < kLogCluster && rows * c <= 2LL * current_sm_count() && cols / (2 * c) >= kLogTile) c *= 2;
+  while (c < kLogCluster && rows * c <= 2LL * current_sm_count() && cols / (2 * c) >= kLogStep) c *= 2;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int rc = dtype == LI4_F32   ? launch_logprobs<float>(a, rows, c, st)
                  : dtype == LI4_F16 ? launch_logprobs<__half>(a, rows, c, st)
